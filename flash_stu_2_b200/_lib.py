@@ -61,6 +61,9 @@ _SIGNATURES = {
     "stu_linear_launches": ([], c_int),
     "stu_linear_can_fuse_norm": ([c_int, c_int, c_int, c_int, c_int], c_int),
     "stu_linear_tile_cost": ([c_int, c_int], c_longlong),
+    "stu_quantize_fp8": ([_P, _P, _P, c_int, c_int, _LL, c_int, _P], c_int),
+    "stu_rmsnorm_fp8": ([_P, _P, _P, _P, _P, _P, c_int, c_int, _LL, _LL, _LL, c_float, c_int, _P], c_int),
+    "stu_linear_fp8": ([_P, _P, _P, _P, _P, _P, _P, _LL, _P, _LL, _P, c_int, c_int, c_int, c_int, _P], c_int),
     "stu_taps_even": ([_P, _P, c_int, c_int, c_int, c_int, _P], c_int),
     "stu_conv_prefill_approx": ([_P, _P, _P, _P, _LL, _LL, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
                                  _P], c_int),

@@ -225,6 +225,145 @@ PyObject* rmsnorm(PyObject*, PyObject* const* args, Py_ssize_t n) {
   Py_RETURN_NONE;
 }
 
+// ---- rows of 8-bit values (stu_quantize_fp8)
+struct Rows8 {
+  const at::Tensor *data = nullptr, *scales = nullptr;
+};
+std::pair<at::Tensor, at::Tensor> new_rows8(long long rows, long long cols, const at::Tensor& like) {
+  const auto bytes = like.options();
+  return {at::empty({rows, (cols + 127) / 128 * 128}, bytes.dtype(at::kFloat8_e4m3fn)),
+          at::empty({(rows + 127) / 128, (cols + 511) / 512, 32, 4, 4}, bytes.dtype(at::kFloat8_e8m0fnu))};
+}
+// `cols` columns in the layout that the kernels read, on device `dev`
+bool rows8(PyObject* data, PyObject* scales, long long cols, int dev, Rows8* r) {
+  if (!plain(data, &r->data) || !plain(scales, &r->scales) || !r->data || !r->scales) return false;
+  const at::Tensor &d = *r->data, &s = *r->scales;
+  return d.scalar_type() == at::kFloat8_e4m3fn && s.scalar_type() == at::kFloat8_e8m0fnu && d.dim() == 2 && d.is_contiguous() && s.is_contiguous() &&
+         d.device().index() == dev && s.device().index() == dev && cols > 0 && d.size(1) == (cols + 127) / 128 * 128 && d.size(0) <= INT32_MAX &&
+         s.sizes() == at::IntArrayRef({(d.size(0) + 127) / 128, (cols + 511) / 512, 32, 4, 4});
+}
+PyObject* pair_of(std::pair<at::Tensor, at::Tensor>&& r) {
+  PyObject *a = THPVariable_Wrap(std::move(r.first)), *b = a ? THPVariable_Wrap(std::move(r.second)) : nullptr;
+  PyObject* t = b ? PyTuple_Pack(2, a, b) : nullptr;
+  Py_XDECREF(a);
+  Py_XDECREF(b);
+  return t;
+}
+// [rows, cols] of a tensor of any number of dimensions without a copy: contiguous, or two dimensions with any row stride
+bool as_rows(const at::Tensor& t, long long* rows, long long* stride) {
+  if (t.dim() < 1 || t.numel() == 0 || t.size(-1) > INT32_MAX) return false;
+  const long long cols = t.size(-1);
+  if (!t.is_contiguous() && !(t.dim() == 2 && t.stride(1) == 1 && t.stride(0) >= cols)) return false;
+  *rows = t.numel() / cols;
+  *stride = t.is_contiguous() ? cols : t.stride(0);
+  return *rows <= INT32_MAX;
+}
+
+// quantize_fp8(x) -> (data, scales); rmsnorm_fp8(x, weight, eps, add, out) -> (data, scales); None: ops.py looks at it.
+PyObject* quantize_fp8(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 1) {
+    PyErr_SetString(PyExc_TypeError, "1 argument expected");
+    return nullptr;
+  }
+  try {
+    const at::Tensor* x;
+    long long rows, stride;
+    if (!plain(args[0], &x) || !x || dtype_code(*x) < 0 || x->device().index() != c10::cuda::current_device() || !as_rows(*x, &rows, &stride)) Py_RETURN_NONE;
+    const int code = dtype_code(*x), cols = (int)x->size(-1);
+    auto out = new_rows8(rows, cols, *x);
+    void *px = data_of(x), *pq = out.first.data_ptr(), *ps = out.second.data_ptr(), *stream = (void*)c10::cuda::getCurrentCUDAStream().stream();
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = stu_quantize_fp8(px, pq, ps, (int)rows, cols, stride, code, stream);
+    Py_END_ALLOW_THREADS
+    if (raised(rc, "stu_quantize_fp8")) return nullptr;
+    if (rc == 0) return pair_of(std::move(out));
+  } catch (const BadArgument&) {
+    PyErr_Clear();
+  } catch (const std::exception&) {
+  }
+  Py_RETURN_NONE;
+}
+PyObject* rmsnorm_fp8(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 5) {
+    PyErr_SetString(PyExc_TypeError, "5 arguments expected");
+    return nullptr;
+  }
+  try {
+    const at::Tensor *x, *w, *add, *out;
+    long long rows, xs, as = 0, os = 0, r = 0;
+    if (!plain(args[0], &x) || !plain(args[1], &w) || !plain(args[3], &add) || !plain(args[4], &out) || !x || !w || dtype_code(*x) < 0 ||
+        x->device().index() != c10::cuda::current_device() || !as_rows(*x, &rows, &xs))
+      Py_RETURN_NONE;
+    const auto alike = [&](const at::Tensor* t) { return t->scalar_type() == x->scalar_type() && t->device() == x->device(); };
+    const long long cols = x->size(-1);
+    if (!alike(w) || w->dim() != 1 || w->size(0) != cols || !w->is_contiguous() || (out && !add)) Py_RETURN_NONE;
+    if (add && (!alike(add) || add->sizes() != x->sizes() || !as_rows(*add, &r, &as))) Py_RETURN_NONE;
+    if (out && (!alike(out) || out->sizes() != x->sizes() || !as_rows(*out, &r, &os))) Py_RETURN_NONE;
+    if (add && !out) {
+      out = x;
+      os = xs;
+    }
+    const int code = dtype_code(*x);
+    const float eps = value_of<float>(args[2]);
+    auto made = new_rows8(rows, cols, *x);
+    void *px = data_of(x), *pa = data_of(add), *pw = data_of(w), *po = data_of(out), *pq = made.first.data_ptr(), *ps = made.second.data_ptr();
+    void* stream = (void*)c10::cuda::getCurrentCUDAStream().stream();
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = stu_rmsnorm_fp8(px, pa, pw, po, pq, ps, (int)rows, (int)cols, xs, as, os, eps, code, stream);
+    Py_END_ALLOW_THREADS
+    if (raised(rc, "stu_rmsnorm_fp8")) return nullptr;
+    if (rc == 0) return pair_of(std::move(made));
+  } catch (const BadArgument&) {
+    PyErr_Clear();
+  } catch (const std::exception&) {
+  }
+  Py_RETURN_NONE;
+}
+// linear_fp8(x data, x scales, W data, W scales, columns, W2 data, W2 scales, resid, out, flags) -> y, with W2 (data, scales); or None as above.
+PyObject* linear_fp8(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 10) {
+    PyErr_SetString(PyExc_TypeError, "10 arguments expected");
+    return nullptr;
+  }
+  try {
+    const long long cols = value_of<long long>(args[4]);
+    const int dev = c10::cuda::current_device(), flags = value_of<int>(args[9]);
+    Rows8 x, w, w2;
+    const at::Tensor *resid, *out;
+    const bool gate = args[5] != Py_None;
+    if (cols > INT32_MAX || !(g_ready.load(std::memory_order_relaxed) >> dev & 1) || !rows8(args[0], args[1], cols, dev, &x) ||
+        !rows8(args[2], args[3], cols, dev, &w) || (gate && !rows8(args[5], args[6], cols, dev, &w2)) || !plain(args[7], &resid) || !plain(args[8], &out))
+      Py_RETURN_NONE;
+    const long long M = x.data->size(0), N = w.data->size(0);
+    if (M == 0 || N == 0 || (gate && (w2.data->size(0) != N || resid || out))) Py_RETURN_NONE;
+    const auto fits = [&](const at::Tensor* t) {
+      return t->scalar_type() == at::kBFloat16 && t->device().index() == dev && t->dim() == 2 && t->size(0) == M && t->size(1) == N && t->stride(1) == 1 &&
+             (M == 1 || t->stride(0) >= N);
+    };
+    if ((resid && !fits(resid)) || (out && !fits(out))) Py_RETURN_NONE;
+    at::Tensor made;
+    std::pair<at::Tensor, at::Tensor> rows;
+    if (gate) rows = new_rows8(M, N, *x.data);
+    else if (!out) made = at::empty({M, N}, x.data->options().dtype(at::kBFloat16));
+    const at::Tensor* y = gate ? &rows.first : out ? out : &made;
+    void *p[] = {data_of(x.data), data_of(x.scales), data_of(w.data), data_of(w.scales), data_of(w2.data), data_of(w2.scales), data_of(resid), data_of(y),
+                 gate ? rows.second.data_ptr() : nullptr, (void*)c10::cuda::getCurrentCUDAStream().stream()};
+    const long long ldr = resid ? resid->stride(0) : 0, ldy = gate ? 0 : y->stride(0);
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = stu_linear_fp8(p[0], p[1], p[2], p[3], p[4], p[5], p[6], ldr, p[7], ldy, p[8], (int)M, (int)N, (int)cols, flags, p[9]);
+    Py_END_ALLOW_THREADS
+    if (raised(rc, "stu_linear_fp8")) return nullptr;
+    if (rc == 0) return gate ? pair_of(std::move(rows)) : made.defined() ? THPVariable_Wrap(std::move(made)) : Py_NewRef(args[8]);
+  } catch (const BadArgument&) {
+    PyErr_Clear();
+  } catch (const std::exception&) {
+  }
+  Py_RETURN_NONE;
+}
+
 // layer_step_f32(x, norm_w, MinT, hist, taps, pos, mid, mlp_norm_w, gate, up, down, eps, mlp_eps, decode_flags, gate_flags, down_flags,
 // status): one cached token of an approx layer in fp32, three launches: mid = x + STU(norm(x)); x = mid + MLP(norm(mid)).  Returns 3,
 // or 1 where the MLP was refused (mid is done; its kernels write nothing that they read, so the caller may run both again), or None
@@ -382,7 +521,10 @@ PyMethodDef methods[] = {
     ENTRY(stu_linear_push),
     ENTRY(stu_peer_combine),
     ENTRY(stu_peer_exchange),
+    ENTRY(stu_linear_fp8),
+    ENTRY(stu_quantize_fp8),
     ENTRY(stu_rmsnorm),
+    ENTRY(stu_rmsnorm_fp8),
     ENTRY(stu_sample),
     ENTRY(stu_swa_forward),
     ENTRY(stu_swa_prefill_scratch_elems),
@@ -395,6 +537,9 @@ PyMethodDef methods[] = {
     {"linear", (PyCFunction)(void (*)(void))linear, METH_FASTCALL, nullptr},
     {"layer_step_f32", (PyCFunction)(void (*)(void))layer_step_f32, METH_FASTCALL, nullptr},
     {"layer_prefill", (PyCFunction)(void (*)(void))layer_prefill, METH_FASTCALL, nullptr},
+    {"quantize_fp8", (PyCFunction)(void (*)(void))quantize_fp8, METH_FASTCALL, nullptr},
+    {"rmsnorm_fp8", (PyCFunction)(void (*)(void))rmsnorm_fp8, METH_FASTCALL, nullptr},
+    {"linear_fp8", (PyCFunction)(void (*)(void))linear_fp8, METH_FASTCALL, nullptr},
     {"rmsnorm", (PyCFunction)(void (*)(void))rmsnorm, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

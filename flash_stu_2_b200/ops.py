@@ -276,6 +276,179 @@ def linear(x: torch.Tensor, W: torch.Tensor, *, W2: Optional[torch.Tensor] = Non
     return out
 
 
+class Fp8Rows:
+    """Rows of 8-bit values: data [rows, columns rounded up to 128] (float8_e4m3fn, zero behind the `cols` columns) and one power-of-two scale for each
+    128 of a row, scales [rows / 128, cols / 512, 32, 4, 4] (float8_e8m0fnu, both rounded up): that of row 128 a + 32 b + c and block 4 g + j is at
+    [a, g, c, b, j], byte 0 where there is no such row or block.  quantize_fp8, rmsnorm_fp8 and linear_fp8(W2=) make them."""
+    __slots__ = ("data", "scales", "cols")
+
+    def __init__(self, data: torch.Tensor, scales: torch.Tensor, cols: int):
+        self.data, self.scales, self.cols = data, scales, cols
+
+    @property
+    def shape(self):
+        return self.data.shape[0], self.cols
+
+    def block_scales(self) -> torch.Tensor:
+        """The scales as numbers, [rows, blocks of 128] fp32."""
+        a, g = self.scales.shape[:2]
+        plain = self.scales.view(torch.uint8).permute(0, 3, 2, 1, 4).reshape(a * 128, g * 4)[:self.data.shape[0], :self.data.shape[1] // 128]
+        return plain.contiguous().view(torch.float8_e8m0fnu).float()
+
+    def dequantize(self) -> torch.Tensor:
+        """What the rows stand for, [rows, cols] fp32 (torch operations: for tests and inspection)."""
+        rows, padded = self.data.shape
+        v = self.data.float().view(rows, padded // 128, 128) * self.block_scales()[:, :, None]
+        return v.view(rows, padded)[:, :self.cols]
+
+    def check(self, what: str):
+        d, s = self.data, self.scales
+        if d.dtype != torch.float8_e4m3fn or s.dtype != torch.float8_e8m0fnu:
+            raise TypeError(f"{what}: 8-bit rows are float8_e4m3fn values with float8_e8m0fnu scales, got {d.dtype} and {s.dtype}")
+        want = ((d.shape[0] + 127) // 128, (self.cols + 511) // 512, 32, 4, 4) if d.dim() == 2 else None
+        if self.cols < 1 or d.dim() != 2 or d.shape[1] != (self.cols + 127) // 128 * 128 or tuple(s.shape) != want or not (
+                d.is_contiguous() and s.is_contiguous()):
+            raise ValueError(f"{what}: values {tuple(d.shape)} and scales {tuple(s.shape)} are not contiguous rows of {self.cols} columns")
+        _cuda(d, s)
+
+
+def _new_fp8(rows: int, cols: int, device) -> Fp8Rows:
+    return Fp8Rows(empty((rows, (cols + 127) // 128 * 128), torch.float8_e4m3fn, device),
+                   empty(((rows + 127) // 128, (cols + 511) // 512, 32, 4, 4), torch.float8_e8m0fnu, device), cols)
+
+
+def _elsewhere(*ts) -> Optional[torch.device]:
+    """The device of the tensors where it is not the current one (launches go to the current device's stream)."""
+    devices = {t.device for t in ts if t is not None}
+    if len(devices) != 1:
+        raise RuntimeError(f"tensors on several devices: {sorted(map(str, devices))}")
+    device = devices.pop()
+    return device if device.index != torch._C._cuda_getDevice() else None
+
+
+def _rows_of(t: torch.Tensor, what: str) -> torch.Tensor:
+    """[rows, cols] of t without a copy."""
+    if t.dim() == 2 and t.stride(1) == 1 and (t.stride(0) >= t.shape[1] or t.shape[0] < 2):
+        return t
+    if t.dim() < 1 or not t.is_contiguous():
+        raise ValueError(f"{what} is written in place: it has to be contiguous, or two-dimensional with contiguous rows")
+    return t.view(-1, t.shape[-1])
+
+
+def quantize_fp8(x: torch.Tensor) -> Fp8Rows:
+    """x [..., cols] (fp32 or bf16) as 8-bit rows: per 128 of a row the smallest power of two with which they fit e4m3's 448; nearest even;
+    infinities and NaN become NaN."""
+    if not _arenas or getattr(_local, "arena", None) is None:
+        made = _lib.native().quantize_fp8(x)
+        if made is not None:
+            _count()
+            return Fp8Rows(made[0], made[1], x.shape[-1])
+    _cuda(x)
+    dt = _dt(x)
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError(f"quantize_fp8: x {tuple(x.shape)} has no columns")
+    device = _elsewhere(x)
+    if device is not None:
+        with torch.cuda.device(device):
+            return quantize_fp8(x)
+    x2 = x.reshape(-1, x.shape[-1])
+    if x2.stride(1) != 1 or x2.stride(0) < x2.shape[1]:
+        x2 = x2.contiguous()
+    out = _new_fp8(*x2.shape, x.device)
+    if x2.shape[0] == 0:
+        return out
+    rc = _lib.native().stu_quantize_fp8(x2.data_ptr(), out.data.data_ptr(), out.scales.data_ptr(), x2.shape[0], x2.shape[1], x2.stride(0), dt, _stream())
+    _lib.check(rc, "stu_quantize_fp8")
+    _count()
+    return out
+
+
+def rmsnorm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float = RMS_EPS, add: Optional[torch.Tensor] = None,
+                out: Optional[torch.Tensor] = None) -> Fp8Rows:
+    """rmsnorm() as 8-bit rows, without a rounding between.  With `add`, x + add is normalised, and stored (rounded) in `out`, or in x itself where
+    that is not given: a residual stream takes in a branch on its way into the next one."""
+    if not _arenas or getattr(_local, "arena", None) is None:
+        made = _lib.native().rmsnorm_fp8(x, weight, eps, add, out)
+        if made is not None:
+            _count()
+            return Fp8Rows(made[0], made[1], x.shape[-1])
+    _cuda(x, weight, add, out)
+    dt = _dt(x)
+    if any(t is not None and t.dtype != x.dtype for t in (weight, add, out)):
+        raise TypeError("rmsnorm_fp8: x, weight, add and out are of one type")
+    if x.dim() < 1 or x.shape[-1] < 1 or weight.shape != x.shape[-1:] or any(t is not None and t.shape != x.shape for t in (add, out)):
+        raise ValueError(f"rmsnorm_fp8: x {tuple(x.shape)} with weight {tuple(weight.shape)}; add and out are of x's shape")
+    if out is not None and add is None:
+        raise ValueError("rmsnorm_fp8: out takes x + add")
+    device = _elsewhere(x, weight, add, out)
+    if device is not None:
+        with torch.cuda.device(device):
+            return rmsnorm_fp8(x, weight, eps, add, out)
+    d = x.shape[-1]
+    total = None if add is None else _rows_of(x if out is None else out, "rmsnorm_fp8: the sum")
+    x2 = _rows_of(x, "x") if add is not None and out is None else x.reshape(-1, d)
+    a2 = None if add is None else add.reshape(-1, d)
+    x2, a2 = (t if t is None or (t.stride(1) == 1 and (t.stride(0) >= d or t.shape[0] < 2)) else t.contiguous() for t in (x2, a2))
+    q = _new_fp8(x2.shape[0], d, x.device)
+    if x2.shape[0] == 0:
+        return q
+    rc = _lib.native().stu_rmsnorm_fp8(x2.data_ptr(), _p(a2), weight.contiguous().data_ptr(), _p(total), q.data.data_ptr(), q.scales.data_ptr(),
+                                       x2.shape[0], d, x2.stride(0), 0 if a2 is None else a2.stride(0), 0 if total is None else total.stride(0),
+                                       eps, dt, _stream())
+    _lib.check(rc, "stu_rmsnorm_fp8")
+    _count()
+    return q
+
+
+def linear_fp8(x: Fp8Rows, W: Fp8Rows, *, W2: Optional[Fp8Rows] = None, resid: Optional[torch.Tensor] = None,
+               out: Optional[torch.Tensor] = None, overlap: bool = False):
+    """linear() of 8-bit rows: x @ W^T as bf16 [rows of x, rows of W]; with `resid` (bf16; `out` may be the same) added to it; with W2
+    gelu_tanh(x @ W^T) * (x @ W2^T) as 8-bit rows.  overlap: the weights are fetched while the kernel before this one drains, which must not be
+    writing them (FLAG_OVERLAP)."""
+    flags = FLAG_OVERLAP if overlap else 0
+    if not _arenas or getattr(_local, "arena", None) is None:
+        if x.cols == W.cols and (W2 is None or W2.cols == W.cols):
+            y = _lib.native().linear_fp8(x.data, x.scales, W.data, W.scales, x.cols, *((None, None) if W2 is None else (W2.data, W2.scales)), resid, out, flags)
+            if y is not None:
+                _count()
+                return y if W2 is None else Fp8Rows(y[0], y[1], W.data.shape[0])
+    for name, rows in (("x", x), ("W", W), ("W2", W2)):
+        if rows is not None:
+            rows.check("linear_fp8: " + name)
+    _cuda(resid, out)
+    (M, K), N = x.shape, W.shape[0]
+    if W.cols != K or (W2 is not None and W2.shape != W.shape):
+        raise ValueError(f"linear_fp8: x {x.shape}, W {W.shape}" + ("" if W2 is None else f", W2 {W2.shape}"))
+    if W2 is not None and (resid is not None or out is not None):
+        raise ValueError("linear_fp8: with W2 the result is new 8-bit rows, nothing is added to it")
+    if N == 0:
+        raise ValueError("linear_fp8: W has no rows")
+    for name, t in (("resid", resid), ("out", out)):
+        if t is not None and t.dtype != torch.bfloat16:
+            raise TypeError(f"linear_fp8: {name} is bfloat16, got {t.dtype}")
+        if t is not None and (t.shape != (M, N) or t.stride(1) != 1 or (M > 1 and t.stride(0) < N)):
+            raise ValueError(f"linear_fp8: {name} {tuple(t.shape)} has to be [{M}, {N}] with contiguous rows")
+    device = _elsewhere(x.data, x.scales, W.data, W.scales, *(() if W2 is None else (W2.data, W2.scales)), resid, out)
+    if device is not None:
+        with torch.cuda.device(device):
+            return linear_fp8(x, W, W2=W2, resid=resid, out=out, overlap=overlap)
+    status_word(x.data.device)
+    if W2 is not None:
+        h = _new_fp8(M, N, x.data.device)
+        y, y_scales, ldy = h.data, h.scales, 0
+    else:
+        h = y = out if out is not None else empty((M, N), torch.bfloat16, x.data.device)
+        y_scales, ldy = None, y.stride(0)
+    if M == 0:
+        return h
+    rc = _lib.native().stu_linear_fp8(x.data.data_ptr(), x.scales.data_ptr(), W.data.data_ptr(), W.scales.data_ptr(), W2 and W2.data.data_ptr(),
+                                      W2 and W2.scales.data_ptr(), _p(resid), 0 if resid is None else resid.stride(0), y.data_ptr(), ldy, _p(y_scales),
+                                      M, N, K, flags, _stream())
+    _lib.check(rc, "stu_linear_fp8")
+    _count()
+    return h
+
+
 def taps_even(fp: torch.Tensor, Lh: int):
     """fp [L, d] (phi @ M_filters in the model dtype) -> even taps, channel-major [d, Lh]."""
     _cuda(fp)

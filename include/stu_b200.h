@@ -103,6 +103,26 @@ int stu_linear_split(const void* x, long long x_row_stride, const void* W, long 
                      int M, int N, int K, int epilogue, int hist_T, int hist_t0, int hist_Lh, const void* norm_w,
                      float eps, int dtype, int backend, float* workspace, long long workspace_elems, void* stream);
 
+/* Rows of 8-bit values (no counterpart in the reference).  values: e4m3 [rows][128 * ceil(cols / 128)], zero behind the columns; every 128 of a row
+ * share the scale 2^e, e the smallest whole number >= -127 with which their largest finite magnitude is at most 448 * 2^e, held as the byte
+ * e + 127 (E8M0).  scales: bytes [ceil(rows / 128)][ceil(cols / 512)][32][4][4]: row 128 a + 32 b + c, block 4 g + j at [a][g][c][b][j]; 0 where there is no
+ * such row or block.  Both 16-byte aligned.  Nearest even; infinities and NaN become NaN.
+ *
+ * stu_quantize_fp8: rows of dtype (x_row_stride elements apart) to such rows.
+ * stu_rmsnorm_fp8: s = x, or round(x + add) stored in sum (which may be x or add); s * rsqrt(mean(s^2) + eps) * w in fp32 to such rows.  All of
+ * dtype; cols <= 32768. */
+int stu_quantize_fp8(const void* x, void* values, void* scales, int rows, int cols, long long x_row_stride, int dtype, void* stream);
+int stu_rmsnorm_fp8(const void* x, const void* add, const void* w, void* sum, void* values, void* scales, int rows, int cols,
+                    long long x_row_stride, long long add_row_stride, long long sum_row_stride, float eps, int dtype, void* stream);
+/* Products of 8-bit rows x [M], W [N] of K columns, sums in fp32.
+ *   W2 = NULL    y[m][n] = round(acc), or round(resid[m][n] + round(acc)), bf16, row strides in elements (y may be resid)
+ *   W2 given     y, y_scales: gelu_tanh(x W^T) * (x W2^T), [M] rows of N columns, as 8-bit rows, without a rounding between
+ * flags: 0x200 = the weights are fetched while the kernel before this one drains (programmatic launch): no kernel still under way may be writing
+ * them.  Sums whose two scales multiply to 2^128 or more are infinite. */
+int stu_linear_fp8(const void* x, const void* x_scales, const void* W, const void* W_scales, const void* W2, const void* W2_scales,
+                   const void* resid, long long resid_row_stride, void* y, long long y_row_stride, void* y_scales, int M, int N, int K,
+                   int flags, void* stream);
+
 /* taps[c][j] = fp[2j][c] for fp = phi @ M_filters ([L,d], model dtype): the even taps that survive when the
  * plus and minus branches of flash_stu/utils/stu_utils.py:223-227 are added (flash_stu/modules/stu.py:88,120). */
 int stu_taps_even(const void* fp, void* taps, int L, int d, int Lh, int dtype, void* stream);

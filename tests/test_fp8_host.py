@@ -1,0 +1,94 @@
+"""8-bit rows without a GPU: the layout, what is refused, and the reference that the GPU tests compare with."""
+import torch
+import pytest
+
+import fp8_reference as R
+
+
+def made(rows, cols, seed=0):
+    from flash_stu_2_b200 import ops
+    g = torch.Generator().manual_seed(seed)
+    q, e = R.quantize((torch.randn(rows, cols, generator=g) * torch.exp2(torch.randint(-20, 20, (rows, 1), generator=g).float())).double())
+    return ops.Fp8Rows(q.to(torch.float8_e4m3fn), R.pieces((e + 127).to(torch.uint8)).view(torch.float8_e8m0fnu), cols)
+
+
+@pytest.mark.parametrize("rows,cols", [(1, 1), (5, 300), (128, 512), (131, 1111)])
+def test_layout(rows, cols):
+    r = made(rows, cols)
+    r_scales = r.scales.view(torch.uint8)
+    plain = r.block_scales()
+    assert plain.shape == (rows, (cols + 127) // 128) and r.shape == (rows, cols) and r.dequantize().shape == (rows, cols)
+    for row in {0, rows // 2, rows - 1}:
+        for k in {0, plain.shape[1] - 1}:
+            byte = int(r_scales[row // 128, k // 4, row % 32, row // 32 % 4, k % 4])
+            assert float(plain[row, k]) == 2.0 ** (byte - 127)
+    assert torch.equal(R.values(r), r.dequantize().double())
+
+
+def test_reference_quantisation_is_the_nearest():
+    """Against every number of the format: the scale is the smallest that fits, each value goes to the nearest, ties to the even one."""
+    g = torch.Generator().manual_seed(1)
+    v = (torch.randn(20, 256, generator=g).double() * 10).float().double()
+    v[0, 0], v[1, :128] = 448.0, 0.0
+    q, e = R.quantize(v)
+    numbers = torch.arange(256, dtype=torch.uint8).view(torch.float8_e4m3fn).double()
+    order = numbers[~numbers.isnan()].unique()
+    top = R.blocks(v.abs()).amax(2)
+    assert bool((top <= 448 * R.power(e)).all()) and bool(((top > 224 * R.power(e)) | (e == -127)).all())
+    z = (R.blocks(v) * R.power(-e)[:, :, None]).reshape(-1, 1)
+    assert bool(((q.reshape(-1, 1) - z).abs() <= (order[None] - z).abs().amin(1, keepdim=True)).all())
+
+
+def test_check_rows_notices():
+    """A wrong value, a wrong scale and a byte where no row is do not pass."""
+    from flash_stu_2_b200 import ops
+    g = torch.Generator().manual_seed(2)
+    v = torch.randn(9, 200, generator=g).double()
+    q, e = R.quantize(v.float().double())
+
+    def rows(q=q, e=e, touch=None):
+        s = R.pieces((e + 127).to(torch.uint8))
+        if touch:
+            s[touch] = 100
+        return ops.Fp8Rows(q.to(torch.float8_e4m3fn), s.view(torch.float8_e8m0fnu), 200)
+
+    R.check_rows(rows(), v, v.abs() * 2.0 ** -20)
+    wrong = q.clone()
+    wrong[3, 7] *= 1.25
+    for bad in (rows(wrong), rows(q / 2, e + 1), rows(touch=(0, 0, 9, 0, 0)), rows(touch=(0, 0, 0, 0, 2))):
+        with pytest.raises(AssertionError):
+            R.check_rows(bad, v, v.abs() * 2.0 ** -20)
+
+
+def test_no_cpu_path():
+    from flash_stu_2_b200 import ops
+    x = torch.zeros(2, 256)
+    r = made(2, 256)
+    for call in (lambda: ops.quantize_fp8(x), lambda: ops.rmsnorm_fp8(x, x[0]), lambda: ops.linear_fp8(r, r), lambda: ops.linear_fp8(r, r, W2=r)):
+        with pytest.raises(RuntimeError, match="no CPU path"):
+            call()
+    with pytest.raises(ValueError, match="contiguous rows of 250"):
+        ops.linear_fp8(ops.Fp8Rows(r.data, r.scales[:, :0], 250), r)
+    with pytest.raises(TypeError, match="float8_e4m3fn"):
+        ops.linear_fp8(ops.Fp8Rows(x, r.scales, 256), r)
+
+
+def test_argument_errors_of_the_library():
+    """Checked on the host before any CUDA call; the addresses are dummies."""
+    from flash_stu_2_b200 import _lib
+    lib, a = _lib.load(), 0x10000
+    assert lib.stu_quantize_fp8(None, a, a, 1, 128, 128, 1, None) == -5
+    assert lib.stu_quantize_fp8(a, a, a, 1, 0, 128, 1, None) == -2 and lib.stu_quantize_fp8(a, a, a, -1, 128, 128, 1, None) == -2
+    assert lib.stu_quantize_fp8(a, a + 8, a, 1, 128, 128, 1, None) == -3 and lib.stu_quantize_fp8(a, a, a, 1, 128, 128, 2, None) == -1
+    assert lib.stu_quantize_fp8(a, a, a, 0, 128, 128, 1, None) == 0
+    assert lib.stu_rmsnorm_fp8(a, a, a, None, a, a, 1, 128, 128, 128, 128, 1e-6, 1, None) == -5
+    assert lib.stu_rmsnorm_fp8(a, None, a, None, a, a, 1, 32769, 32769, 0, 0, 1e-6, 1, None) == -2
+    assert lib.stu_rmsnorm_fp8(a, None, a, None, a, a + 4, 1, 128, 128, 0, 0, 1e-6, 1, None) == -3
+    args = lambda **k: [{**dict(x=a, xs=a, w=a, ws=a, w2=None, w2s=None, r=None, ldr=0, y=a, ldy=8, ys=None, M=4, N=8, K=128, flags=0, st=None), **k}[n]
+                        for n in ("x", "xs", "w", "ws", "w2", "w2s", "r", "ldr", "y", "ldy", "ys", "M", "N", "K", "flags", "st")]
+    call = lambda **k: lib.stu_linear_fp8(*args(**k))
+    assert call(xs=None) == -5 and call(w2=a) == -5 and call(w2=a, w2s=a) == -5
+    assert call(N=0) == -2 and call(K=0) == -2 and call(M=-1) == -2 and call(K=2 ** 31 - 100) == -2
+    assert call(w2=a, w2s=a, ys=a, r=a) == -4 and call(flags=1) == -4
+    assert call(ws=a + 4) == -3 and call(w2=a, w2s=a, ys=a, y=a + 8) == -3
+    assert call(M=0) == 0

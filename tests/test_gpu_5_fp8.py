@@ -1,0 +1,331 @@
+"""Rows of 8-bit values, their norm and their products against the definitions in 64 bits (fp8_reference.py says what each may be off)."""
+import pytest
+import torch
+
+import fp8_reference as R
+
+pytestmark = pytest.mark.gpu
+
+BF16_HALF = torch.finfo(torch.bfloat16).eps / 2
+SHAPES = [(1, 128), (1, 1), (3, 100), (5, 512), (127, 129), (128, 513), (130, 1111), (300, 640), (2, 5000), (1, 18432)]
+
+
+def dev():
+    if not torch.cuda.is_available():
+        pytest.skip("needs a CUDA device")
+    return torch.device("cuda:0")
+
+
+def gen(seed):
+    return torch.Generator(device=dev()).manual_seed(seed)
+
+
+def stream(g, rows, cols, dt):
+    """Values over many powers of two, blocks of zeros among them."""
+    x = torch.randn(rows, cols, device=dev(), generator=g) * torch.exp2(torch.randint(-12, 13, (rows, 1), device=dev(), generator=g).float())
+    x = x * torch.exp(torch.randn(cols, device=dev(), generator=g))
+    x[:, cols // 2:cols // 2 + 128] *= (torch.rand(rows, 1, device=dev(), generator=g) < 0.8).float()
+    return x.to(dt)
+
+
+def rows8(g, rows, cols):
+    from flash_stu_2_b200 import ops
+    return ops.quantize_fp8(stream(g, rows, cols, torch.float32))
+
+
+def weights8(g, rows, cols):
+    from flash_stu_2_b200 import ops
+    return ops.quantize_fp8(torch.randn(rows, cols, device=dev(), generator=g) * torch.exp(torch.randn(rows, 1, device=dev(), generator=g)) * cols ** -0.5)
+
+
+def same_rows(a, b):
+    return a.cols == b.cols and torch.equal(a.data.view(torch.uint8), b.data.view(torch.uint8)) and torch.equal(
+        a.scales.view(torch.uint8), b.scales.view(torch.uint8))
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,cols", SHAPES)
+def test_quantize_is_exact(dt, rows, cols):
+    from flash_stu_2_b200 import ops
+    x = stream(gen(rows + cols), rows, cols, dt)
+    q = ops.quantize_fp8(x)
+    want, e = R.quantize(x.double())
+    assert torch.equal(q.data.double(), want)
+    assert torch.equal(q.scales.view(torch.uint8), R.pieces((e + 127).to(torch.uint8)))
+    assert torch.equal(q.dequantize().double(), (R.blocks(want) * R.power(e)[:, :, None]).view(want.shape)[:, :cols])
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+def test_quantize_borders(dt):
+    """Maxima on, right below and right above 448 * 2^e; ties between neighbours; the smallest numbers; infinities and NaN beside others and alone;
+    zeros of both signs; a maximum below the smallest scale's."""
+    from flash_stu_2_b200 import ops
+    lines = []
+    for top in (448.0, 450.0, 446.0, 1.75, 1.7578125, 2.0 ** -120 * 1.75, 2.0 ** 100):
+        line = torch.linspace(-1, 1, 128, dtype=torch.float64) * top
+        line[0] = top
+        lines.append(line)
+    grid = torch.arange(128, dtype=torch.float64)
+    lines.append(torch.cat([torch.tensor([448.0]), 16 + grid[:127] / 2]))          # ties among steps of 2
+    lines.append(torch.cat([torch.tensor([448.0]), grid[:127] * 2.0 ** -11]))      # below the smallest normal number, ties among steps of 2^-9
+    lines.append(torch.full((128,), 2.0 ** -126, dtype=torch.float64))
+    lines.append(-torch.zeros(128, dtype=torch.float64))
+    for special in (float("inf"), float("-inf"), float("nan")):
+        line = torch.linspace(-3, 3, 128, dtype=torch.float64)
+        line[[5, 77]] = special
+        lines.append(line)
+        lines.append(torch.full((128,), special, dtype=torch.float64))
+    x = torch.stack(lines).to(dt).to(dev())
+    q = ops.quantize_fp8(x)
+    want, e = R.quantize(x.double())
+    assert torch.equal(q.data.double().nan_to_num(7e7), want.nan_to_num(7e7))
+    assert torch.equal(q.scales.view(torch.uint8), R.pieces((e + 127).to(torch.uint8)))
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+def test_quantize_takes_any_strides(dt):
+    from flash_stu_2_b200 import ops
+    g = gen(3)
+    wide = stream(g, 40, 700, dt)
+    for x in (wide[:, 8:608], wide[:, 3:603], wide[::3, :300], wide.t(), wide.view(4, 10, 700), wide.view(4, 10, 700)[:, ::2, 5:400], wide[7], wide[:1, :9]):
+        flat = x.reshape(-1, x.shape[-1])
+        assert same_rows(ops.quantize_fp8(x), ops.quantize_fp8(flat.contiguous()))
+    assert ops.quantize_fp8(wide[:0]).shape == (0, 700) and ops.quantize_fp8(wide[:0]).dequantize().shape == (0, 700)
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("add", [False, True])
+@pytest.mark.parametrize("rows,cols", SHAPES + [(1300, 1536), (2500, 1024), (7, 32768), (1184, 2500)])
+def test_rmsnorm(dt, add, rows, cols):
+    """The stored sum is exact; statistics and scaling in fp32: sums of up to 32768 squares as chains of at most 64, 2^-16 in all."""
+    from flash_stu_2_b200 import ops
+    g = gen(rows + cols)
+    x, w = stream(g, rows, cols, dt), (1 + 0.3 * torch.randn(cols, device=dev(), generator=g)).to(dt)
+    branch = stream(g, rows, cols, dt) if add else None
+    before = x.clone()
+    q = ops.rmsnorm_fp8(x, w, 1e-5, add=branch)
+    s = before if not add else (before.float() + branch.float()).to(dt)
+    assert torch.equal(x, s)
+    v = s.double()
+    v = v / torch.sqrt(v.square().mean(1, keepdim=True) + 1e-5) * w.double()
+    R.check_rows(q, v, v.abs() * 2.0 ** -16)
+
+
+def test_rmsnorm_where_the_sum_goes():
+    """A separate output, the branch itself, strided rows of every operand; x alone stays as it is; rows of another count give the same rows."""
+    from flash_stu_2_b200 import ops
+    g = gen(5)
+    x, b, w = stream(g, 33, 520, torch.bfloat16), stream(g, 33, 520, torch.bfloat16), torch.rand(520, device=dev(), generator=g).bfloat16()
+    want, total = ops.rmsnorm_fp8(x.clone(), w, add=b), (x.float() + b.float()).bfloat16()
+    keep, out = x.clone(), torch.full((33, 600), 9.0, device=dev(), dtype=torch.bfloat16)
+    assert same_rows(ops.rmsnorm_fp8(x, w, add=b, out=out[:, 40:560]), want) and torch.equal(x, keep)
+    assert torch.equal(out[:, 40:560], total) and bool((out[:, :40] == 9).all()) and bool((out[:, 560:] == 9).all())
+    b2 = b.clone()
+    assert same_rows(ops.rmsnorm_fp8(x, w, add=b2, out=b2), want) and torch.equal(b2, total)
+    off = torch.empty(33, 523, device=dev(), dtype=torch.bfloat16)[:, 3:]   # off the 16-byte grid
+    off.copy_(x)
+    assert same_rows(ops.rmsnorm_fp8(off, w, add=b), want) and torch.equal(off, total)
+    assert same_rows(ops.rmsnorm_fp8(x.view(3, 11, 520), w, add=b.view(3, 11, 520), out=torch.empty_like(x).view(3, 11, 520)), want)
+    plain = ops.rmsnorm_fp8(x, w)
+    assert torch.equal(x, keep)
+    many = ops.rmsnorm_fp8(x.repeat(80, 1), w)
+    assert torch.equal(many.data.view(torch.uint8)[-33:], plain.data.view(torch.uint8)) and torch.equal(many.block_scales()[-33:], plain.block_scales())
+    assert ops.rmsnorm_fp8(x[:0], w, add=b[:0]).shape == (0, 520)
+
+
+def test_rmsnorm_of_rows_without_a_size():
+    """Zeros; a value whose square leaves fp32; infinities and NaN: the row's own, no other's."""
+    from flash_stu_2_b200 import ops
+    x = torch.randn(6, 300, device=dev(), generator=gen(1))
+    x[1] = 0
+    x[2, 7] = float("nan")
+    x[3, 299] = float("inf")
+    q = ops.rmsnorm_fp8(x, torch.ones(300, device=dev()), 1e-6)
+    v = x.double()
+    v = v / torch.sqrt(v.square().mean(1, keepdim=True) + 1e-6)
+    R.check_rows(q, v, v.abs().nan_to_num(0) * 2.0 ** -16)
+
+
+LINEAR = [(1, 1, 1), (1, 16, 128), (1, 1536, 18432), (2, 5, 100), (7, 129, 129), (8, 1024, 4096), (9, 200, 513), (16, 96, 1000), (17, 33, 640),
+          (32, 1536, 1536), (33, 1111, 1000), (64, 128, 2048), (127, 257, 300), (130, 520, 1536), (256, 256, 128), (333, 1111, 1000), (700, 1000, 520),
+          (1024, 2048, 1024), (1300, 300, 2000), (2049, 1536, 640), (4100, 260, 384)]
+
+
+def check_linear(y, x, w, resid=None):
+    ref, off = R.product(x, w)
+    off = off + (ref.abs() + off) * BF16_HALF
+    if resid is not None:
+        ref = ref + resid.double()
+        off = off + (ref.abs() + off) * BF16_HALF
+    bad = ~((y.double() - ref).abs() <= off + 1e-38)
+    assert not bool(bad.any()), f"{int(bad.sum())} of {bad.numel()} values, first {bad.nonzero()[0].tolist()}: " \
+                                f"{y[tuple(bad.nonzero()[0].tolist())]} for {ref[tuple(bad.nonzero()[0].tolist())]}"
+
+
+@pytest.mark.parametrize("resid", [False, True])
+@pytest.mark.parametrize("M,N,K", LINEAR)
+def test_linear(M, N, K, resid):
+    from flash_stu_2_b200 import ops
+    g = gen(M + N + K)
+    x, w = rows8(g, M, K), weights8(g, N, K)
+    r = stream(g, M, N, torch.bfloat16) if resid else None
+    y = ops.linear_fp8(x, w, resid=r)
+    check_linear(y, x, w, r)
+    assert torch.equal(ops.linear_fp8(x, w, resid=r), y)
+
+
+GATE = [(1, 1, 1), (1, 128, 128), (1, 4096, 1024), (2, 5, 100), (8, 640, 129), (9, 200, 513), (16, 1000, 1000), (31, 6144, 1536), (33, 129, 640),
+        (64, 1536, 768), (130, 520, 384), (256, 512, 128), (333, 1111, 1000), (1024, 1024, 1024), (1300, 300, 2000), (2049, 2048, 640)]
+
+
+@pytest.mark.parametrize("M,N,K", GATE)
+def test_gate(M, N, K):
+    from flash_stu_2_b200 import ops
+    g = gen(M + N + K)
+    x, w, w2 = rows8(g, M, K), weights8(g, N, K), weights8(g, N, K)
+    h = ops.linear_fp8(x, w, W2=w2)
+    R.check_rows(h, *R.gate(x, w, w2))
+    assert same_rows(ops.linear_fp8(x, w, W2=w2), h)
+
+
+def test_linear_writes_where_it_is_told():
+    """Outputs and residual rows in wider tensors, on and off the 16-byte grid, in place; what lies beside them stays."""
+    from flash_stu_2_b200 import ops
+    for M, N, K in [(5, 96, 256), (40, 200, 300), (300, 264, 256)]:
+        for lead in (8, 3):
+            g = gen(M + lead)
+            x, w, r = rows8(g, M, K), weights8(g, N, K), stream(g, M, N, torch.bfloat16)
+            want = ops.linear_fp8(x, w, resid=r)
+            big = torch.full((M, N + 24), 5.0, device=dev(), dtype=torch.bfloat16)
+            out = big[:, lead:lead + N]
+            assert ops.linear_fp8(x, w, resid=r, out=out) is out
+            assert torch.equal(out, want) and bool((big[:, :lead] == 5).all()) and bool((big[:, lead + N:] == 5).all())
+            out.copy_(r)
+            ops.linear_fp8(x, w, resid=out, out=out)
+            assert torch.equal(out, want) and bool((big[:, :lead] == 5).all()) and bool((big[:, lead + N:] == 5).all())
+            check_linear(ops.linear_fp8(x, w, out=out), x, w)
+    x, w = rows8(gen(1), 4, 256), weights8(gen(2), 8, 256)
+    none = ops.Fp8Rows(x.data[:0], x.scales[:0], 256)
+    assert ops.linear_fp8(none, w).shape == (0, 8) and ops.linear_fp8(none, w, W2=w).shape == (0, 8)
+
+
+@pytest.mark.parametrize("M", [3, 40, 400])
+def test_nan_stays_in_its_row_and_column(M):
+    from flash_stu_2_b200 import ops
+    g = gen(M)
+    a, b = torch.randn(M, 300, device=dev(), generator=g), torch.randn(140, 300, device=dev(), generator=g)
+    a[M - 1, 299] = float("nan")
+    b[7, 0] = float("inf")
+    x, w = ops.quantize_fp8(a), ops.quantize_fp8(b)
+    y = ops.linear_fp8(x, w)
+    nan = torch.zeros(M, 140, dtype=torch.bool, device=dev())
+    nan[M - 1] = True
+    nan[:, 7] = True
+    assert torch.equal(torch.isnan(y), nan)
+    h = ops.linear_fp8(x, w, W2=w)
+    assert torch.equal(torch.isnan(h.data[:, :140].float()), nan)
+    fine = torch.isfinite(a).all(1)
+    one = ops.linear_fp8(ops.quantize_fp8(a[fine]), w)
+    check = ~nan[fine]
+    assert torch.equal(one[check], y[fine][check])
+
+
+@pytest.mark.parametrize("M", [2, 20, 200])
+def test_scales_far_apart(M):
+    """Operands whose scales differ by 2^100 from block to block: products of tiny and huge blocks are exact powers of two apart."""
+    from flash_stu_2_b200 import ops
+    g = gen(M)
+    up = torch.exp2(torch.tensor([0, 50, -50, 20, -100], device=dev()).float()).repeat_interleave(128)
+    a, b = torch.randn(M, 640, device=dev(), generator=g) * up, torch.randn(72, 640, device=dev(), generator=g) / up
+    x, w = ops.quantize_fp8(a), ops.quantize_fp8(b)
+    check_linear(ops.linear_fp8(x, w), x, w)
+
+
+@pytest.mark.parametrize("M,d,inter", [(1, 1024, 4096), (32, 512, 1536), (300, 384, 1000)])
+def test_an_mlp_of_them(M, d, inter):
+    """Norm, gate and up, down onto the stream, one behind the other: within what 8 bits lose of the MLP in 64 bits, and each call against its own inputs.
+    Two quantisations of normal values (2^-4 at most, 2^-5.3 in the mean square) and as much of the weights: every product is off by
+    less than 2^-4 of its terms' root sum of squares; 4 of them compound to less than 1/8 of the branch's."""
+    from flash_stu_2_b200 import ops
+    g = gen(M + d)
+    x = torch.randn(M, d, device=dev(), generator=g).bfloat16()
+    branch, norm = torch.randn(M, d, device=dev(), generator=g).bfloat16(), (1 + 0.1 * torch.randn(d, device=dev(), generator=g)).bfloat16()
+    gate, up, down = (torch.randn(*s, device=dev(), generator=g) * s[1] ** -0.5 for s in ((inter, d), (inter, d), (d, inter)))
+    wg, wu, wd = (ops.quantize_fp8(t) for t in (gate, up, down))
+    total = torch.empty_like(x)
+    xn = ops.rmsnorm_fp8(x, norm, add=branch, out=total)
+    h = ops.linear_fp8(xn, wg, W2=wu, overlap=True)
+    y = ops.linear_fp8(h, wd, resid=total, overlap=True)
+    R.check_rows(h, *R.gate(xn, wg, wu))
+    check_linear(y, h, wd, total)
+    s = (x.float() + branch.float()).bfloat16().double()
+    v = s / torch.sqrt(s.square().mean(1, keepdim=True) + ops.RMS_EPS) * norm.double()
+    mlp = (R.gelu(v @ gate.double().T) * (v @ up.double().T)) @ down.double().T
+    assert float((y.double() - s - mlp).norm() / mlp.norm()) < 0.125
+
+
+def test_another_stream_and_a_replayed_graph():
+    from flash_stu_2_b200 import ops
+    g = gen(8)
+    M, d, inter = 5, 512, 1024
+    xs = [torch.randn(M, d, device=dev(), generator=g).bfloat16() for _ in range(3)]
+    norm = torch.ones(d, device=dev(), dtype=torch.bfloat16)
+    wg, wu, wd = weights8(g, inter, d), weights8(g, inter, d), weights8(g, d, inter)
+
+    def mlp(x):
+        return ops.linear_fp8(ops.linear_fp8(ops.rmsnorm_fp8(x, norm), wg, W2=wu), wd, resid=x)
+
+    want = [mlp(x) for x in xs]
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = [mlp(x) for x in xs]
+    side.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    static = xs[0].clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = mlp(static)
+    for x, w in zip(xs, want):
+        static.copy_(x)
+        graph.replay()
+        assert torch.equal(out, w)
+    # outputs from an arena, as a captured step takes them
+    buffer = torch.zeros(1 << 20, dtype=torch.uint8, device=dev())
+    with ops.arena(buffer):
+        y = mlp(xs[1])
+    assert torch.equal(y, want[1])
+    assert buffer.data_ptr() <= y.data_ptr() < buffer.data_ptr() + buffer.numel()
+    ops.check_status()
+
+
+def test_refusals():
+    from flash_stu_2_b200 import ops
+    g = gen(4)
+    x, w = rows8(g, 4, 256), weights8(g, 8, 256)
+    b = torch.zeros(4, 8, device=dev(), dtype=torch.bfloat16)
+    half = torch.zeros(4, 256, device=dev(), dtype=torch.float16)
+    for call, error, text in [
+            (lambda: ops.quantize_fp8(half), TypeError, "float32 or bfloat16"),
+            (lambda: ops.quantize_fp8(b[:, :0]), ValueError, "no columns"),
+            (lambda: ops.rmsnorm_fp8(b, torch.ones(8, device=dev())), TypeError, "one type"),
+            (lambda: ops.rmsnorm_fp8(b, b[0, :7]), ValueError, "weight"),
+            (lambda: ops.rmsnorm_fp8(b, b[0], add=b[:2]), ValueError, "x's shape"),
+            (lambda: ops.rmsnorm_fp8(b, b[0], out=b), ValueError, "x \\+ add"),
+            (lambda: ops.rmsnorm_fp8(b.t(), b[:, 0].contiguous(), add=b.t()), ValueError, "in place"),
+            (lambda: ops.rmsnorm_fp8(torch.zeros(1, 32769, device=dev()), torch.zeros(32769, device=dev())), RuntimeError, "shape"),
+            (lambda: ops.linear_fp8(x, weights8(g, 8, 300)), ValueError, "linear_fp8"),
+            (lambda: ops.linear_fp8(x, w, W2=weights8(g, 9, 256)), ValueError, "W2"),
+            (lambda: ops.linear_fp8(x, w, W2=w, resid=b), ValueError, "added"),
+            (lambda: ops.linear_fp8(x, w, resid=b.float()), TypeError, "bfloat16"),
+            (lambda: ops.linear_fp8(x, w, out=b[:, :7]), ValueError, "out"),
+            (lambda: ops.linear_fp8(x, w, out=b.t().contiguous().t()), ValueError, "contiguous rows"),
+            (lambda: ops.linear_fp8(ops.Fp8Rows(x.data[:, :128], x.scales, 128), w), ValueError, "contiguous rows"),
+            (lambda: ops.linear_fp8(ops.Fp8Rows(x.data, x.scales[:0], 256), w), ValueError, "scales"),
+            (lambda: ops.linear_fp8(ops.Fp8Rows(x.data.float(), x.scales, 256), w), TypeError, "float8_e4m3fn"),
+            (lambda: ops.linear_fp8(x, ops.Fp8Rows(w.data[:0], w.scales[:0], 256)), ValueError, "no rows"),
+            (lambda: ops.linear_fp8(x, ops.Fp8Rows(w.data.cpu(), w.scales, 256)), RuntimeError, "no CPU path")]:
+        with pytest.raises(error, match=text):
+            call()
+    torch.cuda.synchronize()
