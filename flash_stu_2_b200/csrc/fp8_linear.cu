@@ -9,6 +9,7 @@
 #include <cooperative_groups.h>
 
 #include "fp8.cuh"
+#include "fp8_gemm.cuh"
 
 namespace cg = cooperative_groups;
 
@@ -244,7 +245,9 @@ extern "C" int stu_linear_fp8(const void* x, const void* x_scales, const void* W
 #define STU_STREAM(NG_, DUAL_)                                                                                                       \
   launch_stream<NG_, DUAL_>(a, w, w2, (const bf16*)resid, resid_row_stride, DUAL_ ? nullptr : (bf16*)y, y_row_stride,                \
                             DUAL_ ? (unsigned char*)y : nullptr, (unsigned char*)y_scales, M, N, K, overlap, st)
-  if (M > 65535 * 32) return STU_ERR_SHAPE;
+  if (M > 32)
+    return fp8_gemm({a.q, a.scales, w.q, w.scales, w2.q, w2.scales, (const bf16*)resid, resid_row_stride, W2 ? nullptr : (bf16*)y, y_row_stride,
+                     W2 ? (unsigned char*)y : nullptr, (unsigned char*)y_scales, M, N, K}, st);
   if (M <= 8) return W2 ? STU_STREAM(1, true) : STU_STREAM(1, false);
   if (M <= 16) return W2 ? STU_STREAM(2, true) : STU_STREAM(2, false);
   return W2 ? STU_STREAM(4, true) : STU_STREAM(4, false);

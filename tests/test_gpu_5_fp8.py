@@ -329,3 +329,30 @@ def test_refusals():
         with pytest.raises(error, match=text):
             call()
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("M", [100, 300])
+@pytest.mark.parametrize("two", [False, True])
+def test_a_wait_that_runs_out(M, two):
+    """A CTA alone and a pair of them, plain and gate/up: a first stage that never fills is reported (status 3) within the shortened bound, and the next
+    call is as ever."""
+    import time
+    from flash_stu_2_b200 import _lib, ops
+    lib, g = _lib.load(), gen(M)
+    x, w, w2 = rows8(g, M, 700), weights8(g, 400, 700), weights8(g, 400, 700)
+    call = (lambda: ops.linear_fp8(x, w, W2=w2)) if two else (lambda: ops.linear_fp8(x, w))
+    same = same_rows if two else torch.equal
+    want = call()
+    ops.check_status()
+    assert lib.stu_test_inject_wait_expiry(100) == 0
+    try:
+        t0 = time.monotonic()
+        call()
+        torch.cuda.synchronize()
+        assert time.monotonic() - t0 < 5.0
+        with pytest.raises(RuntimeError, match="status 3"):
+            ops.check_status()
+    finally:
+        assert lib.stu_test_inject_wait_expiry(0) == 0
+    assert same(call(), want)
+    ops.check_status()
