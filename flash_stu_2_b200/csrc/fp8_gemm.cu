@@ -16,115 +16,18 @@
 //
 // Every wait is bounded, as in gemm_tc.cu: on expiry the waiter tells the others, raises the status word, and the CTAs drain their copies, free
 // their tensor memory and return.
-#include <cuda.h>
-
 #include <new>
 
-#include "fp8.cuh"
 #include "fp8_gemm.cuh"
-#include "tma.cuh"
 
 int device_sm_count();      // gemm_tc.cu
 int* device_status_word();  // gemm_tc.cu
 
+using namespace fp8;
+
 namespace {
 
-constexpr int BM = 128, BK = 128;   // rows of x per CTA; bytes of a k-block: a block of 128 columns, one row of the 128-byte swizzle
-constexpr int A_BYTES = BM * BK;
-constexpr int EPI_WARPS = 8, BLOCK_BYTES = 32 * 64 * 2;   // an epilogue warp's block of 32 rows x 64 bf16 columns
-constexpr uint32_t WAIT_LIMIT = 1u << 22;
-
-__device__ __forceinline__ void load_2d_pair(void* dst, const CUtensorMap* map, uint32_t bar, int x, int y) {
-  asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
-               ::"r"(tma::smem_u32(dst)), "l"(map), "r"(bar), "r"(x), "r"(y)
-               : "memory");
-}
-__device__ __forceinline__ void load_3d_pair(void* dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z) {
-  asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
-               ::"r"(tma::smem_u32(dst)), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z)
-               : "memory");
-}
-__device__ __forceinline__ void load_2d(void* dst, const CUtensorMap* map, uint64_t* bar, int x, int y) {
-  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
-               ::"r"(tma::smem_u32(dst)), "l"(map), "r"(tma::smem_u32(bar)), "r"(x), "r"(y)
-               : "memory");
-}
-__device__ __forceinline__ bool mbar_ready(uint64_t* bar, uint32_t parity) {   // without waiting
-  uint32_t ok;
-  asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-               : "=r"(ok) : "r"(tma::smem_u32(bar)), "r"(parity) : "memory");
-  return ok != 0;
-}
-// shared::cluster address of the pair's first CTA's copy of a shared-memory object
-__device__ __forceinline__ uint32_t in_first_cta(const void* p) {
-  uint32_t a;
-  asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(tma::smem_u32(p)));
-  return a;
-}
-__device__ __forceinline__ uint32_t load_from_cta(const volatile int* p, uint32_t cta) {
-  uint32_t a, v;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(tma::smem_u32((const void*)p)), "r"(cta));
-  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
-  return v;
-}
-__device__ __forceinline__ void store_to_cta(const volatile int* p, uint32_t cta, int v) {
-  uint32_t a;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(tma::smem_u32((const void*)p)), "r"(cta));
-  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(a), "r"(v) : "memory");
-}
-__device__ __forceinline__ void pair_sync() {   // both CTAs, all threads; orders no stores
-  asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
-  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-
-// Shared-memory descriptors: an operand tile, rows of 128 bytes in the 128-byte swizzle, 8-row groups 1024 bytes apart; a piece of scales, 32 rows of
-// 16 bytes without a swizzle, 8-row groups 128 bytes apart.
-__device__ __forceinline__ uint64_t operand_desc(uint32_t saddr) {
-  return (uint64_t)((saddr >> 4) & 0x3FFF) | (uint64_t)1 << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
-}
-__device__ __forceinline__ uint64_t scales_desc(uint32_t saddr) {
-  return (uint64_t)((saddr >> 4) & 0x3FFF) | (uint64_t)(128 >> 4) << 32 | (uint64_t)1 << 46;
-}
-
-template <int CTAS> __device__ __forceinline__ void copy_scales(uint32_t tmem, uint64_t desc) {
-  if constexpr (CTAS == 2) asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
-  else asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
-}
-// One instruction: 32 columns of K.  sf: which byte of the scale words.
-template <int CTAS, int N>
-__device__ __forceinline__ void multiply(uint32_t d, uint64_t a, uint64_t b, uint32_t sfa, uint32_t sfb, uint32_t sf, uint32_t accumulate) {
-  // D fp32, A and B e4m3, both K-major, scales E8M0
-  const uint32_t idesc = (1u << 23) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(CTAS * BM >> 4) << 24) | (sf << 29) | (sf << 4);
-  if constexpr (CTAS == 2)
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
-                 "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
-                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate) : "memory");
-  else
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
-                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate) : "memory");
-}
-// Arrives (at the barrier of both CTAs of a pair) when what was issued so far is done.
-template <int CTAS> __device__ __forceinline__ void commit(uint64_t* bar) {
-  if constexpr (CTAS == 2)
-    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(tma::smem_u32(bar)),
-                 "h"((uint16_t)3) : "memory");
-  else
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(tma::smem_u32(bar)) : "memory");
-}
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,"
-      "%28,%29,%30,%31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(taddr));
-}
+constexpr int EPI_WARPS = 8, BLOCK_BYTES = 32 * 32 * 2;   // an epilogue warp's block of 32 rows x 32 bf16 columns
 
 // Bands of group_m row tiles, rows first inside a band.
 __device__ __forceinline__ void tile_coords(int tile, int tiles_m, int tiles_n, int group_m, int& tm, int& tn) {
@@ -144,9 +47,11 @@ struct Out {
 template <bool DUAL, int CTAS, int TN> struct Form {
   static constexpr int MMA_N = DUAL ? 2 * TN : TN;                     // accumulator columns
   static constexpr int B_ROWS = MMA_N / CTAS;                          // rows of B in a CTA's shared memory
-  static constexpr int TILE_BYTES = A_BYTES + B_ROWS * BK;             // of one CTA
+  // k-blocks of a stage: two halve what waiting and sending off take of a pair's stage, a CTA alone has too few stages of them
+  static constexpr int KBS = CTAS == 2 ? 2 : 1;
+  static constexpr int KB_BYTES = A_BYTES + B_ROWS * BK, TILE_BYTES = KBS * KB_BYTES;   // of one CTA
   static constexpr int SCALE_BYTES = fp8::PIECE * (1 + (MMA_N + 127) / 128);
-  static constexpr int STAGES = DUAL ? (CTAS == 2 ? 6 : 4) : 5;
+  static constexpr int STAGES = (227 * 1024 - 2048 - (DUAL ? 2048 : EPI_WARPS * BLOCK_BYTES)) / (TILE_BYTES + SCALE_BYTES);
   // accumulators at columns 0 and SECOND, scales behind them, twice 16 columns (x at 0, W from 4 on)
   static constexpr int SHARED = MMA_N == 256 ? 32 : 0, SECOND = MMA_N - SHARED, SCALES = SECOND + MMA_N;
   static constexpr uint32_t TMEM_COLS = MMA_N == 256 ? 512 : 2 * MMA_N + 32 <= 256 ? 256 : 512;
@@ -162,7 +67,7 @@ __global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__(64 + 32 * EPI_WAR
                     int K, int tiles_m, int tiles_n, int group_m, Out out, int* status, int drop_first_copy, unsigned long long wait_ns) {
   using F = Form<DUAL, CTAS, TN>;
   constexpr bool PAIR = CTAS == 2;
-  constexpr int MMA_N = F::MMA_N, STAGES = F::STAGES, SHARED = F::SHARED;
+  constexpr int MMA_N = F::MMA_N, STAGES = F::STAGES, SHARED = F::SHARED, KBS = F::KBS;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   unsigned char* scales = smem + STAGES * F::TILE_BYTES;            // [stage]: of x, then of W
@@ -225,7 +130,7 @@ __global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__(64 + 32 * EPI_WAR
       int tm, tn;
       tile_coords(tile, tiles_m, tiles_n, group_m, tm, tn);
       const int m0 = (CTAS * tm + rank) * BM, n0 = tn * TN + (DUAL ? 0 : rank * F::B_ROWS), nb = tn * TN / 128;
-      for (int kb = 0; kb < num_kb; kb++, g++) {
+      for (int kb = 0; kb < num_kb; kb += KBS, g++) {
         if (!ready) ok = tma::warp_wait_bounded(&empty_bar[s], ph, abort_flag, wait_ns);
         if (!ok) break;
         const int s1 = s + 1 == STAGES ? 0 : s + 1;
@@ -233,22 +138,31 @@ __global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__(64 + 32 * EPI_WAR
         const bool ready1 = mbar_ready(&empty_bar[s1], ph1);   // asked for here, looked at behind the copies
         if (leader) {
           const bool with_scales = (kb & 3) == 0;
+          const int n = min(KBS, num_kb - kb);
           unsigned char *sa = smem + s * F::TILE_BYTES, *ss = scales + s * F::SCALE_BYTES;
-          if (rank == 0) tma::mbar_expect_tx(&full_bar[s], CTAS * (F::TILE_BYTES + (with_scales ? F::SCALE_BYTES : 0)));   // of both CTAs
+          if (rank == 0) tma::mbar_expect_tx(&full_bar[s], CTAS * (n * F::KB_BYTES + (with_scales ? F::SCALE_BYTES : 0)));   // of both CTAs
           if (!(drop_first_copy && g == 0)) {   // (failure-detection test: the first stage never fills)
             const uint32_t bar = full0 + s * (uint32_t)sizeof(uint64_t);
             if constexpr (PAIR) {
-              load_2d_pair(sa, &tmA, bar, kb * BK, m0);
-              load_2d_pair(sa + A_BYTES, mapB, bar, kb * BK, n0);
+#pragma unroll
+              for (int j = 0; j < KBS; j++)
+                if (j < n) {
+                  load_2d_pair(sa + j * F::KB_BYTES, &tmA, bar, (kb + j) * BK, m0);
+                  load_2d_pair(sa + j * F::KB_BYTES + A_BYTES, mapB, bar, (kb + j) * BK, n0);
+                }
               if (with_scales) {
                 load_3d_pair(ss, &tmSA, bar, 0, kb >> 2, m0 / BM);
                 load_3d_pair(ss + fp8::PIECE, &tmSB, bar, 0, kb >> 2, nb);
                 if (DUAL) load_3d_pair(ss + 2 * fp8::PIECE, &tmSB2, bar, 0, kb >> 2, nb);
               }
             } else {
-              load_2d(sa, &tmA, &full_bar[s], kb * BK, m0);
-              load_2d(sa + A_BYTES, &tmB, &full_bar[s], kb * BK, n0);
-              if (DUAL) load_2d(sa + A_BYTES + TN * BK, &tmB2, &full_bar[s], kb * BK, n0);
+#pragma unroll
+              for (int j = 0; j < KBS; j++)
+                if (j < n) {
+                  load_2d(sa + j * F::KB_BYTES, &tmA, &full_bar[s], (kb + j) * BK, m0);
+                  load_2d(sa + j * F::KB_BYTES + A_BYTES, &tmB, &full_bar[s], (kb + j) * BK, n0);
+                  if (DUAL) load_2d(sa + j * F::KB_BYTES + A_BYTES + TN * BK, &tmB2, &full_bar[s], (kb + j) * BK, n0);
+                }
               if (with_scales) {
                 tma::load_3d(ss, &tmSA, &full_bar[s], 0, kb >> 2, m0 / BM);
                 tma::load_3d(ss + fp8::PIECE, &tmSB, &full_bar[s], 0, kb >> 2, nb);
@@ -280,7 +194,7 @@ __global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__(64 + 32 * EPI_WAR
         ok = tma::warp_wait_bounded(&tmem_empty[buf], (((uint32_t)it >> 1) & 1u) ^ 1u, abort_flag, wait_ns);
         if (SHARED && ok && it > 0) ok = tma::warp_wait_bounded(&shared_read[buf ^ 1], ((uint32_t)(it - 1) >> 1) & 1u, abort_flag, wait_ns);
         if (!ok) break;
-        for (int kb = 0; kb < num_kb; kb++, g++) {
+        for (int kb = 0; kb < num_kb; kb += KBS, g++) {
           if (!ready) ok = tma::warp_wait_bounded(&full_bar[s], ph, abort_flag, wait_ns);
           if (!ok) break;
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -296,8 +210,13 @@ __global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__(64 + 32 * EPI_WAR
             }
             const uint64_t da = da0 + (uint64_t)(s * (F::TILE_BYTES >> 4)), db = db0 + (uint64_t)(s * (F::TILE_BYTES >> 4));
 #pragma unroll
-            for (int kk = 0; kk < BK / 32; kk++)   // 32 bytes along K inside the swizzled row: +2
-              multiply<CTAS, MMA_N>(acc, da + 2 * kk, db + 2 * kk, sf_cols, sf_cols + 4, kb & 3, (kb | kk) ? 1u : 0u);
+            for (int j = 0; j < KBS; j++)
+              if (j == 0 || kb + j < num_kb) {
+#pragma unroll
+                for (int kk = 0; kk < BK / 32; kk++)   // 32 bytes along K inside the swizzled row: +2
+                  multiply<CTAS, MMA_N>(acc, da + j * (F::KB_BYTES >> 4) + 2 * kk, db + j * (F::KB_BYTES >> 4) + 2 * kk, sf_cols, sf_cols + 4, (kb + j) & 3,
+                                        (kb | j | kk) ? 1u : 0u);
+              }
             commit<CTAS>(&empty_bar[s]);
           }
           ready = __all_sync(0xffffffffu, ready1);
@@ -397,63 +316,66 @@ __global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__(64 + 32 * EPI_WAR
         if (!ok) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         bf16* st = reinterpret_cast<bf16*>(blocks + (warp - 2) * BLOCK_BYTES);
-        auto at = [&](int row, int piece) { return st + row * 64 + ((piece ^ (row & 7)) << 3); };   // 8 values, 16 bytes
+        auto at = [&](int row, int piece) { return st + row * 32 + ((piece ^ ((row >> 1) & 3)) << 3); };   // 8 values, 16 bytes
         const bool on_grid = !((out.ldy & 7) || (reinterpret_cast<uintptr_t>(out.y) & 15)) &&
                              !(out.resid && ((out.ldr & 7) || (reinterpret_cast<uintptr_t>(out.resid) & 15)));
         const int rows = min(32, M - first);   // this warp's
+        constexpr int SUBS = TN / 64;          // blocks of this half's columns, 64 of every 128
 #pragma unroll 1
-        for (int i = 0; i < TN / 128; i++) {
-          const int c = 128 * (buf ? i : TN / 128 - 1 - i) + 64 * half, n = tn * TN + c;   // 64 columns
-          uint32_t r[2][32];
-          tmem_ld32(acc + c, r[0]);
-          tmem_ld32(acc + c + 32, r[1]);
+        for (int i = 0; i < SUBS; i++) {
+          const int sub = buf ? i : SUBS - 1 - i, c = 128 * (sub >> 1) + 64 * half + 32 * (sub & 1), n = tn * TN + c;
+          uint32_t r[32];
+          tmem_ld32(acc + c, r);
           asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
           shared_done(i);
-          if (i == TN / 128 - 1) all_done();
+          if (i == SUBS - 1) all_done();
           if (n >= N || rows <= 0) continue;
 #pragma unroll
-          for (int p = 0; p < 8; p++) {
+          for (int p = 0; p < 4; p++) {
             float o[8];
 #pragma unroll
-            for (int j = 0; j < 8; j++) o[j] = __uint_as_float(r[p >> 2][(p & 3) * 8 + j]);
+            for (int j = 0; j < 8; j++) o[j] = __uint_as_float(r[p * 8 + j]);
             store_vec(at(lane, p), o);
           }
           __syncwarp();
-          // whole lines: 8 lanes per row, 4 rows at a time
-          const int piece = lane & 7, r0 = lane >> 3, np = n + piece * 8;
-          if (on_grid && n + 64 <= N) {
+          // 64 bytes of a row by 4 lanes, 8 rows at a time
+          const int piece = lane & 3, r0 = lane >> 2, np = n + piece * 8;
+          if (on_grid && n + 32 <= N) {
             bf16* yc = out.y + (size_t)(first + r0) * out.ldy + np;
-            uint4 v[8];
+            uint4 v[4];
             if (out.resid) {
               const bf16* rc = out.resid + (size_t)(first + r0) * out.ldr + np;
 #pragma unroll
-              for (int j = 0; j < 8; j++)
-                v[j] = r0 + 4 * j < rows ? *reinterpret_cast<const uint4*>(rc + (size_t)(4 * j) * out.ldr) : make_uint4(0, 0, 0, 0);
+              for (int j = 0; j < 4; j++)
+                v[j] = r0 + 8 * j < rows ? *reinterpret_cast<const uint4*>(rc + (size_t)(8 * j) * out.ldr) : make_uint4(0, 0, 0, 0);
             }
 #pragma unroll
-            for (int j = 0; j < 8; j++)
-              if (r0 + 4 * j < rows) {
-                const uint4 mine = *reinterpret_cast<const uint4*>(at(r0 + 4 * j, piece));
+            for (int j = 0; j < 4; j++)
+              if (r0 + 8 * j < rows) {
+                const uint4 mine = *reinterpret_cast<const uint4*>(at(r0 + 8 * j, piece));
                 if (out.resid) {
                   float o[8], s[8];
                   load_vec(reinterpret_cast<const bf16*>(&mine), o);
                   load_vec(reinterpret_cast<const bf16*>(&v[j]), s);
 #pragma unroll
                   for (int e = 0; e < 8; e++) o[e] += s[e];
-                  store_vec(yc + (size_t)(4 * j) * out.ldy, o);
+                  store_vec(yc + (size_t)(8 * j) * out.ldy, o);
                 } else {
-                  *reinterpret_cast<uint4*>(yc + (size_t)(4 * j) * out.ldy) = mine;
+                  *reinterpret_cast<uint4*>(yc + (size_t)(8 * j) * out.ldy) = mine;
                 }
               }
-          } else {   // off the 16-byte grid, or the last columns: single values, 32 columns side by side
+          } else if (n + lane < N) {   // off the 16-byte grid, or the last columns: single values, side by side, 16 rows' residuals ahead of their use
 #pragma unroll 1
-            for (int e = lane; e < min(64, N - n); e += 32)
-#pragma unroll 4
-              for (int j = 0; j < rows; j++) {
-                float v = __bfloat162float(at(j, e >> 3)[e & 7]);
-                if (out.resid) v += __bfloat162float(out.resid[(size_t)(first + j) * out.ldr + n + e]);
-                out.y[(size_t)(first + j) * out.ldy + n + e] = __float2bfloat16_rn(v);
-              }
+            for (int j0 = 0; j0 < rows; j0 += 16) {
+              bf16* yc = out.y + (size_t)(first + j0) * out.ldy + n + lane;
+              float v[16];
+#pragma unroll
+              for (int j = 0; j < 16; j++)
+                v[j] = out.resid && j0 + j < rows ? __bfloat162float(out.resid[(size_t)(first + j0 + j) * out.ldr + n + lane]) : -0.f;   // (adds nothing to any value)
+#pragma unroll
+              for (int j = 0; j < 16; j++)
+                if (j0 + j < rows) yc[(size_t)j * out.ldy] = __float2bfloat16_rn(__bfloat162float(at(j0 + j, lane >> 3)[lane & 7]) + v[j]);
+            }
           }
           __syncwarp();   // the block has been read
         }
@@ -529,7 +451,9 @@ int encode(CUtensorMap* map, const MapKey& k) {
   }
   return r == CUDA_SUCCESS ? STU_OK : STU_ERR_UNSUPPORTED;
 }
-int map_of(CUtensorMap* map, const void* base, long long rows, long long cols, int box) {
+}  // namespace
+
+int fp8_tensor_map(CUtensorMap* map, const void* base, long long rows, long long cols, int box) {
   static thread_local MapSlot* table = nullptr;
   if (!table) table = new (std::nothrow) MapSlot[MAP_SLOTS]();
   const MapKey key{base, rows, cols, box};
@@ -547,6 +471,12 @@ int map_of(CUtensorMap* map, const void* base, long long rows, long long cols, i
   return STU_OK;
 }
 
+namespace {
+
+template <bool DUAL, int CTAS, int TN> cudaError_t allow_shared() {
+  static SmemLimit limit;
+  return allow_smem((const void*)fp8_gemm_kernel<DUAL, CTAS, TN>, Form<DUAL, CTAS, TN>::SMEM, limit);
+}
 // Pairs of CTAs that the current device runs at a time.
 template <bool DUAL, int CTAS, int TN> int device_clusters() {
   static std::atomic<int> found[STU_MAX_DEVICES] = {};
@@ -558,7 +488,7 @@ template <bool DUAL, int CTAS, int TN> int device_clusters() {
     cfg.gridDim = dim3(CTAS * device_sm_count());
     cfg.blockDim = dim3(64 + 32 * EPI_WARPS);
     cfg.dynamicSmemBytes = Form<DUAL, CTAS, TN>::SMEM;
-    if (cudaOccupancyMaxActiveClusters(&n, fp8_gemm_kernel<DUAL, CTAS, TN>, &cfg) != cudaSuccess || n < 1) {
+    if (allow_shared<DUAL, CTAS, TN>() != cudaSuccess || cudaOccupancyMaxActiveClusters(&n, fp8_gemm_kernel<DUAL, CTAS, TN>, &cfg) != cudaSuccess || n < 1) {
       (void)cudaGetLastError();
       n = device_sm_count() / CTAS;
     }
@@ -570,19 +500,18 @@ template <bool DUAL, int CTAS, int TN> int device_clusters() {
 template <bool DUAL, int CTAS, int TN>
 int launch(const Fp8Product& p, cudaStream_t st) {
   using F = Form<DUAL, CTAS, TN>;
-  static SmemLimit limit;
-  cudaError_t e = allow_smem((const void*)fp8_gemm_kernel<DUAL, CTAS, TN>, F::SMEM, limit);
+  cudaError_t e = allow_shared<DUAL, CTAS, TN>();
   if (e != cudaSuccess) return (int)e;
   const int b_box = DUAL ? TN : F::B_ROWS, s_box = DUAL ? -1 : -((TN + 127) / 128);
   CUtensorMap a, b, b2, sa, sb, sb2;
-  int rc = map_of(&a, p.x, p.M, p.K, BM);
-  if (!rc) rc = map_of(&b, p.w, p.N, p.K, b_box);
-  if (!rc) rc = map_of(&sa, p.xs, p.M, p.K, -1);
-  if (!rc) rc = map_of(&sb, p.ws, p.N, p.K, s_box);
+  int rc = fp8_tensor_map(&a, p.x, p.M, p.K, BM);
+  if (!rc) rc = fp8_tensor_map(&b, p.w, p.N, p.K, b_box);
+  if (!rc) rc = fp8_tensor_map(&sa, p.xs, p.M, p.K, -1);
+  if (!rc) rc = fp8_tensor_map(&sb, p.ws, p.N, p.K, s_box);
   b2 = b, sb2 = sb;
   if (DUAL) {
-    if (!rc) rc = map_of(&b2, p.w2, p.N, p.K, b_box);
-    if (!rc) rc = map_of(&sb2, p.w2s, p.N, p.K, s_box);
+    if (!rc) rc = fp8_tensor_map(&b2, p.w2, p.N, p.K, b_box);
+    if (!rc) rc = fp8_tensor_map(&sb2, p.w2s, p.N, p.K, s_box);
   }
   if (rc) return rc;
   const int tiles_m = (p.M + CTAS * BM - 1) / (CTAS * BM), tiles_n = (p.N + TN - 1) / TN, most = device_clusters<DUAL, CTAS, TN>();
@@ -600,7 +529,16 @@ int launch(const Fp8Product& p, cudaStream_t st) {
 }  // namespace
 
 int fp8_gemm(const Fp8Product& p, cudaStream_t st) {
-  if (p.w2) return p.M > BM ? launch<true, 2, 128>(p, st) : launch<true, 1, 128>(p, st);
-  if (p.M <= BM) return launch<false, 1, 128>(p, st);
-  return p.N > 128 ? launch<false, 2, 256>(p, st) : launch<false, 2, 128>(p, st);
+  const auto waves = [&](int rows, int cols, int room) {
+    return ((long long)((p.M + rows - 1) / rows) * ((p.N + cols - 1) / cols) + room - 1) / room;
+  };
+  // Gate/up: a CTA alone on 128 rows where that is fewer rounds than pairs on 256 (us, alone and in pairs: 333 x 6144 x 1536 11.6 and 16.4, 700 18.0 and
+  // 17.0, 1024 24.7 and 22.4, 16384 321 and 266).
+  if (p.w2)
+    return waves(128, 128, device_sm_count()) < waves(256, 128, device_clusters<true, 2, 128>()) || p.M <= BM ? launch<true, 1, 128>(p, st)
+                                                                                                              : launch<true, 2, 128>(p, st);
+  // Plain: tiles of 128 columns where a round of them, about 3/4 of the time of one of 256, makes up for their number (us, 128 and 256 columns:
+  // 1024 x 1536 x 18432 46.7 and 70.8, 1024 x 1536 x 6144 18.7 and 22.0, 2048 x 1536 x 6144 32.8 and 23.4, 8192 x 1536 x 18432 322 and 180).
+  return 3 * waves(256, 128, device_clusters<false, 2, 128>()) < 4 * waves(256, 256, device_clusters<false, 2, 256>()) ? launch<false, 2, 128>(p, st)
+                                                                                                                     : launch<false, 2, 256>(p, st);
 }

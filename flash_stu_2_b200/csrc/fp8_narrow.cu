@@ -1,0 +1,393 @@
+// Products of 8-bit rows (fp8.cuh) for few tokens: the weights are the 128-row operand of the tensor core, the tokens its columns, and K is cut over a
+// thread-block cluster so that a few thousand features occupy all SMs.  What bounds it: HBM, the weights once; for small weights the time
+// from a launch over the first bytes and the cluster's meeting to the last store.
+//
+// Warp 0 of a CTA brings 128 features (gate/up: 128 of both), NT tokens and their scales by TMA into a ring, warp 1 copies the scales into tensor memory
+// and issues kind::mxf8f6f4 (see fp8_gemm.cu), the others drain the sums into shared memory, where the ring was.  Then every CTA of the cluster takes
+// its share of the tokens: a warp adds up a token's 128 features over the cluster, in the order of K, and stores them; gate/up: one warp has the whole
+// block of h and settles its scale by a reduction.  (On mma.sync the conversions to halves and the fragments of tokens took 370 instructions for 2 KB of
+// weights, more than an SM issues in the time that they take to arrive: 18432 x 1536 gate/up of 8 tokens 25.5 us.)
+#include <cooperative_groups.h>
+
+#include "fp8_gemm.cuh"
+
+namespace cg = cooperative_groups;
+using namespace fp8;
+
+int device_sm_count();      // gemm_tc.cu
+int* device_status_word();  // gemm_tc.cu
+
+namespace {
+
+constexpr int MAX_STAGES = 12, MAX_KS = 8;
+
+template <bool DUAL, int NT> struct Narrow {
+  static constexpr int WS = DUAL ? 2 : 1;                           // matrices
+  static constexpr int DRAIN = NT >= 64 ? 8 : 4, THREADS = 64 + 32 * DRAIN;   // warps that read the sums
+  // k-blocks of a stage: waiting for one, announcing its bytes and sending off its copies takes the producer 360 cycles and 27 more per copy, whatever
+  // their size, so that single blocks of 16 KB came at 45 bytes a cycle at most (8 x 1536 x 18432 13.7 us, 66 with K whole)
+  static constexpr int KBS = DUAL ? (NT <= 32 ? 2 : 1) : NT <= 32 ? 4 : 2;
+  static constexpr int W_BYTES = WS * A_BYTES, X_BYTES = NT * BK, KB_BYTES = W_BYTES + X_BYTES;
+  static constexpr int SCALE_BYTES = PIECE * (WS + 1);
+  static constexpr int STAGE = KBS * KB_BYTES + SCALE_BYTES;        // (the scales of all stages lie behind the tiles)
+  static constexpr int ROWS = WS * 128;                             // sums of a token
+  static constexpr int SUM_BYTES = NT * ROWS * 4;
+  static constexpr int SF_COLS = 4 * (WS + 1), SCALES = WS * NT;    // tensor memory: sums, then twice the scales
+  static constexpr uint32_t TMEM_COLS = SCALES + 2 * SF_COLS <= 64 ? 64 : SCALES + 2 * SF_COLS <= 128 ? 128 : SCALES + 2 * SF_COLS <= 256 ? 256 : 512;
+};
+constexpr int TAIL = (2 * MAX_STAGES + 1) * 8 + 32;                 // barriers, tensor memory's address, marks
+template <bool DUAL, int NT> constexpr size_t smem_bytes(int stages) {
+  const size_t ring = (size_t)stages * Narrow<DUAL, NT>::STAGE;
+  return 1024 + (ring > (size_t)Narrow<DUAL, NT>::SUM_BYTES ? ring : (size_t)Narrow<DUAL, NT>::SUM_BYTES) + TAIL;
+}
+
+template <bool DUAL, int NT>
+__global__ void __launch_bounds__(Narrow<DUAL, NT>::THREADS, 1)
+    fp8_narrow_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmW2, const __grid_constant__ CUtensorMap tmX,
+                      const __grid_constant__ CUtensorMap tmSW, const __grid_constant__ CUtensorMap tmSW2, const __grid_constant__ CUtensorMap tmSX,
+                      const bf16* resid, long long ldr, bf16* y, long long ldy, unsigned char* hq, unsigned char* hs, int M, int N, int K, int stages,
+                      int overlap, int* status, int drop_first_copy, unsigned long long wait_ns) {
+  using C = Narrow<DUAL, NT>;
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  constexpr int TILES = C::KBS * C::KB_BYTES, KBS = C::KBS, THREADS = C::THREADS;
+  unsigned char* scales = smem + stages * TILES;
+  float* sums = reinterpret_cast<float*>(smem);   // [token][feature], gate/up: 128 gate, 128 up; once the ring is done with
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + max(stages * C::STAGE, C::SUM_BYTES));
+  uint64_t* empty_bar = full_bar + MAX_STAGES;
+  uint64_t* tmem_full = empty_bar + MAX_STAGES;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tmem_full + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  int* issued_ctr = reinterpret_cast<int*>(tmem_slot + 2);
+  int* consumed_ctr = issued_ctr + 1;
+
+  cg::cluster_group cluster = cg::this_cluster();
+  const int ks = cluster.num_blocks(), rank = cluster.block_rank();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int nb = blockIdx.x, t0 = blockIdx.z * NT, num_kb = blocks_of(K);
+  // this CTA's k-blocks, in stages that begin at multiples of KBS: none reaches over a group of four, whose scales are a piece
+  const int kb0 = (int)((long long)num_kb * rank / ks), kb_end = (int)((long long)num_kb * (rank + 1) / ks), st0 = kb0 / KBS;
+  const int nst = kb_end > kb0 ? (kb_end - 1) / KBS - st0 + 1 : 0;
+  const auto first_kb = [&](int g) { return max(kb0, (st0 + g) * KBS); };
+  const auto blocks_in = [&](int g) { return min(kb_end, (st0 + g + 1) * KBS) - first_kb(g); };
+  const auto with_scales = [&](int g) { return g == 0 || (first_kb(g) & 3) == 0; };
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < stages; s++) {
+      tma::mbar_init(&full_bar[s], 1);
+      tma::mbar_init(&empty_bar[s], 1);
+    }
+    tma::mbar_init(tmem_full, 1);
+    *abort_flag = 0;
+    *issued_ctr = *consumed_ctr = 0;
+    tma::fence_barrier_init();
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tma::smem_u32(tmem_slot)), "r"(C::TMEM_COLS));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem_base = *tmem_slot;
+  // (when the next kernel may start: epilogue.cuh, PdlTrigger)
+  if (overlap && !DUAL) pdl_trigger();
+
+  if (warp == 0) {
+    // ---------------- TMA producer
+    const bool leader = elect_one();
+    const auto load_w = [&](int g, int s) {
+      const int kb = first_kb(g), n = blocks_in(g);
+      unsigned char *tile = smem + s * TILES, *sc = scales + s * C::SCALE_BYTES;
+#pragma unroll
+      for (int j = 0; j < KBS; j++)
+        if (j < n) {
+          load_2d(tile + j * C::KB_BYTES, &tmW, &full_bar[s], (kb + j) * BK, nb * 128);
+          if (DUAL) load_2d(tile + j * C::KB_BYTES + A_BYTES, &tmW2, &full_bar[s], (kb + j) * BK, nb * 128);
+        }
+      if (with_scales(g)) {
+        tma::load_3d(sc, &tmSW, &full_bar[s], 0, kb >> 2, nb);
+        if (DUAL) tma::load_3d(sc + PIECE, &tmSW2, &full_bar[s], 0, kb >> 2, nb);
+      }
+    };
+    const auto load_x = [&](int g, int s) {
+      const int kb = first_kb(g), n = blocks_in(g);
+#pragma unroll
+      for (int j = 0; j < KBS; j++)
+        if (j < n) load_2d(smem + s * TILES + j * C::KB_BYTES + C::W_BYTES, &tmX, &full_bar[s], (kb + j) * BK, t0);
+      if (with_scales(g)) tma::load_3d(scales + s * C::SCALE_BYTES + C::WS * PIECE, &tmSX, &full_bar[s], 0, kb >> 2, t0 / 128);
+    };
+    const auto expect = [&](int g, int s) { tma::mbar_expect_tx(&full_bar[s], blocks_in(g) * C::KB_BYTES + (with_scales(g) ? C::SCALE_BYTES : 0)); };
+    // the first round's weights, ahead of the wait where that is allowed
+    const int pre = min(stages, nst);
+    if (!overlap) pdl_wait();
+    const int first = drop_first_copy ? 1 : 0;   // (failure-detection test: the first stage never fills)
+    if (leader) {
+      for (int g = 0; g < pre; g++) {
+        expect(g, g);
+        if (g >= first) load_w(g, g);
+      }
+    }
+    __syncwarp();
+    if (overlap) pdl_wait();
+    if (!overlap || DUAL) pdl_trigger();
+    if (leader)
+      for (int g = first; g < pre; g++) load_x(g, g);
+    __syncwarp();
+    int g = pre, s = pre == stages ? 0 : pre;
+    uint32_t ph = 0;   // of the stage's first release
+    for (; g < nst; g++) {
+      if (!tma::warp_wait_bounded(&empty_bar[s], ph, abort_flag, wait_ns)) break;
+      if (leader) {
+        expect(g, s);
+        load_w(g, s);
+        load_x(g, s);
+      }
+      if (++s == stages) s = 0, ph ^= 1u;
+    }
+    if (leader) *issued_ctr = g;
+  } else if (warp == 1) {
+    // ---------------- issuer
+    const bool leader = elect_one();
+    const uint64_t dw0 = operand_desc(tma::smem_u32(smem)), dx0 = operand_desc(tma::smem_u32(smem) + C::W_BYTES), ds0 = scales_desc(tma::smem_u32(scales));
+    int g = 0, s = 0, pieces = 0;
+    uint32_t ph = 0, sf = tmem_base + C::SCALES;
+    for (; g < nst; g++) {
+      if (!tma::warp_wait_bounded(&full_bar[s], ph, abort_flag, wait_ns)) break;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const int kb = first_kb(g), n = blocks_in(g);
+      const bool copy = with_scales(g);
+      if (copy) sf = tmem_base + C::SCALES + C::SF_COLS * (pieces++ & 1);
+      if (leader) {
+        if (copy) {   // in order with the instructions around it
+#pragma unroll
+          for (int i = 0; i <= C::WS; i++) copy_scales<1>(sf + 4 * i, ds0 + (uint64_t)((s * C::SCALE_BYTES + i * PIECE) >> 4));
+        }
+        const uint64_t dw = dw0 + (uint64_t)(s * (TILES >> 4)), dx = dx0 + (uint64_t)(s * (TILES >> 4));
+#pragma unroll
+        for (int j = 0; j < KBS; j++)
+          if (j < n) {
+#pragma unroll
+            for (int kk = 0; kk < BK / 32; kk++)
+#pragma unroll
+              for (int i = 0; i < C::WS; i++)
+                multiply<1, NT>(tmem_base + i * NT, dw + ((j * C::KB_BYTES + i * A_BYTES) >> 4) + 2 * kk, dx + ((j * C::KB_BYTES) >> 4) + 2 * kk, sf + 4 * i,
+                                sf + 4 * C::WS, (kb + j) & 3, (g | j | kk) ? 1u : 0u);
+          }
+        if (g + stages < nst) commit<1>(&empty_bar[s]);   // (nobody waits for the last round's)
+        if (g + 1 == nst) commit<1>(tmem_full);
+      }
+      __syncwarp();
+      if (++s == stages) s = 0, ph ^= 1u;
+    }
+    if (leader) *consumed_ctr = g;
+  } else {
+    // ---------------- drain: TMEM lane quarter = warp % 4, a feature per thread
+    const int quarter = warp & 3, half = (warp - 2) >> 2;   // (eight warps: either half of the tokens)
+    const bool ok = nst > 0 && tma::warp_wait_bounded(tmem_full, 0, abort_flag, wait_ns);
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll 1
+    for (int i = 0; i < C::WS; i++)
+#pragma unroll 1
+      for (int c0 = half * (NT / 2); c0 < (C::DRAIN == 8 ? (half + 1) * (NT / 2) : NT); c0 += 32) {
+        uint32_t r[32];
+#pragma unroll
+        for (int c = 0; c < 32; c++) r[c] = 0u;
+        if (ok) {   // (16 tokens: the columns behind them are other sums or scales, unread)
+          tmem_ld32(tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(i * NT + c0), r);
+          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+        }
+#pragma unroll
+        for (int c = 0; c < (NT < 32 ? NT : 32); c++) sums[(c0 + c) * C::ROWS + i * 128 + quarter * 32 + lane] = __uint_as_float(r[c]);
+      }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  }
+  __syncwarp();
+  __syncthreads();
+  cluster.sync();
+  // ---------------- the cluster's sums: a warp per token, four features per lane
+  pdl_wait();   // (returns at once: the producer has waited; the residual rows are read behind it)
+  const int last = min(NT, M - t0), hblocks = blocks_of(N), hgroups = groups_of(N);
+  for (int t = rank + ks * warp; t < last; t += ks * (THREADS / 32)) {
+    float v[C::WS][4];
+#pragma unroll
+    for (int i = 0; i < C::WS; i++)
+#pragma unroll
+      for (int j = 0; j < 4; j++) v[i][j] = 0.f;
+#pragma unroll 4
+    for (int r = 0; r < ks; r++) {
+      const float* from = cluster.map_shared_rank(sums, r) + t * C::ROWS + 4 * lane;
+#pragma unroll
+      for (int i = 0; i < C::WS; i++) {
+        const float4 a = *reinterpret_cast<const float4*>(from + i * 128);
+        v[i][0] += a.x, v[i][1] += a.y, v[i][2] += a.z, v[i][3] += a.w;
+      }
+    }
+    const int m = t0 + t, n = nb * 128 + 4 * lane;
+    if constexpr (DUAL) {
+      float h[4];
+      uint32_t a = 0;
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        h[j] = nan_unless_finite(n + j < N ? gelu(v[0][j]) * v[1][j] : 0.f);
+        a = max(a, h[j] == h[j] ? magnitude(h[j]) : 0u);
+      }
+      a = __reduce_max_sync(0xffffffffu, a);
+      const uint32_t b = scale_byte(a);
+      const float inv = inverse_scale(b);
+      *reinterpret_cast<uint32_t*>(hq + (size_t)m * hblocks * BLOCK + n) = pack4(h[0] * inv, h[1] * inv, h[2] * inv, h[3] * inv);
+      if (lane == 0) hs[scale_word(m, nb >> 2, hgroups) + (nb & 3)] = (unsigned char)b;
+    } else {
+      const size_t ry = (size_t)m * ldy + n, rr = (size_t)m * ldr + n;
+#pragma unroll
+      for (int j = 0; j < 4; j++) v[0][j] = round_to<bf16>(v[0][j]);
+      if (n + 4 <= N && !(reinterpret_cast<uintptr_t>(y + ry) & 7) && !(resid && (reinterpret_cast<uintptr_t>(resid + rr) & 7))) {
+        if (resid) {
+          const uint2 s = *reinterpret_cast<const uint2*>(resid + rr);
+          v[0][0] += __uint_as_float(s.x << 16), v[0][1] += __uint_as_float(s.x & 0xffff0000u);
+          v[0][2] += __uint_as_float(s.y << 16), v[0][3] += __uint_as_float(s.y & 0xffff0000u);
+        }
+        const __nv_bfloat162 p0 = __floats2bfloat162_rn(v[0][0], v[0][1]), p1 = __floats2bfloat162_rn(v[0][2], v[0][3]);
+        *reinterpret_cast<uint2*>(y + ry) = make_uint2(*reinterpret_cast<const uint32_t*>(&p0), *reinterpret_cast<const uint32_t*>(&p1));
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+          if (n + j < N) y[ry + j] = __float2bfloat16_rn(resid ? __bfloat162float(resid[rr + j]) + v[0][j] : v[0][j]);
+      }
+    }
+  }
+  if (DUAL && rank == 0) {   // byte 0 for the rows that fill up the last 128 and for the blocks that fill up the last four
+    const int end = nb == hblocks - 1 ? hgroups * 4 : nb + 1, bottom = min(t0 + NT, M) == M ? (M + 127) & ~127 : t0 + NT;
+    for (int m = t0 + threadIdx.x; m < bottom; m += THREADS)
+      for (int kb = m < M ? nb + 1 : nb; kb < end; kb++) hs[scale_word(m, kb >> 2, hgroups) + (kb & 3)] = 0;
+  }
+  cluster.sync();   // the others have read this CTA's sums
+  if (*abort_flag) {
+    // A wait ran out: report it, and let copies that were issued but never consumed land (bounded) before shared memory is released.
+    if (threadIdx.x == 0) {
+      if (status) atomicExch(status, 3);
+      const uint64_t start = tma::global_ns();
+      for (int g = *consumed_ctr; g < *issued_ctr; g++) {
+        for (uint32_t w = 0; w < WAIT_LIMIT; ++w) {
+          if (tma::mbar_try_wait(&full_bar[g % stages], (uint32_t)(g / stages) & 1u)) break;
+          if ((w & 255u) == 255u && tma::global_ns() - start > wait_ns) break;
+        }
+      }
+    }
+    __syncthreads();
+  }
+  if (warp == 1) {
+    __syncwarp();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(C::TMEM_COLS));
+  }
+}
+
+template <bool DUAL, int NT>
+cudaError_t configure(cudaLaunchConfig_t& cfg, cudaLaunchAttribute* at, dim3 grid, size_t smem) {
+  cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(Narrow<DUAL, NT>::THREADS);
+  cfg.dynamicSmemBytes = smem;
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = at[0].val.clusterDim.z = 1;
+  at[0].val.clusterDim.y = grid.y;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  static SmemLimit limit;
+  return allow_smem((const void*)fp8_narrow_kernel<DUAL, NT>, smem, limit);
+}
+template <bool DUAL, int NT> constexpr int deepest() {
+  int stages = MAX_STAGES;
+  while (stages > 2 && smem_bytes<DUAL, NT>(stages) > 227 * 1024) stages--;
+  return stages;
+}
+
+// Clusters of ks CTAs with the deepest ring that the current device runs at a time (a cluster lies in one of its groups of SMs).
+template <bool DUAL, int NT> int cluster_room(int ks) {
+  static std::atomic<int> found[STU_MAX_DEVICES][MAX_KS + 1] = {};
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= STU_MAX_DEVICES) return 0;
+  if ((n = found[dev][ks].load(std::memory_order_relaxed)) != 0) return n;
+  cudaLaunchConfig_t cfg;
+  cudaLaunchAttribute at[1];
+  if (configure<DUAL, NT>(cfg, at, dim3(1024, ks), smem_bytes<DUAL, NT>(deepest<DUAL, NT>())) != cudaSuccess ||
+      cudaOccupancyMaxActiveClusters(&n, fp8_narrow_kernel<DUAL, NT>, &cfg) != cudaSuccess || n < 1) {
+    (void)cudaGetLastError();
+    n = ks == 1 ? device_sm_count() : -1;   // (none: K is not cut that way)
+  }
+  found[dev][ks].store(n, std::memory_order_relaxed);
+  return n;
+}
+// CTAs that share a tile's K: the most whose clusters run at a time.  us, ks = 1 / 2 / 4 / 8: gate/up of 1 token, 4096 x 1024 (32 tiles) 6.6 / 5.7 / 5.8 /
+// 14.9 (two rounds), 6144 x 1536 (48) 8.3 / 8.0 / 11.7 / 21.8, 18432 x 1536 (144) 13.0 / 17.7; 1536 x 18432 (12) 23.7 / 14.2 / 9.9 / 8.8; 333 tokens,
+// 1536 x 6144 (36) 20.7 / 14.1 / 17.9 / 25.0.
+template <bool DUAL, int NT> int cluster_size(const Fp8Product& p) {
+  const long long tiles = (long long)blocks_of(p.N) * ((p.M + NT - 1) / NT);
+  const int num_kb = blocks_of(p.K);
+  for (int ks = num_kb < MAX_KS ? num_kb : MAX_KS; ks > 1; ks--)
+    if (tiles * ks <= device_sm_count() && tiles <= cluster_room<DUAL, NT>(ks)) return ks;
+  return 1;
+}
+
+template <bool DUAL, int NT>
+int launch(const Fp8Product& p, cudaStream_t st) {
+  using C = Narrow<DUAL, NT>;
+  const int tiles_m = (p.M + NT - 1) / NT, blocks = blocks_of(p.N), num_kb = blocks_of(p.K), ks = cluster_size<DUAL, NT>(p);
+  if (tiles_m > 65535) return STU_ERR_SHAPE;
+  // one deep ring per SM, or two CTAs per SM where there are that many
+  constexpr size_t two = 233472 / 2 - 1024;
+  int stages = deepest<DUAL, NT>();
+  if ((long long)blocks * ks * tiles_m > device_sm_count() && smem_bytes<DUAL, NT>(2) <= two)
+    while (stages > 2 && smem_bytes<DUAL, NT>(stages) > two) stages--;
+  const int most = ((num_kb + ks - 1) / ks + C::KBS - 1) / C::KBS + 1;   // (a range may begin inside a stage)
+  if (stages > most) stages = most;
+  CUtensorMap w, w2, x, sw, sw2, sx;
+  int rc = fp8_tensor_map(&w, p.w, p.N, p.K, 128);
+  if (!rc) rc = fp8_tensor_map(&x, p.x, p.M, p.K, NT);
+  if (!rc) rc = fp8_tensor_map(&sw, p.ws, p.N, p.K, -1);
+  if (!rc) rc = fp8_tensor_map(&sx, p.xs, p.M, p.K, -1);
+  w2 = w, sw2 = sw;
+  if (DUAL) {
+    if (!rc) rc = fp8_tensor_map(&w2, p.w2, p.N, p.K, 128);
+    if (!rc) rc = fp8_tensor_map(&sw2, p.w2s, p.N, p.K, -1);
+  }
+  if (rc) return rc;
+  cudaLaunchConfig_t cfg;
+  cudaLaunchAttribute at[2];
+  cudaError_t e = configure<DUAL, NT>(cfg, at, dim3(blocks, ks, tiles_m), smem_bytes<DUAL, NT>(stages));
+  if (e != cudaSuccess) return (int)e;
+  cfg.stream = st;
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  e = cudaLaunchKernelEx(&cfg, fp8_narrow_kernel<DUAL, NT>, w, w2, x, sw, sw2, sx, p.resid, p.ldr, p.y, p.ldy, p.hq, p.hs, p.M, p.N, p.K, stages, p.overlap,
+                         device_status_word(), (int)take_dropped_stage(), wait_bound_ns());
+  if (e != cudaSuccess) return (int)e;
+  STU_CHECK_LAUNCH();
+  return STU_OK;
+}
+
+template <bool DUAL>
+int launch_tokens(const Fp8Product& p, cudaStream_t st) {
+  if (p.M <= 16) return launch<DUAL, 16>(p, st);
+  if (p.M <= 32) return launch<DUAL, 32>(p, st);
+  if (p.M <= 64) return launch<DUAL, 64>(p, st);
+  return launch<DUAL, 128>(p, st);
+}
+
+}  // namespace
+
+// Whether a product takes less time here than on the tiles of fp8_gemm.cu.  Plain: up to 128 tokens always (1536 x 6144, 128 tokens 9.2 and 17.9 us, 64 tokens
+// 7.5 and 16.5), more while K can still be cut (1536 x 6144, 333 tokens 14.1 and 24.9 us, 700 15.5 and 18.0; 1024 x 4096, 512 tokens 9.8 and 13.6).  Gate/up, whose sums
+// are twice as many to bring together: up to 32 tokens (18432 x 1536, 32 tokens 15.8 and 14.6 us, 16 tokens 14.2 and 14.7; 6144 x 1536, 32 tokens 9.8 and 10.4), more
+// where four or more CTAs share K and there is enough of it (64 tokens: 4096 x 1024 8.1 and 8.6, 6144 x 1536, two CTAs, 11.2 and 10.7; 128 tokens:
+// 4096 x 1024, four, 10.9 and 8.9).
+bool fp8_narrow_takes(const Fp8Product& p) {
+  if (!p.w2) return p.M <= 128 || cluster_size<false, 128>(p) > 1;
+  if (p.M <= 32) return true;
+  if (p.M <= 64) return cluster_size<true, 64>(p) >= 4;
+  return blocks_of(p.K) >= 16 && cluster_size<true, 128>(p) >= 4;
+}
+
+int fp8_narrow(const Fp8Product& p, cudaStream_t st) { return p.w2 ? launch_tokens<true>(p, st) : launch_tokens<false>(p, st); }
