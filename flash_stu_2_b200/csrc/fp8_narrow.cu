@@ -4,7 +4,8 @@
 //
 // Warp 0 of a CTA brings 128 features (gate/up: 128 of both), NT tokens and their scales by TMA into a ring, warp 1 copies the scales into tensor memory
 // and issues kind::mxf8f6f4 (see fp8_gemm.cu), the others drain the sums into shared memory, where the ring was.  Then every CTA of the cluster takes
-// its share of the tokens: a warp adds up a token's 128 features over the cluster, in the order of K, and stores them; gate/up: one warp has the whole
+// its share of the tokens: a warp adds up a token's 128 features over the cluster, in the order of K, and stores them (sums sent to the CTA that adds them up by
+// bulk copies, with no barrier of the cluster ahead of or behind them, came later: 1 x 1024 x 4096 5.2 us, so 4.7); gate/up: one warp has the whole
 // block of h and settles its scale by a reduction.  (On mma.sync the conversions to halves and the fragments of tokens took 370 instructions for 2 KB of
 // weights, more than an SM issues in the time that they take to arrive: 18432 x 1536 gate/up of 8 tokens 25.5 us.)
 #include <cooperative_groups.h>
@@ -64,7 +65,7 @@ __global__ void __launch_bounds__(Narrow<DUAL, NT>::THREADS, 1)
   cg::cluster_group cluster = cg::this_cluster();
   const int ks = cluster.num_blocks(), rank = cluster.block_rank();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int nb = blockIdx.x, t0 = blockIdx.z * NT, num_kb = blocks_of(K);
+  const int nb = blockIdx.x, t0 = blockIdx.z * NT, num_kb = blocks_of(K), last = min(NT, M - t0);   // tokens of this tile
   // this CTA's k-blocks, in stages that begin at multiples of KBS: none reaches over a group of four, whose scales are a piece
   const int kb0 = (int)((long long)num_kb * rank / ks), kb_end = (int)((long long)num_kb * (rank + 1) / ks), st0 = kb0 / KBS;
   const int nst = kb_end > kb0 ? (kb_end - 1) / KBS - st0 + 1 : 0;
@@ -189,7 +190,7 @@ __global__ void __launch_bounds__(Narrow<DUAL, NT>::THREADS, 1)
 #pragma unroll 1
     for (int i = 0; i < C::WS; i++)
 #pragma unroll 1
-      for (int c0 = half * (NT / 2); c0 < (C::DRAIN == 8 ? (half + 1) * (NT / 2) : NT); c0 += 32) {
+      for (int c0 = half * (NT / 2); c0 < min(last, C::DRAIN == 8 ? (half + 1) * (NT / 2) : NT); c0 += 32) {
         uint32_t r[32];
 #pragma unroll
         for (int c = 0; c < 32; c++) r[c] = 0u;
@@ -198,16 +199,17 @@ __global__ void __launch_bounds__(Narrow<DUAL, NT>::THREADS, 1)
           asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
         }
 #pragma unroll
-        for (int c = 0; c < (NT < 32 ? NT : 32); c++) sums[(c0 + c) * C::ROWS + i * 128 + quarter * 32 + lane] = __uint_as_float(r[c]);
+        for (int c = 0; c < (NT < 32 ? NT : 32); c++)
+          if (c0 + c < last) sums[(c0 + c) * C::ROWS + i * 128 + quarter * 32 + lane] = __uint_as_float(r[c]);
       }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   }
   __syncwarp();
   __syncthreads();
-  cluster.sync();
+  if (ks > 1) cluster.sync();
   // ---------------- the cluster's sums: a warp per token, four features per lane
   pdl_wait();   // (returns at once: the producer has waited; the residual rows are read behind it)
-  const int last = min(NT, M - t0), hblocks = blocks_of(N), hgroups = groups_of(N);
+  const int hblocks = blocks_of(N), hgroups = groups_of(N);
   for (int t = rank + ks * warp; t < last; t += ks * (THREADS / 32)) {
     float v[C::WS][4];
 #pragma unroll
@@ -261,7 +263,8 @@ __global__ void __launch_bounds__(Narrow<DUAL, NT>::THREADS, 1)
     for (int m = t0 + threadIdx.x; m < bottom; m += THREADS)
       for (int kb = m < M ? nb + 1 : nb; kb < end; kb++) hs[scale_word(m, kb >> 2, hgroups) + (kb & 3)] = 0;
   }
-  cluster.sync();   // the others have read this CTA's sums
+  if (ks > 1) cluster.sync();   // the others have read this CTA's sums
+  else __syncthreads();
   if (*abort_flag) {
     // A wait ran out: report it, and let copies that were issued but never consumed land (bounded) before shared memory is released.
     if (threadIdx.x == 0) {
