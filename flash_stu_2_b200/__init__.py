@@ -6,12 +6,12 @@ Drop-in for the public names of the reference packages `flash_stu` and `mini_stu
 from .config import FlashSTUConfig
 from .filters import (get_hankel, get_spectral_filters, load_spectral_filters, nearest_power_of_two,
                       save_spectral_filters)
-from .modules import MLP, STU, Attention, RMSNorm
+from .modules import MLP, STU, Attention, Fp8MLP, RMSNorm
 from .layers import AttentionLayer, STULayer
 from .block import FlashSTUBlock
 from .model import FlashSTU
 from .mini_stu import MiniSTU
 
-__all__ = ["FlashSTU", "MiniSTU", "FlashSTUConfig", "FlashSTUBlock", "STU", "Attention", "MLP", "RMSNorm", "STULayer",
+__all__ = ["FlashSTU", "MiniSTU", "FlashSTUConfig", "FlashSTUBlock", "STU", "Attention", "MLP", "Fp8MLP", "RMSNorm", "STULayer",
            "AttentionLayer", "get_spectral_filters", "get_hankel", "save_spectral_filters", "load_spectral_filters",
            "nearest_power_of_two"]

@@ -47,7 +47,7 @@ class FlashSTUBlock(nn.Module):
                 mlp_scale=mlp_scale, dropout=dropout, bias=bias, torch_dtype=torch_dtype, use_attn=use_attention,
                 use_approx=kwargs.get("use_approx", True), use_hankel_L=kwargs.get("use_hankel_L", False),
                 softcap=50.0, n_layers=1, bsz=1, vocab_size=1, stu_enable_mlp_sandwich=stu_enable_mlp_sandwich,
-                stu_mlp_hidden_size=stu_mlp_hidden_size,
+                stu_mlp_hidden_size=stu_mlp_hidden_size, mlp_fp8=kwargs.get("mlp_fp8", False),
             )
             for key, value in (attention_config or {}).items():
                 if key in fields:

@@ -13,6 +13,10 @@ class FlashSTUConfig(PretrainedConfig):
     path has no CUDA kernel here (use_flash_fft is ignored: there is a single convolution path;
     tiling and bias terms raise at module construction) are kept so that
     existing configs load.
+
+    Beyond the reference's: cache_len caps the positions that caches are laid out for; mlp_fp8 runs the layers' MLPs in 8 bits (e4m3
+    weights and activations with a power-of-two scale for each 128 of a row, bfloat16 models): checkpoints are the same, the 8-bit
+    weights are made from them at the first call.
     """
     model_type = "FlashSTU"
 
@@ -44,6 +48,7 @@ class FlashSTUConfig(PretrainedConfig):
         d_in_tile: Optional[int] = None,
         d_out_tile: Optional[int] = None,
         cache_len: Optional[int] = None,
+        mlp_fp8: bool = False,
         **kwargs,
     ):
         # transformers >= 5 serialises a model's dtype under the key `dtype` (and drops `torch_dtype` from the dict it
@@ -61,7 +66,7 @@ class FlashSTUConfig(PretrainedConfig):
             use_hankel_L=use_hankel_L, use_flash_fft=use_flash_fft, use_approx=use_approx, use_attn=use_attn,
             use_cache=use_cache, use_gradient_checkpointing=use_gradient_checkpointing, softcap=softcap,
             stu_enable_mlp_sandwich=stu_enable_mlp_sandwich, stu_mlp_hidden_size=stu_mlp_hidden_size,
-            filter_path=filter_path, d_in_tile=d_in_tile, d_out_tile=d_out_tile, cache_len=cache_len,
+            filter_path=filter_path, d_in_tile=d_in_tile, d_out_tile=d_out_tile, cache_len=cache_len, mlp_fp8=mlp_fp8,
         ).items():
             setattr(self, name, value)
         self.hidden_size = n_embd

@@ -4,7 +4,7 @@ import torch
 import torch.nn as nn
 
 from . import ops
-from .modules import MLP, STU, Attention, RMSNorm, child, host_pos, own, param, uniform_pos
+from .modules import MLP, STU, Attention, RMSNorm, child, host_pos, make_mlp, own, param, uniform_pos
 
 
 def _inplace_target(x: torch.Tensor):
@@ -17,6 +17,14 @@ def _own_step(stu, mlp) -> bool:
     if type(stu) is STU and type(mlp) is MLP:
         return "decode_step" not in stu.__dict__ and "apply_residual" not in mlp.__dict__
     return own(stu, STU, "decode_step") and own(mlp, MLP, "apply_residual")
+
+
+def _mlp_step(mlp, x2, out2, norm, overlap: bool, fuse: bool):
+    """out2 = x2 + mlp(norm(x2)), the norm inside the MLP's kernels (`fuse`, or where its result is the MLP's own) or in front of them."""
+    if fuse or getattr(mlp, "fp8", False):
+        mlp.apply_residual(x2, x2, out2, norm_w=param(norm, "weight"), eps=norm.eps, overlap=overlap)
+    else:
+        mlp.apply_residual(ops.rmsnorm(x2, param(norm, "weight"), norm.eps), x2, out2, overlap=overlap)
 
 
 class STULayer(nn.Module):
@@ -41,7 +49,7 @@ class STULayer(nn.Module):
         else:
             self.stu = STU(config, phi, n)
         self.mlp_norm = RMSNorm(config.n_embd, dtype=config.torch_dtype)
-        self.mlp = MLP(config, dtype=config.torch_dtype)
+        self.mlp = make_mlp(config, dtype=config.torch_dtype)
         self._scratch = {}
 
     def _fused_decode(self, x2, entry):
@@ -109,7 +117,7 @@ class STULayer(nn.Module):
         B, _, d = x.shape
         # the kernel passes the MLP weights through 32 KB shared-memory slots: 16 rows of d and 8 rows of I values
         stu, mlp = child(self, "stu"), child(self, "mlp")
-        return (ops.fused_step and stu.use_approx and not stu.use_hankel_L and x.dtype == torch.bfloat16 and B <= 8 and d % 8 == 0
+        return (ops.fused_step and not getattr(mlp, "fp8", False) and stu.use_approx and not stu.use_hankel_L and x.dtype == torch.bfloat16 and B <= 8 and d % 8 == 0
                 and d <= 1024 and mlp.intermediate_size <= 4096
                 and mlp.intermediate_size % 8 == 0 and STU.pipelined_decode and STU.tensor_core_decode
                 and STU.shared_tap_decode and uniform_pos(entry[1]))
@@ -141,10 +149,7 @@ class STULayer(nn.Module):
             entry = stu.decode_step(x2, param(stu_norm, "weight"), stu_norm.eps, entry, mid)
         else:
             entry = stu.full_decode_step(x2, x2, mid, entry, param(stu_norm, "weight"), stu_norm.eps)
-        if ops.can_fuse_norm(B, mlp.intermediate_size, d, ops.EPI_GELU_MUL, x.dtype):
-            mlp.apply_residual(mid, mid, x2, norm_w=param(mlp_norm, "weight"), eps=mlp_norm.eps, overlap=True)
-        else:
-            mlp.apply_residual(ops.rmsnorm(mid, param(mlp_norm, "weight"), mlp_norm.eps), mid, x2, overlap=True)
+        _mlp_step(mlp, mid, x2, mlp_norm, True, ops.can_fuse_norm(B, mlp.intermediate_size, d, ops.EPI_GELU_MUL, x.dtype))
         return entry
 
     def forward(self, x: torch.Tensor, past_key_value=None, use_cache=False):
@@ -153,7 +158,7 @@ class STULayer(nn.Module):
         if self.stu_mlp_enabled:
             entry = self._sandwich(xc, past_key_value, use_cache)
             x2 = xc.view(B * T, d)
-            self.mlp.apply_residual(ops.rmsnorm(x2, self.mlp_norm.weight, self.mlp_norm.eps), x2, x2)
+            _mlp_step(self.mlp, x2, x2, self.mlp_norm, False, False)
         elif T == 1 and past_key_value is not None:
             entry = self._decode(xc, past_key_value)
         else:
@@ -167,8 +172,7 @@ class STULayer(nn.Module):
                 entry = stu.add_to_residual(xn, xc, entry, use_cache)
             if done != 3:
                 x2 = xc.view(B * T, d)
-                xn2 = ops.rmsnorm(x2, param(mlp_norm, "weight"), mlp_norm.eps)
-                mlp.apply_residual(xn2, x2, x2)
+                _mlp_step(mlp, x2, x2, mlp_norm, False, False)
         if xc is not x:
             x.copy_(xc)
         if use_cache:
@@ -183,7 +187,7 @@ class AttentionLayer(nn.Module):
         self.attn_norm = RMSNorm(config.n_embd, dtype=config.torch_dtype)
         self.attn = Attention(config)
         self.mlp_norm = RMSNorm(config.n_embd, dtype=config.torch_dtype)
-        self.mlp = MLP(config, dtype=config.torch_dtype)
+        self.mlp = make_mlp(config, dtype=config.torch_dtype)
 
     def forward(self, x: torch.Tensor, past_key_value=None, use_cache=True):
         xc = _inplace_target(x)
@@ -197,11 +201,13 @@ class AttentionLayer(nn.Module):
             xn = ops.rmsnorm(xc, param(attn_norm, "weight"), attn_norm.eps)
             y, entry = attn.attend(xn, past_key_value, use_cache)
         ov = ops.FLAG_OVERLAP if (T == 1 and ops.overlap_decode) else 0   # token step: weights fetched early
-        ops.linear(y.view(B * T, d), param(child(attn, "c_proj"), "weight"), resid=x2, out=x2, epilogue=ops.EPI_RESID | ov)
-        if T == 1 and ops.can_fuse_norm(B, mlp.intermediate_size, d, ops.EPI_GELU_MUL, x.dtype):
-            mlp.apply_residual(x2, x2, x2, norm_w=param(mlp_norm, "weight"), eps=mlp_norm.eps, overlap=True)
+        c_proj = param(child(attn, "c_proj"), "weight")
+        if getattr(mlp, "fp8", False):   # the branch joins the stream in the norm
+            branch = ops.linear(y.view(B * T, d), c_proj, epilogue=ops.EPI_STORE | ov)
+            mlp.apply_residual(x2, x2, x2, norm_w=param(mlp_norm, "weight"), eps=mlp_norm.eps, overlap=(T == 1), add=branch)
         else:
-            mlp.apply_residual(ops.rmsnorm(x2, param(mlp_norm, "weight"), mlp_norm.eps), x2, x2, overlap=(T == 1))
+            ops.linear(y.view(B * T, d), c_proj, resid=x2, out=x2, epilogue=ops.EPI_RESID | ov)
+            _mlp_step(mlp, x2, x2, mlp_norm, T == 1, T == 1 and ops.can_fuse_norm(B, mlp.intermediate_size, d, ops.EPI_GELU_MUL, x.dtype))
         if xc is not x:
             x.copy_(xc)
         if use_cache:

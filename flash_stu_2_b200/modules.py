@@ -107,6 +107,7 @@ class RMSNorm(nn.Module):
 
 class MLP(nn.Module):
     """Gated tanh-GELU MLP, down(gelu_tanh(gate(x)) * up(x)) (flash_stu/modules/swiglu.py:4-29)."""
+    fp8 = False   # whether the norm in front is the MLP's own (Fp8MLP: its result is in 8 bits), whatever the size
 
     def __init__(self, config, dtype=None):
         super().__init__()
@@ -137,6 +138,44 @@ class MLP(nn.Module):
         x2 = x.reshape(-1, x.shape[-1])
         h = ops.linear(x2, self.gate_proj.weight, W2=self.up_proj.weight, epilogue=ops.EPI_GELU_MUL)
         return ops.linear(h, self.down_proj.weight).reshape(x.shape)
+
+
+class Fp8MLP(MLP):
+    """The MLP in 8 bits (config.mlp_fp8): its input's norm, both products and what lies between them on e4m3 rows with a scale for each 128
+    of a row (ops.Fp8Rows).  The parameters are MLP's; their 8-bit rows are derived, kept per parameter version."""
+    fp8 = True
+
+    def __init__(self, config, dtype=None):
+        super().__init__(config, dtype=dtype)
+        if self.gate_proj.weight.dtype != torch.bfloat16:
+            raise NotImplementedError("mlp_fp8=True has kernels for bfloat16 models only")
+        self._rows, self._rows_key = None, None
+
+    def rows(self):
+        """gate, up and down as 8-bit rows."""
+        weights = [param(child(self, name), "weight") for name in ("gate_proj", "up_proj", "down_proj")]
+        key = tuple((w._version, w.data_ptr(), w.device) for w in weights)
+        if self._rows_key != key:
+            with torch.no_grad(), ops.no_arena():
+                self._rows, self._rows_key = tuple(ops.quantize_fp8(w.detach()) for w in weights), key
+        return self._rows
+
+    def apply_residual(self, xn2d: torch.Tensor, resid2d: torch.Tensor, out2d: torch.Tensor, norm_w: Optional[torch.Tensor] = None,
+                       eps: float = ops.RMS_EPS, overlap: bool = False, add: Optional[torch.Tensor] = None):
+        """As MLP's; with `add` (and norm_w), xn2d += add first."""
+        gate, up, down = self.rows()
+        ov = overlap and ops.overlap_decode   # (the 8-bit weights are nobody's output here)
+        x = ops.quantize_fp8(xn2d) if norm_w is None else ops.rmsnorm_fp8(xn2d, norm_w, eps, add=add)
+        return ops.linear_fp8(ops.linear_fp8(x, gate, W2=up, overlap=ov), down, resid=resid2d, out=out2d, overlap=ov)
+
+    def forward(self, x):
+        gate, up, down = self.rows()
+        y = ops.linear_fp8(ops.linear_fp8(ops.quantize_fp8(x), gate, W2=up), down)
+        return y.reshape(x.shape)
+
+
+def make_mlp(config, dtype=None) -> MLP:
+    return (Fp8MLP if getattr(config, "mlp_fp8", False) else MLP)(config, dtype=dtype)
 
 
 class STU(nn.Module):

@@ -142,6 +142,16 @@ class arena:
         return piece
 
 
+class no_arena:
+    """Outputs of the ops called by this thread inside the block are allocations of their own: what outlives the step that an `arena` is open for."""
+
+    def __enter__(self):
+        self.outer, _local.arena = getattr(_local, "arena", None), None
+
+    def __exit__(self, *exc):
+        _local.arena = self.outer
+
+
 def empty(shape, dtype: torch.dtype, device) -> torch.Tensor:
     a = getattr(_local, "arena", None) if _arenas else None
     if a is not None:

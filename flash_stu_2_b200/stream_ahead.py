@@ -43,7 +43,8 @@ class StreamAhead:
             stu = layer.stu
             if not (own(layer, STULayer, "forward", "_decode") and own(stu, STU, "decode_step")):
                 return False
-            if (layer.stu_mlp_enabled or not stu.use_approx or stu.use_hankel_L or hist.dtype != torch.bfloat16 or hist.shape != shape
+            # (the norm behind the STU is this form's, in bf16: an MLP in 8 bits has its own)
+            if (layer.stu_mlp_enabled or getattr(layer.mlp, "fp8", False) or not stu.use_approx or stu.use_hankel_L or hist.dtype != torch.bfloat16 or hist.shape != shape
                     or not hist.is_contiguous() or not uniform_pos(pos) or host_pos(pos) != t or hist.shape[1] % 8 or hist.shape[1] > 4096
                     or stu.prepared()[2] is None):
                 return False

@@ -92,3 +92,40 @@ def test_argument_errors_of_the_library():
     assert call(w2=a, w2s=a, ys=a, r=a) == -4 and call(flags=1) == -4
     assert call(ws=a + 4) == -3 and call(w2=a, w2s=a, ys=a, y=a + 8) == -3
     assert call(M=0) == 0
+
+
+def _config(tmp_path, **kw):
+    import os
+    import flash_stu_2_b200 as F
+    path = os.path.join(tmp_path, "phi.pt")
+    F.save_spectral_filters(F.get_spectral_filters(64, 8, dtype=torch.float32, device="cpu"), path, metadata={"seq_len": 64, "K": 8})
+    return F.FlashSTUConfig(**{**dict(n_embd=32, n_layers=4, n_heads=4, seq_len=64, window_size=8, vocab_size=97, mlp_scale=4, num_eigh=8,
+                                      torch_dtype=torch.bfloat16, filter_path=path), **kw})
+
+
+def test_models_with_an_8_bit_mlp(tmp_path):
+    """The switch is the configuration's, survives a round trip, changes no checkpoint, and bfloat16 alone has it."""
+    import flash_stu_2_b200 as F
+    from flash_stu_2_b200.token_step import layer_supported
+    plain, cfg = _config(str(tmp_path)), _config(str(tmp_path), mlp_fp8=True)
+    assert not plain.mlp_fp8 and cfg.mlp_fp8 and F.FlashSTUConfig.from_dict(cfg.to_dict()).mlp_fp8 and not F.FlashSTUConfig.from_dict(plain.to_dict()).mlp_fp8
+    a, b = F.FlashSTU(plain), F.FlashSTU(cfg)
+    assert all(type(layer.mlp) is F.MLP for layer in a.layers) and all(type(layer.mlp) is F.Fp8MLP for layer in b.layers)
+    assert list(a.state_dict()) == list(b.state_dict())
+    b.load_state_dict(a.state_dict())
+    assert all(layer_supported(layer) for layer in a.layers) and not any(layer_supported(layer) for layer in b.layers)
+    assert type(F.FlashSTUBlock(d_model=64, sequence_length=128, num_filters=8, mlp_fp8=True).layer.mlp) is F.Fp8MLP
+    assert type(F.FlashSTUBlock(d_model=64, sequence_length=128, num_filters=8).layer.mlp) is F.MLP
+    with pytest.raises(NotImplementedError, match="bfloat16"):
+        F.FlashSTU(_config(str(tmp_path), mlp_fp8=True, torch_dtype=torch.float32))
+
+
+def test_tensor_parallelism_refuses_an_8_bit_mlp(tmp_path):
+    import torch.distributed as dist
+    from flash_stu_2_b200.tensor_parallel import TensorParallelFlashSTU
+    dist.init_process_group("gloo", init_method=f"file://{tmp_path}/rendezvous", rank=0, world_size=1)
+    try:
+        with pytest.raises(NotImplementedError, match="8 bits"):
+            TensorParallelFlashSTU(_config(str(tmp_path), mlp_fp8=True), {}, "cpu")
+    finally:
+        dist.destroy_process_group()

@@ -356,3 +356,102 @@ def test_a_wait_that_runs_out(M, two):
         assert lib.stu_test_inject_wait_expiry(0) == 0
     assert same(call(), want)
     ops.check_status()
+
+
+# ---------------------------------------------------------------------------------------------------- the models that use them
+def plain_mlp(mlp, x, resid, norm_w, eps):
+    """resid + an 8-bit MLP of norm(x), from the definitions in 64 bits, rounded where the layer rounds."""
+    def rows(v):
+        q, e = R.quantize(v)
+        return (R.blocks(q) * R.power(e)[:, :, None]).view(q.shape)[:, :v.shape[1]]
+    v = x.double()
+    v = rows((v / torch.sqrt(v.square().mean(1, keepdim=True) + eps) * norm_w.double()).float().double())
+    gate, up, down = (rows(getattr(mlp, n).weight.double()) for n in ("gate_proj", "up_proj", "down_proj"))
+    h = rows((R.gelu(v @ gate.T) * (v @ up.T)).float().double())
+    return (resid.float() + (h @ down.T).bfloat16().float()).bfloat16()
+
+
+def model(d=256, layers=4, seed=0, **kw):
+    import flash_stu_2_b200 as F
+    torch.manual_seed(seed)
+    cfg = F.FlashSTUConfig(**{**dict(n_embd=d, n_layers=layers, n_heads=4, seq_len=256, window_size=64, vocab_size=501, mlp_scale=3, num_eigh=8,
+                                     torch_dtype=torch.bfloat16, mlp_fp8=True), **kw})
+    m = F.FlashSTU(cfg).to(dev()).eval()
+    with torch.no_grad():
+        for name, p in m.named_parameters():   # branches that are small against the stream, as a trained model's
+            if p.dim() == 2:
+                p.normal_(0, p.shape[1] ** -0.5 * (0.3 if "down_proj" in name or "c_proj" in name else 1), generator=gen(seed + p.numel()))
+    return m
+
+
+@pytest.mark.parametrize("T", [1, 40, 200])
+@pytest.mark.parametrize("attention", [False, True])
+def test_a_layer_with_an_8_bit_mlp(T, attention):
+    """Prefill and cached steps of a layer against the same layer whose MLP is computed from the definitions; 2e-2 relative is what the layers are held to
+    in bf16.  (Both have the same input to the MLP, so that the 8-bit values differ where fp32 sums put a value on the other side of a rounding.)"""
+    import flash_stu_2_b200 as F
+    from parity import close
+    m = model(layers=2)
+    layer = m.layers[1 if attention else 0]
+    assert type(layer.mlp) is F.Fp8MLP
+    x = torch.randn(3, T + 3, 256, device=dev(), generator=gen(T)).bfloat16()
+
+    def run():
+        with torch.no_grad():
+            y, cache = layer(x[:, :T].clone(), past_key_value=None, use_cache=True)
+            out = [y.clone()]
+            for t in range(T, T + 3):
+                y, cache = layer(x[:, t:t + 1].clone(), past_key_value=cache, use_cache=True)
+                out.append(y.clone())
+        return torch.cat(out, 1)
+
+    got = run()
+
+    def plain(xn2d, resid2d, out2d, norm_w=None, eps=0.0, overlap=False, add=None):
+        if add is not None:
+            xn2d += add   # (bf16 + bf16, rounded once)
+        out2d.copy_(plain_mlp(layer.mlp, xn2d, resid2d, norm_w, eps))
+
+    layer.mlp.apply_residual = plain
+    close(got, run(), 2e-2)
+
+
+@pytest.mark.parametrize("kw", [dict(), dict(use_approx=False), dict(use_attn=False), dict(stu_enable_mlp_sandwich=True, stu_mlp_hidden_size=128)])
+@pytest.mark.parametrize("B", [1, 20])
+def test_generate_with_8_bit_mlps(B, kw):
+    """A captured step and the layers one by one are the same kernels: the same tokens and logits.  The logits are near the bf16 model's: three 8-bit roundings of
+    2^-5.3 in the mean square per MLP (norm, weights, h; the weights' again), whose branches are 0.3 of a stream that grows with them."""
+    m = model(**kw)
+    ids = torch.randint(0, 501, (B, 30), device=dev(), generator=gen(B))
+    with torch.no_grad():
+        a, la = m.generate(ids, max_length=50, do_sample=False, return_logits=True)
+        b, lb = m.generate(ids, max_length=50, do_sample=False, return_logits=True, cuda_graph=False)
+        assert torch.equal(a, b) and torch.equal(la, lb)
+        full = m(a, use_cache=False).logits[:, 29:-1].float()
+        other = model(mlp_fp8=False, **kw)
+        other.load_state_dict(m.state_dict())
+        ref = other(a, use_cache=False).logits[:, 29:-1].float()
+    # a step and a prefill differ where a bf16 rounding puts an 8-bit value elsewhere: within what the 8 bits lose
+    assert float((full - ref).norm() / ref.norm()) < 0.1
+    assert float((la.float() - full).norm() / full.norm()) < 0.1
+
+
+def test_8_bit_weights_follow_the_parameters():
+    from flash_stu_2_b200 import ops
+    m = model(layers=1)
+    mlp, x = m.layers[0].mlp, torch.randn(5, 256, device=dev(), generator=gen(1)).bfloat16()
+    with torch.no_grad():
+        first = mlp(x)
+        assert mlp.rows()[0] is mlp.rows()[0] and torch.equal(mlp(x), first)
+        mlp.down_proj.weight.mul_(2)
+        assert torch.equal(mlp(x).float(), 2 * first.float())   # a power of two: every rounding is the same
+        mlp.gate_proj.weight.data = mlp.gate_proj.weight.data.flip(0).contiguous()
+        assert not torch.equal(mlp(x).float(), 2 * first.float())
+        assert mlp(x.view(1, 5, 256)).shape == (1, 5, 256)
+        want = mlp(x)
+        mlp.up_proj.weight.mul_(1)   # new 8-bit rows, made while an arena is open, are not its pieces
+        buffer = torch.zeros(1 << 20, dtype=torch.uint8, device=dev())
+        with ops.arena(buffer):
+            mlp(x)
+        buffer.fill_(255)
+        assert torch.equal(mlp(x), want)
