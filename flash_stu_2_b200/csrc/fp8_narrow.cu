@@ -327,9 +327,9 @@ template <bool DUAL, int NT> int cluster_room(int ks) {
 // 1536 x 6144 (36) 20.7 / 14.1 / 17.9 / 25.0.
 template <bool DUAL, int NT> int cluster_size(const Fp8Product& p) {
   const long long tiles = (long long)blocks_of(p.N) * ((p.M + NT - 1) / NT);
-  const int num_kb = blocks_of(p.K);
+  const int num_kb = blocks_of(p.K), sms = device_sm_count();
   for (int ks = num_kb < MAX_KS ? num_kb : MAX_KS; ks > 1; ks--)
-    if (tiles * ks <= device_sm_count() && tiles <= cluster_room<DUAL, NT>(ks)) return ks;
+    if (tiles * ks <= sms && tiles <= cluster_room<DUAL, NT>(ks)) return ks;
   return 1;
 }
 

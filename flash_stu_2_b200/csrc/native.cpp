@@ -229,10 +229,17 @@ PyObject* rmsnorm(PyObject*, PyObject* const* args, Py_ssize_t n) {
 struct Rows8 {
   const at::Tensor *data = nullptr, *scales = nullptr;
 };
+// Values and scales in one allocation (of the two that there would be, one costs as much as the rest of the call's checks).
+at::Tensor bytes_of(const at::Tensor& base, long long offset, at::IntArrayRef sizes, at::ScalarType type) {
+  at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(base.storage()), base.key_set(), c10::scalarTypeToTypeMeta(type));
+  t.unsafeGetTensorImpl()->set_storage_offset(offset);
+  t.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
+  return t;
+}
 std::pair<at::Tensor, at::Tensor> new_rows8(long long rows, long long cols, const at::Tensor& like) {
-  const auto bytes = like.options();
-  return {at::empty({rows, (cols + 127) / 128 * 128}, bytes.dtype(at::kFloat8_e4m3fn)),
-          at::empty({(rows + 127) / 128, (cols + 511) / 512, 32, 4, 4}, bytes.dtype(at::kFloat8_e8m0fnu))};
+  const long long padded = (cols + 127) / 128 * 128, a = (rows + 127) / 128, g = (cols + 511) / 512;
+  const at::Tensor base = at::empty({rows * padded + a * g * 512}, like.options().dtype(at::kByte));
+  return {bytes_of(base, 0, {rows, padded}, at::kFloat8_e4m3fn), bytes_of(base, rows * padded, {a, g, 32, 4, 4}, at::kFloat8_e8m0fnu)};
 }
 // `cols` columns in the layout that the kernels read, on device `dev`
 bool rows8(PyObject* data, PyObject* scales, long long cols, int dev, Rows8* r) {
