@@ -12,6 +12,7 @@ extern "C" int stu_linear_fp8(const void* x, const void* x_scales, const void* W
   const void* rows[] = {x, x_scales, W, W_scales, W2, W2_scales, W2 ? y : nullptr, y_scales};
   for (const void* p : rows)
     if (!aligned16(p)) return STU_ERR_ALIGN;
+  if (((uintptr_t)y | (uintptr_t)resid) & 1u) return STU_ERR_ALIGN;
   if (M == 0) return STU_OK;
   const unsigned char *w2 = (const unsigned char*)W2, *w2s = (const unsigned char*)W2_scales;
   const Fp8Product p{(const unsigned char*)x, (const unsigned char*)x_scales, (const unsigned char*)W, (const unsigned char*)W_scales, w2, w2s,

@@ -394,13 +394,16 @@ int launch_rmsnorm(const void* x, const void* add, const void* w, void* sum, voi
   return launch((const T*)x, (const T*)add, (const T*)w, (T*)sum, (unsigned char*)q, (unsigned char*)scales, rows, cols, xs, as, ss, eps, st);
 }
 
+// Whether an address is one of a whole element.
+bool whole(const void* p, int dtype) { return !(reinterpret_cast<uintptr_t>(p) & (dtype == STU_F32 ? 3u : 1u)); }
+
 }  // namespace
 
 extern "C" int stu_quantize_fp8(const void* x, void* q, void* scales, int rows, int cols, long long x_row_stride, int dtype, void* stream) {
   if (!x || !q || !scales) return STU_ERR_NULL;
   if (rows < 0 || cols <= 0 || cols > INT32_MAX - fp8::PIECE) return STU_ERR_SHAPE;
-  if (!aligned16(q) || !aligned16(scales)) return STU_ERR_ALIGN;
   if (dtype != STU_F32 && dtype != STU_BF16) return STU_ERR_DTYPE;
+  if (!aligned16(q) || !aligned16(scales) || !whole(x, dtype)) return STU_ERR_ALIGN;
   if (rows == 0) return STU_OK;
   cudaStream_t st = (cudaStream_t)stream;
   return dtype == STU_F32 ? launch_quantize<float>(x, q, scales, rows, cols, x_row_stride, st)
@@ -411,8 +414,8 @@ extern "C" int stu_rmsnorm_fp8(const void* x, const void* add, const void* w, vo
                                long long x_row_stride, long long add_row_stride, long long sum_row_stride, float eps, int dtype, void* stream) {
   if (!x || !w || !q || !scales || (add && !sum)) return STU_ERR_NULL;
   if (rows < 0 || cols <= 0 || cols > 32768) return STU_ERR_SHAPE;   // 16 warps x 4 pieces
-  if (!aligned16(q) || !aligned16(scales)) return STU_ERR_ALIGN;
   if (dtype != STU_F32 && dtype != STU_BF16) return STU_ERR_DTYPE;
+  if (!aligned16(q) || !aligned16(scales) || !whole(x, dtype) || !whole(add, dtype) || !whole(w, dtype) || !whole(sum, dtype)) return STU_ERR_ALIGN;
   if (rows == 0) return STU_OK;
   cudaStream_t st = (cudaStream_t)stream;
   return dtype == STU_F32 ? launch_rmsnorm<float>(x, add, w, sum, q, scales, rows, cols, x_row_stride, add_row_stride, sum_row_stride, eps, st)

@@ -142,7 +142,8 @@ class MLP(nn.Module):
 
 class Fp8MLP(MLP):
     """The MLP in 8 bits (config.mlp_fp8): its input's norm, both products and what lies between them on e4m3 rows with a scale for each 128
-    of a row (ops.Fp8Rows).  The parameters are MLP's; their 8-bit rows are derived, kept per parameter version."""
+    of a row (ops.Fp8Rows).  The parameters are MLP's; their 8-bit rows are made by the first call behind a change of them (of one through `.data`, which
+    leaves no trace, `mlp.rows(again=True)` tells)."""
     fp8 = True
 
     def __init__(self, config, dtype=None):
@@ -151,20 +152,37 @@ class Fp8MLP(MLP):
             raise NotImplementedError("mlp_fp8=True has kernels for bfloat16 models only")
         self._rows, self._rows_key = None, None
 
-    def rows(self):
+    def __getstate__(self):   # (copies and files: the parameters alone)
+        return {**super().__getstate__(), "_rows": None, "_rows_key": None}
+
+    def rows(self, again: bool = False):
         """gate, up and down as 8-bit rows."""
         weights = [param(child(self, name), "weight") for name in ("gate_proj", "up_proj", "down_proj")]
-        key = tuple((w._version, w.data_ptr(), w.device) for w in weights)
-        if self._rows_key != key:
+        key = [(w._version, w.data_ptr(), w.shape, w.stride()) for w in weights]
+        if again or self._rows_key is None or key != self._rows_key[0]:
             with torch.no_grad(), ops.no_arena():
-                self._rows, self._rows_key = tuple(ops.quantize_fp8(w.detach()) for w in weights), key
+                made = tuple(ops.quantize_fp8(w.detach()) for w in weights)
+                if torch.cuda.is_current_stream_capturing():   # rows that only a graph's replay makes belong to that graph
+                    return made
+                kept = self._rows
+                if kept is not None and all(k.data.device == m.data.device and k.shape == m.shape for k, m in zip(kept, made)):
+                    for k, m in zip(kept, made):   # in place: graphs that were captured with them read the new ones, and never memory that is others'
+                        k.data.copy_(m.data)
+                        k.scales.copy_(m.scales)
+                    made = kept
+                # Calls on other streams, and kernels that fetch weights ahead of the one in front, find them there.
+                torch.cuda.current_stream(made[0].data.device).synchronize()
+            # (the weights that they were made from are kept with the addresses that tell them)
+            self._rows, self._rows_key = made, (key, [w.detach() for w in weights])
         return self._rows
 
     def apply_residual(self, xn2d: torch.Tensor, resid2d: torch.Tensor, out2d: torch.Tensor, norm_w: Optional[torch.Tensor] = None,
                        eps: float = ops.RMS_EPS, overlap: bool = False, add: Optional[torch.Tensor] = None):
-        """As MLP's; with `add` (and norm_w), xn2d += add first."""
-        gate, up, down = self.rows()
-        ov = overlap and ops.overlap_decode   # (the 8-bit weights are nobody's output here)
+        """As MLP's; with `add`, xn2d += add first."""
+        if add is not None and norm_w is None:
+            raise ValueError("add is taken in by the norm: norm_w is missing")
+        gate, up, down = rows = self.rows()
+        ov = overlap and ops.overlap_decode and rows is self._rows   # (others are still being made)
         x = ops.quantize_fp8(xn2d) if norm_w is None else ops.rmsnorm_fp8(xn2d, norm_w, eps, add=add)
         return ops.linear_fp8(ops.linear_fp8(x, gate, W2=up, overlap=ov), down, resid=resid2d, out=out2d, overlap=ov)
 

@@ -413,9 +413,11 @@ def rmsnorm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float = RMS_EPS, add
 def linear_fp8(x: Fp8Rows, W: Fp8Rows, *, W2: Optional[Fp8Rows] = None, resid: Optional[torch.Tensor] = None,
                out: Optional[torch.Tensor] = None, overlap: bool = False):
     """linear() of 8-bit rows: x @ W^T as bf16 [rows of x, rows of W]; with `resid` (bf16; `out` may be the same) added to it; with W2
-    gelu_tanh(x @ W^T) * (x @ W2^T) as 8-bit rows.  overlap: the weights are fetched while the kernel before this one drains, which must not be
-    writing them (FLAG_OVERLAP)."""
+    gelu_tanh(x @ W^T) * (x @ W2^T) as 8-bit rows.  overlap: the weights are fetched while the kernels before this one drain, none of which may be
+    writing them (FLAG_OVERLAP).  The order of a sum over K depends on the number of rows, so that a row alone and among others may differ in fp32's last bits."""
     flags = FLAG_OVERLAP if overlap else 0
+    if not (isinstance(x, Fp8Rows) and isinstance(W, Fp8Rows) and (W2 is None or isinstance(W2, Fp8Rows))):
+        raise TypeError("linear_fp8: x, W and W2 are Fp8Rows")
     if not _arenas or getattr(_local, "arena", None) is None:
         if x.cols == W.cols and (W2 is None or W2.cols == W.cols):
             y = _lib.native().linear_fp8(x.data, x.scales, W.data, W.scales, x.cols, *((None, None) if W2 is None else (W2.data, W2.scales)), resid, out, flags)

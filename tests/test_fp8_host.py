@@ -129,3 +129,106 @@ def test_tensor_parallelism_refuses_an_8_bit_mlp(tmp_path):
             TensorParallelFlashSTU(_config(str(tmp_path), mlp_fp8=True), {}, "cpu")
     finally:
         dist.destroy_process_group()
+
+
+def test_addresses_inside_of_an_element_are_refused():
+    from flash_stu_2_b200 import _lib
+    lib, a = _lib.load(), 0x10000
+    assert lib.stu_quantize_fp8(a + 1, a, a, 1, 128, 128, 1, None) == -3 and lib.stu_quantize_fp8(a + 2, a, a, 1, 128, 128, 0, None) == -3
+    for k in range(4):   # x, add, w, sum
+        p = [a] * 4
+        p[k] += 1
+        assert lib.stu_rmsnorm_fp8(*p, a, a, 1, 128, 128, 128, 128, 1e-6, 1, None) == -3
+    assert lib.stu_linear_fp8(a, a, a, a, None, None, None, 0, a + 1, 8, None, 4, 8, 128, 0, None) == -3
+    assert lib.stu_linear_fp8(a, a, a, a, None, None, a + 1, 8, a, 8, None, 4, 8, 128, 0, None) == -3
+
+
+def test_linear_takes_8_bit_rows():
+    from flash_stu_2_b200 import ops
+    r, t = made(2, 256), torch.zeros(2, 256)
+    for call in (lambda: ops.linear_fp8(t, r), lambda: ops.linear_fp8(r, t), lambda: ops.linear_fp8(r, r, W2=t)):
+        with pytest.raises(TypeError, match="Fp8Rows"):
+            call()
+
+
+def test_when_8_bit_weights_are_made(tmp_path, monkeypatch):
+    """Their kernels stand in for themselves: what is made when, that it is there before anyone reads it ahead of the kernel in front, and what a capture keeps."""
+    import copy
+    import pickle
+    import flash_stu_2_b200 as F
+    from flash_stu_2_b200 import ops
+    calls, capturing = [], [False]
+
+    class Stream:
+        def synchronize(self):
+            calls.append("wait")
+
+    def quantize(w):
+        calls.append("quantize")
+        q, e = R.quantize(w.double())
+        return ops.Fp8Rows(q.to(torch.float8_e4m3fn), R.pieces((e + 127).to(torch.uint8)).view(torch.float8_e8m0fnu), w.shape[1])
+
+    def linear(x, W, *, W2=None, resid=None, out=None, overlap=False):
+        calls.append(overlap)
+        return x if W2 is not None else resid
+
+    monkeypatch.setattr(ops, "quantize_fp8", quantize)
+    monkeypatch.setattr(ops, "rmsnorm_fp8", lambda x, w, eps, add=None: x)
+    monkeypatch.setattr(ops, "linear_fp8", linear)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda *a: Stream())
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing[0])
+    mlp = F.FlashSTU(_config(str(tmp_path), mlp_fp8=True)).layers[0].mlp
+    x, norm = torch.zeros(1, 32, dtype=torch.bfloat16), torch.ones(32, dtype=torch.bfloat16)
+
+    def step():
+        del calls[:]
+        mlp.apply_residual(x, x, x, norm_w=norm, overlap=True)
+        return list(calls)
+
+    made, kept = ["quantize"] * 3, [True, True]
+    capturing[0] = True
+    assert step() == made + [False, False] == step() and mlp._rows is None   # the graph's own, never read ahead of the kernels that make them
+    capturing[0] = False
+    assert step() == made + ["wait"] + kept and step() == kept
+    rows = mlp.rows()
+    capturing[0] = True
+    assert step() == kept
+    capturing[0] = False
+    with torch.no_grad():
+        mlp.up_proj.weight.mul_(2)
+    before = rows[1].dequantize().clone()
+    assert step() == made + ["wait"] + kept and mlp.rows()[1] is rows[1] and torch.equal(rows[1].dequantize(), 2 * before)   # in place
+    mlp.up_proj.weight.data.mul_(2)   # (leaves no trace)
+    assert step() == kept
+    mlp.rows(again=True)
+    assert torch.equal(rows[1].dequantize(), 4 * before)
+    with torch.no_grad():
+        mlp.gate_proj.weight.data = mlp.gate_proj.weight.data.t().contiguous().t()   # the same numbers elsewhere
+    assert step() == made + ["wait"] + kept
+    mlp.down_proj.weight = torch.nn.Parameter(torch.zeros(32, 64, dtype=torch.bfloat16))
+    assert step() == made + ["wait"] + kept and mlp.rows()[2].shape == (32, 64)
+    for other in (copy.deepcopy(mlp), pickle.loads(pickle.dumps(mlp))):
+        assert other._rows is None and mlp._rows is not None
+        assert other.rows()[0] is not mlp.rows()[0] and torch.equal(other.rows()[0].dequantize(), mlp.rows()[0].dequantize())
+    with pytest.raises(ValueError, match="norm_w"):
+        mlp.apply_residual(x, x, x, add=x)
+
+
+def test_a_weight_at_the_address_of_one_that_is_gone(tmp_path, monkeypatch):
+    """The weights that rows were made from are kept with their addresses: nothing else is ever there."""
+    import weakref
+    import flash_stu_2_b200 as F
+    from flash_stu_2_b200 import ops
+    monkeypatch.setattr(ops, "quantize_fp8", lambda w: ops.Fp8Rows(w[:1, :1].clone(), torch.zeros(1), w.shape[1]))
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda *a: type("S", (), {"synchronize": lambda self: None})())
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    mlp = F.FlashSTU(_config(str(tmp_path), mlp_fp8=True)).layers[0].mlp
+    for value in range(8):
+        mlp.up_proj.weight.data = torch.empty(0, dtype=torch.bfloat16)
+        mlp.up_proj.weight.data = torch.full((128, 32), float(value), dtype=torch.bfloat16)
+        assert bool((mlp.rows()[1].data == value).all())
+    gone = weakref.ref(mlp)
+    del mlp
+    import gc
+    gc.collect()
+    assert gone() is None

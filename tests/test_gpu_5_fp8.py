@@ -455,3 +455,90 @@ def test_8_bit_weights_follow_the_parameters():
             mlp(x)
         buffer.fill_(255)
         assert torch.equal(mlp(x), want)
+
+
+def test_8_bit_weights_of_a_graph():
+    """A first call that is captured makes rows of the graph's own; a graph that reads kept rows reads those of new weights too."""
+    from flash_stu_2_b200 import ops
+    m = model(layers=1)
+    mlp, x = m.layers[0].mlp, torch.randn(5, 256, device=dev(), generator=gen(2)).bfloat16()
+    ops.status_word(dev())
+    with torch.no_grad():
+        want = model(layers=1).layers[0].mlp(x)
+        own = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(own):
+            y = mlp(x)
+        assert torch.equal(mlp(x), want)   # nothing has been replayed
+        own.replay()
+        assert torch.equal(y, want)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            z = mlp(x)
+        graph.replay()
+        assert torch.equal(z, want)
+        mlp.down_proj.weight.mul_(2)
+        assert torch.equal(mlp(x).float(), 2 * want.float())
+        for g, out in ((graph, z), (own, y)):
+            g.replay()
+            assert torch.equal(out.float(), 2 * want.float())
+        w = mlp.up_proj.weight
+        twice = w.cpu() * 2
+        w.data = torch.empty(0, device=dev(), dtype=torch.bfloat16)
+        w.data = twice.to(dev())
+        assert torch.equal(mlp(x).float(), 4 * want.float())
+    ops.check_status()
+
+
+@pytest.mark.parametrize("M,d,inter", [(1, 512, 1024), (40, 1536, 2048), (700, 1024, 1100)])
+def test_two_streams_at_once(M, d, inter):
+    """The chain of an MLP on two streams at a time, from threads of their own, many times over: what each gives alone."""
+    import threading
+    from flash_stu_2_b200 import ops
+    g = gen(M)
+    wg, wu, wd = weights8(g, inter, d), weights8(g, inter, d), weights8(g, d, inter)
+    norm = torch.ones(d, device=dev(), dtype=torch.bfloat16)
+    xs = [torch.randn(M, d, device=dev(), generator=g).bfloat16() for _ in range(2)]
+
+    def mlp(x):
+        return ops.linear_fp8(ops.linear_fp8(ops.rmsnorm_fp8(x, norm), wg, W2=wu, overlap=True), wd, resid=x, overlap=True)
+
+    want = [mlp(x) for x in xs]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def run(x, w):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            got = [mlp(x) for _ in range(50)]
+        stream.synchronize()
+        wrong.extend(i for i, y in enumerate(got) if not torch.equal(y, w))
+
+    threads = [threading.Thread(target=run, args=p) for p in zip(xs, want)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+    ops.check_status()
+
+
+@pytest.mark.parametrize("cols", [300, 1536, 4096])
+def test_equal_rows_give_equal_rows(cols):
+    """Within a call wherever they stand; of the norm and the quantisation whatever stands beside them."""
+    from flash_stu_2_b200 import ops
+    g = gen(cols)
+    one = stream(g, 1, cols, torch.bfloat16)
+    w = torch.randn(cols, device=dev(), generator=g).bfloat16()
+    a, b = weights8(g, 200, cols), weights8(g, 200, cols)
+    norms, quantised = [], []
+    for rows in (1, 3, 130, 700, 6000):
+        x = one.expand(rows, cols).contiguous()
+        q, n = ops.quantize_fp8(x), ops.rmsnorm_fp8(x, w)
+        for r in (q, n, ops.linear_fp8(n, a, W2=b)):
+            assert bool((r.data.view(torch.uint8) == r.data.view(torch.uint8)[:1]).all()) and bool((r.block_scales() == r.block_scales()[:1]).all())
+        y = ops.linear_fp8(n, a)
+        assert bool((y == y[:1]).all())
+        quantised.append((q.data.view(torch.uint8)[:1], q.block_scales()[:1]))
+        norms.append((n.data.view(torch.uint8)[:1], n.block_scales()[:1]))
+    for found in (norms, quantised):
+        assert all(torch.equal(d, found[0][0]) and torch.equal(s, found[0][1]) for d, s in found)
