@@ -7,8 +7,10 @@
 // before its epilogue.
 //
 // A pair of CTAs on neighbouring SMs computes tiles of 256 x 256 (gate/up: 256 x 128 of both) with cta_group::2, or a CTA alone tiles of 128
-// rows where those would leave SMs idle.  Warp 0 of a CTA is its TMA producer, warp 1 of the first CTA issues scale copies and instructions, warps 2..9 drain
-// the accumulators.  The kernel is persistent; two accumulators of 256 columns and the scales do not fit 512 columns, so the accumulators
+// rows where those would leave SMs idle.  A thread of warp 0 of a CTA is its TMA producer, one of warp 1 of the first CTA issues scale copies and instructions,
+// warps 2..9 drain the accumulators.  (The tensor core takes few instructions ahead: what the issuer does between two stages is time that it may stand still, and the
+// arithmetic of the other warps draws it out.  Whole warps that agree on every wait and issue by a lane: 16384 x 6144 x 1536 gate/up 250 us, so 230; 2048 x 4096 x
+// 1024 20.5, so 18.4.)  The kernel is persistent; two accumulators of 256 columns and the scales do not fit 512 columns, so the accumulators
 // share 32 columns: the epilogue reads those first and hands them back ahead of the rest.
 //
 // gate/up: a thread has 64 of the 128 features of a block of its row, two warps settle the block's scale through shared memory, and the row
@@ -119,24 +121,23 @@ __global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__(64 + 32 * EPI_WAR
   pdl_trigger();
 
   if (warp == 0) {
-    // ---------------- TMA producer (of either CTA: its 128 rows of x, its part of the rows of W, the scales of both)
-    const bool leader = elect_one();
-    const CUtensorMap* mapB = DUAL && rank ? &tmB2 : &tmB;   // gate/up in a pair: the first CTA brings the gate rows, the second the up rows
-    const uint32_t full0 = in_first_cta(full_bar);
-    int g = 0, s = 0;
-    uint32_t ph = 1;
-    bool ok = true, ready = false;
-    for (int tile = pair; ok && tile < num_tiles; tile += pairs) {
-      int tm, tn;
-      tile_coords(tile, tiles_m, tiles_n, group_m, tm, tn);
-      const int m0 = (CTAS * tm + rank) * BM, n0 = tn * TN + (DUAL ? 0 : rank * F::B_ROWS), nb = tn * TN / 128;
-      for (int kb = 0; kb < num_kb; kb += KBS, g++) {
-        if (!ready) ok = tma::warp_wait_bounded(&empty_bar[s], ph, abort_flag, wait_ns);
-        if (!ok) break;
-        const int s1 = s + 1 == STAGES ? 0 : s + 1;
-        const uint32_t ph1 = s1 ? ph : ph ^ 1u;
-        const bool ready1 = mbar_ready(&empty_bar[s1], ph1);   // asked for here, looked at behind the copies
-        if (leader) {
+    if (elect_one()) {
+      // ---------------- TMA producer, one thread (of either CTA: its 128 rows of x, its part of the rows of W, the scales of both)
+      const CUtensorMap* mapB = DUAL && rank ? &tmB2 : &tmB;   // gate/up in a pair: the first CTA brings the gate rows, the second the up rows
+      const uint32_t full0 = in_first_cta(full_bar);
+      int g = 0, s = 0;
+      uint32_t ph = 1;
+      bool ok = true, ready = false;
+      for (int tile = pair; ok && tile < num_tiles; tile += pairs) {
+        int tm, tn;
+        tile_coords(tile, tiles_m, tiles_n, group_m, tm, tn);
+        const int m0 = (CTAS * tm + rank) * BM, n0 = tn * TN + (DUAL ? 0 : rank * F::B_ROWS), nb = tn * TN / 128;
+        for (int kb = 0; kb < num_kb; kb += KBS, g++) {
+          if (!ready) ok = tma::mbar_wait_bounded(&empty_bar[s], ph, abort_flag, wait_ns);
+          if (!ok) break;
+          const int s1 = s + 1 == STAGES ? 0 : s + 1;
+          const uint32_t ph1 = s1 ? ph : ph ^ 1u;
+          const bool ready1 = mbar_ready(&empty_bar[s1], ph1);   // asked for here, looked at behind the copies
           const bool with_scales = (kb & 3) == 0;
           const int n = min(KBS, num_kb - kb);
           unsigned char *sa = smem + s * F::TILE_BYTES, *ss = scales + s * F::SCALE_BYTES;
@@ -170,19 +171,18 @@ __global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__(64 + 32 * EPI_WAR
               }
             }
           }
+          ready = ready1;
+          s = s1, ph = ph1;
         }
-        ready = __all_sync(0xffffffffu, ready1);
-        s = s1, ph = ph1;
       }
+      *issued_ctr = g;
+      // the last stages' releases arrive in both CTAs: wait for them here, so that none is under way to a CTA that has left
+      for (int h = max(g - STAGES, 0); ok && h < g; h++)
+        ok = tma::mbar_wait_bounded(&empty_bar[h % STAGES], (uint32_t)(h / STAGES) & 1u, abort_flag, wait_ns);
     }
-    if (leader) *issued_ctr = g;
-    // the last stages' releases arrive in both CTAs: wait for them here, so that none is under way to a CTA that has left
-    for (int h = max(g - STAGES, 0); ok && h < g; h++)
-      ok = tma::warp_wait_bounded(&empty_bar[h % STAGES], (uint32_t)(h / STAGES) & 1u, abort_flag, wait_ns);
   } else if (warp == 1) {
-    if (rank == 0) {
-      // ---------------- issuer of the pair
-      const bool leader = elect_one();
+    if (rank == 0 && elect_one()) {
+      // ---------------- issuer of the pair: one thread
       const uint64_t da0 = operand_desc(tma::smem_u32(smem)), db0 = operand_desc(tma::smem_u32(smem) + A_BYTES);
       const uint64_t ds0 = scales_desc(tma::smem_u32(scales));
       int g = 0, s = 0, it = 0, pieces = 0;
@@ -191,41 +191,38 @@ __global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__(64 + 32 * EPI_WAR
       for (int tile = pair; ok && tile < num_tiles; tile += pairs, it++) {
         const int buf = it & 1;
         const uint32_t acc = tmem_base + (uint32_t)buf * F::SECOND;
-        ok = tma::warp_wait_bounded(&tmem_empty[buf], (((uint32_t)it >> 1) & 1u) ^ 1u, abort_flag, wait_ns);
-        if (SHARED && ok && it > 0) ok = tma::warp_wait_bounded(&shared_read[buf ^ 1], ((uint32_t)(it - 1) >> 1) & 1u, abort_flag, wait_ns);
+        ok = tma::mbar_wait_bounded(&tmem_empty[buf], (((uint32_t)it >> 1) & 1u) ^ 1u, abort_flag, wait_ns);
+        if (SHARED && ok && it > 0) ok = tma::mbar_wait_bounded(&shared_read[buf ^ 1], ((uint32_t)(it - 1) >> 1) & 1u, abort_flag, wait_ns);
         if (!ok) break;
         for (int kb = 0; kb < num_kb; kb += KBS, g++) {
-          if (!ready) ok = tma::warp_wait_bounded(&full_bar[s], ph, abort_flag, wait_ns);
+          if (!ready) ok = tma::mbar_wait_bounded(&full_bar[s], ph, abort_flag, wait_ns);
           if (!ok) break;
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
           const int s1 = s + 1 == STAGES ? 0 : s + 1;
           const uint32_t ph1 = s1 ? ph : ph ^ 1u;
           const bool ready1 = mbar_ready(&full_bar[s1], ph1);
           if ((kb & 3) == 0) sf_cols = tmem_base + F::SCALES + 16 * (pieces++ & 1);
-          if (leader) {
-            if ((kb & 3) == 0) {   // in order with the instructions around it
-              const uint64_t ds = ds0 + (uint64_t)(s * (F::SCALE_BYTES >> 4));
+          if ((kb & 3) == 0) {   // in order with the instructions around it
+            const uint64_t ds = ds0 + (uint64_t)(s * (F::SCALE_BYTES >> 4));
 #pragma unroll
-              for (int i = 0; i < F::SCALE_BYTES / fp8::PIECE; i++) copy_scales<CTAS>(sf_cols + 4 * i, ds + i * (fp8::PIECE >> 4));
-            }
-            const uint64_t da = da0 + (uint64_t)(s * (F::TILE_BYTES >> 4)), db = db0 + (uint64_t)(s * (F::TILE_BYTES >> 4));
-#pragma unroll
-            for (int j = 0; j < KBS; j++)
-              if (j == 0 || kb + j < num_kb) {
-#pragma unroll
-                for (int kk = 0; kk < BK / 32; kk++)   // 32 bytes along K inside the swizzled row: +2
-                  multiply<CTAS, MMA_N>(acc, da + j * (F::KB_BYTES >> 4) + 2 * kk, db + j * (F::KB_BYTES >> 4) + 2 * kk, sf_cols, sf_cols + 4, (kb + j) & 3,
-                                        (kb | j | kk) ? 1u : 0u);
-              }
-            commit<CTAS>(&empty_bar[s]);
+            for (int i = 0; i < F::SCALE_BYTES / fp8::PIECE; i++) copy_scales<CTAS>(sf_cols + 4 * i, ds + i * (fp8::PIECE >> 4));
           }
-          ready = __all_sync(0xffffffffu, ready1);
+          const uint64_t da = da0 + (uint64_t)(s * (F::TILE_BYTES >> 4)), db = db0 + (uint64_t)(s * (F::TILE_BYTES >> 4));
+#pragma unroll
+          for (int j = 0; j < KBS; j++)
+            if (j == 0 || kb + j < num_kb) {
+#pragma unroll
+              for (int kk = 0; kk < BK / 32; kk++)   // 32 bytes along K inside the swizzled row: +2
+                multiply<CTAS, MMA_N>(acc, da + j * (F::KB_BYTES >> 4) + 2 * kk, db + j * (F::KB_BYTES >> 4) + 2 * kk, sf_cols, sf_cols + 4, (kb + j) & 3,
+                                      (kb | j | kk) ? 1u : 0u);
+            }
+          commit<CTAS>(&empty_bar[s]);
+          ready = ready1;
           s = s1, ph = ph1;
         }
-        if (ok && leader) commit<CTAS>(&tmem_full[buf]);
-        __syncwarp();
+        if (ok) commit<CTAS>(&tmem_full[buf]);
       }
-      if (leader) *consumed_ctr = g;
+      *consumed_ctr = g;
     }
   } else {
     // ---------------- epilogue warps: TMEM lane quarter = warp % 4 (32 rows), half of the columns

@@ -2,7 +2,7 @@
 // thread-block cluster so that a few thousand features occupy all SMs.  What bounds it: HBM, the weights once; for small weights the time
 // from a launch over the first bytes and the cluster's meeting to the last store.
 //
-// Warp 0 of a CTA brings 128 features (gate/up: 128 of both), NT tokens and their scales by TMA into a ring, warp 1 copies the scales into tensor memory
+// A thread of warp 0 of a CTA brings 128 features (gate/up: 128 of both), NT tokens and their scales by TMA into a ring, one of warp 1 copies the scales into tensor memory
 // and issues kind::mxf8f6f4 (see fp8_gemm.cu), the others drain the sums into shared memory, where the ring was.  Then every CTA of the cluster takes
 // its share of the tokens: a warp adds up a token's 128 features over the cluster, in the order of K, and stores them (sums sent to the CTA that adds them up by
 // bulk copies, with no barrier of the cluster ahead of or behind them, came later: 1 x 1024 x 4096 5.2 us, so 4.7); gate/up: one warp has the whole
@@ -95,7 +95,7 @@ __global__ void __launch_bounds__(Narrow<DUAL, NT>::THREADS, 1)
   if (overlap && !DUAL) pdl_trigger();
 
   if (warp == 0) {
-    // ---------------- TMA producer
+    // ---------------- TMA producer: one thread (the whole warp waits for the kernel in front)
     const bool leader = elect_one();
     const auto load_w = [&](int g, int s) {
       const int kb = first_kb(g), n = blocks_in(g);
@@ -132,34 +132,31 @@ __global__ void __launch_bounds__(Narrow<DUAL, NT>::THREADS, 1)
     __syncwarp();
     if (overlap) pdl_wait();
     if (!overlap || DUAL) pdl_trigger();
-    if (leader)
+    if (leader) {
       for (int g = first; g < pre; g++) load_x(g, g);
-    __syncwarp();
-    int g = pre, s = pre == stages ? 0 : pre;
-    uint32_t ph = 0;   // of the stage's first release
-    for (; g < nst; g++) {
-      if (!tma::warp_wait_bounded(&empty_bar[s], ph, abort_flag, wait_ns)) break;
-      if (leader) {
+      int g = pre, s = pre == stages ? 0 : pre;
+      uint32_t ph = 0;   // of the stage's first release
+      for (; g < nst; g++) {
+        if (!tma::mbar_wait_bounded(&empty_bar[s], ph, abort_flag, wait_ns)) break;
         expect(g, s);
         load_w(g, s);
         load_x(g, s);
+        if (++s == stages) s = 0, ph ^= 1u;
       }
-      if (++s == stages) s = 0, ph ^= 1u;
+      *issued_ctr = g;
     }
-    if (leader) *issued_ctr = g;
   } else if (warp == 1) {
-    // ---------------- issuer
-    const bool leader = elect_one();
-    const uint64_t dw0 = operand_desc(tma::smem_u32(smem)), dx0 = operand_desc(tma::smem_u32(smem) + C::W_BYTES), ds0 = scales_desc(tma::smem_u32(scales));
-    int g = 0, s = 0, pieces = 0;
-    uint32_t ph = 0, sf = tmem_base + C::SCALES;
-    for (; g < nst; g++) {
-      if (!tma::warp_wait_bounded(&full_bar[s], ph, abort_flag, wait_ns)) break;
-      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      const int kb = first_kb(g), n = blocks_in(g);
-      const bool copy = with_scales(g);
-      if (copy) sf = tmem_base + C::SCALES + C::SF_COLS * (pieces++ & 1);
-      if (leader) {
+    if (elect_one()) {
+      // ---------------- issuer: one thread
+      const uint64_t dw0 = operand_desc(tma::smem_u32(smem)), dx0 = operand_desc(tma::smem_u32(smem) + C::W_BYTES), ds0 = scales_desc(tma::smem_u32(scales));
+      int g = 0, s = 0, pieces = 0;
+      uint32_t ph = 0, sf = tmem_base + C::SCALES;
+      for (; g < nst; g++) {
+        if (!tma::mbar_wait_bounded(&full_bar[s], ph, abort_flag, wait_ns)) break;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const int kb = first_kb(g), n = blocks_in(g);
+        const bool copy = with_scales(g);
+        if (copy) sf = tmem_base + C::SCALES + C::SF_COLS * (pieces++ & 1);
         if (copy) {   // in order with the instructions around it
 #pragma unroll
           for (int i = 0; i <= C::WS; i++) copy_scales<1>(sf + 4 * i, ds0 + (uint64_t)((s * C::SCALE_BYTES + i * PIECE) >> 4));
@@ -177,11 +174,10 @@ __global__ void __launch_bounds__(Narrow<DUAL, NT>::THREADS, 1)
           }
         if (g + stages < nst) commit<1>(&empty_bar[s]);   // (nobody waits for the last round's)
         if (g + 1 == nst) commit<1>(tmem_full);
+        if (++s == stages) s = 0, ph ^= 1u;
       }
-      __syncwarp();
-      if (++s == stages) s = 0, ph ^= 1u;
+      *consumed_ctr = g;
     }
-    if (leader) *consumed_ctr = g;
   } else {
     // ---------------- drain: TMEM lane quarter = warp % 4, a feature per thread
     const int quarter = warp & 3, half = (warp - 2) >> 2;   // (eight warps: either half of the tokens)
