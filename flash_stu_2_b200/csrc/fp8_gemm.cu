@@ -49,9 +49,9 @@ struct Out {
 template <bool DUAL, int CTAS, int TN> struct Form {
   static constexpr int MMA_N = DUAL ? 2 * TN : TN;                     // accumulator columns
   static constexpr int B_ROWS = MMA_N / CTAS;                          // rows of B in a CTA's shared memory
-  // k-blocks of a stage: two halve what waiting and sending off take of a pair's stage, a CTA alone has too few stages of them
-  static constexpr int KBS = CTAS == 2 ? 2 : 1;
-  static constexpr int KB_BYTES = A_BYTES + B_ROWS * BK, TILE_BYTES = KBS * KB_BYTES;   // of one CTA
+  // A stage is one k-block.  (Of two, which the producer and the issuer are done with in less time, a pair has room for three, and one of those is on its
+  // way: 8192 x 8192 x 8192 369 us, so 358; 4096 x 6144 x 1536 gate/up 67, so 61.)
+  static constexpr int TILE_BYTES = A_BYTES + B_ROWS * BK;             // of one CTA
   static constexpr int SCALE_BYTES = fp8::PIECE * (1 + (MMA_N + 127) / 128);
   static constexpr int STAGES = (227 * 1024 - 2048 - (DUAL ? 2048 : EPI_WARPS * BLOCK_BYTES)) / (TILE_BYTES + SCALE_BYTES);
   // accumulators at columns 0 and SECOND, scales behind them, twice 16 columns (x at 0, W from 4 on)
@@ -69,7 +69,7 @@ __global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__(64 + 32 * EPI_WAR
                     int K, int tiles_m, int tiles_n, int group_m, Out out, int* status, int drop_first_copy, unsigned long long wait_ns) {
   using F = Form<DUAL, CTAS, TN>;
   constexpr bool PAIR = CTAS == 2;
-  constexpr int MMA_N = F::MMA_N, STAGES = F::STAGES, SHARED = F::SHARED, KBS = F::KBS;
+  constexpr int MMA_N = F::MMA_N, STAGES = F::STAGES, SHARED = F::SHARED;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   unsigned char* scales = smem + STAGES * F::TILE_BYTES;            // [stage]: of x, then of W
@@ -132,38 +132,29 @@ __global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__(64 + 32 * EPI_WAR
         int tm, tn;
         tile_coords(tile, tiles_m, tiles_n, group_m, tm, tn);
         const int m0 = (CTAS * tm + rank) * BM, n0 = tn * TN + (DUAL ? 0 : rank * F::B_ROWS), nb = tn * TN / 128;
-        for (int kb = 0; kb < num_kb; kb += KBS, g++) {
+        for (int kb = 0; kb < num_kb; kb++, g++) {
           if (!ready) ok = tma::mbar_wait_bounded(&empty_bar[s], ph, abort_flag, wait_ns);
           if (!ok) break;
           const int s1 = s + 1 == STAGES ? 0 : s + 1;
           const uint32_t ph1 = s1 ? ph : ph ^ 1u;
           const bool ready1 = mbar_ready(&empty_bar[s1], ph1);   // asked for here, looked at behind the copies
           const bool with_scales = (kb & 3) == 0;
-          const int n = min(KBS, num_kb - kb);
           unsigned char *sa = smem + s * F::TILE_BYTES, *ss = scales + s * F::SCALE_BYTES;
-          if (rank == 0) tma::mbar_expect_tx(&full_bar[s], CTAS * (n * F::KB_BYTES + (with_scales ? F::SCALE_BYTES : 0)));   // of both CTAs
+          if (rank == 0) tma::mbar_expect_tx(&full_bar[s], CTAS * (F::TILE_BYTES + (with_scales ? F::SCALE_BYTES : 0)));   // of both CTAs
           if (!(drop_first_copy && g == 0)) {   // (failure-detection test: the first stage never fills)
             const uint32_t bar = full0 + s * (uint32_t)sizeof(uint64_t);
             if constexpr (PAIR) {
-#pragma unroll
-              for (int j = 0; j < KBS; j++)
-                if (j < n) {
-                  load_2d_pair(sa + j * F::KB_BYTES, &tmA, bar, (kb + j) * BK, m0);
-                  load_2d_pair(sa + j * F::KB_BYTES + A_BYTES, mapB, bar, (kb + j) * BK, n0);
-                }
+              load_2d_pair(sa, &tmA, bar, kb * BK, m0);
+              load_2d_pair(sa + A_BYTES, mapB, bar, kb * BK, n0);
               if (with_scales) {
                 load_3d_pair(ss, &tmSA, bar, 0, kb >> 2, m0 / BM);
                 load_3d_pair(ss + fp8::PIECE, &tmSB, bar, 0, kb >> 2, nb);
                 if (DUAL) load_3d_pair(ss + 2 * fp8::PIECE, &tmSB2, bar, 0, kb >> 2, nb);
               }
             } else {
-#pragma unroll
-              for (int j = 0; j < KBS; j++)
-                if (j < n) {
-                  load_2d(sa + j * F::KB_BYTES, &tmA, &full_bar[s], (kb + j) * BK, m0);
-                  load_2d(sa + j * F::KB_BYTES + A_BYTES, &tmB, &full_bar[s], (kb + j) * BK, n0);
-                  if (DUAL) load_2d(sa + j * F::KB_BYTES + A_BYTES + TN * BK, &tmB2, &full_bar[s], (kb + j) * BK, n0);
-                }
+              load_2d(sa, &tmA, &full_bar[s], kb * BK, m0);
+              load_2d(sa + A_BYTES, &tmB, &full_bar[s], kb * BK, n0);
+              if (DUAL) load_2d(sa + A_BYTES + TN * BK, &tmB2, &full_bar[s], kb * BK, n0);
               if (with_scales) {
                 tma::load_3d(ss, &tmSA, &full_bar[s], 0, kb >> 2, m0 / BM);
                 tma::load_3d(ss + fp8::PIECE, &tmSB, &full_bar[s], 0, kb >> 2, nb);
@@ -194,7 +185,7 @@ __global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__(64 + 32 * EPI_WAR
         ok = tma::mbar_wait_bounded(&tmem_empty[buf], (((uint32_t)it >> 1) & 1u) ^ 1u, abort_flag, wait_ns);
         if (SHARED && ok && it > 0) ok = tma::mbar_wait_bounded(&shared_read[buf ^ 1], ((uint32_t)(it - 1) >> 1) & 1u, abort_flag, wait_ns);
         if (!ok) break;
-        for (int kb = 0; kb < num_kb; kb += KBS, g++) {
+        for (int kb = 0; kb < num_kb; kb++, g++) {
           if (!ready) ok = tma::mbar_wait_bounded(&full_bar[s], ph, abort_flag, wait_ns);
           if (!ok) break;
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -209,13 +200,8 @@ __global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__(64 + 32 * EPI_WAR
           }
           const uint64_t da = da0 + (uint64_t)(s * (F::TILE_BYTES >> 4)), db = db0 + (uint64_t)(s * (F::TILE_BYTES >> 4));
 #pragma unroll
-          for (int j = 0; j < KBS; j++)
-            if (j == 0 || kb + j < num_kb) {
-#pragma unroll
-              for (int kk = 0; kk < BK / 32; kk++)   // 32 bytes along K inside the swizzled row: +2
-                multiply<CTAS, MMA_N>(acc, da + j * (F::KB_BYTES >> 4) + 2 * kk, db + j * (F::KB_BYTES >> 4) + 2 * kk, sf_cols, sf_cols + 4, (kb + j) & 3,
-                                      (kb | j | kk) ? 1u : 0u);
-            }
+          for (int kk = 0; kk < BK / 32; kk++)   // 32 bytes along K inside the swizzled row: +2
+            multiply<CTAS, MMA_N>(acc, da + 2 * kk, db + 2 * kk, sf_cols, sf_cols + 4, kb & 3, (kb | kk) ? 1u : 0u);
           commit<CTAS>(&empty_bar[s]);
           ready = ready1;
           s = s1, ph = ph1;
@@ -534,13 +520,12 @@ int fp8_gemm(const Fp8Product& p, cudaStream_t st) {
   const auto waves = [&](int rows, int cols, int room) {
     return ((long long)((p.M + rows - 1) / rows) * ((p.N + cols - 1) / cols) + room - 1) / room;
   };
-  // Gate/up: a CTA alone on 128 rows where that is fewer rounds than pairs on 256 (us, alone and in pairs: 333 x 6144 x 1536 11.6 and 16.4, 700 18.0 and
-  // 17.0, 1024 24.7 and 22.4, 16384 321 and 266).
+  // Gate/up: a CTA alone on 128 rows where that is fewer rounds than pairs on 256 (us, alone and in pairs: 128 x 18432 x 1536 14.1 and 15.7, 333 x 6144 x 1536
+  // 11.0 and 14.5, 700 16.1 and 14.9, 1024 21.3 and 19.1, 2048 37.6 and 33.3).
   if (p.w2)
-    return waves(128, 128, device_sm_count()) < waves(256, 128, device_clusters<true, 2, 128>()) || p.M <= BM ? launch<true, 1, 128>(p, st)
-                                                                                                              : launch<true, 2, 128>(p, st);
+    return waves(128, 128, device_sm_count()) < waves(256, 128, device_clusters<true, 2, 128>()) ? launch<true, 1, 128>(p, st) : launch<true, 2, 128>(p, st);
   // Plain: tiles of 128 columns where a round of them, about 3/4 of the time of one of 256, makes up for their number (us, 128 and 256 columns:
-  // 1024 x 1536 x 18432 46.7 and 70.8, 1024 x 1536 x 6144 18.7 and 22.0, 2048 x 1536 x 6144 32.8 and 23.4, 8192 x 1536 x 18432 322 and 180).
+  // 1024 x 1536 x 18432 34.7 and 47.3, 1024 x 1536 x 6144 15.2 and 20.2, 2048 x 1536 x 6144 24.4 and 21.9, 1024 x 8192 x 2048 20.2 and 17.9).
   return 3 * waves(256, 128, device_clusters<false, 2, 128>()) < 4 * waves(256, 256, device_clusters<false, 2, 256>()) ? launch<false, 2, 128>(p, st)
                                                                                                                      : launch<false, 2, 256>(p, st);
 }

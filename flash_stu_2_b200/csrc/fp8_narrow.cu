@@ -27,7 +27,7 @@ template <bool DUAL, int NT> struct Narrow {
   static constexpr int DRAIN = NT >= 64 ? 8 : 4, THREADS = 64 + 32 * DRAIN;   // warps that read the sums
   // k-blocks of a stage: waiting for one, announcing its bytes and sending off its copies takes the producer 360 cycles and 27 more per copy, whatever
   // their size, so that single blocks of 16 KB came at 45 bytes a cycle at most (8 x 1536 x 18432 13.7 us, 66 with K whole)
-  static constexpr int KBS = DUAL ? (NT <= 32 ? 2 : 1) : NT <= 32 ? 4 : 2;
+  static constexpr int KBS = DUAL ? 2 : NT <= 32 ? 4 : 2;
   static constexpr int W_BYTES = WS * A_BYTES, X_BYTES = NT * BK, KB_BYTES = W_BYTES + X_BYTES;
   static constexpr int SCALE_BYTES = PIECE * (WS + 1);
   static constexpr int STAGE = KBS * KB_BYTES + SCALE_BYTES;        // (the scales of all stages lie behind the tiles)
@@ -367,26 +367,22 @@ int launch(const Fp8Product& p, cudaStream_t st) {
   return STU_OK;
 }
 
-template <bool DUAL>
-int launch_tokens(const Fp8Product& p, cudaStream_t st) {
-  if (p.M <= 16) return launch<DUAL, 16>(p, st);
-  if (p.M <= 32) return launch<DUAL, 32>(p, st);
-  if (p.M <= 64) return launch<DUAL, 64>(p, st);
-  return launch<DUAL, 128>(p, st);
-}
-
 }  // namespace
 
-// Whether a product takes less time here than on the tiles of fp8_gemm.cu.  Plain: up to 128 tokens always (1536 x 6144, 128 tokens 9.2 and 17.9 us, 64 tokens
-// 7.5 and 16.5), more while K can still be cut (1536 x 6144, 333 tokens 14.1 and 24.9 us, 700 15.5 and 18.0; 1024 x 4096, 512 tokens 9.8 and 13.6).  Gate/up, whose sums
-// are twice as many to bring together: up to 32 tokens (18432 x 1536, 32 tokens 15.8 and 14.6 us, 16 tokens 14.2 and 14.7; 6144 x 1536, 32 tokens 9.8 and 10.4), more
-// where four or more CTAs share K and there is enough of it (64 tokens: 4096 x 1024 8.1 and 8.6, 6144 x 1536, two CTAs, 11.2 and 10.7; 128 tokens:
-// 4096 x 1024, four, 10.9 and 8.9).
+// Whether a product takes less time here than on the tiles of fp8_gemm.cu (us, here and there).  Plain: up to 64 tokens (64: 1024 x 4096 8.2 and 14.3,
+// 18432 x 1536 11.6 and 12.0, 8192 x 2048 9.4 and 8.6).  More: 128 of them take 8 + 0.26 per k-block of a CTA here, one round of tiles there
+// 5.4 + 0.195 per k-block (K over 8 CTAs: 128 x 1024 x 4096 7.9 and 11.3, 128 x 2048 x 1024 7.7 and 6.1; over 4: 512 x 1024 x 4096 9.5 and 11.4, 128 x 4096 x 2048 8.6
+// and 8.5; over 3: 384 x 1536 x 6144 12.2 and 14.6; over 2: 700 x 1536 x 18432 26.4 and 33.5, 700 x 1024 x 4096 12.1 and 11.3, 128 x 8192 x 2048 12.2 and 9.0).
+// Gate/up, whose sums are twice as many to bring together: up to 16 tokens (18432 x 1536 13.8 and 15.1), up to 32 where K is
+// shared (4096 x 1024 7.3 and 7.9, 6144 x 1536 9.8 and 10.0; not: 18432 x 1536 15.4 and 14.6, 12288 x 1024 10.8 and 10.3).
 bool fp8_narrow_takes(const Fp8Product& p) {
-  if (!p.w2) return p.M <= 128 || cluster_size<false, 128>(p) > 1;
-  if (p.M <= 32) return true;
-  if (p.M <= 64) return cluster_size<true, 64>(p) >= 4;
-  return blocks_of(p.K) >= 16 && cluster_size<true, 128>(p) >= 4;
+  if (p.w2) return p.M <= 16 || (p.M <= 32 && cluster_size<true, 32>(p) > 1);
+  if (p.M <= 64) return true;
+  const long long ks = cluster_size<false, 128>(p), num_kb = blocks_of(p.K);
+  return 195 * num_kb * ks > 260 * num_kb + 2600 * ks;
 }
 
-int fp8_narrow(const Fp8Product& p, cudaStream_t st) { return p.w2 ? launch_tokens<true>(p, st) : launch_tokens<false>(p, st); }
+int fp8_narrow(const Fp8Product& p, cudaStream_t st) {
+  if (p.w2) return p.M <= 16 ? launch<true, 16>(p, st) : launch<true, 32>(p, st);
+  return p.M <= 16 ? launch<false, 16>(p, st) : p.M <= 32 ? launch<false, 32>(p, st) : p.M <= 64 ? launch<false, 64>(p, st) : launch<false, 128>(p, st);
+}

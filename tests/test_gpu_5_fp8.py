@@ -542,3 +542,57 @@ def test_equal_rows_give_equal_rows(cols):
         norms.append((n.data.view(torch.uint8)[:1], n.block_scales()[:1]))
     for found in (norms, quantised):
         assert all(torch.equal(d, found[0][0]) and torch.equal(s, found[0][1]) for d, s in found)
+
+
+# up to 64 tokens, and more whose K is long enough to be cut: the forms that have the weights as the 128-row operand, at the edges of their tiles and clusters
+CUT = [(17, 300, 2000), (48, 1111, 1536), (64, 257, 4000), (65, 300, 2100), (96, 1, 2177), (128, 128, 2304), (129, 520, 2560), (200, 257, 4096), (300, 520, 2305),
+       (384, 1000, 2400), (500, 1100, 9000), (64, 20000, 200)]
+
+
+@pytest.mark.parametrize("resid", [False, True])
+@pytest.mark.parametrize("M,N,K", CUT)
+def test_linear_whose_K_is_cut(M, N, K, resid):
+    from flash_stu_2_b200 import ops
+    g = gen(M + N + K)
+    x, w = rows8(g, M, K), weights8(g, N, K)
+    big = torch.full((M + 2, N + 9), 5.0, device=dev(), dtype=torch.bfloat16)
+    out = big[1:M + 1, 4:4 + N]
+    r = stream(g, M, N, torch.bfloat16) if resid else None
+    ops.linear_fp8(x, w, resid=r, out=out)
+    check_linear(out, x, w, r)
+    assert torch.equal(ops.linear_fp8(x, w, resid=r, overlap=True), out)
+    big[1:M + 1, 4:4 + N] = 5.0
+    assert bool((big == 5).all())
+    ops.check_status()
+
+
+@pytest.mark.parametrize("M,N,K", [(16, 300, 700), (17, 700, 1111), (32, 2000, 300), (32, 18400, 256), (33, 300, 700), (128, 18400, 200)])
+def test_gate_of_few_tokens(M, N, K):
+    from flash_stu_2_b200 import ops
+    g = gen(M + N + K)
+    x, w, w2 = rows8(g, M, K), weights8(g, N, K), weights8(g, N, K)
+    h = ops.linear_fp8(x, w, W2=w2)
+    R.check_rows(h, *R.gate(x, w, w2))
+    assert same_rows(ops.linear_fp8(x, w, W2=w2, overlap=True), h)
+    ops.check_status()
+
+
+@pytest.mark.parametrize("M,K,two", [(5, 700, False), (5, 700, True), (30, 2100, False), (30, 2100, True), (50, 2100, False), (100, 2100, False)])
+def test_a_wait_that_runs_out_where_K_is_cut(M, K, two):
+    from flash_stu_2_b200 import _lib, ops
+    lib, g = _lib.load(), gen(M)
+    x, w, w2 = rows8(g, M, K), weights8(g, 400, K), weights8(g, 400, K)
+    call = (lambda: ops.linear_fp8(x, w, W2=w2)) if two else (lambda: ops.linear_fp8(x, w))
+    same = same_rows if two else torch.equal
+    want = call()
+    ops.check_status()
+    assert lib.stu_test_inject_wait_expiry(100) == 0
+    try:
+        call()
+        torch.cuda.synchronize()
+        with pytest.raises(RuntimeError, match="status 3"):
+            ops.check_status()
+    finally:
+        assert lib.stu_test_inject_wait_expiry(0) == 0
+    assert same(call(), want)
+    ops.check_status()
