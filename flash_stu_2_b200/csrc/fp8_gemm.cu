@@ -214,11 +214,39 @@ __global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__(64 + 32 * EPI_WAR
     // ---------------- epilogue warps: TMEM lane quarter = warp % 4 (32 rows), half of the columns
     const int quarter = warp & 3, half = (warp - 2) >> 2;
     const uint32_t hand_back = in_first_cta(tmem_empty), hand_shared = in_first_cta(shared_read);
+    const bool on_grid = !((out.ldy & 7) || (reinterpret_cast<uintptr_t>(out.y) & 15)) &&
+                         !(out.resid && ((out.ldr & 7) || (reinterpret_cast<uintptr_t>(out.resid) & 15)));
     int it = 0;
     for (int tile = pair; tile < num_tiles; tile += pairs, it++) {
       int tm, tn;
       tile_coords(tile, tiles_m, tiles_n, group_m, tm, tn);
       const int m0 = (CTAS * tm + rank) * BM, first = m0 + quarter * 32, buf = it & 1;
+      // plain: a half's columns, 64 of every 128, in SUBS blocks of 32; a block's residuals (four vectors, or 32 rows' values of a column), asked for ahead of its
+      // sums (3000 x 1111 x 1000 off the 16-byte grid, behind them and with loads and stores in turn 25.3 us, so 17.2; on it 700 rows 10.1, so 9.2)
+      constexpr int SUBS = TN / 64;
+      const int rows = min(32, M - first);   // this warp's
+      const int piece = lane & 3, r0 = lane >> 2;   // 64 bytes of a row by 4 lanes, 8 rows at a time
+      const auto column = [&](int i) {
+        const int sub = buf ? i : SUBS - 1 - i;
+        return 128 * (sub >> 1) + 64 * half + 32 * (sub & 1);
+      };
+      uint32_t v[32];
+      const auto ask = [&](int i) {
+        const int n = tn * TN + column(i);
+        if (on_grid && n + 32 <= N) {
+          const bf16* rc = out.resid + (size_t)(first + r0) * out.ldr + n + piece * 8;
+#pragma unroll
+          for (int j = 0; j < 4; j++) {
+            const uint4 u = r0 + 8 * j < rows ? *reinterpret_cast<const uint4*>(rc + (size_t)(8 * j) * out.ldr) : make_uint4(0, 0, 0, 0);
+            v[4 * j] = u.x, v[4 * j + 1] = u.y, v[4 * j + 2] = u.z, v[4 * j + 3] = u.w;
+          }
+        } else {
+          const uint16_t* rc = reinterpret_cast<const uint16_t*>(out.resid) + (size_t)first * out.ldr + n + lane;
+#pragma unroll
+          for (int j = 0; j < 32; j++) v[j] = n + lane < N && j < rows ? rc[(size_t)j * out.ldr] : 0u;
+        }
+      };
+      if (!DUAL && out.resid) ask(0);
       bool ok = tma::warp_wait_bounded(&tmem_full[buf], ((uint32_t)it >> 1) & 1u, abort_flag, wait_ns);
       const uint32_t acc = tmem_base + (uint32_t)buf * F::SECOND + ((uint32_t)(quarter * 32) << 16);
       const bool shares = SHARED && half == (buf ^ 1);   // the first accumulator's last columns, the second one's first
@@ -304,67 +332,60 @@ __global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__(64 + 32 * EPI_WAR
         if (!ok) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         bf16* st = reinterpret_cast<bf16*>(blocks + (warp - 2) * BLOCK_BYTES);
-        auto at = [&](int row, int piece) { return st + row * 32 + ((piece ^ ((row >> 1) & 3)) << 3); };   // 8 values, 16 bytes
-        const bool on_grid = !((out.ldy & 7) || (reinterpret_cast<uintptr_t>(out.y) & 15)) &&
-                             !(out.resid && ((out.ldr & 7) || (reinterpret_cast<uintptr_t>(out.resid) & 15)));
-        const int rows = min(32, M - first);   // this warp's
-        constexpr int SUBS = TN / 64;          // blocks of this half's columns, 64 of every 128
+        auto at = [&](int row, int p) { return st + row * 32 + ((p ^ ((row >> 1) & 3)) << 3); };   // 8 values, 16 bytes
 #pragma unroll 1
         for (int i = 0; i < SUBS; i++) {
-          const int sub = buf ? i : SUBS - 1 - i, c = 128 * (sub >> 1) + 64 * half + 32 * (sub & 1), n = tn * TN + c;
+          const int c = column(i), n = tn * TN + c;
           uint32_t r[32];
           tmem_ld32(acc + c, r);
           asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
           shared_done(i);
           if (i == SUBS - 1) all_done();
-          if (n >= N || rows <= 0) continue;
+          if (n < N && rows > 0) {
 #pragma unroll
-          for (int p = 0; p < 4; p++) {
-            float o[8];
+            for (int p = 0; p < 4; p++) {
+              float o[8];
 #pragma unroll
-            for (int j = 0; j < 8; j++) o[j] = __uint_as_float(r[p * 8 + j]);
-            store_vec(at(lane, p), o);
-          }
-          __syncwarp();
-          // 64 bytes of a row by 4 lanes, 8 rows at a time
-          const int piece = lane & 3, r0 = lane >> 2, np = n + piece * 8;
-          if (on_grid && n + 32 <= N) {
-            bf16* yc = out.y + (size_t)(first + r0) * out.ldy + np;
-            uint4 v[4];
-            if (out.resid) {
-              const bf16* rc = out.resid + (size_t)(first + r0) * out.ldr + np;
-#pragma unroll
-              for (int j = 0; j < 4; j++)
-                v[j] = r0 + 8 * j < rows ? *reinterpret_cast<const uint4*>(rc + (size_t)(8 * j) * out.ldr) : make_uint4(0, 0, 0, 0);
+              for (int j = 0; j < 8; j++) o[j] = __uint_as_float(r[p * 8 + j]);
+              store_vec(at(lane, p), o);
             }
+            __syncwarp();
+            // (what is read of the block is read ahead of the first store: that might be to it, for all that the compiler knows)
+            if (on_grid && n + 32 <= N) {
+              bf16* yc = out.y + (size_t)(first + r0) * out.ldy + n + piece * 8;
+              uint4 mine[4];
 #pragma unroll
-            for (int j = 0; j < 4; j++)
-              if (r0 + 8 * j < rows) {
-                const uint4 mine = *reinterpret_cast<const uint4*>(at(r0 + 8 * j, piece));
-                if (out.resid) {
+              for (int j = 0; j < 4; j++) mine[j] = *reinterpret_cast<const uint4*>(at(r0 + 8 * j, piece));
+              if (out.resid) {
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
                   float o[8], s[8];
-                  load_vec(reinterpret_cast<const bf16*>(&mine), o);
-                  load_vec(reinterpret_cast<const bf16*>(&v[j]), s);
+                  load_vec(reinterpret_cast<const bf16*>(&mine[j]), o);
+                  load_vec(reinterpret_cast<const bf16*>(&v[4 * j]), s);
 #pragma unroll
                   for (int e = 0; e < 8; e++) o[e] += s[e];
-                  store_vec(yc + (size_t)(8 * j) * out.ldy, o);
-                } else {
-                  *reinterpret_cast<uint4*>(yc + (size_t)(8 * j) * out.ldy) = mine;
+                  store_vec(reinterpret_cast<bf16*>(&mine[j]), o);
                 }
               }
-          } else if (n + lane < N) {   // off the 16-byte grid, or the last columns: single values, side by side, 16 rows' residuals ahead of their use
-#pragma unroll 1
-            for (int j0 = 0; j0 < rows; j0 += 16) {
-              bf16* yc = out.y + (size_t)(first + j0) * out.ldy + n + lane;
-              float v[16];
 #pragma unroll
-              for (int j = 0; j < 16; j++)
-                v[j] = out.resid && j0 + j < rows ? __bfloat162float(out.resid[(size_t)(first + j0 + j) * out.ldr + n + lane]) : -0.f;   // (adds nothing to any value)
+              for (int j = 0; j < 4; j++)
+                if (r0 + 8 * j < rows) *reinterpret_cast<uint4*>(yc + (size_t)(8 * j) * out.ldy) = mine[j];
+            } else {   // off the 16-byte grid, or the last columns: single values, side by side
+              uint16_t* yc = reinterpret_cast<uint16_t*>(out.y) + (size_t)first * out.ldy + n + lane;
+              uint16_t mine[32];
 #pragma unroll
-              for (int j = 0; j < 16; j++)
-                if (j0 + j < rows) yc[(size_t)j * out.ldy] = __float2bfloat16_rn(__bfloat162float(at(j0 + j, lane >> 3)[lane & 7]) + v[j]);
+              for (int j = 0; j < 32; j++) mine[j] = reinterpret_cast<const uint16_t*>(at(j, lane >> 3))[lane & 7];
+              if (out.resid) {
+#pragma unroll
+                for (int j = 0; j < 32; j++)
+                  mine[j] = __bfloat16_as_ushort(__float2bfloat16_rn(__uint_as_float((uint32_t)mine[j] << 16) + __uint_as_float(v[j] << 16)));
+              }
+#pragma unroll
+              for (int j = 0; j < 32; j++)
+                if (n + lane < N && j < rows) yc[(size_t)j * out.ldy] = mine[j];
             }
           }
+          if (out.resid && i + 1 < SUBS) ask(i + 1);
           __syncwarp();   // the block has been read
         }
       }
