@@ -18,6 +18,7 @@
 //
 // Every wait is bounded, as in gemm_tc.cu: on expiry the waiter tells the others, raises the status word, and the CTAs drain their copies, free
 // their tensor memory and return.
+#include <memory>
 #include <new>
 
 #include "fp8_gemm.cuh"
@@ -427,7 +428,7 @@ __global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__(64 + 32 * EPI_WAR
 }
 
 // ---------------------------------------------------------------------------------------------- host
-// Tensor maps are an address and a shape: kept per thread (encoding one takes a microsecond, a launch needs up to six).
+// Tensor maps are an address and a shape, whatever lies there: kept per thread (encoding one takes a microsecond, a launch needs up to six).
 struct MapKey {
   const void* base;
   long long rows, cols;
@@ -463,8 +464,8 @@ int encode(CUtensorMap* map, const MapKey& k) {
 }  // namespace
 
 int fp8_tensor_map(CUtensorMap* map, const void* base, long long rows, long long cols, int box) {
-  static thread_local MapSlot* table = nullptr;
-  if (!table) table = new (std::nothrow) MapSlot[MAP_SLOTS]();
+  static thread_local std::unique_ptr<MapSlot[]> table;
+  if (!table) table.reset(new (std::nothrow) MapSlot[MAP_SLOTS]());
   const MapKey key{base, rows, cols, box};
   if (!table) return encode(map, key);
   const unsigned long long h = (unsigned long long)(uintptr_t)base * 0x9E3779B97F4A7C15ull + (unsigned long long)rows * 0xC2B2AE3D27D4EB4Full +

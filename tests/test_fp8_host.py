@@ -232,3 +232,14 @@ def test_a_weight_at_the_address_of_one_that_is_gone(tmp_path, monkeypatch):
     import gc
     gc.collect()
     assert gone() is None
+
+
+def test_the_device_that_is_launched_on(monkeypatch):
+    from types import SimpleNamespace
+    from flash_stu_2_b200 import ops
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 0, raising=False)
+    on = lambda i: SimpleNamespace(device=torch.device("cuda", i))
+    assert ops._elsewhere(on(0), None, on(0)) is None
+    assert ops._elsewhere(on(1), None, on(1)) == torch.device("cuda", 1)
+    with pytest.raises(RuntimeError, match="several devices"):
+        ops._elsewhere(on(0), on(1))

@@ -596,3 +596,49 @@ def test_a_wait_that_runs_out_where_K_is_cut(M, K, two):
         assert lib.stu_test_inject_wait_expiry(0) == 0
     assert same(call(), want)
     ops.check_status()
+
+
+@pytest.mark.parametrize("M", [3, 200])
+def test_the_librarys_calls(M):
+    """The three calls by addresses, as a host of another kind makes them."""
+    from flash_stu_2_b200 import _lib, ops
+    lib, g, d, inter, eps = _lib.load(), gen(M), 520, 1100, 1e-5
+    stream = torch.cuda.current_stream().cuda_stream
+    gate, up, down = (torch.randn(*s, device=dev(), generator=g) * s[1] ** -0.5 for s in ((inter, d), (inter, d), (d, inter)))
+    x, branch = (torch.randn(M, d, device=dev(), generator=g).bfloat16() for _ in range(2))
+    norm = torch.ones(d, device=dev(), dtype=torch.bfloat16)
+
+    def rows8(n, cols):
+        return (torch.empty(n, -(-cols // 128) * 128, dtype=torch.float8_e4m3fn, device=dev()),
+                torch.empty(-(-n // 128), -(-cols // 512), 32, 4, 4, dtype=torch.float8_e8m0fnu, device=dev()))
+
+    p = lambda r: (r[0].data_ptr(), r[1].data_ptr())
+    weights = []
+    for w in (gate, up, down):
+        weights.append(rows8(*w.shape))
+        assert lib.stu_quantize_fp8(w.data_ptr(), *p(weights[-1]), w.shape[0], w.shape[1], w.stride(0), 0, stream) == 0
+    q = [ops.quantize_fp8(w) for w in (gate, up, down)]
+    assert all(same_rows(ops.Fp8Rows(*a, b.cols), b) for a, b in zip(weights, q))
+    want = x.clone()
+    ops.linear_fp8(ops.linear_fp8(ops.rmsnorm_fp8(want, norm, eps, add=branch), q[0], W2=q[1]), q[2], resid=want, out=want)
+    xn, h = rows8(M, d), rows8(M, inter)
+    assert lib.stu_rmsnorm_fp8(x.data_ptr(), branch.data_ptr(), norm.data_ptr(), x.data_ptr(), *p(xn), M, d, d, d, d, eps, 1, stream) == 0
+    assert lib.stu_linear_fp8(*p(xn), *p(weights[0]), *p(weights[1]), None, 0, h[0].data_ptr(), 0, h[1].data_ptr(), M, inter, d, 0, stream) == 0
+    assert lib.stu_linear_fp8(*p(h), *p(weights[2]), None, None, x.data_ptr(), d, x.data_ptr(), d, None, M, d, inter, 0, stream) == 0
+    assert torch.equal(x, want)
+    ops.check_status()
+
+
+def test_two_devices_at_once_are_refused():
+    """Operands on several devices have no kernel; one of them alone is launched where it lies, whichever device is current."""
+    from flash_stu_2_b200 import ops
+    if torch.cuda.device_count() < 2:
+        pytest.skip("needs two CUDA devices")
+    g = gen(0)
+    x, w = rows8(g, 4, 256), weights8(g, 8, 256)
+    want = ops.linear_fp8(x, w)
+    there = ops.Fp8Rows(w.data.to("cuda:1"), w.scales.to("cuda:1"), 256)
+    with pytest.raises(RuntimeError, match="several devices"):
+        ops.linear_fp8(x, there)
+    with torch.cuda.device(1):
+        assert torch.equal(ops.linear_fp8(x, w), want)
