@@ -2,12 +2,13 @@
 // thread-block cluster so that a few thousand features occupy all SMs.  What bounds it: HBM, the weights once; for small weights the time
 // from a launch over the first bytes and the cluster's meeting to the last store.
 //
-// A thread of warp 0 of a CTA brings 128 features (gate/up: 128 of both), NT tokens and their scales by TMA into a ring, one of warp 1 copies the scales into tensor memory
-// and issues kind::mxf8f6f4 (see fp8_gemm.cu), the others drain the sums into shared memory, where the ring was.  Then every CTA of the cluster takes
-// its share of the tokens: a warp adds up a token's 128 features over the cluster, in the order of K, and stores them (sums sent to the CTA that adds them up by
-// bulk copies, with no barrier of the cluster ahead of or behind them, came later: 1 x 1024 x 4096 5.2 us, so 4.7); gate/up: one warp has the whole
-// block of h and settles its scale by a reduction.  (On mma.sync the conversions to halves and the fragments of tokens took 370 instructions for 2 KB of
-// weights, more than an SM issues in the time that they take to arrive: 18432 x 1536 gate/up of 8 tokens 25.5 us.)
+// A thread of warp 0 of a CTA brings 128 features (gate/up: 128 of both), NT tokens and their scales by TMA into a ring, one of warp 1 copies the scales into tensor
+// memory and issues kind::mxf8f6f4 (see fp8_gemm.cu), the others drain the sums and send each to the CTA of the cluster whose share its token is in, where it
+// counts towards a barrier.  A warp there adds up a token's 128 features over the cluster, in the order of K, and stores them; gate/up: one warp has the whole
+// block of h and settles its scale by a reduction.  The cluster meets once, behind the set-up and unnoticed; a CTA alone passes its sums on in shared memory.  (Sums left in shared memory and fetched between two meetings of the cluster
+// took 700 and 600 ns for those and 1000 for the rest: 1 x 1024 x 4096 4.7 us, so 3.8; gate/up 1 x 4096 x 1024 5.8, so 5.1; 128 x 1536 x 6144 9.2, so 8.6; but 333 tokens, whose
+// sends are many, 12.1, so 12.3.  Sent by bulk copies of staged rows 5.2.)  On mma.sync the conversions to halves and the fragments of tokens took 370 instructions for 2 KB of
+// weights, more than an SM issues in the time that they take to arrive: 18432 x 1536 gate/up of 8 tokens 25.5 us.
 #include <cooperative_groups.h>
 
 #include "fp8_gemm.cuh"
@@ -27,22 +28,38 @@ template <bool DUAL, int NT> struct Narrow {
   static constexpr int DRAIN = NT >= 64 ? 8 : 4, THREADS = 64 + 32 * DRAIN;   // warps that read the sums
   // k-blocks of a stage: waiting for one, announcing its bytes and sending off its copies takes the producer 360 cycles and 27 more per copy, whatever
   // their size, so that single blocks of 16 KB came at 45 bytes a cycle at most (8 x 1536 x 18432 13.7 us, 66 with K whole)
-  static constexpr int KBS = DUAL ? 2 : NT <= 32 ? 4 : 2;
+  static constexpr int KBS = DUAL ? 2 : NT <= 32 ? 4 : NT <= 64 ? 2 : 1;
   static constexpr int W_BYTES = WS * A_BYTES, X_BYTES = NT * BK, KB_BYTES = W_BYTES + X_BYTES;
   static constexpr int SCALE_BYTES = PIECE * (WS + 1);
   static constexpr int STAGE = KBS * KB_BYTES + SCALE_BYTES;        // (the scales of all stages lie behind the tiles)
   static constexpr int ROWS = WS * 128;                             // sums of a token
-  static constexpr int SUM_BYTES = NT * ROWS * 4;
+  static constexpr int SUM_BYTES = (NT + MAX_KS) * ROWS * 4;        // room for a CTA's share of the tokens, from each of the cluster
   static constexpr int SF_COLS = 4 * (WS + 1), SCALES = WS * NT;    // tensor memory: sums, then twice the scales
   static constexpr uint32_t TMEM_COLS = SCALES + 2 * SF_COLS <= 64 ? 64 : SCALES + 2 * SF_COLS <= 128 ? 128 : SCALES + 2 * SF_COLS <= 256 ? 256 : 512;
 };
-constexpr int TAIL = (2 * MAX_STAGES + 1) * 8 + 32;                 // barriers, tensor memory's address, marks
-template <bool DUAL, int NT> constexpr size_t smem_bytes(int stages) {
-  const size_t ring = (size_t)stages * Narrow<DUAL, NT>::STAGE;
-  return 1024 + (ring > (size_t)Narrow<DUAL, NT>::SUM_BYTES ? ring : (size_t)Narrow<DUAL, NT>::SUM_BYTES) + TAIL;
+constexpr int TAIL = (2 * MAX_STAGES + 2) * 8 + 32;                 // barriers, tensor memory's address, marks
+// Sums of a cluster come while a CTA's ring may still be in use: they have memory of their own.  A CTA by itself puts them where its ring was, so that two fit an SM.
+template <bool DUAL, int NT> __host__ __device__ constexpr int before_tail(int stages, int ks) {
+  const int ring = stages * Narrow<DUAL, NT>::STAGE, sums = Narrow<DUAL, NT>::SUM_BYTES;
+  return ks > 1 ? ring + sums : ring > sums ? ring : sums;
+}
+template <bool DUAL, int NT> constexpr size_t smem_bytes(int stages, int ks) {
+  return 1024 + (size_t)before_tail<DUAL, NT>(stages, ks) + TAIL;
 }
 
-template <bool DUAL, int NT>
+// A value to CTA `to` of the cluster, where it counts towards what the barrier expects.
+__device__ __forceinline__ void send(uint32_t addr, uint32_t bar, int to, uint32_t v) {
+  asm volatile("{\n\t.reg .b32 a, b;\n\tmapa.shared::cluster.u32 a, %0, %2;\n\tmapa.shared::cluster.u32 b, %1, %2;\n\t"
+               "st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.b32 [a], %3, [b];\n\t}"
+               ::"r"(addr), "r"(bar), "r"(to), "r"(v) : "memory");
+}
+// Behind a wait for the barrier: what other CTAs stored before they arrived is seen.
+__device__ __forceinline__ void acquire_cluster(uint64_t* bar) {
+  asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.acquire.cluster.shared::cta.b64 p, [%0], 0;\n\t}" ::"r"(tma::smem_u32(bar)) : "memory");
+}
+
+// ALONE: K is not cut.
+template <bool DUAL, int NT, bool ALONE>
 __global__ void __launch_bounds__(Narrow<DUAL, NT>::THREADS, 1)
     fp8_narrow_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmW2, const __grid_constant__ CUtensorMap tmX,
                       const __grid_constant__ CUtensorMap tmSW, const __grid_constant__ CUtensorMap tmSW2, const __grid_constant__ CUtensorMap tmSX,
@@ -53,19 +70,21 @@ __global__ void __launch_bounds__(Narrow<DUAL, NT>::THREADS, 1)
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   constexpr int TILES = C::KBS * C::KB_BYTES, KBS = C::KBS, THREADS = C::THREADS;
   unsigned char* scales = smem + stages * TILES;
-  float* sums = reinterpret_cast<float*>(smem);   // [token][feature], gate/up: 128 gate, 128 up; once the ring is done with
-  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + max(stages * C::STAGE, C::SUM_BYTES));
+  cg::cluster_group cluster = cg::this_cluster();
+  const int ks = ALONE ? 1 : cluster.num_blocks(), rank = ALONE ? 0 : cluster.block_rank();
+  float* sums = reinterpret_cast<float*>(smem + (ALONE ? 0 : stages * C::STAGE));   // [this CTA's tokens][CTA that they come from][feature], gate/up: 128 gate, 128 up
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + before_tail<DUAL, NT>(stages, ks));
   uint64_t* empty_bar = full_bar + MAX_STAGES;
   uint64_t* tmem_full = empty_bar + MAX_STAGES;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tmem_full + 1);
+  uint64_t* received = tmem_full + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(received + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* issued_ctr = reinterpret_cast<int*>(tmem_slot + 2);
   int* consumed_ctr = issued_ctr + 1;
 
-  cg::cluster_group cluster = cg::this_cluster();
-  const int ks = cluster.num_blocks(), rank = cluster.block_rank();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int nb = blockIdx.x, t0 = blockIdx.z * NT, num_kb = blocks_of(K), last = min(NT, M - t0);   // tokens of this tile
+  const int owned = max(last - rank + ks - 1, 0) / ks;   // of these tokens, every ks-th is this CTA's to add up
   // this CTA's k-blocks, in stages that begin at multiples of KBS: none reaches over a group of four, whose scales are a piece
   const int kb0 = (int)((long long)num_kb * rank / ks), kb_end = (int)((long long)num_kb * (rank + 1) / ks), st0 = kb0 / KBS;
   const int nst = kb_end > kb0 ? (kb_end - 1) / KBS - st0 + 1 : 0;
@@ -79,9 +98,11 @@ __global__ void __launch_bounds__(Narrow<DUAL, NT>::THREADS, 1)
       tma::mbar_init(&empty_bar[s], 1);
     }
     tma::mbar_init(tmem_full, 1);
+    tma::mbar_init(received, 1);
     *abort_flag = 0;
     *issued_ctr = *consumed_ctr = 0;
     tma::fence_barrier_init();
+    tma::mbar_expect_tx(received, ALONE ? 0 : owned * ks * C::ROWS * 4);
   }
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tma::smem_u32(tmem_slot)), "r"(C::TMEM_COLS));
@@ -91,6 +112,7 @@ __global__ void __launch_bounds__(Narrow<DUAL, NT>::THREADS, 1)
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem_base = *tmem_slot;
+  if (!ALONE) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");   // sums may come
   // (when the next kernel may start: epilogue.cuh, PdlTrigger)
   if (overlap && !DUAL) pdl_trigger();
 
@@ -181,8 +203,11 @@ __global__ void __launch_bounds__(Narrow<DUAL, NT>::THREADS, 1)
   } else {
     // ---------------- drain: TMEM lane quarter = warp % 4, a feature per thread
     const int quarter = warp & 3, half = (warp - 2) >> 2;   // (eight warps: either half of the tokens)
-    const bool ok = nst > 0 && tma::warp_wait_bounded(tmem_full, 0, abort_flag, wait_ns);
+    if (!ALONE) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    const bool ok = nst > 0 && tma::warp_wait_bounded(tmem_full, 0, abort_flag, wait_ns);   // (else zeros: the others count on them)
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    float* mine = sums + rank * C::ROWS + quarter * 32 + lane;
+    const uint32_t to = tma::smem_u32(mine), bar = tma::smem_u32(received);
 #pragma unroll 1
     for (int i = 0; i < C::WS; i++)
 #pragma unroll 1
@@ -194,19 +219,41 @@ __global__ void __launch_bounds__(Narrow<DUAL, NT>::THREADS, 1)
           tmem_ld32(tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(i * NT + c0), r);
           asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
         }
+        if constexpr (ALONE) {
 #pragma unroll
-        for (int c = 0; c < (NT < 32 ? NT : 32); c++)
-          if (c0 + c < last) sums[(c0 + c) * C::ROWS + i * 128 + quarter * 32 + lane] = __uint_as_float(r[c]);
+          for (int c = 0; c < (NT < 32 ? NT : 32); c++)
+            if (c0 + c < last) mine[(c0 + c) * C::ROWS + i * 128] = __uint_as_float(r[c]);
+        } else {
+          int owner = c0 % ks, at = c0 / ks;
+#pragma unroll
+          for (int c = 0; c < (NT < 32 ? NT : 32); c++)
+            if (c0 + c < last) {
+              send(to + (uint32_t)(at * ks * C::ROWS + i * 128) * 4, bar, owner, r[c]);
+              if (++owner == ks) owner = 0, at++;
+            }
+        }
       }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   }
   __syncwarp();
-  __syncthreads();
-  if (ks > 1) cluster.sync();
-  // ---------------- the cluster's sums: a warp per token, four features per lane
-  pdl_wait();   // (returns at once: the producer has waited; the residual rows are read behind it)
+  if (!ALONE && warp < 2) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  pdl_wait();   // (returns at once: the producer has waited; outputs and residual rows are touched behind it)
   const int hblocks = blocks_of(N), hgroups = groups_of(N);
-  for (int t = rank + ks * warp; t < last; t += ks * (THREADS / 32)) {
+  if (DUAL && rank == 0) {   // byte 0 for the rows that fill up the last 128 and for the blocks that fill up the last four
+    const int end = nb == hblocks - 1 ? hgroups * 4 : nb + 1, bottom = min(t0 + NT, M) == M ? (M + 127) & ~127 : t0 + NT;
+    for (int m = t0 + threadIdx.x; m < bottom; m += THREADS)
+      for (int kb = m < M ? nb + 1 : nb; kb < end; kb++) hs[scale_word(m, kb >> 2, hgroups) + (kb & 3)] = 0;
+  }
+  // ---------------- this CTA's share of the cluster's sums: a warp per token, four features per lane
+  bool all = true;
+  if constexpr (!ALONE) {
+    all = tma::warp_wait_bounded(received, 0, abort_flag, 4 * wait_ns);   // (the others send by the end of their own waits)
+    acquire_cluster(received);
+  } else {
+    __syncthreads();
+  }
+  for (int own = warp; all && own < owned; own += THREADS / 32) {
+    const int t = rank + ks * own;
     float v[C::WS][4];
 #pragma unroll
     for (int i = 0; i < C::WS; i++)
@@ -214,7 +261,7 @@ __global__ void __launch_bounds__(Narrow<DUAL, NT>::THREADS, 1)
       for (int j = 0; j < 4; j++) v[i][j] = 0.f;
 #pragma unroll 4
     for (int r = 0; r < ks; r++) {
-      const float* from = cluster.map_shared_rank(sums, r) + t * C::ROWS + 4 * lane;
+      const float* from = sums + (own * ks + r) * C::ROWS + 4 * lane;
 #pragma unroll
       for (int i = 0; i < C::WS; i++) {
         const float4 a = *reinterpret_cast<const float4*>(from + i * 128);
@@ -254,24 +301,21 @@ __global__ void __launch_bounds__(Narrow<DUAL, NT>::THREADS, 1)
       }
     }
   }
-  if (DUAL && rank == 0) {   // byte 0 for the rows that fill up the last 128 and for the blocks that fill up the last four
-    const int end = nb == hblocks - 1 ? hgroups * 4 : nb + 1, bottom = min(t0 + NT, M) == M ? (M + 127) & ~127 : t0 + NT;
-    for (int m = t0 + threadIdx.x; m < bottom; m += THREADS)
-      for (int kb = m < M ? nb + 1 : nb; kb < end; kb++) hs[scale_word(m, kb >> 2, hgroups) + (kb & 3)] = 0;
-  }
-  if (ks > 1) cluster.sync();   // the others have read this CTA's sums
-  else __syncthreads();
+  __syncthreads();
   if (*abort_flag) {
-    // A wait ran out: report it, and let copies that were issued but never consumed land (bounded) before shared memory is released.
+    // A wait ran out: report it, and let copies that were issued but never consumed, and the others' sums, land (bounded) before shared memory is released.
+    if (!ALONE) cluster.sync();   // (with those that gave up; who has left counts as here)
     if (threadIdx.x == 0) {
       if (status) atomicExch(status, 3);
       const uint64_t start = tma::global_ns();
-      for (int g = *consumed_ctr; g < *issued_ctr; g++) {
+      const auto land = [&](uint64_t* bar, uint32_t parity) {
         for (uint32_t w = 0; w < WAIT_LIMIT; ++w) {
-          if (tma::mbar_try_wait(&full_bar[g % stages], (uint32_t)(g / stages) & 1u)) break;
+          if (tma::mbar_try_wait(bar, parity)) break;
           if ((w & 255u) == 255u && tma::global_ns() - start > wait_ns) break;
         }
-      }
+      };
+      land(received, 0);
+      for (int g = *consumed_ctr; g < *issued_ctr; g++) land(&full_bar[g % stages], (uint32_t)(g / stages) & 1u);
     }
     __syncthreads();
   }
@@ -282,7 +326,7 @@ __global__ void __launch_bounds__(Narrow<DUAL, NT>::THREADS, 1)
   }
 }
 
-template <bool DUAL, int NT>
+template <bool DUAL, int NT, bool ALONE>
 cudaError_t configure(cudaLaunchConfig_t& cfg, cudaLaunchAttribute* at, dim3 grid, size_t smem) {
   cfg = {};
   cfg.gridDim = grid;
@@ -294,11 +338,11 @@ cudaError_t configure(cudaLaunchConfig_t& cfg, cudaLaunchAttribute* at, dim3 gri
   cfg.attrs = at;
   cfg.numAttrs = 1;
   static SmemLimit limit;
-  return allow_smem((const void*)fp8_narrow_kernel<DUAL, NT>, smem, limit);
+  return allow_smem((const void*)fp8_narrow_kernel<DUAL, NT, ALONE>, smem, limit);
 }
-template <bool DUAL, int NT> constexpr int deepest() {
+template <bool DUAL, int NT> constexpr int deepest(int ks) {
   int stages = MAX_STAGES;
-  while (stages > 2 && smem_bytes<DUAL, NT>(stages) > 227 * 1024) stages--;
+  while (stages > 2 && smem_bytes<DUAL, NT>(stages, ks) > 227 * 1024) stages--;
   return stages;
 }
 
@@ -310,16 +354,16 @@ template <bool DUAL, int NT> int cluster_room(int ks) {
   if ((n = found[dev][ks].load(std::memory_order_relaxed)) != 0) return n;
   cudaLaunchConfig_t cfg;
   cudaLaunchAttribute at[1];
-  if (configure<DUAL, NT>(cfg, at, dim3(1024, ks), smem_bytes<DUAL, NT>(deepest<DUAL, NT>())) != cudaSuccess ||
-      cudaOccupancyMaxActiveClusters(&n, fp8_narrow_kernel<DUAL, NT>, &cfg) != cudaSuccess || n < 1) {
+  if (configure<DUAL, NT, false>(cfg, at, dim3(1024, ks), smem_bytes<DUAL, NT>(deepest<DUAL, NT>(ks), ks)) != cudaSuccess ||
+      cudaOccupancyMaxActiveClusters(&n, fp8_narrow_kernel<DUAL, NT, false>, &cfg) != cudaSuccess || n < 1) {
     (void)cudaGetLastError();
-    n = ks == 1 ? device_sm_count() : -1;   // (none: K is not cut that way)
+    n = -1;   // (none: K is not cut that way)
   }
   found[dev][ks].store(n, std::memory_order_relaxed);
   return n;
 }
 // CTAs that share a tile's K: the most whose clusters run at a time.  us, ks = 1 / 2 / 4 / 8: gate/up of 1 token, 4096 x 1024 (32 tiles) 6.6 / 5.7 / 5.8 /
-// 14.9 (two rounds), 6144 x 1536 (48) 8.3 / 8.0 / 11.7 / 21.8, 18432 x 1536 (144) 13.0 / 17.7; 1536 x 18432 (12) 23.7 / 14.2 / 9.9 / 8.8; 333 tokens,
+// 14.9 (two rounds; all of these with sums that are fetched), 6144 x 1536 (48) 8.3 / 8.0 / 11.7 / 21.8, 18432 x 1536 (144) 13.0 / 17.7; 1536 x 18432 (12) 23.7 / 14.2 / 9.9 / 8.8; 333 tokens,
 // 1536 x 6144 (36) 20.7 / 14.1 / 17.9 / 25.0.
 template <bool DUAL, int NT> int cluster_size(const Fp8Product& p) {
   const long long tiles = (long long)blocks_of(p.N) * ((p.M + NT - 1) / NT);
@@ -336,9 +380,9 @@ int launch(const Fp8Product& p, cudaStream_t st) {
   if (tiles_m > 65535) return STU_ERR_SHAPE;
   // one deep ring per SM, or two CTAs per SM where there are that many
   constexpr size_t two = 233472 / 2 - 1024;
-  int stages = deepest<DUAL, NT>();
-  if ((long long)blocks * ks * tiles_m > device_sm_count() && smem_bytes<DUAL, NT>(2) <= two)
-    while (stages > 2 && smem_bytes<DUAL, NT>(stages) > two) stages--;
+  int stages = deepest<DUAL, NT>(ks);
+  if ((long long)blocks * ks * tiles_m > device_sm_count() && smem_bytes<DUAL, NT>(2, ks) <= two)
+    while (stages > 2 && smem_bytes<DUAL, NT>(stages, ks) > two) stages--;
   const int most = ((num_kb + ks - 1) / ks + C::KBS - 1) / C::KBS + 1;   // (a range may begin inside a stage)
   if (stages > most) stages = most;
   CUtensorMap w, w2, x, sw, sw2, sx;
@@ -354,13 +398,16 @@ int launch(const Fp8Product& p, cudaStream_t st) {
   if (rc) return rc;
   cudaLaunchConfig_t cfg;
   cudaLaunchAttribute at[2];
-  cudaError_t e = configure<DUAL, NT>(cfg, at, dim3(blocks, ks, tiles_m), smem_bytes<DUAL, NT>(stages));
+  const size_t smem = smem_bytes<DUAL, NT>(stages, ks);
+  constexpr bool MAY_BE_ALONE = NT < 128;   // (fp8_narrow_takes)
+  const bool alone = MAY_BE_ALONE && ks == 1;
+  cudaError_t e = (alone ? configure<DUAL, NT, MAY_BE_ALONE> : configure<DUAL, NT, false>)(cfg, at, dim3(blocks, ks, tiles_m), smem);
   if (e != cudaSuccess) return (int)e;
   cfg.stream = st;
   at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.numAttrs = pdl_enabled() ? 2 : 1;
-  e = cudaLaunchKernelEx(&cfg, fp8_narrow_kernel<DUAL, NT>, w, w2, x, sw, sw2, sx, p.resid, p.ldr, p.y, p.ldy, p.hq, p.hs, p.M, p.N, p.K, stages, p.overlap,
+  e = cudaLaunchKernelEx(&cfg, alone ? fp8_narrow_kernel<DUAL, NT, MAY_BE_ALONE> : fp8_narrow_kernel<DUAL, NT, false>, w, w2, x, sw, sw2, sx, p.resid, p.ldr, p.y, p.ldy, p.hq, p.hs, p.M, p.N, p.K, stages, p.overlap,
                          device_status_word(), (int)take_dropped_stage(), wait_bound_ns());
   if (e != cudaSuccess) return (int)e;
   STU_CHECK_LAUNCH();
