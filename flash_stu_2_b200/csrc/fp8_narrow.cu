@@ -27,8 +27,9 @@ template <bool DUAL, int NT> struct Narrow {
   static constexpr int WS = DUAL ? 2 : 1;                           // matrices
   static constexpr int DRAIN = NT >= 64 ? 8 : 4, THREADS = 64 + 32 * DRAIN;   // warps that read the sums
   // k-blocks of a stage: waiting for one, announcing its bytes and sending off its copies takes the producer 360 cycles and 27 more per copy, whatever
-  // their size, so that single blocks of 16 KB came at 45 bytes a cycle at most (8 x 1536 x 18432 13.7 us, 66 with K whole)
-  static constexpr int KBS = DUAL ? 2 : NT <= 32 ? 4 : NT <= 64 ? 2 : 1;
+  // their size, so that single blocks of 16 KB came at 45 bytes a cycle at most (8 x 1536 x 18432 13.7 us, 66 with K whole);
+  // where blocks are of 32 KB and the sums that come from elsewhere leave room for few, stages of one (32 x 6144 x 1536 gate/up 10.0 us, so 9.75)
+  static constexpr int KBS = DUAL ? (NT <= 16 ? 2 : 1) : NT <= 32 ? 4 : NT <= 64 ? 2 : 1;
   static constexpr int W_BYTES = WS * A_BYTES, X_BYTES = NT * BK, KB_BYTES = W_BYTES + X_BYTES;
   static constexpr int SCALE_BYTES = PIECE * (WS + 1);
   static constexpr int STAGE = KBS * KB_BYTES + SCALE_BYTES;        // (the scales of all stages lie behind the tiles)
