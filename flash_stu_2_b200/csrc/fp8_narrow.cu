@@ -5,7 +5,7 @@
 // A thread of warp 0 of a CTA brings 128 features (gate/up: 128 of both), NT tokens and their scales by TMA into a ring, one of warp 1 copies the scales into tensor
 // memory and issues kind::mxf8f6f4 (see fp8_gemm.cu), the others drain the sums and send each to the CTA of the cluster whose share its token is in, where it
 // counts towards a barrier.  A warp there adds up a token's 128 features over the cluster, in the order of K, and stores them; gate/up: one warp has the whole
-// block of h and settles its scale by a reduction.  The cluster meets once, behind the set-up and unnoticed; a CTA alone passes its sums on in shared memory.  (Sums left in shared memory and fetched between two meetings of the cluster
+// block of h and settles its scale by a reduction.  The cluster meets once, behind the set-up and unnoticed (Mode: or behind the products); a CTA alone passes its sums on in shared memory.  (Sums left in shared memory and fetched between two meetings of the cluster
 // took 700 and 600 ns for those and 1000 for the rest: 1 x 1024 x 4096 4.7 us, so 3.8; gate/up 1 x 4096 x 1024 5.8, so 5.1; 128 x 1536 x 6144 9.2, so 8.6; but 333 tokens, whose
 // sends are many, 12.1, so 12.3.  Sent by bulk copies of staged rows 5.2.)  On mma.sync the conversions to halves and the fragments of tokens took 370 instructions for 2 KB of
 // weights, more than an SM issues in the time that they take to arrive: 18432 x 1536 gate/up of 8 tokens 25.5 us.
@@ -23,13 +23,19 @@ namespace {
 
 constexpr int MAX_STAGES = 12, MAX_KS = 8;
 
-template <bool DUAL, int NT> struct Narrow {
+// Where sums go.  ALONE (K is not cut): where the CTA's ring was, so that two CTAs fit an SM.  EARLY: they come while the ring may still be in use, to memory of their own; the
+// cluster has met ahead of the products.  LATE, for 128 tokens, whose sums would leave a ring of four k-blocks instead of three stages of two: where the ring was, behind a meeting of CTAs that are
+// done with theirs.  (us, early with stages of one, and late, by k-blocks of a CTA: 6 of 128 x 1536 x 6144 8.7 and 9.15, 8 of 512 x 1024 x 4096 9.85 and 10.2, 16 of 333 x 1536 x 6144 12.25 and
+// 12.15, 24 of 512 x 1536 x 6144 15.3 and 14.8, 72 of 512 x 1536 x 18432 29.4 and 26.9.)
+enum Mode { ALONE, EARLY, LATE };
+
+template <bool DUAL, int NT, Mode MODE> struct Narrow {
   static constexpr int WS = DUAL ? 2 : 1;                           // matrices
   static constexpr int DRAIN = NT >= 64 ? 8 : 4, THREADS = 64 + 32 * DRAIN;   // warps that read the sums
   // k-blocks of a stage: waiting for one, announcing its bytes and sending off its copies takes the producer 360 cycles and 27 more per copy, whatever
   // their size, so that single blocks of 16 KB came at 45 bytes a cycle at most (8 x 1536 x 18432 13.7 us, 66 with K whole);
   // where blocks are of 32 KB and the sums that come from elsewhere leave room for few, stages of one (32 x 6144 x 1536 gate/up 10.0 us, so 9.75)
-  static constexpr int KBS = DUAL ? (NT <= 16 ? 2 : 1) : NT <= 32 ? 4 : NT <= 64 ? 2 : 1;
+  static constexpr int KBS = DUAL ? (NT <= 16 ? 2 : 1) : NT <= 32 ? 4 : NT <= 64 || MODE == LATE ? 2 : 1;
   static constexpr int W_BYTES = WS * A_BYTES, X_BYTES = NT * BK, KB_BYTES = W_BYTES + X_BYTES;
   static constexpr int SCALE_BYTES = PIECE * (WS + 1);
   static constexpr int STAGE = KBS * KB_BYTES + SCALE_BYTES;        // (the scales of all stages lie behind the tiles)
@@ -39,14 +45,11 @@ template <bool DUAL, int NT> struct Narrow {
   static constexpr uint32_t TMEM_COLS = SCALES + 2 * SF_COLS <= 64 ? 64 : SCALES + 2 * SF_COLS <= 128 ? 128 : SCALES + 2 * SF_COLS <= 256 ? 256 : 512;
 };
 constexpr int TAIL = (2 * MAX_STAGES + 2) * 8 + 32;                 // barriers, tensor memory's address, marks
-// Sums of a cluster come while a CTA's ring may still be in use: they have memory of their own.  A CTA by itself puts them where its ring was, so that two fit an SM.
-template <bool DUAL, int NT> __host__ __device__ constexpr int before_tail(int stages, int ks) {
-  const int ring = stages * Narrow<DUAL, NT>::STAGE, sums = Narrow<DUAL, NT>::SUM_BYTES;
-  return ks > 1 ? ring + sums : ring > sums ? ring : sums;
+template <bool DUAL, int NT, Mode MODE> __host__ __device__ constexpr int before_tail(int stages) {
+  const int ring = stages * Narrow<DUAL, NT, MODE>::STAGE, sums = Narrow<DUAL, NT, MODE>::SUM_BYTES;
+  return MODE == EARLY ? ring + sums : ring > sums ? ring : sums;
 }
-template <bool DUAL, int NT> constexpr size_t smem_bytes(int stages, int ks) {
-  return 1024 + (size_t)before_tail<DUAL, NT>(stages, ks) + TAIL;
-}
+template <bool DUAL, int NT, Mode MODE> constexpr size_t smem_bytes(int stages) { return 1024 + (size_t)before_tail<DUAL, NT, MODE>(stages) + TAIL; }
 
 // A value to CTA `to` of the cluster, where it counts towards what the barrier expects.
 __device__ __forceinline__ void send(uint32_t addr, uint32_t bar, int to, uint32_t v) {
@@ -54,27 +57,29 @@ __device__ __forceinline__ void send(uint32_t addr, uint32_t bar, int to, uint32
                "st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.b32 [a], %3, [b];\n\t}"
                ::"r"(addr), "r"(bar), "r"(to), "r"(v) : "memory");
 }
+__device__ __forceinline__ void meet() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
 // Behind a wait for the barrier: what other CTAs stored before they arrived is seen.
 __device__ __forceinline__ void acquire_cluster(uint64_t* bar) {
   asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.acquire.cluster.shared::cta.b64 p, [%0], 0;\n\t}" ::"r"(tma::smem_u32(bar)) : "memory");
 }
 
-// ALONE: K is not cut.
-template <bool DUAL, int NT, bool ALONE>
-__global__ void __launch_bounds__(Narrow<DUAL, NT>::THREADS, 1)
+template <bool DUAL, int NT, Mode MODE>
+__global__ void __launch_bounds__(Narrow<DUAL, NT, MODE>::THREADS, 1)
     fp8_narrow_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmW2, const __grid_constant__ CUtensorMap tmX,
                       const __grid_constant__ CUtensorMap tmSW, const __grid_constant__ CUtensorMap tmSW2, const __grid_constant__ CUtensorMap tmSX,
                       const bf16* resid, long long ldr, bf16* y, long long ldy, unsigned char* hq, unsigned char* hs, int M, int N, int K, int stages,
                       int overlap, int* status, int drop_first_copy, unsigned long long wait_ns) {
-  using C = Narrow<DUAL, NT>;
+  using C = Narrow<DUAL, NT, MODE>;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   constexpr int TILES = C::KBS * C::KB_BYTES, KBS = C::KBS, THREADS = C::THREADS;
   unsigned char* scales = smem + stages * TILES;
   cg::cluster_group cluster = cg::this_cluster();
-  const int ks = ALONE ? 1 : cluster.num_blocks(), rank = ALONE ? 0 : cluster.block_rank();
-  float* sums = reinterpret_cast<float*>(smem + (ALONE ? 0 : stages * C::STAGE));   // [this CTA's tokens][CTA that they come from][feature], gate/up: 128 gate, 128 up
-  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + before_tail<DUAL, NT>(stages, ks));
+  const int ks = MODE == ALONE ? 1 : cluster.num_blocks(), rank = MODE == ALONE ? 0 : cluster.block_rank();
+  float* sums = reinterpret_cast<float*>(smem + (MODE == EARLY ? stages * C::STAGE : 0));   // [this CTA's tokens][CTA that they come from][feature], gate/up: 128 gate, 128 up
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + before_tail<DUAL, NT, MODE>(stages));
   uint64_t* empty_bar = full_bar + MAX_STAGES;
   uint64_t* tmem_full = empty_bar + MAX_STAGES;
   uint64_t* received = tmem_full + 1;
@@ -103,7 +108,7 @@ __global__ void __launch_bounds__(Narrow<DUAL, NT>::THREADS, 1)
     *abort_flag = 0;
     *issued_ctr = *consumed_ctr = 0;
     tma::fence_barrier_init();
-    tma::mbar_expect_tx(received, ALONE ? 0 : owned * ks * C::ROWS * 4);
+    tma::mbar_expect_tx(received, MODE == ALONE ? 0 : owned * ks * C::ROWS * 4);
   }
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tma::smem_u32(tmem_slot)), "r"(C::TMEM_COLS));
@@ -113,7 +118,7 @@ __global__ void __launch_bounds__(Narrow<DUAL, NT>::THREADS, 1)
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem_base = *tmem_slot;
-  if (!ALONE) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");   // sums may come
+  if (MODE == EARLY) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");   // sums may come
   // (when the next kernel may start: epilogue.cuh, PdlTrigger)
   if (overlap && !DUAL) pdl_trigger();
 
@@ -204,8 +209,9 @@ __global__ void __launch_bounds__(Narrow<DUAL, NT>::THREADS, 1)
   } else {
     // ---------------- drain: TMEM lane quarter = warp % 4, a feature per thread
     const int quarter = warp & 3, half = (warp - 2) >> 2;   // (eight warps: either half of the tokens)
-    if (!ALONE) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (MODE == EARLY) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     const bool ok = nst > 0 && tma::warp_wait_bounded(tmem_full, 0, abort_flag, wait_ns);   // (else zeros: the others count on them)
+    if (MODE == LATE) meet();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     float* mine = sums + rank * C::ROWS + quarter * 32 + lane;
     const uint32_t to = tma::smem_u32(mine), bar = tma::smem_u32(received);
@@ -220,7 +226,7 @@ __global__ void __launch_bounds__(Narrow<DUAL, NT>::THREADS, 1)
           tmem_ld32(tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(i * NT + c0), r);
           asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
         }
-        if constexpr (ALONE) {
+        if constexpr (MODE == ALONE) {
 #pragma unroll
           for (int c = 0; c < (NT < 32 ? NT : 32); c++)
             if (c0 + c < last) mine[(c0 + c) * C::ROWS + i * 128] = __uint_as_float(r[c]);
@@ -237,7 +243,10 @@ __global__ void __launch_bounds__(Narrow<DUAL, NT>::THREADS, 1)
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   }
   __syncwarp();
-  if (!ALONE && warp < 2) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  if (warp < 2) {
+    if (MODE == LATE) meet();
+    else if (MODE == EARLY) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  }
   pdl_wait();   // (returns at once: the producer has waited; outputs and residual rows are touched behind it)
   const int hblocks = blocks_of(N), hgroups = groups_of(N);
   if (DUAL && rank == 0) {   // byte 0 for the rows that fill up the last 128 and for the blocks that fill up the last four
@@ -247,7 +256,7 @@ __global__ void __launch_bounds__(Narrow<DUAL, NT>::THREADS, 1)
   }
   // ---------------- this CTA's share of the cluster's sums: a warp per token, four features per lane
   bool all = true;
-  if constexpr (!ALONE) {
+  if constexpr (MODE != ALONE) {
     all = tma::warp_wait_bounded(received, 0, abort_flag, 4 * wait_ns);   // (the others send by the end of their own waits)
     acquire_cluster(received);
   } else {
@@ -305,7 +314,7 @@ __global__ void __launch_bounds__(Narrow<DUAL, NT>::THREADS, 1)
   __syncthreads();
   if (*abort_flag) {
     // A wait ran out: report it, and let copies that were issued but never consumed, and the others' sums, land (bounded) before shared memory is released.
-    if (!ALONE) cluster.sync();   // (with those that gave up; who has left counts as here)
+    if (MODE != ALONE) cluster.sync();   // (with those that gave up; who has left counts as here)
     if (threadIdx.x == 0) {
       if (status) atomicExch(status, 3);
       const uint64_t start = tma::global_ns();
@@ -327,11 +336,11 @@ __global__ void __launch_bounds__(Narrow<DUAL, NT>::THREADS, 1)
   }
 }
 
-template <bool DUAL, int NT, bool ALONE>
+template <bool DUAL, int NT, Mode MODE>
 cudaError_t configure(cudaLaunchConfig_t& cfg, cudaLaunchAttribute* at, dim3 grid, size_t smem) {
   cfg = {};
   cfg.gridDim = grid;
-  cfg.blockDim = dim3(Narrow<DUAL, NT>::THREADS);
+  cfg.blockDim = dim3(Narrow<DUAL, NT, MODE>::THREADS);
   cfg.dynamicSmemBytes = smem;
   at[0].id = cudaLaunchAttributeClusterDimension;
   at[0].val.clusterDim.x = at[0].val.clusterDim.z = 1;
@@ -339,11 +348,11 @@ cudaError_t configure(cudaLaunchConfig_t& cfg, cudaLaunchAttribute* at, dim3 gri
   cfg.attrs = at;
   cfg.numAttrs = 1;
   static SmemLimit limit;
-  return allow_smem((const void*)fp8_narrow_kernel<DUAL, NT, ALONE>, smem, limit);
+  return allow_smem((const void*)fp8_narrow_kernel<DUAL, NT, MODE>, smem, limit);
 }
-template <bool DUAL, int NT> constexpr int deepest(int ks) {
+template <bool DUAL, int NT, Mode MODE> constexpr int deepest() {
   int stages = MAX_STAGES;
-  while (stages > 2 && smem_bytes<DUAL, NT>(stages, ks) > 227 * 1024) stages--;
+  while (stages > 2 && smem_bytes<DUAL, NT, MODE>(stages) > 227 * 1024) stages--;
   return stages;
 }
 
@@ -355,8 +364,8 @@ template <bool DUAL, int NT> int cluster_room(int ks) {
   if ((n = found[dev][ks].load(std::memory_order_relaxed)) != 0) return n;
   cudaLaunchConfig_t cfg;
   cudaLaunchAttribute at[1];
-  if (configure<DUAL, NT, false>(cfg, at, dim3(1024, ks), smem_bytes<DUAL, NT>(deepest<DUAL, NT>(ks), ks)) != cudaSuccess ||
-      cudaOccupancyMaxActiveClusters(&n, fp8_narrow_kernel<DUAL, NT, false>, &cfg) != cudaSuccess || n < 1) {
+  if (configure<DUAL, NT, EARLY>(cfg, at, dim3(1024, ks), smem_bytes<DUAL, NT, EARLY>(deepest<DUAL, NT, EARLY>())) != cudaSuccess ||
+      cudaOccupancyMaxActiveClusters(&n, fp8_narrow_kernel<DUAL, NT, EARLY>, &cfg) != cudaSuccess || n < 1) {
     (void)cudaGetLastError();
     n = -1;   // (none: K is not cut that way)
   }
@@ -374,16 +383,16 @@ template <bool DUAL, int NT> int cluster_size(const Fp8Product& p) {
   return 1;
 }
 
-template <bool DUAL, int NT>
-int launch(const Fp8Product& p, cudaStream_t st) {
-  using C = Narrow<DUAL, NT>;
-  const int tiles_m = (p.M + NT - 1) / NT, blocks = blocks_of(p.N), num_kb = blocks_of(p.K), ks = cluster_size<DUAL, NT>(p);
+template <bool DUAL, int NT, Mode MODE>
+int launch(const Fp8Product& p, int ks, cudaStream_t st) {
+  using C = Narrow<DUAL, NT, MODE>;
+  const int tiles_m = (p.M + NT - 1) / NT, blocks = blocks_of(p.N), num_kb = blocks_of(p.K);
   if (tiles_m > 65535) return STU_ERR_SHAPE;
   // one deep ring per SM, or two CTAs per SM where there are that many
   constexpr size_t two = 233472 / 2 - 1024;
-  int stages = deepest<DUAL, NT>(ks);
-  if ((long long)blocks * ks * tiles_m > device_sm_count() && smem_bytes<DUAL, NT>(2, ks) <= two)
-    while (stages > 2 && smem_bytes<DUAL, NT>(stages, ks) > two) stages--;
+  int stages = deepest<DUAL, NT, MODE>();
+  if ((long long)blocks * ks * tiles_m > device_sm_count() && smem_bytes<DUAL, NT, MODE>(2) <= two)
+    while (stages > 2 && smem_bytes<DUAL, NT, MODE>(stages) > two) stages--;
   const int most = ((num_kb + ks - 1) / ks + C::KBS - 1) / C::KBS + 1;   // (a range may begin inside a stage)
   if (stages > most) stages = most;
   CUtensorMap w, w2, x, sw, sw2, sx;
@@ -399,20 +408,23 @@ int launch(const Fp8Product& p, cudaStream_t st) {
   if (rc) return rc;
   cudaLaunchConfig_t cfg;
   cudaLaunchAttribute at[2];
-  const size_t smem = smem_bytes<DUAL, NT>(stages, ks);
-  constexpr bool MAY_BE_ALONE = NT < 128;   // (fp8_narrow_takes)
-  const bool alone = MAY_BE_ALONE && ks == 1;
-  cudaError_t e = (alone ? configure<DUAL, NT, MAY_BE_ALONE> : configure<DUAL, NT, false>)(cfg, at, dim3(blocks, ks, tiles_m), smem);
+  cudaError_t e = configure<DUAL, NT, MODE>(cfg, at, dim3(blocks, ks, tiles_m), smem_bytes<DUAL, NT, MODE>(stages));
   if (e != cudaSuccess) return (int)e;
   cfg.stream = st;
   at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.numAttrs = pdl_enabled() ? 2 : 1;
-  e = cudaLaunchKernelEx(&cfg, alone ? fp8_narrow_kernel<DUAL, NT, MAY_BE_ALONE> : fp8_narrow_kernel<DUAL, NT, false>, w, w2, x, sw, sw2, sx, p.resid, p.ldr, p.y, p.ldy, p.hq, p.hs, p.M, p.N, p.K, stages, p.overlap,
-                         device_status_word(), (int)take_dropped_stage(), wait_bound_ns());
+  e = cudaLaunchKernelEx(&cfg, fp8_narrow_kernel<DUAL, NT, MODE>, w, w2, x, sw, sw2, sx, p.resid, p.ldr, p.y, p.ldy, p.hq, p.hs, p.M, p.N, p.K, stages,
+                         p.overlap, device_status_word(), (int)take_dropped_stage(), wait_bound_ns());
   if (e != cudaSuccess) return (int)e;
   STU_CHECK_LAUNCH();
   return STU_OK;
+}
+template <bool DUAL, int NT> int launch(const Fp8Product& p, cudaStream_t st) {
+  const int ks = cluster_size<DUAL, NT>(p);
+  constexpr Mode OTHER = NT < 128 ? ALONE : LATE;   // (128 tokens come here where K is cut: fp8_narrow_takes)
+  const bool early = NT < 128 ? ks > 1 : blocks_of(p.K) < 16 * ks;
+  return early ? launch<DUAL, NT, EARLY>(p, ks, st) : launch<DUAL, NT, OTHER>(p, ks, st);
 }
 
 }  // namespace
