@@ -160,7 +160,7 @@ class Fp8MLP(MLP):
         weights = [param(child(self, name), "weight") for name in ("gate_proj", "up_proj", "down_proj")]
         key = [(w._version, w.data_ptr(), w.shape, w.stride()) for w in weights]
         if again or self._rows_key is None or key != self._rows_key[0]:
-            with torch.no_grad(), ops.no_arena():
+            with torch.inference_mode(False), torch.no_grad(), ops.no_arena():   # (inference tensors could not be renewed outside of that mode)
                 made = tuple(ops.quantize_fp8(w.detach()) for w in weights)
                 if torch.cuda.is_current_stream_capturing():   # rows that only a graph's replay makes belong to that graph
                     return made

@@ -243,3 +243,20 @@ def test_the_device_that_is_launched_on(monkeypatch):
     assert ops._elsewhere(on(1), None, on(1)) == torch.device("cuda", 1)
     with pytest.raises(RuntimeError, match="several devices"):
         ops._elsewhere(on(0), on(1))
+
+
+def test_8_bit_weights_made_in_inference_mode(tmp_path, monkeypatch):
+    """What a call in inference mode made is renewed by one outside of it, and the other way around."""
+    import flash_stu_2_b200 as F
+    from flash_stu_2_b200 import ops
+    monkeypatch.setattr(ops, "quantize_fp8", lambda w: ops.Fp8Rows(w.float().clone(), torch.zeros(1), w.shape[1]))
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda *a: type("S", (), {"synchronize": lambda self: None})())
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    mlp = F.FlashSTU(_config(str(tmp_path), mlp_fp8=True)).layers[0].mlp
+    for first, then in ((torch.inference_mode, torch.no_grad), (torch.no_grad, torch.inference_mode)):
+        with first():
+            before = mlp.rows()[0].data.clone()
+        with torch.no_grad():
+            mlp.gate_proj.weight.mul_(2)
+        with then():
+            assert torch.equal(mlp.rows()[0].data, 2 * before)
