@@ -140,17 +140,31 @@ class MLP(nn.Module):
         return ops.linear(h, self.down_proj.weight).reshape(x.shape)
 
 
+def _changes(w: torch.Tensor) -> Optional[int]:
+    """How often a weight has been written in place; None where nobody counts (inference tensors, and parameters that were one or were given one's data)."""
+    try:
+        return None if w.is_inference() else w._version
+    except RuntimeError:
+        return None
+
+
 class Fp8MLP(MLP):
     """The MLP in 8 bits (config.mlp_fp8): its input's norm, both products and what lies between them on e4m3 rows with a scale for each 128
     of a row (ops.Fp8Rows).  The parameters are MLP's; their 8-bit rows are made by the first call behind a change of them (of one through `.data`, which
-    leaves no trace, `mlp.rows(again=True)` tells)."""
+    leaves no trace, `mlp.rows(again=True)` tells).  Parameters that are inference tensors do not tell of their changes: every call makes its rows anew then.  (Those
+    of a model that is made and moved in inference mode are none; those that load_state_dict(assign=True) is given there are.)"""
     fp8 = True
 
     def __init__(self, config, dtype=None):
-        super().__init__(config, dtype=dtype)
+        with torch.inference_mode(False):
+            super().__init__(config, dtype=dtype)
         if self.gate_proj.weight.dtype != torch.bfloat16:
             raise NotImplementedError("mlp_fp8=True has kernels for bfloat16 models only")
         self._rows, self._rows_key = None, None
+
+    def _apply(self, fn, recurse=True):
+        with torch.inference_mode(False):
+            return super()._apply(fn, recurse)
 
     def __getstate__(self):   # (copies and files: the parameters alone)
         return {**super().__getstate__(), "_rows": None, "_rows_key": None}
@@ -158,11 +172,12 @@ class Fp8MLP(MLP):
     def rows(self, again: bool = False):
         """gate, up and down as 8-bit rows."""
         weights = [param(child(self, name), "weight") for name in ("gate_proj", "up_proj", "down_proj")]
-        key = [(w._version, w.data_ptr(), w.shape, w.stride()) for w in weights]
-        if again or self._rows_key is None or key != self._rows_key[0]:
+        key = [(_changes(w), w.data_ptr(), w.shape, w.stride()) for w in weights]
+        told = all(k[0] is not None for k in key)
+        if not told or again or self._rows_key is None or key != self._rows_key[0]:
             with torch.inference_mode(False), torch.no_grad(), ops.no_arena():   # (inference tensors could not be renewed outside of that mode)
                 made = tuple(ops.quantize_fp8(w.detach()) for w in weights)
-                if torch.cuda.is_current_stream_capturing():   # rows that only a graph's replay makes belong to that graph
+                if not told or torch.cuda.is_current_stream_capturing():   # rows that only a graph's replay makes belong to that graph
                     return made
                 kept = self._rows
                 if kept is not None and all(k.data.device == m.data.device and k.shape == m.shape for k, m in zip(kept, made)):
