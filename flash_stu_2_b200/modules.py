@@ -10,6 +10,7 @@ import math
 from typing import Optional, Tuple
 
 import os
+import weakref
 
 import torch
 import torch.nn as nn
@@ -140,19 +141,29 @@ class MLP(nn.Module):
         return ops.linear(h, self.down_proj.weight).reshape(x.shape)
 
 
-def _changes(w: torch.Tensor) -> Optional[int]:
-    """How often a weight has been written in place; None where nobody counts (inference tensors, and parameters that were one or were given one's data)."""
-    try:
-        return None if w.is_inference() else w._version
-    except RuntimeError:
-        return None
+class _Seen:
+    """A weight as it was when something was made from it.  It is told by what holds its memory, not by its address, which may be another's by now; the memory
+    is not kept from being freed by that."""
+    __slots__ = ("memory", "version", "address", "shape", "stride")
+
+    def __init__(self, w: torch.Tensor):
+        self.memory, self.address, self.shape, self.stride = weakref.ref(w.untyped_storage()), w.data_ptr(), w.shape, w.stride()
+        try:
+            self.version = None if w.is_inference() else w._version
+        except RuntimeError:
+            self.version = None   # nobody counts its changes: an inference tensor, or a parameter that was one or was given one's data
+
+    def still(self, w: torch.Tensor) -> bool:
+        return (self.memory() is w.untyped_storage() and self.address == w.data_ptr() and not w.is_inference() and self.version == w._version
+                and self.shape == w.shape and self.stride == w.stride())
 
 
 class Fp8MLP(MLP):
     """The MLP in 8 bits (config.mlp_fp8): its input's norm, both products and what lies between them on e4m3 rows with a scale for each 128
     of a row (ops.Fp8Rows).  The parameters are MLP's; their 8-bit rows are made by the first call behind a change of them (of one through `.data`, which
     leaves no trace, `mlp.rows(again=True)` tells).  Parameters that are inference tensors do not tell of their changes: every call makes its rows anew then.  (Those
-    of a model that is made and moved in inference mode are none; those that load_state_dict(assign=True) is given there are.)"""
+    of a model that is made and moved in inference mode are none; those that load_state_dict(assign=True) is given there are.)  A model that leaves a device takes its rows off it: like its
+    other weights, they are not there any more for graphs that were captured before."""
     fp8 = True
 
     def __init__(self, config, dtype=None):
@@ -164,7 +175,10 @@ class Fp8MLP(MLP):
 
     def _apply(self, fn, recurse=True):
         with torch.inference_mode(False):
-            return super()._apply(fn, recurse)
+            super()._apply(fn, recurse)
+        if self._rows is not None and any(p.device != self._rows[0].data.device for p in self.parameters()):
+            self._rows, self._rows_key = None, None   # (a model that leaves a device holds nothing there)
+        return self
 
     def __getstate__(self):   # (copies and files: the parameters alone)
         return {**super().__getstate__(), "_rows": None, "_rows_key": None}
@@ -172,23 +186,27 @@ class Fp8MLP(MLP):
     def rows(self, again: bool = False):
         """gate, up and down as 8-bit rows."""
         weights = [param(child(self, name), "weight") for name in ("gate_proj", "up_proj", "down_proj")]
-        key = [(_changes(w), w.data_ptr(), w.shape, w.stride()) for w in weights]
-        told = all(k[0] is not None for k in key)
-        if not told or again or self._rows_key is None or key != self._rows_key[0]:
-            with torch.inference_mode(False), torch.no_grad(), ops.no_arena():   # (inference tensors could not be renewed outside of that mode)
-                made = tuple(ops.quantize_fp8(w.detach()) for w in weights)
-                if not told or torch.cuda.is_current_stream_capturing():   # rows that only a graph's replay makes belong to that graph
-                    return made
-                kept = self._rows
-                if kept is not None and all(k.data.device == m.data.device and k.shape == m.shape for k, m in zip(kept, made)):
-                    for k, m in zip(kept, made):   # in place: graphs that were captured with them read the new ones, and never memory that is others'
-                        k.data.copy_(m.data)
-                        k.scales.copy_(m.scales)
-                    made = kept
-                # Calls on other streams, and kernels that fetch weights ahead of the one in front, find them there.
-                torch.cuda.current_stream(made[0].data.device).synchronize()
-            # (the weights that they were made from are kept with the addresses that tell them)
-            self._rows, self._rows_key = made, (key, [w.detach() for w in weights])
+        seen = self._rows_key
+        if not again and seen is not None and seen[0].still(weights[0]) and seen[1].still(weights[1]) and seen[2].still(weights[2]):
+            return self._rows
+        seen = [_Seen(w) for w in weights]
+        with torch.inference_mode(False), torch.no_grad(), ops.no_arena():   # (inference tensors could not be renewed outside of that mode)
+            if any(k.version is None for k in seen) or torch.cuda.is_current_stream_capturing():   # rows that only a graph's replay makes belong to that graph
+                return tuple(ops.quantize_fp8(w.detach()) for w in weights)
+            self._rows_key = None
+            made = []
+            for k, w in zip(self._rows or (None,) * 3, weights):
+                m = ops.quantize_fp8(w.detach())
+                if k is not None and k.data.device == m.data.device and k.shape == m.shape:
+                    k.data.copy_(m.data)   # in place: graphs that were captured with them read the new ones, and never memory that is others'
+                    k.scales.copy_(m.scales)
+                    m = k
+                made.append(m)
+            # Calls on other streams, and kernels that fetch weights ahead of the one in front, find them there.
+            torch.cuda.current_stream(made[0].data.device).synchronize()
+        if self._rows is None or any(k is not m for k, m in zip(self._rows, made)):
+            self._rows = tuple(made)
+        self._rows_key = seen
         return self._rows
 
     def apply_residual(self, xn2d: torch.Tensor, resid2d: torch.Tensor, out2d: torch.Tensor, norm_w: Optional[torch.Tensor] = None,

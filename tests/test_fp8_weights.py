@@ -88,3 +88,106 @@ def test_parameters_that_do_not_tell_of_their_changes(kernels, how):
     with torch.inference_mode():
         mlp.up_proj.weight.mul_(2)
         assert torch.equal(of(mlp), 4 * before)
+
+
+def stored(t):
+    """Tells whether a tensor's memory is still somebody's."""
+    import weakref
+    return weakref.ref(t.untyped_storage())
+
+
+def alive(refs):
+    gc.collect()
+    return [r() is not None for r in refs]
+
+
+def test_a_model_that_leaves_a_device_holds_nothing_there(kernels):
+    """Neither the weights that rows were made from nor the rows; a move that changes nothing keeps both."""
+    mlp = make()
+    rows = mlp.rows()
+    refs = [stored(p.data) for p in mlp.parameters()] + [stored(t) for r in rows for t in (r.data, r.scales)]
+    mlp.to("cpu")
+    assert mlp.rows() is rows and alive(refs) == [True] * 9
+    del rows
+    mlp.to("meta")
+    assert alive(refs) == [False] * 9
+
+
+@pytest.mark.parametrize("how", ["assigned", "replaced", "data", "type"])
+def test_weights_that_are_replaced_are_not_held(kernels, how):
+    """Not until the next call, and not while that makes the rows of their successors; the rows stay where they are."""
+    mlp = make()
+    rows = mlp.rows()
+    before = of(mlp).clone()
+    old = stored(mlp.up_proj.weight.data)
+    twice = (2 * mlp.up_proj.weight.detach()).clone()
+    if how == "assigned":
+        mlp.load_state_dict({**{k: v.clone() for k, v in mlp.state_dict().items()}, "up_proj.weight": twice}, assign=True)
+    elif how == "replaced":
+        mlp.up_proj.weight = torch.nn.Parameter(twice)
+    elif how == "data":
+        mlp.up_proj.weight.data = twice
+    else:
+        twice = mlp.to(torch.float32).up_proj.weight.detach().mul_(2)
+    assert alive([old]) == [False]
+    assert mlp.rows()[1] is rows[1] and torch.equal(of(mlp), 2 * before)
+
+
+def test_one_matrix_at_a_time(kernels, monkeypatch):
+    """A renewal has the new rows of one matrix beside the old ones of all."""
+    from flash_stu_2_b200 import ops
+    made, most, quantize = [], [0], ops.quantize_fp8
+
+    def counted(w):
+        r = quantize(w)
+        made.append(stored(r.data))
+        most[0] = max(most[0], sum(alive(made)))
+        return r
+
+    monkeypatch.setattr(ops, "quantize_fp8", counted)
+    mlp = make()
+    mlp.rows()
+    most[0] = 0
+    with torch.no_grad():
+        mlp.up_proj.weight.mul_(2)
+    mlp.rows()
+    assert most[0] == 3 + 1
+
+
+def test_another_weight_in_the_same_memory(kernels):
+    """Told by what holds the memory, not by its address: a new weight where one that is gone was."""
+    mlp = make()
+    held = mlp.up_proj.weight.data
+    first = of(mlp).clone()
+    memory = held.untyped_storage()
+    # another tensor over the same bytes: the same storage, the same version
+    mlp.up_proj.weight.data = held.view(128, 32)
+    assert mlp.rows()[1] is mlp.rows()[1] and torch.equal(of(mlp), first)
+    del held, memory
+    for value in range(8):
+        mlp.up_proj.weight.data = torch.empty(0, dtype=torch.bfloat16)
+        mlp.up_proj.weight.data = torch.full((128, 32), 2.0 ** value, dtype=torch.bfloat16)
+        assert bool((of(mlp) == 2.0 ** value).all())
+
+
+def test_a_first_call_that_fails_leaves_nothing_behind(kernels, monkeypatch):
+    """Rows of which one could not be made are no model's rows: the next call makes them all."""
+    from flash_stu_2_b200 import ops
+    mlp = make()
+    first = of(mlp).clone()
+    quantize, left = ops.quantize_fp8, [1]
+
+    def fails(w):
+        if left[0] == 0:
+            raise torch.OutOfMemoryError("no room")
+        left[0] -= 1
+        return quantize(w)
+
+    with torch.no_grad():
+        for p in mlp.parameters():
+            p.mul_(2)
+    monkeypatch.setattr(ops, "quantize_fp8", fails)
+    with pytest.raises(torch.OutOfMemoryError):
+        mlp.rows()
+    monkeypatch.setattr(ops, "quantize_fp8", quantize)
+    assert torch.equal(of(mlp), 2 * first) and torch.equal(of(mlp, 2), R.values(quantize(mlp.down_proj.weight.detach())).float())
