@@ -10,6 +10,7 @@ import math
 from typing import Optional, Tuple
 
 import os
+import threading
 import weakref
 
 import torch
@@ -158,6 +159,9 @@ class _Seen:
                 and self.shape == w.shape and self.stride == w.stride())
 
 
+_renewals = threading.RLock()   # held while 8-bit rows are made that a model keeps
+
+
 class Fp8MLP(MLP):
     """The MLP in 8 bits (config.mlp_fp8): its input's norm, both products and what lies between them on e4m3 rows with a scale for each 128
     of a row (ops.Fp8Rows).  The parameters are MLP's; their 8-bit rows are made by the first call behind a change of them (of one through `.data`, which
@@ -183,14 +187,22 @@ class Fp8MLP(MLP):
     def __getstate__(self):   # (copies and files: the parameters alone)
         return {**super().__getstate__(), "_rows": None, "_rows_key": None}
 
+    def _kept(self, weights):
+        """The rows that were made from these weights as they are, or None."""
+        seen = self._rows_key
+        return self._rows if seen is not None and seen[0].still(weights[0]) and seen[1].still(weights[1]) and seen[2].still(weights[2]) else None
+
     def rows(self, again: bool = False):
         """gate, up and down as 8-bit rows."""
         weights = [param(child(self, name), "weight") for name in ("gate_proj", "up_proj", "down_proj")]
-        seen = self._rows_key
-        if not again and seen is not None and seen[0].still(weights[0]) and seen[1].still(weights[1]) and seen[2].still(weights[2]):
-            return self._rows
-        seen = [_Seen(w) for w in weights]
-        with torch.inference_mode(False), torch.no_grad(), ops.no_arena():   # (inference tensors could not be renewed outside of that mode)
+        kept = None if again else self._kept(weights)
+        if kept is not None:
+            return kept
+        with _renewals, torch.inference_mode(False), torch.no_grad(), ops.no_arena():   # (inference tensors could not be renewed outside of that mode)
+            kept = None if again else self._kept(weights)   # (another thread's first call may have made them meanwhile)
+            if kept is not None:
+                return kept
+            seen = [_Seen(w) for w in weights]
             if any(k.version is None for k in seen) or torch.cuda.is_current_stream_capturing():   # rows that only a graph's replay makes belong to that graph
                 return tuple(ops.quantize_fp8(w.detach()) for w in weights)
             self._rows_key = None
@@ -204,10 +216,10 @@ class Fp8MLP(MLP):
                 made.append(m)
             # Calls on other streams, and kernels that fetch weights ahead of the one in front, find them there.
             torch.cuda.current_stream(made[0].data.device).synchronize()
-        if self._rows is None or any(k is not m for k, m in zip(self._rows, made)):
-            self._rows = tuple(made)
-        self._rows_key = seen
-        return self._rows
+            if self._rows is None or any(k is not m for k, m in zip(self._rows, made)):
+                self._rows = tuple(made)
+            self._rows_key = seen
+            return self._rows
 
     def apply_residual(self, xn2d: torch.Tensor, resid2d: torch.Tensor, out2d: torch.Tensor, norm_w: Optional[torch.Tensor] = None,
                        eps: float = ops.RMS_EPS, overlap: bool = False, add: Optional[torch.Tensor] = None):

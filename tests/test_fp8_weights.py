@@ -191,3 +191,27 @@ def test_a_first_call_that_fails_leaves_nothing_behind(kernels, monkeypatch):
         mlp.rows()
     monkeypatch.setattr(ops, "quantize_fp8", quantize)
     assert torch.equal(of(mlp), 2 * first) and torch.equal(of(mlp, 2), R.values(quantize(mlp.down_proj.weight.detach())).float())
+
+
+def test_first_calls_of_two_threads(kernels, monkeypatch):
+    """Both get the rows that are kept: a graph that one of them captures next reads memory that stays."""
+    import threading
+    from flash_stu_2_b200 import ops
+    quantize, inside, go = ops.quantize_fp8, threading.Semaphore(0), threading.Event()
+
+    def slow(w):
+        inside.release()
+        go.wait(10)
+        return quantize(w)
+
+    monkeypatch.setattr(ops, "quantize_fp8", slow)
+    mlp, got = make(), []
+    threads = [threading.Thread(target=lambda: got.append(mlp.rows())) for _ in range(2)]
+    threads[0].start()
+    assert inside.acquire(timeout=10)
+    threads[1].start()
+    inside.acquire(timeout=0.5)   # (the second one is inside too, or waits)
+    go.set()
+    for t in threads:
+        t.join()
+    assert got[0] is got[1] is mlp.rows()
