@@ -364,7 +364,7 @@ int launch_rmsnorm_on(const T* x, const T* add, const T* w, T* sum, unsigned cha
   const int groups = fp8::groups_of(cols);
   int wpr = 1;
   while (wpr * 4 < groups) wpr *= 2;
-  while (wpr < groups && wpr < 16 && (long long)rows * wpr < 148 * 8) wpr *= 2;   // few rows: a shorter chain each
+  while (wpr < groups && wpr < 16 && (long long)rows * wpr < device_sm_count() * WARPS) wpr *= 2;   // few rows: a shorter chain each
   const int nch = (groups + wpr - 1) / wpr, warps = wpr > WARPS ? wpr : WARPS, per_cta = warps / wpr;
   const dim3 grid((rows + per_cta - 1) / per_cta + 1), block(warps * 32);
   if constexpr (GRID != ANY && sizeof(T) == 2) {
