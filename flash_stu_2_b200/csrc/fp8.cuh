@@ -28,9 +28,8 @@ __device__ __forceinline__ uint32_t scale_byte(uint32_t amax_bits) {
   const int b = (int)(amax_bits >> 23) - 8 + ((amax_bits & 0x7fffffu) > 0x600000u ? 1 : 0);
   return b > 0 ? b : 0;
 }
-// 2^-e and 2^e of a scale byte
+// 2^-e of a scale byte
 __device__ __forceinline__ float inverse_scale(uint32_t b) { return __uint_as_float((254u - b) << 23); }
-__device__ __forceinline__ float scale_of(uint32_t b) { return __uint_as_float(b ? b << 23 : 1u << 22); }
 
 // Four values to e4m3, nearest even, the first in the lowest byte.
 __device__ __forceinline__ uint32_t pack4(float a, float b, float c, float d) {
