@@ -16,6 +16,11 @@
 // gate/up: a thread has 64 of the 128 features of a block of its row, two warps settle the block's scale through shared memory, and the row
 // leaves in 8 bits.
 //
+// Sums: the tensor core cuts what it adds off towards zero, so that they are short by a few 2^-24 (K = 18432: some 10^-6) of the magnitudes in them where rounded fp32 sums
+// would be off to either side.  Of a gate/up product's 8-bit results (2048 x 6144 x 1536) 5 in a million are the neighbour of the right one for it, 21 with fp32 sums and
+// the tanh form; where it is a block's largest value that lies on a scale's border, the block has the other scale.  bf16 results that are not the nearest, here and with
+// rounded fp32 sums: K = 1536 6 and 5 in 100,000, 6144 31 and 8.
+//
 // Every wait is bounded, as in gemm_tc.cu: on expiry the waiter tells the others, raises the status word, and the CTAs drain their copies, free
 // their tensor memory and return.
 #include <memory>
