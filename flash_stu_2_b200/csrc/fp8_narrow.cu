@@ -429,19 +429,19 @@ template <bool DUAL, int NT> int launch(const Fp8Product& p, cudaStream_t st) {
 
 }  // namespace
 
-// Whether a product takes less time here than on the tiles of fp8_gemm.cu (us, here and there).  Plain: up to 64 tokens (64: 1024 x 4096 8.2 and 14.3,
-// 18432 x 1536 11.6 and 12.0, 8192 x 2048 9.4 and 8.6).  More: 128 of them take 8 + 0.26 per k-block of a CTA here, one round of tiles there
-// 5.4 + 0.195 per k-block (K over 8 CTAs: 128 x 1024 x 4096 7.9 and 11.3, 128 x 2048 x 1024 7.7 and 6.1; over 4: 512 x 1024 x 4096 9.5 and 11.4, 128 x 4096 x 2048 8.6
-// and 8.5; over 3: 384 x 1536 x 6144 12.2 and 14.6; over 2: 700 x 1536 x 18432 26.4 and 33.5, 700 x 1024 x 4096 12.1 and 11.3, 128 x 8192 x 2048 12.2 and 9.0),
-// and 2.6 more there for rows off the 16-byte grid (333 x 1111 x 1000 7.0 and 9.9).
-// Gate/up, whose sums are twice as many to bring together: up to 16 tokens (18432 x 1536 13.8 and 15.1), up to 32 where K is
-// shared (4096 x 1024 7.3 and 7.9, 6144 x 1536 9.8 and 10.0; not: 18432 x 1536 15.4 and 14.6, 12288 x 1024 10.8 and 10.3).
+// Whether a product takes less time here than on the tiles of fp8_gemm.cu (us, here and there, weights from HBM).  Plain: up to 64 tokens (64: 1024 x 4096 5.1 and 10.1, 18432 x 1536 9.2 and
+// 10.8, 4096 x 1024 5.4 and 5.5; of 48 such products 64 x 8192 x 2048 alone is slower, 8.2 and 7.9).  More: 128 of them take 6.05 + 0.32 per k-block of a CTA here, one round of tiles
+// there 4.1 + 0.2 per k-block, 1.4 more where the last columns are not 32 and 4.5 more for rows off the 16-byte grid, which leave in single values (K over 8 CTAs: 128 x 1024 x 4096 7.1 and 10.4;
+// 128 x 1024 x 1024 5.9 and 5.7; over 6: 128 x 2048 x 2048 7.1 and 7.4, 200 x 520 x 700 5.8 and 6.7; over 4: 512 x 1024 x 4096 8.9 and 10.4, 256 x 2048 x 2048 8.0 and 7.5, 128 x 4096 x 1024 7.1 and 5.9; over 3:
+// 384 x 1536 x 6144 11.1 and 13.8; over 2: 700 x 1536 x 18432 25.1 and 33.3, 700 x 1024 x 4096 11.3 and 10.4, 700 x 1111 x 1000 8.3 and 10.3).
+// Gate/up, whose sums are twice as many to bring together: up to 24 tokens (24: 18432 x 1536 15.1 and 16.0, 12288 x 1024 10.1 and 10.6), up to 32 where K is shared (4096 x 1024 7.5 and 7.9, 6144 x 1536
+// 10.1 and 11.7; not: 18432 x 1536 16.0 and 16.0, 12288 x 1024 11.0 and 10.6).
 bool fp8_narrow_takes(const Fp8Product& p) {
-  if (p.w2) return p.M <= 16 || (p.M <= 32 && cluster_size<true, 32>(p) > 1);
+  if (p.w2) return p.M <= 24 || (p.M <= 32 && cluster_size<true, 32>(p) > 1);
   if (p.M <= 64) return true;
   const long long ks = cluster_size<false, 128>(p), num_kb = blocks_of(p.K);
   const bool on_grid = !((p.ldy | (p.resid ? p.ldr : 0)) & 7) && aligned16(p.y) && aligned16(p.resid);
-  return ks > 1 && 195 * num_kb * ks + (on_grid ? 0 : 2600 * ks) > 260 * num_kb + 2600 * ks;
+  return ks > 1 && (4100 + 200 * num_kb + (!on_grid ? 4500 : p.N & 31 ? 1400 : 0)) * ks > 6050 * ks + 320 * num_kb;
 }
 
 int fp8_narrow(const Fp8Product& p, cudaStream_t st) {

@@ -64,6 +64,32 @@ def test_gate_of_many_tiles(M, N, K):
     ops.check_status()
 
 
+# K of few blocks cut over a cluster, and products on either side of the choice between the kernels
+@pytest.mark.parametrize("resid", [False, True])
+@pytest.mark.parametrize("M,N,K", [(1, 520, 700), (16, 1000, 1024), (32, 1536, 1536), (48, 768, 1152), (65, 1000, 1024), (200, 520, 700), (129, 1240, 1536), (96, 2048, 2048), (160, 2048, 2048),
+                                   (1024, 520, 700), (1024, 1111, 1000), (512, 1536, 3000), (130, 1001, 2560), (700, 1024, 4096)])
+def test_linear_near_the_choice(M, N, K, resid):
+    from flash_stu_2_b200 import ops
+    g = gen(M + N + K)
+    x, w = rows8(g, M, K), weights8(g, N, K)
+    r = stream(g, M, N, torch.bfloat16) if resid else None
+    y = ops.linear_fp8(x, w, resid=r)
+    check_linear(y, x, w, r)
+    assert torch.equal(ops.linear_fp8(x, w, resid=r, overlap=True), y)
+    ops.check_status()
+
+
+@pytest.mark.parametrize("M,N,K", [(17, 18400, 256), (24, 12300, 300), (24, 18432, 1536), (25, 18400, 256), (20, 1000, 1000), (32, 768, 700)])
+def test_gate_near_the_choice(M, N, K):
+    from flash_stu_2_b200 import ops
+    g = gen(M + N + K)
+    x, w, w2 = rows8(g, M, K), weights8(g, N, K), weights8(g, N, K)
+    h = ops.linear_fp8(x, w, W2=w2)
+    R.check_rows(h, *gate(x, w, w2))
+    assert same_rows(ops.linear_fp8(x, w, W2=w2, overlap=True), h)
+    ops.check_status()
+
+
 # bf16 rows without a branch, on the 32-byte grid and on the 16-byte one, of one to four pieces, up to three laps
 @pytest.mark.parametrize("rows,cols", [(3600, 512), (9001, 512), (4001, 1024), (4001, 1000), (3555, 328), (2400, 1536), (2501, 1288), (2500, 2048), (5003, 2040), (4999, 1)])
 def test_norm_of_many_rows(rows, cols):
