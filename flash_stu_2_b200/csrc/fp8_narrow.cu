@@ -372,13 +372,15 @@ template <bool DUAL, int NT> int cluster_room(int ks) {
   found[dev][ks].store(n, std::memory_order_relaxed);
   return n;
 }
-// CTAs that share a tile's K: the most whose clusters run at a time.  us, ks = 1 / 2 / 4 / 8: gate/up of 1 token, 4096 x 1024 (32 tiles) 6.6 / 5.7 / 5.8 /
-// 14.9 (two rounds; all of these with sums that are fetched), 6144 x 1536 (48) 8.3 / 8.0 / 11.7 / 21.8, 18432 x 1536 (144) 13.0 / 17.7; 1536 x 18432 (12) 23.7 / 14.2 / 9.9 / 8.8; 333 tokens,
-// 1536 x 6144 (36) 20.7 / 14.1 / 17.9 / 25.0.
+// CTAs that share a tile's K: the most whose clusters run at a time (74, 45, 33, 26, 22, 15, 15 of 2 to 8), up to 6 for plain products of up to 32 tokens whose K has fewer than 16 blocks.  us, ks = 1 / 2 /
+// 4 / 6 / 8, weights from HBM: gate/up of 1 token, 4096 x 1024 (32 tiles) 5.9 / 5.3 / 5.2 / 9.4 (two rounds) / 12.8, 6144 x 1536 (48) 7.8 / 7.5 / 11.3, 18432 x 1536 (144) 13.5 / 17.6, 1000 x 1000 (8) 5.6 / 4.4 / 3.9 /
+// 4.0 / 3.9; plain of 1 token, 8 k-blocks, x 1024 3.5 / 3.2 / 2.9 / 2.8 / 3.1; 12, x 1536 4.2 / 3.6 / 3.3 / 3.3 / 3.6; 20, x 1001 5.4 / 4.7 / 3.5 / 3.4 / 3.5; of 32, 32 k-blocks, x 1024 9.4 / 7.3 / 5.3 / 4.9 / 4.7; 144, x 1536
+// 32.5 / 19.8 / 13.1 / 10.9 / 10.1; of 64, 8 k-blocks, x 1000 5.8 / 5.5 / 4.6 / 4.6 / 4.3.  (3, 5 and 7 lie between their neighbours.  16 tiles of 8 and 16 blocks take 5 to 13 % less with 4 than with 6.)
 template <bool DUAL, int NT> int cluster_size(const Fp8Product& p) {
   const long long tiles = (long long)blocks_of(p.N) * ((p.M + NT - 1) / NT);
   const int num_kb = blocks_of(p.K), sms = device_sm_count();
-  for (int ks = num_kb < MAX_KS ? num_kb : MAX_KS; ks > 1; ks--)
+  const int most = !DUAL && NT <= 32 && num_kb < 16 ? 6 : MAX_KS;
+  for (int ks = num_kb < most ? num_kb : most; ks > 1; ks--)
     if (tiles * ks <= sms && tiles <= cluster_room<DUAL, NT>(ks)) return ks;
   return 1;
 }
