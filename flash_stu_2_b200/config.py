@@ -16,7 +16,8 @@ class FlashSTUConfig(PretrainedConfig):
 
     Beyond the reference's: cache_len caps the positions that caches are laid out for; mlp_fp8 runs the layers' MLPs in 8 bits (e4m3
     weights and activations with a power-of-two scale for each 128 of a row, bfloat16 models): checkpoints are the same, the 8-bit
-    weights are made from them at the first call.
+    weights are made from them at the first call.  Prefills and MLPs of 1536 and wider gain; token steps of small layers lose, whose bf16
+    sub-layers are one kernel (a block of d=1024: 8 sequences 21 -> 27 us).
     """
     model_type = "FlashSTU"
 

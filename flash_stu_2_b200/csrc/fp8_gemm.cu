@@ -17,9 +17,9 @@
 // leaves in 8 bits.
 //
 // Sums: the tensor core cuts what it adds off towards zero, so that they are short by a few 2^-24 (K = 18432: some 10^-6) of the magnitudes in them where rounded fp32 sums
-// would be off to either side.  Of a gate/up product's 8-bit results (2048 x 6144 x 1536) 5 in a million are the neighbour of the right one for it, 21 with fp32 sums and
-// the tanh form; where it is a block's largest value that lies on a scale's border, the block has the other scale.  bf16 results that are not the nearest, here and with
-// rounded fp32 sums: K = 1536 6 and 5 in 100,000, 6144 31 and 8.
+// would be off to either side.  Of a gate/up product's 8-bit results (16384 x 6144 x 1536) 5 in a million are the neighbour of the right one for it, 20 with fp32 sums and
+// the tanh form; where a block's largest value is that close to a scale's border, the block can have the other scale (one of 5.5 million).  bf16 results that are not the
+// nearest, here and with rounded fp32 sums: K = 1536 6 and 5 in 100,000, 6144 31 and 8, 18432 109 and 18.
 //
 // Every wait is bounded, as in gemm_tc.cu: on expiry the waiter tells the others, raises the status word, and the CTAs drain their copies, free
 // their tensor memory and return.
@@ -282,8 +282,8 @@ __global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__(64 + 32 * EPI_WAR
             asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
             shared_done(i);
             if (i == 1) all_done();
-            // The arithmetic behind the arrivals, not between loads and arrivals, where the compiler would put it: the issuer waited 1700 cycles for the shared
-            // columns of every tile, so 440 (16384 x 6144 x 1536 in a loop 260 us, so 253).
+            // The arithmetic behind the arrivals, not between loads and arrivals, where the compiler would put it and the issuer would wait for it at every tile
+            // (16384 x 6144 x 1536 in a loop 287 us, so 254; in bursts 244, so 227).
             __syncwarp();
 #pragma unroll
             for (int j = 0; j < 32; j++) asm volatile("" : "+r"(r[j]), "+r"(r2[j]));
