@@ -413,8 +413,8 @@ def rmsnorm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float = RMS_EPS, add
 def linear_fp8(x: Fp8Rows, W: Fp8Rows, *, W2: Optional[Fp8Rows] = None, resid: Optional[torch.Tensor] = None,
                out: Optional[torch.Tensor] = None, overlap: bool = False):
     """linear() of 8-bit rows: x @ W^T as bf16 [rows of x, rows of W]; with `resid` (bf16; `out` may be the same) added to it; with W2
-    gelu_tanh(x @ W^T) * (x @ W2^T) as 8-bit rows.  overlap: the weights are fetched while the kernels before this one drain, none of which may be
-    writing them (FLAG_OVERLAP).  The order of a sum over K depends on the sizes and on whether out and resid lie on the 16-byte grid, so that a row
+    gelu_tanh(x @ W^T) * (x @ W2^T) as 8-bit rows.  overlap: the weights may be fetched while the kernels before this one drain (few tokens: they are), none of which
+    may be writing them (FLAG_OVERLAP).  The order of a sum over K depends on the sizes and on whether out and resid lie on the 16-byte grid, so that a row
     alone and among others may differ in fp32's last bits."""
     flags = FLAG_OVERLAP if overlap else 0
     if not (isinstance(x, Fp8Rows) and isinstance(W, Fp8Rows) and (W2 is None or isinstance(W2, Fp8Rows))):

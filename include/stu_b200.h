@@ -117,8 +117,8 @@ int stu_rmsnorm_fp8(const void* x, const void* add, const void* w, void* sum, vo
 /* Products of 8-bit rows x [M], W [N] of K columns, sums in fp32.
  *   W2 = NULL    y[m][n] = round(acc), or round(resid[m][n] + round(acc)), bf16, row strides in elements (y may be resid)
  *   W2 given     y, y_scales: gelu_tanh(x W^T) * (x W2^T), [M] rows of N columns, as 8-bit rows, without a rounding between
- * flags: 0x200 = the weights are fetched while the kernel before this one drains (programmatic launch): no kernel still under way may be writing
- * them.  Sums whose two scales multiply to 2^128 or more are infinite.  How K is cut, and with it the order of fp32 sums, depends on M, N, K, the device's
+ * flags: 0x200 = the weights may be fetched while the kernel before this one drains (programmatic launch; the kernel of few tokens does): no kernel
+ * still under way may be writing them.  Sums whose two scales multiply to 2^128 or more are infinite.  How K is cut, and with it the order of fp32 sums, depends on M, N, K, the device's
  * SMs and whether y and resid lie on the 16-byte grid.  Status 3: a bounded wait of the kernel ran out. */
 int stu_linear_fp8(const void* x, const void* x_scales, const void* W, const void* W_scales, const void* W2, const void* W2_scales,
                    const void* resid, long long resid_row_stride, void* y, long long y_row_stride, void* y_scales, int M, int N, int K,

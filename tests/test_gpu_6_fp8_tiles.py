@@ -170,3 +170,22 @@ def test_memory_behind_a_move():
         for layer in m.layers:
             layer.mlp.to(dev())
         assert torch.equal(m(ids, use_cache=False).logits, want)
+
+
+def test_offsets_that_pass_32_bits():
+    """Rows whose bytes lie behind the first 2^31 and 2^32: what the same rows give alone (K of one block: sums do not depend on the form)."""
+    from flash_stu_2_b200 import ops
+    g = gen(0)
+    M, N, last = 550001, 4096, 301
+    norm_w = torch.ones(N, device=dev(), dtype=torch.bfloat16)
+    x, w, w2 = rows8(g, M, 128), weights8(g, N, 128), weights8(g, N, 128)
+    few = ops.quantize_fp8(x.dequantize()[-last:])
+    y = ops.linear_fp8(x, w)
+    assert torch.equal(y[-last:], ops.linear_fp8(few, w))
+    q, n = ops.quantize_fp8(y), ops.rmsnorm_fp8(y, norm_w)
+    for rows, alone in ((q, ops.quantize_fp8(y[-last:])), (n, ops.rmsnorm_fp8(y[-last:], norm_w)), (ops.linear_fp8(x, w, W2=w2), ops.linear_fp8(few, w, W2=w2))):
+        assert torch.equal(rows.data[-last:].view(torch.uint8), alone.data.view(torch.uint8)) and torch.equal(rows.block_scales()[-last:], alone.block_scales())
+    half = y[-last:].clone()
+    ops.rmsnorm_fp8(y, norm_w, add=y, out=y)
+    assert torch.equal(y[-last:], (2 * half.float()).bfloat16())
+    ops.check_status()
