@@ -134,6 +134,10 @@ _SIGNATURES = {
     "stu_swa_prefill_scratch_elems": ([c_int, c_int, c_int, c_int], c_longlong),
     "stu_swa_prefill_tc5": ([_P, _P, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int, _P,
                              c_int, _P], c_int),
+    "stu_swa_packed": ([_P, _LL, _P, c_int, _P, _P, _LL, _LL, c_int, c_int, c_int, c_int, c_float, _P, c_int, _P], c_int),
+    "stu_kv4_write": ([_P, _LL, _P, _P, _P, _P, c_int, _LL, c_int, c_int, c_int, c_int, c_int, _P], c_int),
+    "stu_kv4_read": ([_P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, _P], c_int),
+    "stu_kv4_step": ([_P, _LL, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, _P], c_int),
     "stu_sample": ([_P, _LL, c_int, c_int, c_float, c_int, c_float, c_int, _P, _P, _LL, _P, c_int, _P], c_int),
 }
 

@@ -1,0 +1,148 @@
+// Attention of whole prompts, packed behind one another: causal, sliding window, ALiBi, soft cap, several query heads to a key head.
+//
+// Every position of a packed row is relative (i - j is the same counted from the sequence's start or from the first row), so the sequences are one
+// long one in which query i sees keys from max(its sequence's first row, i - window) on.  A tile of queries may span sequences; nothing but the
+// first visible key of each row tells them apart, and that grows with i.
+//   score = cap tanh(q.k / sqrt(hd) / cap) - slope_h (i - j);  out = softmax(score) . V     (flash_stu/modules/attention.py:72-101)
+#include "common.cuh"
+
+namespace {
+
+constexpr int QT = 32, KT = 32;
+
+// First visible key of row i: INT_MAX for a row of no sequence (before the first or behind the last).
+__device__ __forceinline__ int first_key(const int* __restrict__ cu, int S, int i, int rows, int window) {
+  if (i >= rows || i < cu[0] || i >= cu[S]) return 0x7fffffff;
+  int lo = 0, hi = S;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (cu[mid] <= i) lo = mid;
+    else hi = mid;
+  }
+  return min(max(max(cu[lo], 0), window < 0 ? 0 : i - window), i);
+}
+
+// Any head dimension, fp32 or bf16, in fp32 on the CUDA cores: a CTA per 32 queries of one head, eight warps of four queries; keys and values of 32
+// positions in shared memory as fp32 (keys transposed), lane = key for the scores, lane = dimension for the weighted values.
+template <typename T>
+__global__ void __launch_bounds__(256) packed_attend_kernel(const T* __restrict__ qkv, long long row_stride, const int* __restrict__ cu, int S,
+                                                            const float* __restrict__ slopes, T* __restrict__ out, long long out_stride, int rows, int H,
+                                                            int Hk, int hd, int window, float scale, float softcap) {
+  extern __shared__ __align__(16) float smem[];
+  __shared__ int first[QT];
+  const int hdp = (hd + 31) & ~31, dpl = hdp >> 5;
+  float (*Qs)[QT] = reinterpret_cast<float (*)[QT]>(smem);                              // [dim][query]
+  float (*Kt)[KT + 1] = reinterpret_cast<float (*)[KT + 1]>(smem + hdp * QT);           // [dim][key]
+  float* Vs = smem + hdp * QT + hdp * (KT + 1);                                         // [key][hdp]
+  const int h = blockIdx.y, g = h / (H / Hk), q0 = blockIdx.x * QT, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  for (int e = threadIdx.x; e < QT * hdp; e += 256) {
+    const int qi = e / hdp, c = e % hdp, i = q0 + qi;
+    Qs[c][qi] = i < rows && c < hd ? Elem<T>::to_f(qkv[i * row_stride + (long long)h * hd + c]) * scale : 0.f;
+  }
+  if (threadIdx.x < QT) first[threadIdx.x] = first_key(cu, S, q0 + threadIdx.x, rows, window);
+  __syncthreads();
+  float m[4], l[4], acc[4][4];
+#pragma unroll
+  for (int u = 0; u < 4; u++) {
+    m[u] = -INFINITY;
+    l[u] = 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; e++) acc[u][e] = 0.f;
+  }
+  const float slope = slopes ? slopes[h] : 0.f;
+  int j_lo = 0x7fffffff, j_hi = -1;   // keys that any row of the tile sees
+  for (int qi = 0; qi < QT; qi++) {
+    j_lo = min(j_lo, first[qi]);
+    if (first[qi] != 0x7fffffff) j_hi = q0 + qi;
+  }
+  for (int jt = j_lo; jt <= j_hi; jt += KT) {
+    __syncthreads();
+    for (int e = threadIdx.x; e < KT * hdp; e += 256) {
+      const int kj = e / hdp, c = e % hdp, j = jt + kj;
+      const bool ok = j <= j_hi && c < hd;
+      const T* at = qkv + j * row_stride + (long long)(H + g) * hd + c;
+      Kt[c][kj] = ok ? Elem<T>::to_f(*at) : 0.f;
+      Vs[kj * hdp + c] = ok ? Elem<T>::to_f(at[(long long)Hk * hd]) : 0.f;
+    }
+    __syncthreads();
+    const int j = jt + lane;
+    float s[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int c = 0; c < hd; c++) {
+      const float kv = Kt[c][lane];
+      const float4 q4 = *reinterpret_cast<const float4*>(&Qs[c][warp * 4]);
+      s[0] = fmaf(q4.x, kv, s[0]);
+      s[1] = fmaf(q4.y, kv, s[1]);
+      s[2] = fmaf(q4.z, kv, s[2]);
+      s[3] = fmaf(q4.w, kv, s[3]);
+    }
+    float pr[4];
+    bool seen[4];
+#pragma unroll
+    for (int u = 0; u < 4; u++) {
+      const int i = q0 + warp * 4 + u;
+      seen[u] = j >= first[warp * 4 + u] && j <= i;
+      float sc = s[u];
+      if (softcap > 0.f) sc = softcap * tanhf(sc / softcap);
+      sc = seen[u] ? sc - slope * (float)(i - j) : -INFINITY;
+      const float top = fmaxf(m[u], warp_max(sc)), corr = top == -INFINITY ? 1.f : __expf(m[u] - top);
+      pr[u] = seen[u] ? __expf(sc - top) : 0.f;
+      l[u] = l[u] * corr + warp_sum(pr[u]);
+      m[u] = top;
+#pragma unroll
+      for (int e = 0; e < 4; e++) acc[u][e] *= corr;
+    }
+    for (int kj = 0; kj < KT; kj++) {
+      float pv[4];
+#pragma unroll
+      for (int u = 0; u < 4; u++) pv[u] = __shfl_sync(0xffffffffu, pr[u], kj);
+#pragma unroll
+      for (int u = 0; u < 4; u++) {
+        if (!__shfl_sync(0xffffffffu, (int)seen[u], kj)) continue;   // (a masked value may be NaN)
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+          if (e < dpl) acc[u][e] = fmaf(pv[u], Vs[kj * hdp + lane + 32 * e], acc[u][e]);
+      }
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < 4; u++) {
+    const int i = q0 + warp * 4 + u;
+    if (first[warp * 4 + u] == 0x7fffffff) continue;
+    const float inv = 1.f / l[u];
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      const int c = lane + 32 * e;
+      if (e < dpl && c < hd) out[i * out_stride + (long long)h * hd + c] = Elem<T>::from_f(acc[u][e] * inv);
+    }
+  }
+}
+
+}  // namespace
+
+extern "C" int stu_swa_packed(const void* qkv, long long row_stride, const int* cu_seqlens, int S, const float* slopes, void* out, long long out_stride,
+                              long long rows, int H, int Hk, int hd, int window, float softcap, int* status, int dtype, void* stream) {
+  if (!qkv || !cu_seqlens || !out) return STU_ERR_NULL;
+  if (dtype != STU_F32 && dtype != STU_BF16) return STU_ERR_DTYPE;
+  if (S <= 0 || rows <= 0 || rows > 0x7fffff00ll || Hk <= 0 || H < Hk || H % Hk || H > 65535 || hd <= 0 ||
+      row_stride < (long long)(H + 2 * Hk) * hd || out_stride < (long long)H * hd)
+    return STU_ERR_SHAPE;
+  if (hd > 128) return STU_ERR_UNSUPPORTED;
+  (void)status;
+  cudaStream_t st = (cudaStream_t)stream;
+  const float scale = 1.0f / sqrtf((float)hd);
+  const dim3 grid((unsigned)((rows + QT - 1) / QT), H);
+  const int hdp = (hd + 31) & ~31;
+  const size_t smem = (size_t)(hdp * QT + hdp * (KT + 1) + KT * hdp) * sizeof(float);
+  static SmemLimit limit, limit16;
+  cudaError_t e = dtype == STU_F32 ? allow_smem((const void*)packed_attend_kernel<float>, 64 * 1024, limit)
+                                   : allow_smem((const void*)packed_attend_kernel<bf16>, 64 * 1024, limit16);
+  if (e != cudaSuccess) return (int)e;
+  if (dtype == STU_F32)
+    packed_attend_kernel<float><<<grid, 256, smem, st>>>((const float*)qkv, row_stride, cu_seqlens, S, slopes, (float*)out, out_stride, (int)rows, H, Hk,
+                                                         hd, window, scale, softcap);
+  else
+    packed_attend_kernel<bf16><<<grid, 256, smem, st>>>((const bf16*)qkv, row_stride, cu_seqlens, S, slopes, (bf16*)out, out_stride, (int)rows, H, Hk, hd,
+                                                        window, scale, softcap);
+  STU_CHECK_LAUNCH();
+  return STU_OK;
+}

@@ -516,6 +516,9 @@ PyMethodDef methods[] = {
     ENTRY(stu_full_decode_prepare),
     ENTRY(stu_full_decode_step),
     ENTRY(stu_full_decode_step_tc5),
+    ENTRY(stu_kv4_read),
+    ENTRY(stu_kv4_step),
+    ENTRY(stu_kv4_write),
     ENTRY(stu_lds_chunk_scan),
     ENTRY(stu_lds_decode_step),
     ENTRY(stu_lds_final_state),
@@ -534,6 +537,7 @@ PyMethodDef methods[] = {
     ENTRY(stu_rmsnorm_fp8),
     ENTRY(stu_sample),
     ENTRY(stu_swa_forward),
+    ENTRY(stu_swa_packed),
     ENTRY(stu_swa_prefill_scratch_elems),
     ENTRY(stu_swa_prefill_tc5),
     ENTRY(stu_taps_even),

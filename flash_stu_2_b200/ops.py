@@ -1058,6 +1058,188 @@ def swa_prefill_tc5(qkv, k_ring, v_ring, pos, slopes, H: int, window: int, softc
     return out
 
 
+def _heads_of(qkv: torch.Tensor, H: int, kv_heads: int, what: str) -> int:
+    """hd of rows of H query heads, then kv_heads keys and as many values."""
+    if H < 1 or kv_heads < 1 or H % kv_heads:
+        raise ValueError(f"{what}: {H} query heads do not share {kv_heads} key heads evenly")
+    if qkv.dim() < 2 or qkv.shape[-1] == 0 or qkv.shape[-1] % (H + 2 * kv_heads):
+        raise ValueError(f"{what}: qkv {tuple(qkv.shape)} does not hold {H} query heads, {kv_heads} keys and as many values")
+    return qkv.shape[-1] // (H + 2 * kv_heads)
+
+
+def _int32(t: torch.Tensor, shape, what: str):
+    if t.dtype != torch.int32:
+        raise TypeError(f"{what} is int32, got {t.dtype}")
+    if tuple(t.shape) != tuple(shape) or not t.is_contiguous():
+        raise ValueError(f"{what} {tuple(t.shape)} has to be contiguous {tuple(shape)}")
+
+
+def _check_scores(slopes: Optional[torch.Tensor], H: int, softcap: float, what: str):
+    if slopes is not None and (slopes.dtype != torch.float32 or tuple(slopes.shape) != (H,) or not slopes.is_contiguous()):
+        raise ValueError(f"{what}: slopes are contiguous float32 [{H}], or None")
+    if not 0 <= softcap < math.inf:
+        raise ValueError(f"{what}: softcap is a finite number, 0 for none")
+
+
+def _dense_rows(t: torch.Tensor) -> torch.Tensor:
+    return t if t.stride(1) == 1 and (t.stride(0) >= t.shape[1] or t.shape[0] < 2) else t.contiguous()
+
+
+def _row_stride(t: torch.Tensor) -> int:
+    """(Of a single row, whose stride says nothing, at least its length.)"""
+    return max(t.stride(0), t.shape[1])
+
+
+def swa_packed(qkv: torch.Tensor, cu_seqlens: torch.Tensor, slopes: Optional[torch.Tensor], H: int, window: Optional[int] = None, softcap: float = 0.0,
+               kv_heads: Optional[int] = None, out: Optional[torch.Tensor] = None):
+    """Attention of whole prompts that lie behind one another in qkv [N, (H + 2 kv_heads) hd]: sequence s in rows cu_seqlens[s] .. cu_seqlens[s+1] - 1
+    (int32 [S + 1] on the device, ascending).  Causal; window: how many earlier positions a query sees (None: all of its sequence); slopes: ALiBi's,
+    or None; kv_heads: H unless query heads share keys.  Returns [N, H hd]; rows that belong to no sequence are left as they are in `out`, which may not
+    lie in qkv's memory."""
+    softcap, kv_heads = float(softcap or 0.0), H if kv_heads is None else kv_heads
+    dt = _dt(qkv)
+    hd = _heads_of(qkv, H, kv_heads, "swa_packed")
+    if qkv.dim() != 2 or hd > 128:
+        raise ValueError(f"swa_packed: qkv {tuple(qkv.shape)} has to be packed rows of heads of at most 128")
+    if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1:
+        raise ValueError(f"swa_packed: cu_seqlens {tuple(cu_seqlens.shape)} has to be [sequences + 1]")
+    _int32(cu_seqlens, cu_seqlens.shape, "swa_packed: cu_seqlens")
+    _check_scores(slopes, H, softcap, "swa_packed")
+    if window is not None and window < 0:
+        raise ValueError("swa_packed: window is the number of earlier positions that are seen, or None")
+    N = qkv.shape[0]
+    if out is not None and (out.dtype != qkv.dtype or out.shape != (N, H * hd) or out.stride(1) != 1 or (N > 1 and out.stride(0) < H * hd)):
+        raise ValueError(f"swa_packed: out has to be {qkv.dtype} [{N}, {H * hd}] with contiguous rows")
+    _cuda(qkv, cu_seqlens, slopes, out)
+    device = _elsewhere(qkv, cu_seqlens, slopes, out)
+    if device is not None:
+        with torch.cuda.device(device):
+            return swa_packed(qkv, cu_seqlens, slopes, H, window, softcap, kv_heads, out)
+    qkv = _dense_rows(qkv)
+    if out is None:
+        out = empty((N, H * hd), qkv.dtype, qkv.device)
+    if N == 0 or cu_seqlens.numel() == 1:
+        return out
+    rc = _lib.native().stu_swa_packed(qkv.data_ptr(), _row_stride(qkv), cu_seqlens.data_ptr(), cu_seqlens.numel() - 1, _p(slopes), out.data_ptr(),
+                                      _row_stride(out), N, H, kv_heads, hd, -1 if window is None else min(window, 2 ** 31 - 1), softcap,
+                                      status_word(qkv.device).data_ptr(), dt, _stream())
+    _lib.check(rc, "stu_swa_packed")
+    _count()
+    return out
+
+
+def _kv4_row_bytes(hd: int) -> int:
+    """Bytes of a slot of one head: 4 bits for each of its dimensions, rounded up to 32, 64 or 128, and 4 bytes for each 64 of them."""
+    if hd < 8 or hd % 8 or hd > 128:
+        raise NotImplementedError(f"a cache in 4 bits has kernels for heads of a multiple of 8 dimensions up to 128, not {hd}")
+    return 20 if hd <= 32 else 36 if hd <= 64 else 72
+
+
+def kv4_slots(window: int) -> int:
+    """Slots of a ring that `window` earlier positions are read from: with the new one, up to a multiple of 16."""
+    return (window + 16) // 16 * 16
+
+
+def kv4_rings(batch: int, slots: int, kv_heads: int, hd: int, device):
+    """Empty rings (keys, values) of 4 bits per number: uint8 [batch, kv_heads, slots * bytes of a slot] (see stu_b200.h).  The token at position t is in
+    slot t % slots; positions are a tensor [batch, 2] int32 as other caches have it."""
+    if batch < 0 or slots < 16 or slots % 16 or kv_heads < 1:
+        raise ValueError(f"kv4_rings: {slots} slots (a multiple of 16) of {kv_heads} heads for {batch} sequences")
+    shape = (batch, kv_heads, slots * _kv4_row_bytes(hd))
+    return torch.zeros(shape, dtype=torch.uint8, device=device), torch.zeros(shape, dtype=torch.uint8, device=device)
+
+
+def _kv4_check(k4: torch.Tensor, v4: torch.Tensor, hd: int, what: str) -> int:
+    """Slots of the rings."""
+    row = _kv4_row_bytes(hd)
+    if k4.dtype != torch.uint8 or v4.dtype != torch.uint8:
+        raise TypeError(f"{what}: rings are uint8, got {k4.dtype} and {v4.dtype}")
+    if k4.dim() != 3 or k4.shape != v4.shape or not (k4.is_contiguous() and v4.is_contiguous()) or k4.shape[2] == 0 or k4.shape[2] % (16 * row):
+        raise ValueError(f"{what}: {tuple(k4.shape)} and {tuple(v4.shape)} are not contiguous rings of heads of {hd} dimensions")
+    return k4.shape[2] // row
+
+
+def kv4_write(qkv: torch.Tensor, k4: torch.Tensor, v4: torch.Tensor, pos: torch.Tensor, H: int, cu_seqlens: Optional[torch.Tensor] = None):
+    """The keys and values of new tokens into rings of 4 bits (kv4_rings), which move on: qkv [batch, tokens, (H + 2 kv_heads) hd], or packed rows
+    [N, ...] with cu_seqlens as in swa_packed.  Of more tokens than slots the last are kept."""
+    dt = _dt(qkv)
+    if k4.dim() != 3:
+        raise ValueError(f"kv4_write: {tuple(k4.shape)} is no ring")
+    B, kv_heads = k4.shape[:2]
+    hd = _heads_of(qkv, H, kv_heads, "kv4_write")
+    slots = _kv4_check(k4, v4, hd, "kv4_write")
+    _int32(pos, (B, 2), "kv4_write: pos")
+    if cu_seqlens is not None:
+        _int32(cu_seqlens, (B + 1,), "kv4_write: cu_seqlens")
+    if qkv.dim() != (3 if cu_seqlens is None else 2) or (cu_seqlens is None and qkv.shape[0] != B):
+        raise ValueError(f"kv4_write: qkv {tuple(qkv.shape)} for rings of {B} sequences")
+    _cuda(qkv, k4, v4, pos, cu_seqlens)
+    device = _elsewhere(qkv, k4, v4, pos, cu_seqlens)
+    if device is not None:
+        with torch.cuda.device(device):
+            return kv4_write(qkv, k4, v4, pos, H, cu_seqlens)
+    rows = _dense_rows(qkv.reshape(-1, qkv.shape[-1]))
+    if rows.shape[0] == 0 or B == 0:
+        return
+    rc = _lib.native().stu_kv4_write(rows.data_ptr(), _row_stride(rows), k4.data_ptr(), v4.data_ptr(), pos.data_ptr(), _p(cu_seqlens), B, rows.shape[0], H,
+                                     kv_heads, hd, slots, dt, _stream())
+    _lib.check(rc, "stu_kv4_write")
+    _count()
+
+
+def kv4_read(k4: torch.Tensor, v4: torch.Tensor, hd: int, dtype: torch.dtype):
+    """What rings of 4 bits stand for: (keys, values) [batch, slots, kv_heads hd], rings as swa_forward reads them.  Slots that nothing was written to
+    are zeros."""
+    slots = _kv4_check(k4, v4, hd, "kv4_read")
+    if dtype not in (torch.float32, torch.bfloat16):
+        raise TypeError(f"kv4_read: values are float32 or bfloat16, not {dtype}")
+    _cuda(k4, v4)
+    device = _elsewhere(k4, v4)
+    if device is not None:
+        with torch.cuda.device(device):
+            return kv4_read(k4, v4, hd, dtype)
+    B, kv_heads = k4.shape[:2]
+    k, v = (empty((B, slots, kv_heads * hd), dtype, k4.device) for _ in range(2))
+    if B == 0:
+        return k, v
+    rc = _lib.native().stu_kv4_read(k4.data_ptr(), v4.data_ptr(), k.data_ptr(), v.data_ptr(), B, kv_heads, hd, slots, _dt(k), _stream())
+    _lib.check(rc, "stu_kv4_read")
+    _count()
+    return k, v
+
+
+def kv4_step(qkv: torch.Tensor, k4: torch.Tensor, v4: torch.Tensor, pos: torch.Tensor, slopes: Optional[torch.Tensor], H: int, window: int,
+             softcap: float = 0.0, update_cache: bool = True):
+    """swa_forward of one new token per sequence, qkv [batch, 1, (H + 2 kv_heads) hd], over rings of 4 bits: its own key and value as they are,
+    those of the `window` positions before it as the rings hold them.  update_cache: they are stored, and pos moves on.  Returns [batch, 1, H hd]."""
+    softcap, dt = float(softcap or 0.0), _dt(qkv)
+    if k4.dim() != 3:
+        raise ValueError(f"kv4_step: {tuple(k4.shape)} is no ring")
+    B, kv_heads = k4.shape[:2]
+    hd = _heads_of(qkv, H, kv_heads, "kv4_step")
+    slots = _kv4_check(k4, v4, hd, "kv4_step")
+    _int32(pos, (B, 2), "kv4_step: pos")
+    _check_scores(slopes, H, softcap, "kv4_step")
+    if qkv.dim() != 3 or qkv.shape[:2] != (B, 1):
+        raise ValueError(f"kv4_step: qkv {tuple(qkv.shape)} is not one token for each of {B} sequences")
+    if not 0 <= window < slots:
+        raise ValueError(f"kv4_step: a window of {window} earlier positions and the new one do not fit {slots} slots")
+    _cuda(qkv, k4, v4, pos, slopes)
+    device = _elsewhere(qkv, k4, v4, pos, slopes)
+    if device is not None:
+        with torch.cuda.device(device):
+            return kv4_step(qkv, k4, v4, pos, slopes, H, window, softcap, update_cache)
+    rows = _dense_rows(qkv[:, 0])
+    out = empty((B, 1, H * hd), qkv.dtype, qkv.device)
+    if B == 0:
+        return out
+    rc = _lib.native().stu_kv4_step(rows.data_ptr(), _row_stride(rows), k4.data_ptr(), v4.data_ptr(), pos.data_ptr(), _p(slopes), out.data_ptr(), B, H,
+                                    kv_heads, hd, slots, window, softcap, int(update_cache), dt, _stream())
+    _lib.check(rc, "stu_kv4_step")
+    _count(2 if update_cache else 1)
+    return out
+
+
 def sample(logits, temperature: float, top_k: Optional[int], top_p: Optional[float], do_sample: bool,
            uniforms: Optional[torch.Tensor], out: torch.Tensor, out_stride: int = 1):
     """Pick one token per row of logits [B,V]; writes int64 ids to out[b*out_stride]."""

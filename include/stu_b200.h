@@ -387,6 +387,29 @@ int stu_swa_prefill_tc5(const void* qkv, void* vt_scratch, void* k_ring, void* v
                         void* out, int B, int Tn, int H, int hd, int W, int window, float softcap, int update_cache,
                         int* status, int dtype, void* stream);
 
+/* Attention of whole prompts, packed behind one another: qkv rows of (H + 2 Hk) * hd values (queries, keys, values; H a multiple of Hk: query
+ * head h reads key head h / (H / Hk)), sequence s in rows cu_seqlens[s] .. cu_seqlens[s + 1] - 1 (int32 [S + 1] on the device, ascending, in
+ * 0 .. rows; empty sequences are none).  Causal; window < 0: every earlier position of the sequence is seen, else the last `window`; slopes (fp32
+ * [H]) may be NULL; softcap 0: none.  out rows of H * hd values; rows that belong to no sequence are left as they are.  For sequences of one length what
+ * stu_swa_forward computes without a cache. */
+int stu_swa_packed(const void* qkv, long long row_stride, const int* cu_seqlens, int S, const float* slopes, void* out,
+                   long long out_stride, long long rows, int H, int Hk, int hd, int window, float softcap, int* status, int dtype,
+                   void* stream);
+
+/* A ring cache of 4 bits for the keys or the values of B sequences: [B][Hk] runs of slots * (width / 2 + 4 * pieces) bytes, slots a multiple of 16,
+ * hd a multiple of 8 up to 128 (kv4.cuh: the layout and how numbers get into it).  The token at position t is in slot t % slots; pos [B][2] as for
+ * stu_swa_forward.
+ * stu_kv4_write: the keys and values of qkv's rows (as in stu_swa_packed; without cu_seqlens rows / B of each sequence) from position pos[2 b] on, of each
+ * sequence the last `slots`; pos moves on by all of them.
+ * stu_kv4_read: both rings as values [B][slots][Hk * hd], in the order of the slots.
+ * stu_kv4_step: attention of one new token per sequence (qkv: B rows) over its own key and value, as they are, and the last `window` < slots earlier
+ * ones, as the rings hold them; out [B][H * hd].  update_cache: the new key and value are stored, and pos moves on. */
+int stu_kv4_write(const void* qkv, long long row_stride, void* k4, void* v4, int* pos, const int* cu_seqlens, int B, long long rows,
+                  int H, int Hk, int hd, int slots, int dtype, void* stream);
+int stu_kv4_read(const void* k4, const void* v4, void* k, void* v, int B, int Hk, int hd, int slots, int dtype, void* stream);
+int stu_kv4_step(const void* qkv, long long row_stride, void* k4, void* v4, int* pos, const float* slopes, void* out, int B, int H,
+                 int Hk, int hd, int slots, int window, float softcap, int update_cache, int dtype, void* stream);
+
 /* ---- exchange between the GPUs of a tensor-parallel group, fused into the token loop's kernels ----------------
  * The reference is single-GPU (its sub-layers: flash_stu/layers/stu_layer.py:78-98,
  * flash_stu/layers/attention_layer.py); these calls replace the all-gather after a channel-sharded STU sub-layer and the
