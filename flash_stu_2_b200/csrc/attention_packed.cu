@@ -4,23 +4,11 @@
 // long one in which query i sees keys from max(its sequence's first row, i - window) on.  A tile of queries may span sequences; nothing but the
 // first visible key of each row tells them apart, and that grows with i.
 //   score = cap tanh(q.k / sqrt(hd) / cap) - slope_h (i - j);  out = softmax(score) . V     (flash_stu/modules/attention.py:72-101)
-#include "common.cuh"
+#include "attention_packed.cuh"
 
 namespace {
 
 constexpr int QT = 32, KT = 32;
-
-// First visible key of row i: INT_MAX for a row of no sequence (before the first or behind the last).
-__device__ __forceinline__ int first_key(const int* __restrict__ cu, int S, int i, int rows, int window) {
-  if (i >= rows || i < cu[0] || i >= cu[S]) return 0x7fffffff;
-  int lo = 0, hi = S;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (cu[mid] <= i) lo = mid;
-    else hi = mid;
-  }
-  return min(max(max(cu[lo], 0), window < 0 ? 0 : i - window), i);
-}
 
 // Any head dimension, fp32 or bf16, in fp32 on the CUDA cores: a CTA per 32 queries of one head, eight warps of four queries; keys and values of 32
 // positions in shared memory as fp32 (keys transposed), lane = key for the scores, lane = dimension for the weighted values.
@@ -39,7 +27,7 @@ __global__ void __launch_bounds__(256) packed_attend_kernel(const T* __restrict_
     const int qi = e / hdp, c = e % hdp, i = q0 + qi;
     Qs[c][qi] = i < rows && c < hd ? Elem<T>::to_f(qkv[i * row_stride + (long long)h * hd + c]) * scale : 0.f;
   }
-  if (threadIdx.x < QT) first[threadIdx.x] = first_key(cu, S, q0 + threadIdx.x, rows, window);
+  if (threadIdx.x < QT) first[threadIdx.x] = packed::first_key(cu, S, q0 + threadIdx.x, rows, window);
   __syncthreads();
   float m[4], l[4], acc[4][4];
 #pragma unroll
@@ -50,10 +38,10 @@ __global__ void __launch_bounds__(256) packed_attend_kernel(const T* __restrict_
     for (int e = 0; e < 4; e++) acc[u][e] = 0.f;
   }
   const float slope = slopes ? slopes[h] : 0.f;
-  int j_lo = 0x7fffffff, j_hi = -1;   // keys that any row of the tile sees
+  int j_lo = packed::NOBODY, j_hi = -1;   // keys that any row of the tile sees
   for (int qi = 0; qi < QT; qi++) {
     j_lo = min(j_lo, first[qi]);
-    if (first[qi] != 0x7fffffff) j_hi = q0 + qi;
+    if (first[qi] != packed::NOBODY) j_hi = q0 + qi;
   }
   for (int jt = j_lo; jt <= j_hi; jt += KT) {
     __syncthreads();
@@ -107,7 +95,7 @@ __global__ void __launch_bounds__(256) packed_attend_kernel(const T* __restrict_
 #pragma unroll
   for (int u = 0; u < 4; u++) {
     const int i = q0 + warp * 4 + u;
-    if (first[warp * 4 + u] == 0x7fffffff) continue;
+    if (first[warp * 4 + u] == packed::NOBODY) continue;
     const float inv = 1.f / l[u];
 #pragma unroll
     for (int e = 0; e < 4; e++) {
@@ -127,8 +115,9 @@ extern "C" int stu_swa_packed(const void* qkv, long long row_stride, const int* 
       row_stride < (long long)(H + 2 * Hk) * hd || out_stride < (long long)H * hd)
     return STU_ERR_SHAPE;
   if (hd > 128) return STU_ERR_UNSUPPORTED;
-  (void)status;
   cudaStream_t st = (cudaStream_t)stream;
+  if (dtype == STU_BF16 && hd % 8 == 0 && aligned16(qkv) && row_stride % 8 == 0 && aligned16(out) && out_stride % 8 == 0)
+    return launch_packed_umma(qkv, row_stride, cu_seqlens, S, slopes, out, out_stride, (int)rows, H, Hk, hd, window, softcap, status, st);
   const float scale = 1.0f / sqrtf((float)hd);
   const dim3 grid((unsigned)((rows + QT - 1) / QT), H);
   const int hdp = (hd + 31) & ~31;

@@ -1,0 +1,492 @@
+// Attention of packed prompts on the 5th-generation tensor cores: bf16, heads of a multiple of 8 dimensions up to 128 (attention_packed.cu says what
+// is computed, and how one tile of queries may span sequences).
+//
+// One CTA = 256 rows of one head as two tiles of 128 queries, which take turns: while the softmax of one runs, the tensor core works for the other.  Key tiles of
+// 128 rows, on multiples of 128, from the first key that any row sees to the diagonal; each tile of queries skips those that none of its rows sees.
+//   S = Q K^T   tcgen05.mma, M = 128 queries, N = 128 keys; Q, K and V come by cp.async.bulk.tensor from qkv itself, seen as [rows][heads][hd] (what a
+//               box has past hd is filled with zeros: a head of 96 is one of 128 with zeros behind it); S lands in tensor memory
+//   softmax     four warps per tile, a row per thread: soft cap, ALiBi, mask, exponentials in the exp2 domain against a maximum that moves only
+//               when the row's outgrows it by 2^8 (then the row of O in tensor memory is rescaled); P in bf16 goes back over S
+//   O += P V    tcgen05.mma, P from tensor memory, V as it lies (rows of keys: the operand whose rows are the sum's index), accumulating in tensor memory
+// The two tiles' S and O are the 512 columns that there are, so P has to take S's place; the next S of a tile is issued behind the product
+// that reads its P, and a CTA's products run in the order of issue.
+// The tensor core adds 0 times what a masked key's value holds: where that is NaN or infinite, a row with a finite sum of weights has a result that is not, and is
+// computed again on the CUDA cores over the keys that it sees.
+#include <cuda.h>
+
+#include "attention_packed.cuh"
+#include "tma.cuh"
+
+namespace {
+
+constexpr int BM = 128, BN = 128, STAGES = 4;
+constexpr int STATUS_PACKED = 13;
+constexpr float LOG2E = 1.4426950408889634f;
+// tanh(y) = y (T0 + T1 y^2 + T2 y^4) for |y| <= 1/2: relative error 2.3e-5
+constexpr float T0 = 0.999977239f, T1 = -0.331685329f, T2 = 0.115185198f;
+constexpr float LAG = 8.f;
+
+template <int HD> struct Smem {
+  static constexpr int KB = HD / 64;                   // blocks of 64 dimensions
+  static constexpr int TILE = KB * 16384;              // 128 rows
+  static constexpr int KV = 2 * TILE;                  // behind the two tiles of queries
+  static constexpr int BYTES = KV + STAGES * TILE + 1024;
+};
+
+struct Ctl {
+  uint64_t q_full[2], s_full[2], p_full[2], pv_done[2], kv_full[STAGES], kv_empty[STAGES];
+  uint32_t tmem_slot, again[2 * BM / 32];
+  int abort_flag, range[4], first[2 * BM];
+};
+
+// K-major rows of 64 values (128-byte swizzle), groups of 8 rows 1 KB apart
+__device__ __forceinline__ uint64_t desc_k(uint32_t saddr) {
+  return (uint64_t)((saddr >> 4) & 0x3FFF) | (uint64_t)1 << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+// rows are the sum's index: 64 columns a row, the next 64 columns a whole block of 128 rows further
+__device__ __forceinline__ uint64_t desc_mn(uint32_t saddr) {
+  return (uint64_t)((saddr >> 4) & 0x3FFF) | (uint64_t)(16384 >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+__host__ __device__ constexpr uint32_t idesc(int n, bool b_rows_k) {   // D fp32, A and B bf16, M = 128
+  return (1u << 4) | (1u << 7) | (1u << 10) | (b_rows_k ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+}
+__device__ __forceinline__ void umma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t accumulate) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(id),
+               "r"(accumulate)
+               : "memory");
+}
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t accumulate) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(id),
+               "r"(accumulate)
+               : "memory");
+}
+__device__ __forceinline__ void umma_commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(tma::smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,"
+      "%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,"
+      "%29,%30,%31,%32};"
+      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+        "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]),
+        "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]),
+        "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+// pairs of fp32 values in 64-bit registers
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pair_of(float lo, float hi) {
+  f32x2 d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(lo), "f"(hi));
+  return d;
+}
+__device__ __forceinline__ f32x2 pair_of(uint32_t lo, uint32_t hi) { return (f32x2)hi << 32 | lo; }
+__device__ __forceinline__ void split(f32x2 v, uint32_t& lo, uint32_t& hi) { asm("mov.b64 {%0, %1}, %2;" : "=r"(lo), "=r"(hi) : "l"(v)); }
+__device__ __forceinline__ void split(f32x2 v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+  f32x2 d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ float exp2_hw(float x) {   // 0 for -infinity
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ bool seen_bit(const uint32_t (&m)[4], int c) { return m[c >> 5] >> (c & 31) & 1u; }
+
+// Row i once more, by a warp, over the keys that it sees and no other.
+__device__ void row_again(const bf16* __restrict__ qkv, long long row_stride, bf16* __restrict__ dst, int i, int first, int h, int g, int H, int Hk, int hd,
+                          float slope, float scale, float softcap, int lane) {
+  float q[4], o[4] = {0.f, 0.f, 0.f, 0.f}, m = -INFINITY, l = 0.f;
+#pragma unroll
+  for (int e = 0; e < 4; e++) q[e] = lane + 32 * e < hd ? __bfloat162float(qkv[i * row_stride + (long long)h * hd + lane + 32 * e]) * scale : 0.f;
+  for (int j = first; j <= i; j++) {
+    const bf16 *k = qkv + j * row_stride + (long long)(H + g) * hd, *v = k + (long long)Hk * hd;
+    float s = 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+      if (lane + 32 * e < hd) s = fmaf(q[e], __bfloat162float(k[lane + 32 * e]), s);
+    s = warp_sum(s);
+    if (softcap > 0.f) s = softcap * tanhf(s / softcap);
+    s -= slope * (float)(i - j);
+    const float top = fmaxf(m, s), corr = top == -INFINITY ? 1.f : __expf(m - top), p = __expf(s - top);
+    m = top;
+    l = l * corr + p;
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+      if (lane + 32 * e < hd) o[e] = fmaf(p, __bfloat162float(v[lane + 32 * e]), o[e] * corr);
+  }
+#pragma unroll
+  for (int e = 0; e < 4; e++)
+    if (lane + 32 * e < hd) dst[lane + 32 * e] = __float2bfloat16_rn(o[e] / l);
+}
+
+template <int HD, bool CAP, bool ALIBI>
+__global__ void __launch_bounds__(320, 1) packed_umma_kernel(const __grid_constant__ CUtensorMap map, const bf16* __restrict__ qkv, long long row_stride,
+                                                             const int* __restrict__ cu, int S, const float* __restrict__ slopes, bf16* __restrict__ out,
+                                                             long long out_stride, int rows, int H, int Hk, int hd, int window, float scale,
+                                                             float softcap, int* status) {
+  typedef Smem<HD> L;
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  __shared__ Ctl ctl;
+  volatile int* abort_flag = &ctl.abort_flag;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int h = blockIdx.y, g = h / (H / Hk);
+  const int q0 = (int)(gridDim.x - 1 - blockIdx.x) * 2 * BM;   // (without a window the last rows see most: they go first)
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; i++) {
+      tma::mbar_init(&ctl.q_full[i], 1);
+      tma::mbar_init(&ctl.s_full[i], 1);
+      tma::mbar_init(&ctl.p_full[i], 128);
+      tma::mbar_init(&ctl.pv_done[i], 1);
+    }
+    for (int s = 0; s < STAGES; s++) {
+      tma::mbar_init(&ctl.kv_full[s], 1);
+      tma::mbar_init(&ctl.kv_empty[s], 1);
+    }
+    ctl.abort_flag = 0;
+    tma::fence_barrier_init();
+  }
+  if (threadIdx.x < 2 * BM / 32) ctl.again[threadIdx.x] = 0;
+  if (warp == 8) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(tma::smem_u32(&ctl.tmem_slot)));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
+  }
+  // The sequences of the first and of the last row of the CTA (counted by all threads: one reading of cu, however many there are), and every row's first key
+  const int row_lo = max(q0, cu[0]), row_hi = min(min(q0 + 2 * BM, rows), cu[S]) - 1;   // rows of sequences
+  int below = 0, upto = 0;
+  for (int s0 = 0; s0 < S; s0 += 320) {   // (block-uniform)
+    const int at = s0 + threadIdx.x < S ? cu[s0 + threadIdx.x] : 0x7fffffff;
+    below += __syncthreads_count(at <= row_lo);
+    upto += __syncthreads_count(at <= row_hi);
+  }
+  const int seq_lo = max(below - 1, 0), seq_hi = max(upto, seq_lo + 1);
+  if (threadIdx.x < 2 * BM) {
+    const int i = q0 + threadIdx.x;
+    ctl.first[threadIdx.x] = i >= row_lo && i <= row_hi ? packed::first_key_in(cu, seq_lo, seq_hi, i, window) : packed::NOBODY;
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = ctl.tmem_slot;
+  // key tiles of the two tiles of queries: begin .. end - 1
+  int begin[2], end[2];
+#pragma unroll
+  for (int i = 0; i < 2; i++) {
+    const int lo = max(row_lo, q0 + i * BM), hi = min(row_hi, q0 + i * BM + BM - 1);
+    begin[i] = lo <= hi ? ctl.first[lo - q0] / BN : 0;
+    end[i] = lo <= hi ? hi / BN + 1 : 0;
+    begin[i] = min(begin[i], end[i]);
+  }
+  const int t_lo = end[0] == 0 ? begin[1] : end[1] == 0 ? begin[0] : min(begin[0], begin[1]), t_hi = max(end[0], end[1]);
+  auto active = [&](int i, int t) { return t >= begin[i] && t < end[i]; };
+
+  if (warp == 9) {
+    // ------------------------------------------------------------------ producer
+    const bool leader = elect_one();
+    auto load = [&](unsigned char* dst, uint64_t* bar, int head, int row) {
+      if (leader) {
+        tma::mbar_expect_tx(bar, L::TILE);
+#pragma unroll
+        for (int kb = 0; kb < L::KB; kb++) tma::load_3d(dst + kb * 16384, &map, bar, kb * 64, head, row);
+      }
+      __syncwarp();
+    };
+    bool ok = true;
+    int n = 0;
+    auto load_kv = [&](int head, int t) {
+      const int s = n % STAGES;
+      ok = ok && tma::warp_wait_bounded(&ctl.kv_empty[s], ((uint32_t)(n / STAGES) & 1u) ^ 1u, abort_flag);
+      if (ok) load(smem + L::KV + s * L::TILE, &ctl.kv_full[s], head, t * BN);
+      n++;
+    };
+    for (int t = t_lo; ok && t < t_hi; t++) {
+      for (int i = 0; i < 2; i++)
+        if (t == begin[i] && end[i] > begin[i]) load(smem + i * L::TILE, &ctl.q_full[i], h, q0 + i * BM);
+      load_kv(H + g, t);
+      load_kv(H + Hk + g, t);
+    }
+  } else if (warp == 8) {
+    // ------------------------------------------------------------------ MMA issuer
+    const bool leader = elect_one();
+    const uint32_t base = tma::smem_u32(smem);
+    bool ok = true;
+    auto stage_of = [&](int n) { return base + L::KV + (uint32_t)(n % STAGES) * L::TILE; };
+    auto wait_kv = [&](int n) { return tma::warp_wait_bounded(&ctl.kv_full[n % STAGES], (uint32_t)(n / STAGES) & 1u, abort_flag); };
+    for (int t = t_lo; ok && t <= t_hi; t++) {
+      const int nk = 2 * (t - t_lo), nv = nk - 1;   // the stages of K of t and V of t - 1
+      for (int i = 0; ok && i < 2; i++) {
+        if (active(i, t - 1)) {
+          const int n = t - 1 - begin[i];
+          ok = tma::warp_wait_bounded(&ctl.p_full[i], (uint32_t)n & 1u, abort_flag) && wait_kv(nv);
+          if (!ok) break;
+          fence_after();
+          if (leader) {
+            const uint64_t v = desc_mn(stage_of(nv));
+#pragma unroll
+            for (int kk = 0; kk < BN / 16; kk++)
+              umma_ts(tmem + 256 + i * HD, tmem + i * 128 + kk * 8, v + (uint64_t)(kk * (2048 >> 4)), idesc(HD, true), (n | kk) ? 1u : 0u);
+            umma_commit(&ctl.pv_done[i]);
+            if (i == 1 || !active(1, t - 1)) umma_commit(&ctl.kv_empty[nv % STAGES]);
+          }
+          __syncwarp();
+        }
+        if (active(i, t)) {
+          if (t == begin[i]) ok = tma::warp_wait_bounded(&ctl.q_full[i], 0, abort_flag);
+          ok = ok && wait_kv(nk);
+          if (!ok) break;
+          fence_after();
+          if (leader) {
+#pragma unroll
+            for (int kb = 0; kb < L::KB; kb++)
+#pragma unroll
+              for (int kk = 0; kk < 4; kk++)
+                umma_ss(tmem + i * 128, desc_k(base + i * L::TILE + kb * 16384) + 2 * kk, desc_k(stage_of(nk) + kb * 16384) + 2 * kk, idesc(BN, false),
+                        (kb | kk) ? 1u : 0u);
+            umma_commit(&ctl.s_full[i]);
+            if (i == 1 || !active(1, t)) umma_commit(&ctl.kv_empty[nk % STAGES]);
+          }
+          __syncwarp();
+        }
+      }
+    }
+  } else {
+    // -------------------------------------------------------------------- softmax warps (a quarter of the lanes of tensor memory each)
+    const int tile = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane;
+    const int i = q0 + tile * BM + row, first = ctl.first[tile * BM + row];
+    const int last_first = max(row_lo, q0 + tile * BM) <= min(row_hi, q0 + tile * BM + BM - 1) ? ctl.first[min(row_hi, q0 + tile * BM + BM - 1) - q0] : 0;
+    const bool whole = row_lo <= q0 + tile * BM && row_hi >= q0 + tile * BM + BM - 1;
+    const uint32_t lanes = (uint32_t)(quarter * 32) << 16, tm_s = tmem + tile * 128 + lanes, tm_o = tmem + 256 + tile * HD + lanes;
+    const float c2 = ALIBI ? slopes[h] * LOG2E : 0.f;
+    const float k0 = CAP ? scale / softcap : 0.f, k1 = CAP ? softcap * LOG2E : scale * LOG2E;
+    const float kk0 = k0 * k0;
+    const f32x2 cap0 = pair_of(k0 * k1 * T0, k0 * k1 * T0), cap1 = pair_of(k0 * k1 * kk0 * T1, k0 * k1 * kk0 * T1),
+                cap2 = pair_of(k0 * k1 * kk0 * kk0 * T2, k0 * k1 * kk0 * kk0 * T2), kp = pair_of(k1, k1), cc = pair_of(c2, c2);
+    const float most_small = CAP ? 0.25f / kk0 : 0.f;   // tanh(s k0) k1 = s (cap0 + cap1 s^2 + cap2 s^4) while s^2 is below it
+    float m_ref = -INFINITY, l = 0.f;
+    bool ok = true;
+    const int nt = end[tile] - begin[tile];
+    for (int n = 0; n < nt; n++) {
+      const int jt = (begin[tile] + n) * BN;
+      ok = tma::warp_wait_bounded(&ctl.s_full[tile], (uint32_t)n & 1u, abort_flag);
+      if (!ok) break;
+      fence_after();
+      uint32_t sr[128];
+#pragma unroll
+      for (int c = 0; c < 4; c++) tmem_ld32(tm_s + c * 32, sr + c * 32);
+      tmem_wait_ld();
+      const bool interior = whole && jt >= last_first && jt + BN - 1 <= q0 + tile * BM;   // all rows of the tile see all keys of this one
+      uint32_t seen[4];
+      if (!interior) {
+        const int lo = max(first - jt, 0), hi = first == packed::NOBODY ? -1 : min(i - jt, BN - 1);
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+          const int a = max(lo - 32 * w, 0), b = min(hi - 32 * w, 31);
+          seen[w] = a > b ? 0u : (0xffffffffu >> (31 - (b - a))) << a;
+        }
+      }
+      const float base_t = ALIBI ? c2 * (float)(jt - i) : 0.f;
+      if (CAP) {
+        if (!interior) {   // a masked score decides nothing
+#pragma unroll
+          for (int c = 0; c < 128; c++)
+            if (!seen_bit(seen, c)) sr[c] = 0;
+        }
+        float most = 0.f;   // the largest square (a NaN score is not in it: both forms carry it on)
+        const f32x2 bt = pair_of(base_t, base_t);
+#pragma unroll
+        for (int c = 0; c < 128; c += 2) {
+          const f32x2 sv = pair_of(sr[c], sr[c + 1]), sq = mul2(sv, sv);
+          float s0, s1;
+          split(sq, s0, s1);
+          most = fmaxf(most, fmaxf(s0, s1));
+          const f32x2 p = fma2(sq, fma2(sq, cap2, cap1), cap0);
+          split(ALIBI ? fma2(sv, p, fma2(cc, pair_of((float)c, (float)(c + 1)), bt)) : mul2(sv, p), sr[c], sr[c + 1]);
+        }
+        const bool large = !(most < most_small);   // (a row's own scores decide for it)
+        if (__any_sync(0xffffffffu, large)) {
+#pragma unroll
+          for (int q = 0; q < 4; q++) {
+            uint32_t raw[32];
+            tmem_ld32(tm_s + q * 32, raw);
+            tmem_wait_ld();
+#pragma unroll
+            for (int c = 0; c < 32; c++) {
+              float th;   // the hardware's: relative error 2^-11
+              asm("tanh.approx.f32 %0, %1;" : "=f"(th) : "f"(__uint_as_float(raw[c]) * k0));
+              if (large) sr[q * 32 + c] = __float_as_uint(ALIBI ? fmaf(th, k1, fmaf(c2, (float)(q * 32 + c), base_t)) : th * k1);
+            }
+          }
+        }
+      } else {
+        const f32x2 bt = pair_of(base_t, base_t);
+#pragma unroll
+        for (int c = 0; c < 128; c += 2) {
+          const f32x2 sv = pair_of(sr[c], sr[c + 1]);
+          split(ALIBI ? fma2(sv, kp, fma2(cc, pair_of((float)c, (float)(c + 1)), bt)) : mul2(sv, kp), sr[c], sr[c + 1]);
+        }
+      }
+      if (!interior) {
+#pragma unroll
+        for (int c = 0; c < 128; c++)
+          if (!seen_bit(seen, c)) sr[c] = 0xff800000u;   // -infinity
+      }
+      float mx[4];
+#pragma unroll
+      for (int c = 0; c < 4; c++) mx[c] = fmaxf(__uint_as_float(sr[c]), __uint_as_float(sr[c + 4]));
+#pragma unroll
+      for (int c = 8; c < 128; c += 8)
+#pragma unroll
+        for (int e = 0; e < 4; e++) mx[e] = fmaxf(mx[e], fmaxf(__uint_as_float(sr[c + e]), __uint_as_float(sr[c + e + 4])));
+      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+      const bool grow = top > m_ref + LAG || (m_ref == -INFINITY && top > -INFINITY);
+      if (__any_sync(0xffffffffu, grow)) {
+        const float m_new = fmaxf(m_ref, top), corr = m_new == -INFINITY ? 1.f : exp2_hw(m_ref - m_new);   // 0 for a row that had no key yet
+        m_ref = m_new;
+        l *= corr;
+        if (n > 0) {
+          ok = tma::warp_wait_bounded(&ctl.pv_done[tile], (uint32_t)(n - 1) & 1u, abort_flag);
+          if (!ok) break;
+          fence_after();
+#pragma unroll 1
+          for (int c = 0; c < HD / 32; c++) {
+            uint32_t o[32];
+            tmem_ld32(tm_o + c * 32, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * corr);
+            tmem_st32(tm_o + c * 32, o);
+          }
+          tmem_wait_st();
+        }
+      }
+      const float ref = m_ref == -INFINITY ? 0.f : m_ref;
+      const f32x2 neg = pair_of(-ref, -ref);
+      f32x2 sum[2] = {0, 0};
+#pragma unroll
+      for (int c = 0; c < 128; c += 2) {
+        float p0, p1;
+        split(add2(pair_of(sr[c], sr[c + 1]), neg), p0, p1);
+        p0 = exp2_hw(p0);
+        p1 = exp2_hw(p1);
+        sum[c >> 1 & 1] = add2(sum[c >> 1 & 1], pair_of(p0, p1));
+        sr[c >> 1] = pack_bf16(p0, p1);
+      }
+      float s0, s1;
+      split(add2(sum[0], sum[1]), s0, s1);
+      l += s0 + s1;
+      tmem_st32(tm_s, sr);
+      tmem_st32(tm_s + 32, sr + 32);
+      tmem_wait_st();
+      fence_before();
+      tma::mbar_arrive(&ctl.p_full[tile]);
+    }
+    if (ok && nt > 0) ok = tma::warp_wait_bounded(&ctl.pv_done[tile], (uint32_t)(nt - 1) & 1u, abort_flag);
+    if (ok && nt > 0) {
+      fence_after();
+      const float inv_l = 1.f / l;
+      bf16* dst = out + i * out_stride + (long long)h * hd;
+      bool finite = true;
+#pragma unroll 1
+      for (int c = 0; c < HD / 32; c++) {
+        uint32_t o[32];
+        tmem_ld32(tm_o + c * 32, o);
+        tmem_wait_ld();
+        if (first != packed::NOBODY) {
+#pragma unroll
+          for (int v = 0; v < 4; v++) {
+            if (c * 32 + v * 8 < hd) {
+              float f[8];
+#pragma unroll
+              for (int e = 0; e < 8; e++) {
+                f[e] = __uint_as_float(o[v * 8 + e]) * inv_l;
+                finite &= fabsf(f[e]) < INFINITY;
+              }
+              store_vec(dst + c * 32 + v * 8, f);
+            }
+          }
+        }
+      }
+      if (!finite && fabsf(l) < INFINITY) atomicOr(&ctl.again[tile * 4 + quarter], 1u << lane);
+    }
+    fence_before();
+  }
+  __syncthreads();
+  if (*abort_flag) {
+    if (threadIdx.x == 0) {
+      if (status) atomicExch(status, STATUS_PACKED);
+      const uint64_t start = tma::global_ns();   // copies under way still land in this CTA's shared memory: it keeps it for longer than any copy takes
+      while (tma::global_ns() - start < 200000ull) {}
+    }
+    __syncthreads();
+  }
+  if (warp == 8) {
+    fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+  }
+  for (int r = warp; r < 2 * BM; r += 10)
+    if (ctl.again[r >> 5] >> (r & 31) & 1u)
+      row_again(qkv, row_stride, out + (long long)(q0 + r) * out_stride + (long long)h * hd, q0 + r, ctl.first[r], h, g, H, Hk, hd, ALIBI ? slopes[h] : 0.f,
+                scale, CAP ? softcap : 0.f, lane);
+}
+
+template <int HD, bool CAP, bool ALIBI>
+int launch(const CUtensorMap& map, const void* qkv, long long row_stride, const int* cu, int S, const float* slopes, void* out, long long out_stride, int rows,
+           int H, int Hk, int hd, int window, float softcap, int* status, cudaStream_t st) {
+  static SmemLimit limit;
+  const cudaError_t e = allow_smem((const void*)packed_umma_kernel<HD, CAP, ALIBI>, Smem<HD>::BYTES, limit);
+  if (e != cudaSuccess) return (int)e;
+  packed_umma_kernel<HD, CAP, ALIBI><<<dim3((unsigned)((rows + 2 * BM - 1) / (2 * BM)), H), 320, Smem<HD>::BYTES, st>>>(
+      map, (const bf16*)qkv, row_stride, cu, S, slopes, (bf16*)out, out_stride, rows, H, Hk, hd, window, 1.0f / sqrtf((float)hd), softcap, status);
+  STU_CHECK_LAUNCH();
+  return STU_OK;
+}
+
+}  // namespace
+
+int launch_packed_umma(const void* qkv, long long row_stride, const int* cu, int S, const float* slopes, void* out, long long out_stride, int rows, int H,
+                       int Hk, int hd, int window, float softcap, int* status, cudaStream_t st) {
+  CUtensorMap map;
+  const cuuint64_t dims[3] = {(cuuint64_t)hd, (cuuint64_t)(H + 2 * Hk), (cuuint64_t)rows};
+  const cuuint64_t strides[2] = {(cuuint64_t)hd * 2, (cuuint64_t)row_stride * 2};
+  const cuuint32_t box[3] = {64, 1, BM};
+  const int rc = tma::encode_bf16(&map, qkv, 3, dims, strides, box, true);
+  if (rc != STU_OK) return rc;
+  auto go = [&](auto kernel) { return kernel(map, qkv, row_stride, cu, S, slopes, out, out_stride, rows, H, Hk, hd, window, softcap, status, st); };
+  if (hd <= 64)
+    return softcap > 0.f ? slopes ? go(launch<64, true, true>) : go(launch<64, true, false>) : slopes ? go(launch<64, false, true>) : go(launch<64, false, false>);
+  return softcap > 0.f ? slopes ? go(launch<128, true, true>) : go(launch<128, true, false>) : slopes ? go(launch<128, false, true>) : go(launch<128, false, false>);
+}

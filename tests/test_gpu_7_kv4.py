@@ -304,24 +304,26 @@ def test_packed(case, cap, alibi, dt):
 @pytest.mark.parametrize("dt", DTYPES)
 @pytest.mark.parametrize("hd", [64, 128, 40])
 def test_packed_sequences_do_not_touch(dt, hd):
-    """NaN and infinities in the keys and values of one sequence are in no other's rows."""
+    """NaN and infinities in the keys and values of one sequence are in no other's rows.  (Rows that share a tile with them may be computed in another
+    way, so each is held to the reference's tolerance, which is the same for both, and not to the other's bits.)"""
     from flash_stu_2_b200 import ops
     g, H, kv, lengths = gen(hd), 2, 1, (70, 33, 200, 5)
-    qkv, cu = activations(g, sum(lengths), H, kv, hd, dt), cu_of(lengths)
-    plain = ops.swa_packed(qkv, cu, slopes_of(H), H, None, 50.0, kv_heads=kv)
+    qkv, cu, slopes = activations(g, sum(lengths), H, kv, hd, dt), cu_of(lengths), slopes_of(H)
+    want, tol = R.packed(qkv, lengths, 0, slopes, H, kv, None, 50.0, dt)
     for bad in range(4):
         for value in (math.nan, math.inf):
             x = qkv.clone()
             a, b = int(cu[bad]), int(cu[bad + 1])
             x[a:b, H * hd:] = value
-            got = ops.swa_packed(x, cu, slopes_of(H), H, None, 50.0, kv_heads=kv)
-            assert torch.equal(got[:a], plain[:a]) and torch.equal(got[b:], plain[b:]) and bool(got[a:b].isnan().all())
+            got = ops.swa_packed(x, cu, slopes, H, None, 50.0, kv_heads=kv)
+            assert bool(got[a:b].isnan().all())
+            R.check(torch.cat([got[:a], got[b:]]), torch.cat([want[:a], want[b:]]), torch.cat([tol[:a], tol[b:]]))
+    want, tol = R.packed(qkv, lengths, 0, slopes, H, kv, 8, 50.0, dt)
     x = qkv.clone()
-    x[90, H * hd:] = math.nan                      # a key in the middle of the second: rows from it on
-    got = ops.swa_packed(x, cu, slopes_of(H), H, 8, 50.0, kv_heads=kv)
-    plain = ops.swa_packed(qkv, cu, slopes_of(H), H, 8, 50.0, kv_heads=kv)
-    rows = got.isnan().any(1).nonzero().flatten().tolist()
-    assert rows == list(range(90, 99)) and torch.equal(got[:90], plain[:90]) and torch.equal(got[99:], plain[99:])
+    x[90, H * hd:] = math.nan                      # a key in the middle of the second: the rows from it on that see it
+    got = ops.swa_packed(x, cu, slopes, H, 8, 50.0, kv_heads=kv)
+    assert got.isnan().any(1).nonzero().flatten().tolist() == list(range(90, 99))
+    R.check(torch.cat([got[:90], got[99:]]), torch.cat([want[:90], want[99:]]), torch.cat([tol[:90], tol[99:]]))
 
 
 @pytest.mark.parametrize("dt", DTYPES)
