@@ -20,11 +20,17 @@
 namespace {
 
 constexpr int BM = 128, BN = 128, STAGES = 4;
+// Eight warps of softmax, the issuer, the producer, and two without work that make these a warpgroup, whose registers go to the softmax: 256 threads of
+// 208 and 128 of 80 are less than the launch's 384 of 168.
+constexpr int THREADS = 384, REGS_SOFTMAX = 208, REGS_OTHERS = 80;
 constexpr int STATUS_PACKED = 13;
 constexpr float LOG2E = 1.4426950408889634f;
 // tanh(y) = y (T0 + T1 y^2 + T2 y^4) for |y| <= 1/2: relative error 2.3e-5
 constexpr float T0 = 0.999977239f, T1 = -0.331685329f, T2 = 0.115185198f;
 constexpr float LAG = 8.f;
+
+// Of 8 pairs of weights those that the FMA pipe makes
+constexpr int POLY_OF_8 = 2;
 
 template <int HD> struct Smem {
   static constexpr int KB = HD / 64;                   // blocks of 64 dimensions
@@ -34,9 +40,9 @@ template <int HD> struct Smem {
 };
 
 struct Ctl {
-  uint64_t q_full[2], s_full[2], p_full[2], pv_done[2], kv_full[STAGES], kv_empty[STAGES];
-  uint32_t tmem_slot, again[2 * BM / 32];
-  int abort_flag, range[4], first[2 * BM];
+  uint64_t q_full[2], s_full[2], p_full[2][2], pv_done[2], kv_full[STAGES], kv_empty[STAGES];
+  uint32_t tmem_slot;
+  int abort_flag, first[2 * BM];
 };
 
 // K-major rows of 64 values (128-byte swizzle), groups of 8 rows 1 KB apart
@@ -85,7 +91,21 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
         "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
       : "memory");
 }
-__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* r) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+               : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+               : "memory");
+}
+// Loads have landed: nothing that reads r may move ahead of this.
+template <int N> __device__ __forceinline__ void tmem_wait_ld(uint32_t (&r)[N]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < N; i++) asm volatile("" : "+r"(r[i]));
+}
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -120,11 +140,37 @@ __device__ __forceinline__ float exp2_hw(float x) {   // 0 for -infinity
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+// 2^x on the FMA pipe, beside the special-function unit, which takes 8 clocks of a warp for every exponential: x = k + f with f in [-1/2, 1/2] (adding 1.5 2^23
+// rounds to whole numbers), a polynomial of degree 3 in f (minimax, relative error 7.5e-5 against 2^-9 of the weights' rounding), k added to the exponent.  At least 2^-125: what is
+// masked adds that to the sum of weights and to none of the products of finite values, as far as fp32 tells.  NaN stays NaN.
+__device__ __forceinline__ f32x2 exp2_poly(f32x2 x) {
+  float x0, x1;
+  split(x, x0, x1);
+  x0 = x0 < -125.f ? -125.f : x0;
+  x1 = x1 < -125.f ? -125.f : x1;
+  x = pair_of(x0, x1);
+  const f32x2 big = pair_of(12582912.f, 12582912.f), t = add2(x, big), k = add2(t, pair_of(-12582912.f, -12582912.f));
+  const f32x2 f = fma2(k, pair_of(-1.f, -1.f), x);
+  f32x2 p = fma2(f, pair_of(0.05517167f, 0.05517167f), pair_of(0.24261112f, 0.24261112f));
+  p = fma2(f, p, pair_of(0.69326099f, 0.69326099f));
+  p = fma2(f, p, pair_of(0.99992807f, 0.99992807f));
+  uint32_t p0, p1, t0, t1;
+  split(p, p0, p1);
+  split(t, t0, t1);
+  return pair_of(p0 + (t0 << 23), p1 + (t1 << 23));
+}
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 __device__ __forceinline__ bool seen_bit(const uint32_t (&m)[4], int c) { return m[c >> 5] >> (c & 31) & 1u; }
+
+__device__ __forceinline__ void give_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_OTHERS)); }
 
 // Row i once more, by a warp, over the keys that it sees and no other.
 __device__ void row_again(const bf16* __restrict__ qkv, long long row_stride, bf16* __restrict__ dst, int i, int first, int h, int g, int H, int Hk, int hd,
@@ -154,11 +200,12 @@ __device__ void row_again(const bf16* __restrict__ qkv, long long row_stride, bf
 }
 
 template <int HD, bool CAP, bool ALIBI>
-__global__ void __launch_bounds__(320, 1) packed_umma_kernel(const __grid_constant__ CUtensorMap map, const bf16* __restrict__ qkv, long long row_stride,
+__global__ void __launch_bounds__(THREADS, 1) packed_umma_kernel(const __grid_constant__ CUtensorMap map, const bf16* __restrict__ qkv, long long row_stride,
                                                              const int* __restrict__ cu, int S, const float* __restrict__ slopes, bf16* __restrict__ out,
                                                              long long out_stride, int rows, int H, int Hk, int hd, int window, float scale,
                                                              float softcap, int* status) {
   typedef Smem<HD> L;
+  constexpr int POLY = CAP ? 1 : POLY_OF_8;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   __shared__ Ctl ctl;
@@ -170,7 +217,8 @@ __global__ void __launch_bounds__(320, 1) packed_umma_kernel(const __grid_consta
     for (int i = 0; i < 2; i++) {
       tma::mbar_init(&ctl.q_full[i], 1);
       tma::mbar_init(&ctl.s_full[i], 1);
-      tma::mbar_init(&ctl.p_full[i], 128);
+      tma::mbar_init(&ctl.p_full[i][0], 128);
+      tma::mbar_init(&ctl.p_full[i][1], 128);
       tma::mbar_init(&ctl.pv_done[i], 1);
     }
     for (int s = 0; s < STAGES; s++) {
@@ -180,7 +228,6 @@ __global__ void __launch_bounds__(320, 1) packed_umma_kernel(const __grid_consta
     ctl.abort_flag = 0;
     tma::fence_barrier_init();
   }
-  if (threadIdx.x < 2 * BM / 32) ctl.again[threadIdx.x] = 0;
   if (warp == 8) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(tma::smem_u32(&ctl.tmem_slot)));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
@@ -188,7 +235,7 @@ __global__ void __launch_bounds__(320, 1) packed_umma_kernel(const __grid_consta
   // The sequences of the first and of the last row of the CTA (counted by all threads: one reading of cu, however many there are), and every row's first key
   const int row_lo = max(q0, cu[0]), row_hi = min(min(q0 + 2 * BM, rows), cu[S]) - 1;   // rows of sequences
   int below = 0, upto = 0;
-  for (int s0 = 0; s0 < S; s0 += 320) {   // (block-uniform)
+  for (int s0 = 0; s0 < S; s0 += THREADS) {   // (block-uniform)
     const int at = s0 + threadIdx.x < S ? cu[s0 + threadIdx.x] : 0x7fffffff;
     below += __syncthreads_count(at <= row_lo);
     upto += __syncthreads_count(at <= row_hi);
@@ -216,6 +263,7 @@ __global__ void __launch_bounds__(320, 1) packed_umma_kernel(const __grid_consta
 
   if (warp == 9) {
     // ------------------------------------------------------------------ producer
+    give_registers();
     const bool leader = elect_one();
     auto load = [&](unsigned char* dst, uint64_t* bar, int head, int row) {
       if (leader) {
@@ -241,6 +289,7 @@ __global__ void __launch_bounds__(320, 1) packed_umma_kernel(const __grid_consta
     }
   } else if (warp == 8) {
     // ------------------------------------------------------------------ MMA issuer
+    give_registers();
     const bool leader = elect_one();
     const uint32_t base = tma::smem_u32(smem);
     bool ok = true;
@@ -251,14 +300,22 @@ __global__ void __launch_bounds__(320, 1) packed_umma_kernel(const __grid_consta
       for (int i = 0; ok && i < 2; i++) {
         if (active(i, t - 1)) {
           const int n = t - 1 - begin[i];
-          ok = tma::warp_wait_bounded(&ctl.p_full[i], (uint32_t)n & 1u, abort_flag) && wait_kv(nv);
-          if (!ok) break;
-          fence_after();
-          if (leader) {
-            const uint64_t v = desc_mn(stage_of(nv));
+          ok = wait_kv(nv);
+          const uint64_t v = desc_mn(stage_of(nv));
 #pragma unroll
-            for (int kk = 0; kk < BN / 16; kk++)
-              umma_ts(tmem + 256 + i * HD, tmem + i * 128 + kk * 8, v + (uint64_t)(kk * (2048 >> 4)), idesc(HD, true), (n | kk) ? 1u : 0u);
+          for (int half = 0; half < 2; half++) {   // (the first 64 keys' weights come while the others' are made)
+            ok = ok && tma::warp_wait_bounded(&ctl.p_full[i][half], (uint32_t)n & 1u, abort_flag);
+            if (!ok) break;
+            fence_after();
+            if (leader) {
+#pragma unroll
+              for (int kk = half * 4; kk < half * 4 + 4; kk++)
+                umma_ts(tmem + 256 + i * HD, tmem + i * 128 + kk * 8, v + (uint64_t)(kk * (2048 >> 4)), idesc(HD, true), (n | kk) ? 1u : 0u);
+            }
+            __syncwarp();
+          }
+          if (!ok) break;
+          if (leader) {
             umma_commit(&ctl.pv_done[i]);
             if (i == 1 || !active(1, t - 1)) umma_commit(&ctl.kv_empty[nv % STAGES]);
           }
@@ -283,8 +340,9 @@ __global__ void __launch_bounds__(320, 1) packed_umma_kernel(const __grid_consta
         }
       }
     }
-  } else {
+  } else if (warp < 8) {
     // -------------------------------------------------------------------- softmax warps (a quarter of the lanes of tensor memory each)
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_SOFTMAX));
     const int tile = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane;
     const int i = q0 + tile * BM + row, first = ctl.first[tile * BM + row];
     const int last_first = max(row_lo, q0 + tile * BM) <= min(row_hi, q0 + tile * BM + BM - 1) ? ctl.first[min(row_hi, q0 + tile * BM + BM - 1) - q0] : 0;
@@ -295,9 +353,9 @@ __global__ void __launch_bounds__(320, 1) packed_umma_kernel(const __grid_consta
     const float kk0 = k0 * k0;
     const f32x2 cap0 = pair_of(k0 * k1 * T0, k0 * k1 * T0), cap1 = pair_of(k0 * k1 * kk0 * T1, k0 * k1 * kk0 * T1),
                 cap2 = pair_of(k0 * k1 * kk0 * kk0 * T2, k0 * k1 * kk0 * kk0 * T2), kp = pair_of(k1, k1), cc = pair_of(c2, c2);
-    const float most_small = CAP ? 0.25f / kk0 : 0.f;   // tanh(s k0) k1 = s (cap0 + cap1 s^2 + cap2 s^4) while s^2 is below it
-    float m_ref = -INFINITY, l = 0.f;
-    bool ok = true;
+    const float most_small = CAP ? 0.5f / k0 : 0.f;   // tanh(s k0) k1 = s (cap0 + cap1 s^2 + cap2 s^4) while |s| is below it
+    float ref = 0.f, l = 0.f;   // what scores are counted from: the row's maximum, or one that it has outgrown by less than LAG
+    bool any_key = false, ok = true;
     const int nt = end[tile] - begin[tile];
     for (int n = 0; n < nt; n++) {
       const int jt = (begin[tile] + n) * BN;
@@ -307,7 +365,7 @@ __global__ void __launch_bounds__(320, 1) packed_umma_kernel(const __grid_consta
       uint32_t sr[128];
 #pragma unroll
       for (int c = 0; c < 4; c++) tmem_ld32(tm_s + c * 32, sr + c * 32);
-      tmem_wait_ld();
+      tmem_wait_ld(sr);
       const bool interior = whole && jt >= last_first && jt + BN - 1 <= q0 + tile * BM;   // all rows of the tile see all keys of this one
       uint32_t seen[4];
       if (!interior) {
@@ -318,101 +376,103 @@ __global__ void __launch_bounds__(320, 1) packed_umma_kernel(const __grid_consta
           seen[w] = a > b ? 0u : (0xffffffffu >> (31 - (b - a))) << a;
         }
       }
-      const float base_t = ALIBI ? c2 * (float)(jt - i) : 0.f;
+      // scores in the exp2 domain, counted from ref: s k1 (or its cap) + c2 (j - i) - ref
+      const float base_t = ALIBI ? fmaf(c2, (float)(jt - i), -ref) : -ref;
+      const f32x2 bt = pair_of(base_t, base_t);
       if (CAP) {
         if (!interior) {   // a masked score decides nothing
 #pragma unroll
           for (int c = 0; c < 128; c++)
             if (!seen_bit(seen, c)) sr[c] = 0;
         }
-        float most = 0.f;   // the largest square (a NaN score is not in it: both forms carry it on)
-        const f32x2 bt = pair_of(base_t, base_t);
+        float most[4] = {0.f, 0.f, 0.f, 0.f};   // (a NaN score is not in it: both forms carry it on)
 #pragma unroll
         for (int c = 0; c < 128; c += 2) {
+          most[c >> 1 & 3] = max3(most[c >> 1 & 3], fabsf(__uint_as_float(sr[c])), fabsf(__uint_as_float(sr[c + 1])));
           const f32x2 sv = pair_of(sr[c], sr[c + 1]), sq = mul2(sv, sv);
-          float s0, s1;
-          split(sq, s0, s1);
-          most = fmaxf(most, fmaxf(s0, s1));
           const f32x2 p = fma2(sq, fma2(sq, cap2, cap1), cap0);
-          split(ALIBI ? fma2(sv, p, fma2(cc, pair_of((float)c, (float)(c + 1)), bt)) : mul2(sv, p), sr[c], sr[c + 1]);
+          split(fma2(sv, p, ALIBI ? fma2(cc, pair_of((float)c, (float)(c + 1)), bt) : bt), sr[c], sr[c + 1]);
         }
-        const bool large = !(most < most_small);   // (a row's own scores decide for it)
+        const bool large = !(fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])) < most_small);   // (a row's own scores decide for it)
         if (__any_sync(0xffffffffu, large)) {
 #pragma unroll
           for (int q = 0; q < 4; q++) {
             uint32_t raw[32];
             tmem_ld32(tm_s + q * 32, raw);
-            tmem_wait_ld();
+            tmem_wait_ld(raw);
 #pragma unroll
             for (int c = 0; c < 32; c++) {
               float th;   // the hardware's: relative error 2^-11
               asm("tanh.approx.f32 %0, %1;" : "=f"(th) : "f"(__uint_as_float(raw[c]) * k0));
-              if (large) sr[q * 32 + c] = __float_as_uint(ALIBI ? fmaf(th, k1, fmaf(c2, (float)(q * 32 + c), base_t)) : th * k1);
+              if (large) sr[q * 32 + c] = __float_as_uint(fmaf(th, k1, ALIBI ? fmaf(c2, (float)(q * 32 + c), base_t) : base_t));
             }
           }
         }
       } else {
-        const f32x2 bt = pair_of(base_t, base_t);
 #pragma unroll
-        for (int c = 0; c < 128; c += 2) {
-          const f32x2 sv = pair_of(sr[c], sr[c + 1]);
-          split(ALIBI ? fma2(sv, kp, fma2(cc, pair_of((float)c, (float)(c + 1)), bt)) : mul2(sv, kp), sr[c], sr[c + 1]);
-        }
+        for (int c = 0; c < 128; c += 2)
+          split(fma2(pair_of(sr[c], sr[c + 1]), kp, ALIBI ? fma2(cc, pair_of((float)c, (float)(c + 1)), bt) : bt), sr[c], sr[c + 1]);
       }
       if (!interior) {
 #pragma unroll
         for (int c = 0; c < 128; c++)
           if (!seen_bit(seen, c)) sr[c] = 0xff800000u;   // -infinity
       }
-      float mx[4];
+      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int c = 0; c < 4; c++) mx[c] = fmaxf(__uint_as_float(sr[c]), __uint_as_float(sr[c + 4]));
-#pragma unroll
-      for (int c = 8; c < 128; c += 8)
-#pragma unroll
-        for (int e = 0; e < 4; e++) mx[e] = fmaxf(mx[e], fmaxf(__uint_as_float(sr[c + e]), __uint_as_float(sr[c + e + 4])));
+      for (int c = 0; c < 128; c += 2) mx[c >> 1 & 3] = max3(mx[c >> 1 & 3], __uint_as_float(sr[c]), __uint_as_float(sr[c + 1]));
       const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-      const bool grow = top > m_ref + LAG || (m_ref == -INFINITY && top > -INFINITY);
-      if (__any_sync(0xffffffffu, grow)) {
-        const float m_new = fmaxf(m_ref, top), corr = m_new == -INFINITY ? 1.f : exp2_hw(m_ref - m_new);   // 0 for a row that had no key yet
-        m_ref = m_new;
+      if (__any_sync(0xffffffffu, top > LAG || (!any_key && top > -INFINITY))) {
+        const float shift = any_key ? fmaxf(top, 0.f) : top > -INFINITY ? top : 0.f, corr = any_key ? exp2_hw(-shift) : top > -INFINITY ? 0.f : 1.f;
+        any_key |= top > -INFINITY;
+        ref += shift;
         l *= corr;
+        const f32x2 neg = pair_of(-shift, -shift);
+#pragma unroll
+        for (int c = 0; c < 128; c += 2) split(add2(pair_of(sr[c], sr[c + 1]), neg), sr[c], sr[c + 1]);
         if (n > 0) {
           ok = tma::warp_wait_bounded(&ctl.pv_done[tile], (uint32_t)(n - 1) & 1u, abort_flag);
           if (!ok) break;
           fence_after();
 #pragma unroll 1
-          for (int c = 0; c < HD / 32; c++) {
-            uint32_t o[32];
-            tmem_ld32(tm_o + c * 32, o);
-            tmem_wait_ld();
+          for (int c = 0; c < HD / 16; c++) {
+            uint32_t o[16];
+            tmem_ld16(tm_o + c * 16, o);
+            tmem_wait_ld(o);
 #pragma unroll
-            for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * corr);
-            tmem_st32(tm_o + c * 32, o);
+            for (int e = 0; e < 16; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * corr);
+            tmem_st16(tm_o + c * 16, o);
           }
           tmem_wait_st();
         }
       }
-      const float ref = m_ref == -INFINITY ? 0.f : m_ref;
-      const f32x2 neg = pair_of(-ref, -ref);
       f32x2 sum[2] = {0, 0};
 #pragma unroll
-      for (int c = 0; c < 128; c += 2) {
-        float p0, p1;
-        split(add2(pair_of(sr[c], sr[c + 1]), neg), p0, p1);
-        p0 = exp2_hw(p0);
-        p1 = exp2_hw(p1);
-        sum[c >> 1 & 1] = add2(sum[c >> 1 & 1], pair_of(p0, p1));
-        sr[c >> 1] = pack_bf16(p0, p1);
+      for (int half = 0; half < 2; half++) {
+#pragma unroll
+        for (int c = half * 64; c < half * 64 + 64; c += 2) {
+          const f32x2 x = pair_of(sr[c], sr[c + 1]);
+          f32x2 p;
+          if ((c >> 1) % 8 < POLY) {
+            p = exp2_poly(x);
+          } else {
+            float p0, p1;
+            split(x, p0, p1);
+            p = pair_of(exp2_hw(p0), exp2_hw(p1));
+          }
+          sum[c >> 1 & 1] = add2(sum[c >> 1 & 1], p);
+          float p0, p1;
+          split(p, p0, p1);
+          sr[c >> 1] = pack_bf16(p0, p1);
+        }
+        tmem_st32(tm_s + half * 32, sr + half * 32);
+        tmem_wait_st();
+        fence_before();
+        tma::mbar_arrive(&ctl.p_full[tile][half]);
       }
       float s0, s1;
       split(add2(sum[0], sum[1]), s0, s1);
       l += s0 + s1;
-      tmem_st32(tm_s, sr);
-      tmem_st32(tm_s + 32, sr + 32);
-      tmem_wait_st();
-      fence_before();
-      tma::mbar_arrive(&ctl.p_full[tile]);
     }
     if (ok && nt > 0) ok = tma::warp_wait_bounded(&ctl.pv_done[tile], (uint32_t)(nt - 1) & 1u, abort_flag);
     if (ok && nt > 0) {
@@ -424,7 +484,7 @@ __global__ void __launch_bounds__(320, 1) packed_umma_kernel(const __grid_consta
       for (int c = 0; c < HD / 32; c++) {
         uint32_t o[32];
         tmem_ld32(tm_o + c * 32, o);
-        tmem_wait_ld();
+        tmem_wait_ld(o);
         if (first != packed::NOBODY) {
 #pragma unroll
           for (int v = 0; v < 4; v++) {
@@ -440,9 +500,16 @@ __global__ void __launch_bounds__(320, 1) packed_umma_kernel(const __grid_consta
           }
         }
       }
-      if (!finite && fabsf(l) < INFINITY) atomicOr(&ctl.again[tile * 4 + quarter], 1u << lane);
+      uint32_t again = __ballot_sync(0xffffffffu, !finite && fabsf(l) < INFINITY);
+      for (; again; again &= again - 1) {   // (stored above by the row's thread, here by all of them: the ballot has ordered the two)
+        const int r = tile * BM + quarter * 32 + __ffs(again) - 1;
+        row_again(qkv, row_stride, out + (long long)(q0 + r) * out_stride + (long long)h * hd, q0 + r, ctl.first[r], h, g, H, Hk, hd, ALIBI ? slopes[h] : 0.f,
+                  scale, CAP ? softcap : 0.f, lane);
+      }
     }
     fence_before();
+  } else {
+    give_registers();
   }
   __syncthreads();
   if (*abort_flag) {
@@ -457,10 +524,6 @@ __global__ void __launch_bounds__(320, 1) packed_umma_kernel(const __grid_consta
     fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
   }
-  for (int r = warp; r < 2 * BM; r += 10)
-    if (ctl.again[r >> 5] >> (r & 31) & 1u)
-      row_again(qkv, row_stride, out + (long long)(q0 + r) * out_stride + (long long)h * hd, q0 + r, ctl.first[r], h, g, H, Hk, hd, ALIBI ? slopes[h] : 0.f,
-                scale, CAP ? softcap : 0.f, lane);
 }
 
 template <int HD, bool CAP, bool ALIBI>
@@ -469,7 +532,7 @@ int launch(const CUtensorMap& map, const void* qkv, long long row_stride, const 
   static SmemLimit limit;
   const cudaError_t e = allow_smem((const void*)packed_umma_kernel<HD, CAP, ALIBI>, Smem<HD>::BYTES, limit);
   if (e != cudaSuccess) return (int)e;
-  packed_umma_kernel<HD, CAP, ALIBI><<<dim3((unsigned)((rows + 2 * BM - 1) / (2 * BM)), H), 320, Smem<HD>::BYTES, st>>>(
+  packed_umma_kernel<HD, CAP, ALIBI><<<dim3((unsigned)((rows + 2 * BM - 1) / (2 * BM)), H), THREADS, Smem<HD>::BYTES, st>>>(
       map, (const bf16*)qkv, row_stride, cu, S, slopes, (bf16*)out, out_stride, rows, H, Hk, hd, window, 1.0f / sqrtf((float)hd), softcap, status);
   STU_CHECK_LAUNCH();
   return STU_OK;
