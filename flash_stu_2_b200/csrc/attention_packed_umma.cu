@@ -10,6 +10,8 @@
 //   O += P V    tcgen05.mma, P from tensor memory, V as it lies (rows of keys: the operand whose rows are the sum's index), accumulating in tensor memory
 // The two tiles' S and O are the 512 columns that there are, so P has to take S's place; the next S of a tile is issued behind the product
 // that reads its P, and a CTA's products run in the order of issue.
+// With ALiBi the maximum is taken for what it will be at the row's end if the scores stay as they are.  Where they do not, all of a row's weights may be too small for fp32:
+// the row is computed again, as below.
 // The tensor core adds 0 times what a masked key's value holds: where that is NaN or infinite, a row with a finite sum of weights has a result that is not, and is
 // computed again on the CUDA cores over the keys that it sees.
 #include <cuda.h>
@@ -27,10 +29,13 @@ constexpr int STATUS_PACKED = 13;
 constexpr float LOG2E = 1.4426950408889634f;
 // tanh(y) = y (T0 + T1 y^2 + T2 y^4) for |y| <= 1/2: relative error 2.3e-5
 constexpr float T0 = 0.999977239f, T1 = -0.331685329f, T2 = 0.115185198f;
-constexpr float LAG = 8.f;
+// ... = y (T0_TINY + T1_TINY y^2) for |y| <= 1/5: 2.6e-5
+constexpr float T0_TINY = 0.999973796f, T1_TINY = -0.328076375f;
+// How far a score may outgrow what scores are counted from; the least sum of weights (what it leaves out is below 2^-126 a key)
+constexpr float LAG = 8.f, LEAST = 0x1p-90f;
 
-// Of 8 pairs of weights those that the FMA pipe makes
-constexpr int POLY_OF_8 = 2;
+// Of 8 pairs of weights those that the FMA pipe makes; pairs whose arithmetic is interleaved
+constexpr int POLY_OF_8 = 2, ILP = 8;
 
 template <int HD> struct Smem {
   static constexpr int KB = HD / 64;                   // blocks of 64 dimensions
@@ -148,21 +153,33 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 // 2^x on the FMA pipe, beside the special-function unit, which takes 8 clocks of a warp for every exponential: x = k + f with f in [-1/2, 1/2] (adding 1.5 2^23
 // rounds to whole numbers), a polynomial of degree 3 in f (minimax, relative error 7.5e-5 against 2^-9 of the weights' rounding), k added to the exponent.  At least 2^-125: what is
 // masked adds that to the sum of weights and to none of the products of finite values, as far as fp32 tells.  NaN stays NaN.
-__device__ __forceinline__ f32x2 exp2_poly(f32x2 x) {
-  float x0, x1;
-  split(x, x0, x1);
-  x0 = x0 < -125.f ? -125.f : x0;
-  x1 = x1 < -125.f ? -125.f : x1;
-  x = pair_of(x0, x1);
-  const f32x2 big = pair_of(12582912.f, 12582912.f), t = add2(x, big), k = add2(t, pair_of(-12582912.f, -12582912.f));
-  const f32x2 f = fma2(k, pair_of(-1.f, -1.f), x);
-  f32x2 p = fma2(f, pair_of(0.05517167f, 0.05517167f), pair_of(0.24261112f, 0.24261112f));
-  p = fma2(f, p, pair_of(0.69326099f, 0.69326099f));
-  p = fma2(f, p, pair_of(0.99992807f, 0.99992807f));
-  uint32_t p0, p1, t0, t1;
-  split(p, p0, p1);
-  split(t, t0, t1);
-  return pair_of(p0 + (t0 << 23), p1 + (t1 << 23));
+template <int N> __device__ __forceinline__ void exp2_poly(const uint32_t* x, f32x2* y) {
+  f32x2 f[N], t[N], p[N];
+  const f32x2 big = pair_of(12582912.f, 12582912.f), unbig = pair_of(-12582912.f, -12582912.f), minus = pair_of(-1.f, -1.f);
+#pragma unroll
+  for (int u = 0; u < N; u++) {
+    const float x0 = __uint_as_float(x[2 * u]), x1 = __uint_as_float(x[2 * u + 1]);
+    f[u] = pair_of(x0 < -125.f ? -125.f : x0, x1 < -125.f ? -125.f : x1);
+  }
+#pragma unroll
+  for (int u = 0; u < N; u++) t[u] = add2(f[u], big);
+#pragma unroll
+  for (int u = 0; u < N; u++) p[u] = add2(t[u], unbig);
+#pragma unroll
+  for (int u = 0; u < N; u++) f[u] = fma2(p[u], minus, f[u]);
+#pragma unroll
+  for (int u = 0; u < N; u++) p[u] = fma2(f[u], pair_of(0.05517167f, 0.05517167f), pair_of(0.24261112f, 0.24261112f));
+#pragma unroll
+  for (int u = 0; u < N; u++) p[u] = fma2(f[u], p[u], pair_of(0.69326099f, 0.69326099f));
+#pragma unroll
+  for (int u = 0; u < N; u++) p[u] = fma2(f[u], p[u], pair_of(0.99992807f, 0.99992807f));
+#pragma unroll
+  for (int u = 0; u < N; u++) {
+    uint32_t p0, p1, t0, t1;
+    split(p[u], p0, p1);
+    split(t[u], t0, t1);
+    y[u] = pair_of(p0 + (t0 << 23), p1 + (t1 << 23));
+  }
 }
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
@@ -171,6 +188,42 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
 __device__ __forceinline__ bool seen_bit(const uint32_t (&m)[4], int c) { return m[c >> 5] >> (c & 31) & 1u; }
 
 __device__ __forceinline__ void give_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_OTHERS)); }
+
+// A bounded wait whose first look costs little: most of these barriers have completed by the time they are asked for (tma::warp_wait_bounded takes 115 clocks
+// then, of the 1024 that a tile's two products take).
+__device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  if (__all_sync(0xffffffffu, tma::mbar_try_wait(bar, parity))) return true;
+  return tma::warp_wait_bounded(bar, parity, abort_flag);
+}
+
+// 128 scores s -> cap(s) + c2 (column) + bt, by the polynomial of degree 2 or 1 in s^2, eight pairs at a time
+template <bool SMALL, bool ALIBI>
+__device__ __forceinline__ void capped(uint32_t (&sr)[128], f32x2 cap0, f32x2 cap1, f32x2 cap2, f32x2 tiny0, f32x2 tiny1, f32x2 cc, f32x2 bt) {
+  f32x2 add[ILP];
+#pragma unroll
+  for (int u = 0; u < ILP; u++) add[u] = ALIBI ? fma2(cc, pair_of((float)(2 * u), (float)(2 * u + 1)), bt) : bt;
+  const f32x2 further = mul2(cc, pair_of(2.f * ILP, 2.f * ILP));
+#pragma unroll
+  for (int c0 = 0; c0 < 128; c0 += 2 * ILP) {
+    f32x2 sv[ILP], sq[ILP], p[ILP];
+#pragma unroll
+    for (int u = 0; u < ILP; u++) sv[u] = pair_of(sr[c0 + 2 * u], sr[c0 + 2 * u + 1]);
+#pragma unroll
+    for (int u = 0; u < ILP; u++) sq[u] = mul2(sv[u], sv[u]);
+#pragma unroll
+    for (int u = 0; u < ILP; u++) p[u] = SMALL ? fma2(sq[u], cap2, cap1) : fma2(sq[u], tiny1, tiny0);
+    if (SMALL) {
+#pragma unroll
+      for (int u = 0; u < ILP; u++) p[u] = fma2(sq[u], p[u], cap0);
+    }
+#pragma unroll
+    for (int u = 0; u < ILP; u++) split(fma2(sv[u], p[u], add[u]), sr[c0 + 2 * u], sr[c0 + 2 * u + 1]);
+    if (ALIBI && c0 + 2 * ILP < 128) {
+#pragma unroll
+      for (int u = 0; u < ILP; u++) add[u] = add2(add[u], further);
+    }
+  }
+}
 
 // Row i once more, by a warp, over the keys that it sees and no other.
 __device__ void row_again(const bf16* __restrict__ qkv, long long row_stride, bf16* __restrict__ dst, int i, int first, int h, int g, int H, int Hk, int hd,
@@ -205,7 +258,7 @@ __global__ void __launch_bounds__(THREADS, 1) packed_umma_kernel(const __grid_co
                                                              long long out_stride, int rows, int H, int Hk, int hd, int window, float scale,
                                                              float softcap, int* status) {
   typedef Smem<HD> L;
-  constexpr int POLY = CAP ? 1 : POLY_OF_8;
+  constexpr int POLY = CAP ? 2 : POLY_OF_8;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   __shared__ Ctl ctl;
@@ -217,8 +270,8 @@ __global__ void __launch_bounds__(THREADS, 1) packed_umma_kernel(const __grid_co
     for (int i = 0; i < 2; i++) {
       tma::mbar_init(&ctl.q_full[i], 1);
       tma::mbar_init(&ctl.s_full[i], 1);
-      tma::mbar_init(&ctl.p_full[i][0], 128);
-      tma::mbar_init(&ctl.p_full[i][1], 128);
+      tma::mbar_init(&ctl.p_full[i][0], 4);
+      tma::mbar_init(&ctl.p_full[i][1], 4);
       tma::mbar_init(&ctl.pv_done[i], 1);
     }
     for (int s = 0; s < STAGES; s++) {
@@ -294,17 +347,23 @@ __global__ void __launch_bounds__(THREADS, 1) packed_umma_kernel(const __grid_co
     const uint32_t base = tma::smem_u32(smem);
     bool ok = true;
     auto stage_of = [&](int n) { return base + L::KV + (uint32_t)(n % STAGES) * L::TILE; };
-    auto wait_kv = [&](int n) { return tma::warp_wait_bounded(&ctl.kv_full[n % STAGES], (uint32_t)(n / STAGES) & 1u, abort_flag); };
+    int landed = 0;   // stages that have been waited for
+    auto wait_kv = [&](int n) {
+      for (; ok && landed <= n; landed++) ok = wait_for(&ctl.kv_full[landed % STAGES], (uint32_t)(landed / STAGES) & 1u, abort_flag);
+      return ok;
+    };
     for (int t = t_lo; ok && t <= t_hi; t++) {
       const int nk = 2 * (t - t_lo), nv = nk - 1;   // the stages of K of t and V of t - 1
-      for (int i = 0; ok && i < 2; i++) {
-        if (active(i, t - 1)) {
-          const int n = t - 1 - begin[i];
-          ok = wait_kv(nv);
-          const uint64_t v = desc_mn(stage_of(nv));
+      const uint64_t k = desc_k(stage_of(nk)), v = desc_mn(stage_of(nv + STAGES));
+#pragma unroll
+      for (int i = 0; i < 2; i++) {
+        const bool product = active(i, t - 1), scores = active(i, t);
+        if (!wait_kv(scores ? nk : nv)) break;
+        if (product) {
+          const uint32_t n = (uint32_t)(t - 1 - begin[i]);
 #pragma unroll
           for (int half = 0; half < 2; half++) {   // (the first 64 keys' weights come while the others' are made)
-            ok = ok && tma::warp_wait_bounded(&ctl.p_full[i][half], (uint32_t)n & 1u, abort_flag);
+            ok = ok && wait_for(&ctl.p_full[i][half], n & 1u, abort_flag);
             if (!ok) break;
             fence_after();
             if (leader) {
@@ -315,29 +374,29 @@ __global__ void __launch_bounds__(THREADS, 1) packed_umma_kernel(const __grid_co
             __syncwarp();
           }
           if (!ok) break;
-          if (leader) {
-            umma_commit(&ctl.pv_done[i]);
-            if (i == 1 || !active(1, t - 1)) umma_commit(&ctl.kv_empty[nv % STAGES]);
-          }
-          __syncwarp();
+          if (leader && !scores) umma_commit(&ctl.pv_done[i]);   // the tile's last
         }
-        if (active(i, t)) {
-          if (t == begin[i]) ok = tma::warp_wait_bounded(&ctl.q_full[i], 0, abort_flag);
-          ok = ok && wait_kv(nk);
-          if (!ok) break;
+        if (scores) {
+          if (t == begin[i]) {
+            ok = wait_for(&ctl.q_full[i], 0, abort_flag);
+            if (!ok) break;
+          }
           fence_after();
           if (leader) {
+            const uint64_t q = desc_k(base + i * L::TILE);
 #pragma unroll
             for (int kb = 0; kb < L::KB; kb++)
 #pragma unroll
               for (int kk = 0; kk < 4; kk++)
-                umma_ss(tmem + i * 128, desc_k(base + i * L::TILE + kb * 16384) + 2 * kk, desc_k(stage_of(nk) + kb * 16384) + 2 * kk, idesc(BN, false),
-                        (kb | kk) ? 1u : 0u);
-            umma_commit(&ctl.s_full[i]);
-            if (i == 1 || !active(1, t)) umma_commit(&ctl.kv_empty[nk % STAGES]);
+                umma_ss(tmem + i * 128, q + kb * (16384 >> 4) + 2 * kk, k + kb * (16384 >> 4) + 2 * kk, idesc(BN, false), (kb | kk) ? 1u : 0u);
+            umma_commit(&ctl.s_full[i]);   // (the products before are complete then, too)
           }
-          __syncwarp();
         }
+        if (leader) {
+          if (product && (i == 1 || !active(1, t - 1))) umma_commit(&ctl.kv_empty[(nv + STAGES) % STAGES]);
+          if (scores && (i == 1 || !active(1, t))) umma_commit(&ctl.kv_empty[nk % STAGES]);
+        }
+        __syncwarp();
       }
     }
   } else if (warp < 8) {
@@ -351,15 +410,17 @@ __global__ void __launch_bounds__(THREADS, 1) packed_umma_kernel(const __grid_co
     const float c2 = ALIBI ? slopes[h] * LOG2E : 0.f;
     const float k0 = CAP ? scale / softcap : 0.f, k1 = CAP ? softcap * LOG2E : scale * LOG2E;
     const float kk0 = k0 * k0;
+    // tanh(s k0) k1 = s times a polynomial in s^2, while |s| is below most_tiny (degree 1) or most_small (degree 2)
     const f32x2 cap0 = pair_of(k0 * k1 * T0, k0 * k1 * T0), cap1 = pair_of(k0 * k1 * kk0 * T1, k0 * k1 * kk0 * T1),
                 cap2 = pair_of(k0 * k1 * kk0 * kk0 * T2, k0 * k1 * kk0 * kk0 * T2), kp = pair_of(k1, k1), cc = pair_of(c2, c2);
-    const float most_small = CAP ? 0.5f / k0 : 0.f;   // tanh(s k0) k1 = s (cap0 + cap1 s^2 + cap2 s^4) while |s| is below it
+    const f32x2 cap_tiny0 = pair_of(k0 * k1 * T0_TINY, k0 * k1 * T0_TINY), cap_tiny1 = pair_of(k0 * k1 * kk0 * T1_TINY, k0 * k1 * kk0 * T1_TINY);
+    const float most_tiny = CAP ? 0.2f / k0 : 0.f, most_small = CAP ? 0.5f / k0 : 0.f;
     float ref = 0.f, l = 0.f;   // what scores are counted from: the row's maximum, or one that it has outgrown by less than LAG
     bool any_key = false, ok = true;
     const int nt = end[tile] - begin[tile];
     for (int n = 0; n < nt; n++) {
       const int jt = (begin[tile] + n) * BN;
-      ok = tma::warp_wait_bounded(&ctl.s_full[tile], (uint32_t)n & 1u, abort_flag);
+      ok = wait_for(&ctl.s_full[tile], (uint32_t)n & 1u, abort_flag);
       if (!ok) break;
       fence_after();
       uint32_t sr[128];
@@ -385,15 +446,13 @@ __global__ void __launch_bounds__(THREADS, 1) packed_umma_kernel(const __grid_co
           for (int c = 0; c < 128; c++)
             if (!seen_bit(seen, c)) sr[c] = 0;
         }
-        float most[4] = {0.f, 0.f, 0.f, 0.f};   // (a NaN score is not in it: both forms carry it on)
+        float most[4] = {0.f, 0.f, 0.f, 0.f};   // (a NaN score is not in it: every form carries it on)
 #pragma unroll
-        for (int c = 0; c < 128; c += 2) {
-          most[c >> 1 & 3] = max3(most[c >> 1 & 3], fabsf(__uint_as_float(sr[c])), fabsf(__uint_as_float(sr[c + 1])));
-          const f32x2 sv = pair_of(sr[c], sr[c + 1]), sq = mul2(sv, sv);
-          const f32x2 p = fma2(sq, fma2(sq, cap2, cap1), cap0);
-          split(fma2(sv, p, ALIBI ? fma2(cc, pair_of((float)c, (float)(c + 1)), bt) : bt), sr[c], sr[c + 1]);
-        }
-        const bool large = !(fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])) < most_small);   // (a row's own scores decide for it)
+        for (int c = 0; c < 128; c += 2) most[c >> 1 & 3] = max3(most[c >> 1 & 3], fabsf(__uint_as_float(sr[c])), fabsf(__uint_as_float(sr[c + 1])));
+        const float biggest = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
+        if (__all_sync(0xffffffffu, biggest < most_tiny)) capped<false, ALIBI>(sr, cap0, cap1, cap2, cap_tiny0, cap_tiny1, cc, bt);
+        else capped<true, ALIBI>(sr, cap0, cap1, cap2, cap_tiny0, cap_tiny1, cc, bt);
+        const bool large = !(biggest < most_small);
         if (__any_sync(0xffffffffu, large)) {
 #pragma unroll
           for (int q = 0; q < 4; q++) {
@@ -422,20 +481,19 @@ __global__ void __launch_bounds__(THREADS, 1) packed_umma_kernel(const __grid_co
 #pragma unroll
       for (int c = 0; c < 128; c += 2) mx[c >> 1 & 3] = max3(mx[c >> 1 & 3], __uint_as_float(sr[c]), __uint_as_float(sr[c + 1]));
       const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-      if (__any_sync(0xffffffffu, top > LAG || (!any_key && top > -INFINITY))) {
-        const float shift = any_key ? fmaxf(top, 0.f) : top > -INFINITY ? top : 0.f, corr = any_key ? exp2_hw(-shift) : top > -INFINITY ? 0.f : 1.f;
-        any_key |= top > -INFINITY;
+      const bool grow = top > (any_key ? LAG : -INFINITY);   // the row has outgrown ref, or has its first key: ref moves, and what has been summed up shrinks
+      if (__any_sync(0xffffffffu, grow)) {
+        // (ALiBi alone lifts what is to come by up to c2 (i - the last key here): ref is set as high, or heads with steep slopes would move it in every tile)
+        const float rise = ALIBI ? c2 * (float)max(i - jt - (BN - 1), 0) : 0.f;
+        const float shift = grow ? top + rise : 0.f, corr = grow && any_key ? exp2_hw(-shift) : 1.f;
+        const f32x2 neg = pair_of(-shift, -shift);
         ref += shift;
         l *= corr;
-        const f32x2 neg = pair_of(-shift, -shift);
 #pragma unroll
         for (int c = 0; c < 128; c += 2) split(add2(pair_of(sr[c], sr[c + 1]), neg), sr[c], sr[c + 1]);
-        if (n > 0) {
-          ok = tma::warp_wait_bounded(&ctl.pv_done[tile], (uint32_t)(n - 1) & 1u, abort_flag);
-          if (!ok) break;
-          fence_after();
+        if (__any_sync(0xffffffffu, corr != 1.f)) {
 #pragma unroll 1
-          for (int c = 0; c < HD / 16; c++) {
+          for (int c = 0; c < HD / 16; c++) {   // (the product of the tile before is complete: these scores were issued behind it)
             uint32_t o[16];
             tmem_ld16(tm_o + c * 16, o);
             tmem_wait_ld(o);
@@ -445,36 +503,37 @@ __global__ void __launch_bounds__(THREADS, 1) packed_umma_kernel(const __grid_co
           }
           tmem_wait_st();
         }
+        any_key |= grow;
       }
       f32x2 sum[2] = {0, 0};
 #pragma unroll
       for (int half = 0; half < 2; half++) {
 #pragma unroll
-        for (int c = half * 64; c < half * 64 + 64; c += 2) {
-          const f32x2 x = pair_of(sr[c], sr[c + 1]);
-          f32x2 p;
-          if ((c >> 1) % 8 < POLY) {
-            p = exp2_poly(x);
-          } else {
+        for (int c0 = half * 64; c0 < half * 64 + 64; c0 += 16) {   // 8 pairs: the first POLY of them on the FMA pipe
+          f32x2 p[8];
+          exp2_poly<POLY>(sr + c0, p);
+#pragma unroll
+          for (int u = POLY; u < 8; u++) p[u] = pair_of(exp2_hw(__uint_as_float(sr[c0 + 2 * u])), exp2_hw(__uint_as_float(sr[c0 + 2 * u + 1])));
+#pragma unroll
+          for (int u = 0; u < 8; u++) sum[u & 1] = add2(sum[u & 1], p[u]);
+#pragma unroll
+          for (int u = 0; u < 8; u++) {
             float p0, p1;
-            split(x, p0, p1);
-            p = pair_of(exp2_hw(p0), exp2_hw(p1));
+            split(p[u], p0, p1);
+            sr[(c0 >> 1) + u] = pack_bf16(p0, p1);
           }
-          sum[c >> 1 & 1] = add2(sum[c >> 1 & 1], p);
-          float p0, p1;
-          split(p, p0, p1);
-          sr[c >> 1] = pack_bf16(p0, p1);
         }
         tmem_st32(tm_s + half * 32, sr + half * 32);
         tmem_wait_st();
         fence_before();
-        tma::mbar_arrive(&ctl.p_full[tile][half]);
+        __syncwarp();
+        if (lane == 0) tma::mbar_arrive(&ctl.p_full[tile][half]);
       }
       float s0, s1;
       split(add2(sum[0], sum[1]), s0, s1);
       l += s0 + s1;
     }
-    if (ok && nt > 0) ok = tma::warp_wait_bounded(&ctl.pv_done[tile], (uint32_t)(nt - 1) & 1u, abort_flag);
+    if (ok && nt > 0) ok = wait_for(&ctl.pv_done[tile], 0, abort_flag);
     if (ok && nt > 0) {
       fence_after();
       const float inv_l = 1.f / l;
@@ -500,7 +559,7 @@ __global__ void __launch_bounds__(THREADS, 1) packed_umma_kernel(const __grid_co
           }
         }
       }
-      uint32_t again = __ballot_sync(0xffffffffu, !finite && fabsf(l) < INFINITY);
+      uint32_t again = __ballot_sync(0xffffffffu, first != packed::NOBODY && (l < LEAST || (!finite && fabsf(l) < INFINITY)));
       for (; again; again &= again - 1) {   // (stored above by the row's thread, here by all of them: the ballot has ordered the two)
         const int r = tile * BM + quarter * 32 + __ffs(again) - 1;
         row_again(qkv, row_stride, out + (long long)(q0 + r) * out_stride + (long long)h * hd, q0 + r, ctl.first[r], h, g, H, Hk, hd, ALIBI ? slopes[h] : 0.f,
