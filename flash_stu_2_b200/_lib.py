@@ -137,7 +137,7 @@ _SIGNATURES = {
     "stu_swa_packed": ([_P, _LL, _P, c_int, _P, _P, _LL, _LL, c_int, c_int, c_int, c_int, c_float, _P, c_int, _P], c_int),
     "stu_kv4_write": ([_P, _LL, _P, _P, _P, _P, c_int, _LL, c_int, c_int, c_int, c_int, c_int, _P], c_int),
     "stu_kv4_read": ([_P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, _P], c_int),
-    "stu_kv4_step": ([_P, _LL, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, _P], c_int),
+    "stu_kv4_step": ([_P, _LL, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int, _P, c_int, _P], c_int),
     "stu_sample": ([_P, _LL, c_int, c_int, c_float, c_int, c_float, c_int, _P, _P, _LL, _P, c_int, _P], c_int),
 }
 

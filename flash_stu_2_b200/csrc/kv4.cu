@@ -97,100 +97,6 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const unsigned char* __re
   }
 }
 
-// One token per sequence against its ring, any number of query heads to a key head: a CTA per (head, sequence), a warp per 32 keys.  Scores:
-// a lane per key; weighted values: a lane per dimension.
-template <typename T>
-__global__ void __launch_bounds__(256) kv4_step_kernel(const T* __restrict__ qkv, long long row_stride, const unsigned char* __restrict__ k4,
-                                                       const unsigned char* __restrict__ v4, const int* __restrict__ pos,
-                                                       const float* __restrict__ slopes, T* __restrict__ out, int H, int Hk, int hd, int slots,
-                                                       int window, float scale, float softcap) {
-  __shared__ float q[128], s_m[8], s_l[8], s_o[8][128];
-  const int h = blockIdx.x, b = blockIdx.y, g = h / (H / Hk), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int pieces = kv4::pieces_of(hd), width = kv4::width_of(hd);
-  const long long base = ((long long)b * Hk + g) * kv4::head_bytes(hd, slots);
-  const uint32_t *kw = reinterpret_cast<const uint32_t*>(k4 + base), *vw = reinterpret_cast<const uint32_t*>(v4 + base);
-  const uint32_t *ks = kw + (long long)slots * (width / 8), *vs = vw + (long long)slots * (width / 8);
-  const T* row = qkv + (long long)b * row_stride;
-  if (threadIdx.x < hd) q[threadIdx.x] = Elem<T>::to_f(row[(long long)h * hd + threadIdx.x]) * scale;
-  __syncthreads();
-  const int t = pos[2 * b], newest = kv4::slot_of(t, slots);
-  const float slope = slopes ? slopes[h] : 0.f;
-  auto bent = [&](float s) { return softcap > 0.f ? softcap * tanhf(s / softcap) : s; };
-  float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-  if (warp == 0) {   // the new token itself, as it is
-    float s = 0.f;
-    for (int c = lane; c < hd; c += 32) s = fmaf(q[c], Elem<T>::to_f(row[(long long)(H + g) * hd + c]), s);
-    m = bent(warp_sum(s));
-    l = 1.f;
-    for (int e = 0; e < 4; e++)
-      if (lane + 32 * e < hd) o[e] = Elem<T>::to_f(row[(long long)(H + Hk + g) * hd + lane + 32 * e]);
-  }
-  for (int s0 = warp * 32; s0 < slots; s0 += 256) {
-    const int slot = s0 + lane;
-    const int behind = newest > slot ? newest - slot : newest - slot + slots;   // 1 .. slots
-    const bool seen = slot < slots && behind <= window && behind <= t;
-    if (!__any_sync(0xffffffffu, seen)) continue;
-    float s = -INFINITY;
-    if (seen) {
-      float sum[2] = {0.f, 0.f}, all[2] = {0.f, 0.f};
-      for (int w = 0; w < hd / 8; w++) {
-        const int p = w >> 3;
-        const uint32_t word = kw[(long long)slot * (width / 8) + kv4::word_at(w & 7, p, pieces)];
-        for (int e = 0; e < 8; e++) {
-          sum[p] = fmaf((float)(word >> 4 * e & 15u), q[w * 8 + e], sum[p]);
-          all[p] += q[w * 8 + e];
-        }
-      }
-      float dot = 0.f;
-      for (int p = 0; p < pieces; p++) {
-        const uint32_t sc = ks[(long long)slot * pieces + p];
-        dot += fmaf(__uint_as_float(sc & 0xffff0000u), sum[p], __uint_as_float(sc << 16) * all[p]);
-      }
-      s = bent(dot) - slope * (float)behind;
-    }
-    const float top = fmaxf(m, warp_max(s)), corr = top == -INFINITY ? 1.f : __expf(m - top);
-    const float pw = seen ? __expf(s - top) : 0.f;
-    m = top;
-    l = l * corr + warp_sum(pw);
-    for (int e = 0; e < 4; e++) o[e] *= corr;
-    for (int k = 0; k < 32; k++) {
-      const float w = __shfl_sync(0xffffffffu, pw, k);
-      if (!__shfl_sync(0xffffffffu, (int)seen, k)) continue;
-      for (int e = 0; e < 4; e++) {
-        const int c = lane + 32 * e, p = c >> 6;
-        if (c < hd) {
-          const uint32_t word = vw[(long long)(s0 + k) * (width / 8) + kv4::word_at((c & 63) >> 3, p, pieces)];
-          const uint32_t sc = vs[(long long)(s0 + k) * pieces + p];
-          o[e] = fmaf(w, fmaf((float)(word >> 4 * (c & 7) & 15u), __uint_as_float(sc & 0xffff0000u), __uint_as_float(sc << 16)), o[e]);
-        }
-      }
-    }
-  }
-  if (lane == 0) {
-    s_m[warp] = m;
-    s_l[warp] = l;
-  }
-  for (int e = 0; e < 4; e++) s_o[warp][lane + 32 * e] = o[e];
-  __syncthreads();
-  if (threadIdx.x < hd) {
-    float M = -INFINITY, num = 0.f, den = 0.f;
-    for (int w = 0; w < 8; w++) M = fmaxf(M, s_m[w]);
-    for (int w = 0; w < 8; w++) {
-      const float f = s_m[w] > -INFINITY ? __expf(s_m[w] - M) : 0.f;
-      num = fmaf(s_o[w][threadIdx.x], f, num);
-      den = fmaf(s_l[w], f, den);
-    }
-    out[((long long)b * H + h) * hd + threadIdx.x] = Elem<T>::from_f(num / den);
-  }
-}
-
-int geometry(int B, int H, int Hk, int hd, int slots, int dtype) {
-  if (dtype != STU_F32 && dtype != STU_BF16) return STU_ERR_DTYPE;
-  if (B <= 0 || Hk <= 0 || H < Hk || H % Hk || hd <= 0 || slots <= 0 || slots % 16) return STU_ERR_SHAPE;
-  if (hd % 8 || hd > 128) return STU_ERR_UNSUPPORTED;
-  return STU_OK;
-}
-
 template <typename T>
 int launch_write(const void* qkv, long long row_stride, void* k4, void* v4, int* pos, const int* cu, int B, long long rows, int per_seq, int H, int Hk,
                  int hd, int slots, cudaStream_t st) {
@@ -212,7 +118,7 @@ int launch_write(const void* qkv, long long row_stride, void* k4, void* v4, int*
 extern "C" int stu_kv4_write(const void* qkv, long long row_stride, void* k4, void* v4, int* pos, const int* cu_seqlens, int B, long long rows, int H,
                              int Hk, int hd, int slots, int dtype, void* stream) {
   if (!qkv || !k4 || !v4 || !pos) return STU_ERR_NULL;
-  const int rc = geometry(B, H, Hk, hd, slots, dtype);
+  const int rc = kv4::geometry(B, H, Hk, hd, slots, dtype);
   if (rc != STU_OK) return rc;
   if (rows <= 0 || rows > 0x7fffffffll || row_stride < (long long)(H + 2 * Hk) * hd || (!cu_seqlens && rows % B)) return STU_ERR_SHAPE;
   if (!aligned16(k4) || !aligned16(v4)) return STU_ERR_ALIGN;
@@ -223,7 +129,7 @@ extern "C" int stu_kv4_write(const void* qkv, long long row_stride, void* k4, vo
 
 extern "C" int stu_kv4_read(const void* k4, const void* v4, void* k, void* v, int B, int Hk, int hd, int slots, int dtype, void* stream) {
   if (!k4 || !v4 || !k || !v) return STU_ERR_NULL;
-  const int rc = geometry(B, Hk, Hk, hd, slots, dtype);
+  const int rc = kv4::geometry(B, Hk, Hk, hd, slots, dtype);
   if (rc != STU_OK) return rc;
   if (!aligned16(k4) || !aligned16(v4) || !aligned16(k) || !aligned16(v)) return STU_ERR_ALIGN;
   const long long blocks = ((long long)B * slots * Hk * (hd / 8) + 255) / 256;
@@ -235,24 +141,4 @@ extern "C" int stu_kv4_read(const void* k4, const void* v4, void* k, void* v, in
     kv4_read_kernel<bf16><<<grid, 256, 0, st>>>((const unsigned char*)k4, (const unsigned char*)v4, (bf16*)k, (bf16*)v, B, Hk, hd, slots);
   STU_CHECK_LAUNCH();
   return STU_OK;
-}
-
-extern "C" int stu_kv4_step(const void* qkv, long long row_stride, void* k4, void* v4, int* pos, const float* slopes, void* out, int B, int H, int Hk,
-                            int hd, int slots, int window, float softcap, int update_cache, int dtype, void* stream) {
-  if (!qkv || !k4 || !v4 || !pos || !out) return STU_ERR_NULL;
-  const int rc = geometry(B, H, Hk, hd, slots, dtype);
-  if (rc != STU_OK) return rc;
-  if (window < 0 || window >= slots || B > 65535 || row_stride < (long long)(H + 2 * Hk) * hd) return STU_ERR_SHAPE;
-  if (!aligned16(k4) || !aligned16(v4)) return STU_ERR_ALIGN;
-  cudaStream_t st = (cudaStream_t)stream;
-  const float scale = 1.0f / sqrtf((float)hd);
-  if (dtype == STU_F32)
-    kv4_step_kernel<float><<<dim3(H, B), 256, 0, st>>>((const float*)qkv, row_stride, (const unsigned char*)k4, (const unsigned char*)v4, pos, slopes,
-                                                       (float*)out, H, Hk, hd, slots, window, scale, softcap);
-  else
-    kv4_step_kernel<bf16><<<dim3(H, B), 256, 0, st>>>((const bf16*)qkv, row_stride, (const unsigned char*)k4, (const unsigned char*)v4, pos, slopes,
-                                                      (bf16*)out, H, Hk, hd, slots, window, scale, softcap);
-  STU_CHECK_LAUNCH();
-  if (!update_cache) return STU_OK;
-  return stu_kv4_write(qkv, row_stride, k4, v4, pos, nullptr, B, B, H, Hk, hd, slots, dtype, stream);
 }

@@ -89,4 +89,11 @@ __device__ __forceinline__ int word_at(int i, int piece, int pieces) { return i 
 // Slot of the token at position t.  (A position that no sequence has, below 0, still falls into the ring.)
 __device__ __forceinline__ int slot_of(int t, int slots) { return (int)((unsigned)t % (unsigned)slots); }
 
+inline int geometry(int B, int H, int Hk, int hd, int slots, int dtype) {
+  if (dtype != STU_F32 && dtype != STU_BF16) return STU_ERR_DTYPE;
+  if (B <= 0 || Hk <= 0 || H < Hk || H % Hk || hd <= 0 || slots <= 0 || slots % 16) return STU_ERR_SHAPE;
+  if (hd % 8 || hd > 128) return STU_ERR_UNSUPPORTED;
+  return STU_OK;
+}
+
 }  // namespace kv4

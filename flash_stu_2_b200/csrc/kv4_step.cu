@@ -1,0 +1,475 @@
+// Attention of one new token per sequence over its ring of 4 bits (kv4.cuh), which takes the token's key and value in.
+//
+// A CTA (or a cluster of up to 8 that share the keys) works for one key head of one sequence and up to 8 of its query heads; a warp takes 32 slots at a time.
+//   scores   mma.sync, queries as rows, the numbers of 8 keys as columns: a number n becomes bf16 by putting its bits under those of 128 (128 + n is exact), so
+//            that two of them cost a shift and a logical operation.  A piece's scale is the same for all of a row's products:
+//              q.k = sum over pieces of  step (q.(128 + n)) + (lowest - 128 step) sum(q)
+//   softmax  a lane per key, the scores handed over through shared memory: cap, ALiBi, window, exponentials in the exp2 domain against a maximum that moves only when
+//            a score outgrows it by 2^8
+//   values   mma.sync, weights times the values' steps as rows; a number enters as n - 8 (the tensor core's sums are cut off, not rounded: with 128 + n the error of
+//            16384 of them was four times the output's rounding); what lowest and the 8s add is summed up beside, one number per piece.  The weights' rows are 8 of 16: a
+//            weight is two bf16, its rounding and what that left, in rows r and r + 8 (error 2^-17)
+// fp32: queries and weights are three bf16 each (the third in a product of its own), and scores are made of n - 8, too.
+// A warp's slots come by bulk copies into two stages of its own, 4.6 KB each (heads of 128).
+// Warps are merged through shared memory, CTAs of a cluster through distributed shared memory, in a fixed order; the new token's own key and value join there, as
+// they are.  The ring's slot of the new token holds one that is out of everyone's window; it is written by one warp.
+// Bound by HBM where the grid is large (4.5 bits a number), by latency where it is small.
+#include <cooperative_groups.h>
+
+#include "kv4.cuh"
+#include "tma.cuh"
+
+namespace cg = cooperative_groups;
+
+int device_sm_count();   // gemm_tc.cu
+
+namespace {
+
+constexpr int WARPS = 4, TILE = 32;      // warps of a CTA; slots that a warp takes at a time
+constexpr float LAG = 8.f;               // exp2 domain
+constexpr int STATUS_KV4 = 14;
+constexpr int PITCH = TILE * 2 + 16;     // bytes between rows of weights: eight rows' 16 bytes lie in different banks
+
+template <typename T, int W> struct Geometry {
+  static constexpr bool F32 = sizeof(T) == 4;
+  static constexpr int NP = W / 64 ? W / 64 : 1;          // pieces
+  static constexpr int WPL = W == 32 ? 1 : 2;             // words of a key's piece per lane
+  static constexpr int KS = 2 * WPL;                      // steps of 16 dimensions per piece
+  static constexpr int NT = W == 32 ? 4 : 8;              // tiles of 8 dimensions per piece
+  static constexpr int PROWS = F32 ? 24 : 16;             // rows of weights
+  static constexpr int ROWS_BYTES = TILE * W / 2, SCALE_BYTES = TILE * 4 * NP, STAGE = 2 * (ROWS_BYTES + SCALE_BYTES);   // keys, values, their scales
+  static constexpr int P_BYTES = NP * PROWS * PITCH;
+  __host__ __device__ static constexpr int warp_bytes(int rows) { return 2 * STAGE + NP * rows * TILE * 4 + P_BYTES; }
+};
+
+__device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t a) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+}
+__device__ __forceinline__ void ldmatrix_x2(uint32_t (&r)[2], uint32_t a) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x2.shared.b16 {%0,%1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "r"(a) : "memory");
+}
+// numbers s of the two halves of w, as bf16: 128 + n, or n - 8 (CENTRED)
+template <bool CENTRED> __device__ __forceinline__ uint32_t numbers(uint32_t w, int s) {
+  uint32_t v = ((w >> 4 * s) & 0x000f000fu) | 0x43004300u;
+  if (CENTRED) asm("sub.rn.bf16x2 %0, %0, %1;" : "+r"(v) : "r"(0x43084308u));
+  return v;
+}
+__device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float rounded(float x) { return __bfloat162float(__float2bfloat16_rn(x)); }
+__device__ __forceinline__ float exp2_fast(float x) {   // relative error 2^-22; 0 for -infinity
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+template <int N> __device__ __forceinline__ void load_words(uint32_t (&w)[N], const unsigned char* p) {
+  if constexpr (N == 4) *reinterpret_cast<uint4*>(w) = *reinterpret_cast<const uint4*>(p);
+  if constexpr (N == 2) *reinterpret_cast<uint2*>(w) = *reinterpret_cast<const uint2*>(p);
+  if constexpr (N == 1) w[0] = *reinterpret_cast<const uint32_t*>(p);
+}
+
+// NR: rows of queries that there is room for
+template <typename T, int W, int NR>
+__global__ void __launch_bounds__(WARPS * 32, W == 128 && (sizeof(T) == 4 || NR > 2) ? 3 : 4) kv4_step_kernel(
+    const T* __restrict__ qkv, long long row_stride, unsigned char* k4, unsigned char* v4, int* __restrict__ pos, const float* __restrict__ slopes,
+    T* __restrict__ out, int B, int H, int Hk, int hd, int slots, int window, float scale, float softcap, int update_cache, int splits, int* status) {
+  typedef Geometry<T, W> G;
+  constexpr bool F32 = G::F32;
+  constexpr int NP = G::NP, KS = G::KS, NT = G::NT;
+  constexpr float LOG2E = 1.4426950408889634f;
+  extern __shared__ __align__(16) unsigned char smem[];
+  __shared__ float s_qsum[8][2], s_own[8], s_m[WARPS][8], s_l[WARPS][8], c_m[8], c_l[8];
+  const int g = blockIdx.x / splits, part = blockIdx.x - g * splits, b = blockIdx.y;
+  const int R = H / Hk, r0 = blockIdx.z * 8, rows = min(8, R - r0), h0 = g * R + r0;   // the query heads h0 .. h0 + rows - 1
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, gr = lane >> 2, c = lane & 3;
+  __shared__ uint64_t full[WARPS][2];
+  __shared__ int abort_flag;
+  unsigned char* mine = smem + warp * G::warp_bytes(NR);            // two stages
+  float* sS = reinterpret_cast<float*>(mine + 2 * G::STAGE);        // [piece][row][32 keys]
+  unsigned char* sP = mine + 2 * G::STAGE + NP * NR * TILE * 4;     // [piece][hi 8, mid 8 (, lo 8) rows][32 keys] bf16
+  for (int e = lane; e < G::P_BYTES / 4; e += 32) reinterpret_cast<uint32_t*>(sP)[e] = 0;   // (rows without a query stay as they are)
+  if (lane == 0) {
+    tma::mbar_init(&full[warp][0], 1);
+    tma::mbar_init(&full[warp][1], 1);
+    if (warp == 0) abort_flag = 0;
+    tma::fence_barrier_init();
+  }
+  pdl_trigger();   // launched with the programmatic attribute: resident while the projection in front of it drains
+  pdl_wait();
+  const int t = pos[2 * b];
+  if (update_cache) {   // every CTA has read its position before it arrives here; the last one to arrive moves all of them on
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      const int total = gridDim.x * gridDim.y * gridDim.z;
+      if (atomicAdd(&pos[1], 1) == total - 1) {
+        pos[1] = 0;
+        for (int i = 0; i < B; i++) pos[2 * i] += 1;
+      }
+    }
+  }
+  const int newest = kv4::slot_of(t, slots), live = min(max(t, 0), window);   // the `live` slots before slot `newest`, around the ring's end
+  const int first = newest >= live ? newest - live : newest - live + slots, tiles_all = (slots + TILE - 1) / TILE, tile0 = first / TILE;
+  int tiles = 0;
+  if (live > 0) {
+    const int last = newest > 0 ? newest - 1 : slots - 1;
+    tiles = first <= last ? last / TILE - tile0 + 1 : min(tiles_all, tiles_all - tile0 + last / TILE + 1);
+  }
+  const int parts = min(splits, max(1, (tiles + WARPS - 1) / WARPS));   // CTAs that have something to do (a barrier of the cluster waits for none that has left)
+  if (part >= parts) return;
+  const long long head_bytes = kv4::head_bytes(W, slots);
+  unsigned char *kb = k4 + ((long long)b * Hk + g) * head_bytes, *vb = v4 + ((long long)b * Hk + g) * head_bytes;
+  const long long scales_at = (long long)slots * (W / 2);
+  const T* row = qkv + (long long)b * row_stride;
+
+  auto fetch = [&](int n, int stage) {   // the n-th tile (of the ring's last, what there is)
+    int tile = tile0 + n;
+    if (tile >= tiles_all) tile -= tiles_all;
+    const int s0 = tile * TILE, here = min(TILE, slots - s0);
+    if (lane == 0) {
+      unsigned char* to = mine + stage * G::STAGE;
+      uint64_t* bar = &full[warp][stage];
+      tma::mbar_expect_tx(bar, 2 * here * (W / 2 + 4 * NP));
+      tma::bulk_load(to, kb + (long long)s0 * (W / 2), here * (W / 2), bar);
+      tma::bulk_load(to + 2 * G::ROWS_BYTES, kb + scales_at + (long long)s0 * 4 * NP, here * 4 * NP, bar);
+      tma::bulk_load(to + G::ROWS_BYTES, vb + (long long)s0 * (W / 2), here * (W / 2), bar);
+      tma::bulk_load(to + 2 * G::ROWS_BYTES + G::SCALE_BYTES, vb + scales_at + (long long)s0 * 4 * NP, here * 4 * NP, bar);
+    }
+  };
+  const int stride = parts * WARPS;
+  int n = part * WARPS + warp;
+  __syncwarp();
+  if (n < tiles) fetch(n, 0);
+  if (n + stride < tiles) fetch(n + stride, 1);
+
+  // queries in the order of the numbers: step u of piece p holds, of word i = 2 c + u / 2 (or c), dimensions s, s + 4 (columns 2 c, 2 c + 1) and s + 1, s + 5
+  uint32_t qa[NP][KS][F32 ? 6 : 2];
+  {
+    const T* q = row + (long long)(h0 + gr) * hd;
+#pragma unroll
+    for (int p = 0; p < NP; p++)
+#pragma unroll
+      for (int u = 0; u < KS; u++)
+#pragma unroll
+        for (int half = 0; half < 2; half++) {
+          const int d = 64 * p + 8 * (G::WPL * c + (u >> 1)) + 2 * (u & 1) + half;
+          const float x0 = gr < rows && d < hd ? Elem<T>::to_f(q[d]) : 0.f, x1 = gr < rows && d + 4 < hd ? Elem<T>::to_f(q[d + 4]) : 0.f;
+          if (F32) {
+            const float h0_ = rounded(x0), h1_ = rounded(x1), m0_ = rounded(x0 - h0_), m1_ = rounded(x1 - h1_);
+            qa[p][u][half] = bf16_pair(h0_, h1_);
+            qa[p][u][2 + half] = bf16_pair(m0_, m1_);
+            qa[p][u][4 + half] = bf16_pair(x0 - h0_ - m0_, x1 - h1_ - m1_);
+          } else {
+            qa[p][u][half] = bf16_pair(x0, x1);
+          }
+        }
+  }
+  for (int r = warp; r < rows; r += WARPS) {   // each query's sums, and its score with the new token's own key
+    const T *q = row + (long long)(h0 + r) * hd, *k = row + (long long)(H + g) * hd;
+    float sum0 = 0.f, sum1 = 0.f, dot = 0.f;
+    for (int d = lane; d < hd; d += 32) {
+      const float x = Elem<T>::to_f(q[d]);
+      (d < 64 ? sum0 : sum1) += x;
+      dot = fmaf(x, Elem<T>::to_f(k[d]), dot);
+    }
+    sum0 = warp_sum(sum0);
+    sum1 = warp_sum(sum1);
+    dot = warp_sum(dot) * scale;
+    if (softcap > 0.f) dot = softcap * tanhf(dot / softcap);
+    if (lane == 0) {
+      s_qsum[r][0] = sum0;
+      s_qsum[r][1] = sum1;
+      s_own[r] = dot * LOG2E;
+    }
+  }
+  __syncthreads();
+  if (update_cache && part == 0 && blockIdx.z == 0 && warp == WARPS - 1) {   // the new key and value: eight lanes per piece
+    const int unit = lane >> 3, which = unit / NP, piece = unit % NP, i = lane & 7;
+    const bool on = unit < 2 * NP, there = on && piece * 64 + i * 8 < hd;
+    float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (there) kv4::load8<false>(row + (long long)(H + which * Hk + g) * hd + piece * 64 + i * 8, x);
+    uint32_t word, sc;
+    kv4::quantize(x, there, word, sc);
+    unsigned char* ring = which ? vb : kb;
+    if (on && i * 8 < W / NP) reinterpret_cast<uint32_t*>(ring)[(long long)newest * (W / 8) + kv4::word_at(i, piece, NP)] = word;
+    if (on && i == 0) reinterpret_cast<uint32_t*>(ring + scales_at)[(long long)newest * NP + piece] = sc;
+  }
+
+  float qs[NR][NP], slope[NR], m[NR], l[NR], low[NR][NP], o[NP][NT][4];
+  const float k0 = softcap > 0.f ? scale / softcap : 0.f, k1 = softcap > 0.f ? softcap * LOG2E : scale * LOG2E;
+#pragma unroll
+  for (int r = 0; r < NR; r++) {
+    m[r] = -INFINITY;
+    l[r] = 0.f;
+    slope[r] = slopes && r < rows ? slopes[h0 + r] * LOG2E : 0.f;
+#pragma unroll
+    for (int p = 0; p < NP; p++) {
+      low[r][p] = 0.f;
+      qs[r][p] = r < rows ? s_qsum[r][p] : 0.f;
+    }
+  }
+#pragma unroll
+  for (int p = 0; p < NP; p++)
+#pragma unroll
+    for (int d = 0; d < NT; d++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) o[p][d][e] = 0.f;
+
+  // the column of this lane's key among 16: the keys whose words a lane of the second product takes together, c, c + 4, c + 8 and c + 12, are in rows that lie in
+  // more banks than neighbours
+  const int column = (lane & 16) + 2 * (lane & 3) + ((lane >> 2) & 1) + (lane & 8);
+  bool ok = true;
+  for (int turn = 0; n < tiles; n += stride, turn++) {   // (the same for the whole warp)
+    int tile = tile0 + n;
+    if (tile >= tiles_all) tile -= tiles_all;
+    const unsigned char* held = mine + (turn & 1) * G::STAGE;
+    ok = tma::warp_wait_bounded(&full[warp][turn & 1], (uint32_t)(turn >> 1) & 1u, &abort_flag);
+    if (!ok) break;
+    // ---- scores of 8 queries with 4 x 8 keys
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      uint32_t k[NP * G::WPL];
+      load_words(k, held + (8 * j + gr) * (W / 2) + c * (W / 8));
+#pragma unroll
+      for (int p = 0; p < NP; p++) {
+        float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int u = 0; u < KS; u++) {
+          const uint32_t w = k[(u >> 1) * NP + p], b0 = numbers<F32>(w, 2 * (u & 1)), b1 = numbers<F32>(w, 2 * (u & 1) + 1);
+          mma(s, qa[p][u][0], F32 ? qa[p][u][2] : 0u, qa[p][u][1], F32 ? qa[p][u][3] : 0u, b0, b1);
+          if (F32) mma(s, qa[p][u][4], 0u, qa[p][u][5], 0u, b0, b1);
+        }
+        if (gr < NR) *reinterpret_cast<float2*>(sS + (p * NR + gr) * TILE + 8 * j + 2 * c) = F32 ? make_float2(s[0] + s[2], s[1] + s[3]) : make_float2(s[0], s[1]);
+      }
+    }
+    __syncwarp();
+    // ---- a lane per key
+    const int slot = tile * TILE + lane, behind = newest > slot ? newest - slot : newest - slot + slots;   // 1 .. slots
+    const bool seen = slot < slots && behind <= live;
+    const float far = (float)behind;
+    float kstep[NP], klow[NP], vstep[NP], vlow[NP];
+    uint32_t ks[NP], vs[NP];
+    load_words(ks, held + 2 * G::ROWS_BYTES + lane * 4 * NP);
+    load_words(vs, held + 2 * G::ROWS_BYTES + G::SCALE_BYTES + lane * 4 * NP);
+#pragma unroll
+    for (int p = 0; p < NP; p++) {
+      kstep[p] = __uint_as_float(ks[p] & 0xffff0000u);
+      klow[p] = fmaf(F32 ? 8.f : -128.f, kstep[p], __uint_as_float(ks[p] << 16));
+      vstep[p] = seen ? __uint_as_float(vs[p] & 0xffff0000u) : 0.f;
+      vlow[p] = seen ? __uint_as_float(vs[p] << 16) : 0.f;
+    }
+    bool moved = false;
+    float shrink = 1.f;   // of row gr
+#pragma unroll
+    for (int r = 0; r < NR; r++) {
+      if (r < rows) {   // (the same for the whole CTA)
+        float x = 0.f;
+#pragma unroll
+        for (int p = 0; p < NP; p++) x = fmaf(kstep[p], sS[(p * NR + r) * TILE + lane], fmaf(klow[p], qs[r][p], x));
+        if (softcap > 0.f) {
+          x *= k0;
+          if (F32) x = tanhf(x);
+          else asm("tanh.approx.f32 %0, %0;" : "+f"(x));   // relative error 2^-11
+        }
+        x = fmaf(-slope[r], far, x * k1);
+        if (!seen) x = -INFINITY;
+        if (__any_sync(0xffffffffu, x > (m[r] == -INFINITY ? m[r] : m[r] + LAG))) {
+          const float top = fmaxf(m[r], warp_max(x)), corr = exp2_fast(m[r] - top);   // (0 where there was no key yet)
+          m[r] = top;
+          l[r] *= corr;
+#pragma unroll
+          for (int p = 0; p < NP; p++) low[r][p] *= corr;
+          if (gr == r) shrink = corr;
+          moved = true;
+        }
+        const float w = seen ? exp2_fast(x - m[r]) : 0.f;
+        l[r] += w;
+#pragma unroll
+        for (int p = 0; p < NP; p++) {
+          const float a = w * vstep[p], hi = rounded(a), mid = rounded(a - hi);
+          __nv_bfloat16* at = reinterpret_cast<__nv_bfloat16*>(sP + (p * G::PROWS + r) * PITCH) + column;
+          at[0] = __float2bfloat16_rn(hi);
+          at[8 * PITCH / 2] = __float2bfloat16_rn(mid);
+          if (F32) at[16 * PITCH / 2] = __float2bfloat16_rn(a - hi - mid);
+          low[r][p] += fmaf(w, vlow[p], 8.f * (F32 ? a : hi + mid));
+        }
+      }
+    }
+    if (moved) {   // (for the whole warp)
+#pragma unroll
+      for (int p = 0; p < NP; p++)
+#pragma unroll
+        for (int d = 0; d < NT; d++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) o[p][d][e] *= shrink;
+    }
+    __syncwarp();
+    // ---- weighted values: 2 x 16 keys
+#pragma unroll
+    for (int kk = 0; kk < 2; kk++) {
+      uint32_t v[4][NP];   // (of a head of 32 a lane's word holds its four numbers and those of the next row's lane)
+#pragma unroll
+      for (int e = 0; e < 4; e++) load_words(v[e], held + G::ROWS_BYTES + (16 * kk + c + 4 * e) * (W / 2) + (W == 32 ? gr >> 1 : gr * NP) * 4);
+#pragma unroll
+      for (int p = 0; p < NP; p++) {
+        uint32_t a[4], a3[2] = {0u, 0u};
+        const uint32_t at = (uint32_t)__cvta_generic_to_shared(sP + (p * G::PROWS + (lane & 15)) * PITCH + kk * 32 + (lane >> 4) * 16);
+        ldmatrix_x4(a, at);   // rows 0 - 7 and 8 - 15 of keys 0 - 7, then of keys 8 - 15
+        if (F32) ldmatrix_x2(a3, (uint32_t)__cvta_generic_to_shared(sP + (p * G::PROWS + 16 + (lane & 7)) * PITCH + kk * 32 + ((lane >> 3) & 1) * 16));
+        uint32_t lo[2], hi[2];   // numbers 0 - 3 and 4 - 7 of two keys
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+          const uint32_t x = v[2 * e][p], y = v[2 * e + 1][p];
+          lo[e] = __byte_perm(x, y, W == 32 && (gr & 1) ? 0x7632 : 0x5410);
+          hi[e] = __byte_perm(x, y, 0x7632);
+        }
+#pragma unroll
+        for (int d = 0; d < NT; d++) {
+          const uint32_t b0 = numbers<true>(d < 4 ? lo[0] : hi[0], d & 3), b1 = numbers<true>(d < 4 ? lo[1] : hi[1], d & 3);
+          mma(o[p][d], a[0], a[1], a[2], a[3], b0, b1);
+          if (F32) mma(o[p][d], a3[0], 0u, a3[1], 0u, b0, b1);
+        }
+      }
+    }
+    __syncwarp();
+    if (n + 2 * stride < tiles) fetch(n + 2 * stride, turn & 1);
+  }
+  // ---- this warp's rows; then the CTA's
+  __syncthreads();   // (what they are written to is other warps' scratch)
+  if (abort_flag) {   // a copy that did not land in time: none is under way any more when the CTA ends
+    if (threadIdx.x == 0) {
+      if (status) atomicExch(status, STATUS_KV4);
+      const uint64_t start = tma::global_ns();
+      while (tma::global_ns() - start < 200000ull) {}
+    }
+    __syncthreads();
+  }
+  float* sO = reinterpret_cast<float*>(smem);   // [warp][row][W]
+#pragma unroll
+  for (int r = 0; r < NR; r++) {
+    if (r < rows) {
+      const float sum = warp_sum(l[r]);
+#pragma unroll
+      for (int p = 0; p < NP; p++) low[r][p] = warp_sum(low[r][p]);
+      if (lane == 0) {
+        s_m[warp][r] = m[r];
+        s_l[warp][r] = sum;
+      }
+      if (gr == r) {
+#pragma unroll
+        for (int p = 0; p < NP; p++)
+#pragma unroll
+          for (int d = 0; d < NT; d++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) sO[(warp * NR + r) * W + 64 * p + (2 * c + e) * NT + d] = o[p][d][e] + o[p][d][2 + e] + low[r][p];
+      }
+    }
+  }
+  __syncthreads();
+  const bool one = parts == 1;
+  for (int e = threadIdx.x; e < rows * W; e += WARPS * 32) {
+    const int r = e / W, d = e % W;
+    float top = one ? s_own[r] : -INFINITY, num = 0.f, den = 0.f;
+#pragma unroll
+    for (int w = 0; w < WARPS; w++) top = fmaxf(top, s_m[w][r]);
+#pragma unroll
+    for (int w = 0; w < WARPS; w++) {
+      const float f = s_m[w][r] > -INFINITY ? exp2_fast(s_m[w][r] - top) : (s_l[w][r] == s_l[w][r] ? 0.f : s_l[w][r]);   // (a warp that saw NaN alone has no maximum)
+      if (s_m[w][r] > -INFINITY || !(f == 0.f)) num = fmaf(sO[(w * NR + r) * W + d], f, num);
+      den = fmaf(s_l[w][r], f, den);
+    }
+    if (one) {
+      const float f = exp2_fast(s_own[r] - top);
+      if (d < hd) out[((long long)b * H + h0 + r) * hd + d] = Elem<T>::from_f(fmaf(f, Elem<T>::to_f(row[(long long)(H + Hk + g) * hd + d]), num) / (den + f));
+    } else {
+      sO[r * W + d] = num;   // (each thread reads its own column of all warps before)
+      if (d == 0) {
+        c_m[r] = top;
+        c_l[r] = den;
+      }
+    }
+  }
+  if (one) return;
+  cg::cluster_group cluster = cg::this_cluster();
+  cluster.sync();
+  if (part == 0) {
+    for (int e = threadIdx.x; e < rows * W; e += WARPS * 32) {
+      const int r = e / W, d = e % W;
+      float ms[8], top = s_own[r];
+      for (int i = 0; i < parts; i++) top = fmaxf(top, ms[i & 7] = *cluster.map_shared_rank(&c_m[r], i));
+      float num = 0.f, den = 0.f;
+      for (int i = 0; i < parts; i++) {
+        const float li = *cluster.map_shared_rank(&c_l[r], i);
+        const float f = ms[i & 7] > -INFINITY ? exp2_fast(ms[i & 7] - top) : (li == li ? 0.f : li);
+        if (!(f == 0.f)) num = fmaf(*cluster.map_shared_rank(&sO[r * W + d], i), f, num);
+        den = fmaf(li, f, den);
+      }
+      const float f = exp2_fast(s_own[r] - top);
+      if (d < hd) out[((long long)b * H + h0 + r) * hd + d] = Elem<T>::from_f(fmaf(f, Elem<T>::to_f(row[(long long)(H + Hk + g) * hd + d]), num) / (den + f));
+    }
+  }
+  cluster.sync();   // the other CTAs' results stay alive until they are read
+}
+
+template <typename T, int W, int NR>
+int launch(const void* qkv, long long row_stride, void* k4, void* v4, int* pos, const float* slopes, void* out, int B, int H, int Hk, int hd, int slots,
+           int window, float softcap, int update_cache, int* status, cudaStream_t st) {
+  typedef Geometry<T, W> G;
+  const size_t smem = (size_t)WARPS * G::warp_bytes(NR);
+  static_assert(G::warp_bytes(NR) >= NR * W * 4, "the warps' rows are merged there");
+  static SmemLimit limit;
+  cudaError_t e = allow_smem((const void*)kv4_step_kernel<T, W, NR>, smem, limit);
+  if (e != cudaSuccess) return (int)e;
+  const int groups = (H / Hk + 7) / 8;
+  int splits = 1;
+  while (splits < 8 && 2ll * splits * Hk * B * groups <= 4ll * device_sm_count() && window / (2 * splits) >= WARPS * TILE / 2) splits *= 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(Hk * splits, B, groups);
+  cfg.blockDim = dim3(WARPS * 32);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[2];
+  cfg.attrs = at;
+  if (splits > 1) {
+    at[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+    at[cfg.numAttrs].val.clusterDim.x = splits;
+    at[cfg.numAttrs].val.clusterDim.y = at[cfg.numAttrs].val.clusterDim.z = 1;
+    cfg.numAttrs++;
+  }
+  if (pdl_enabled()) {
+    at[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
+    cfg.numAttrs++;
+  }
+  e = cudaLaunchKernelEx(&cfg, kv4_step_kernel<T, W, NR>, (const T*)qkv, row_stride, (unsigned char*)k4, (unsigned char*)v4, pos, slopes, (T*)out, B, H, Hk, hd,
+                         slots, window, 1.0f / sqrtf((float)hd), softcap, update_cache, splits, status);
+  return (int)e;
+}
+
+}  // namespace
+
+extern "C" int stu_kv4_step(const void* qkv, long long row_stride, void* k4, void* v4, int* pos, const float* slopes, void* out, int B, int H, int Hk,
+                            int hd, int slots, int window, float softcap, int update_cache, int* status, int dtype, void* stream) {
+  if (!qkv || !k4 || !v4 || !pos || !out) return STU_ERR_NULL;
+  const int rc = kv4::geometry(B, H, Hk, hd, slots, dtype);
+  if (rc != STU_OK) return rc;
+  if (window < 0 || window >= slots || B > 65535 || row_stride < (long long)(H + 2 * Hk) * hd) return STU_ERR_SHAPE;
+  if (!aligned16(k4) || !aligned16(v4)) return STU_ERR_ALIGN;
+  const int R = H / Hk < 8 ? H / Hk : 8;
+  auto go = [&](auto f) { return f(qkv, row_stride, k4, v4, pos, slopes, out, B, H, Hk, hd, slots, window, softcap, update_cache, status, (cudaStream_t)stream); };
+  auto by_rows = [&](auto one, auto two, auto four, auto eight) { return R == 1 ? go(one) : R == 2 ? go(two) : R <= 4 ? go(four) : go(eight); };
+  if (dtype == STU_F32) {
+    if (hd <= 32) return by_rows(launch<float, 32, 1>, launch<float, 32, 2>, launch<float, 32, 4>, launch<float, 32, 8>);
+    if (hd <= 64) return by_rows(launch<float, 64, 1>, launch<float, 64, 2>, launch<float, 64, 4>, launch<float, 64, 8>);
+    return by_rows(launch<float, 128, 1>, launch<float, 128, 2>, launch<float, 128, 4>, launch<float, 128, 8>);
+  }
+  if (hd <= 32) return by_rows(launch<bf16, 32, 1>, launch<bf16, 32, 2>, launch<bf16, 32, 4>, launch<bf16, 32, 8>);
+  if (hd <= 64) return by_rows(launch<bf16, 64, 1>, launch<bf16, 64, 2>, launch<bf16, 64, 4>, launch<bf16, 64, 8>);
+  return by_rows(launch<bf16, 128, 1>, launch<bf16, 128, 2>, launch<bf16, 128, 4>, launch<bf16, 128, 8>);
+}

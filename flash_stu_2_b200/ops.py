@@ -97,7 +97,8 @@ STATUS_TEXT = {1: "token id outside the vocabulary", 2: "position outside the ca
                10: "a tensor-parallel rank waited in vain for another rank's sub-layer output",
                11: "tcgen05 attention prefill: a bounded wait ran out, or a sequence was not at position 0",
                12: "a bounded wait ran out inside the token-step kernel",
-               13: "a bounded wait ran out inside the attention over packed prompts"}
+               13: "a bounded wait ran out inside the attention over packed prompts",
+               14: "a bounded wait ran out inside the attention over a ring of 4 bits"}
 
 
 def check_status(device=None):
@@ -1235,9 +1236,9 @@ def kv4_step(qkv: torch.Tensor, k4: torch.Tensor, v4: torch.Tensor, pos: torch.T
     if B == 0:
         return out
     rc = _lib.native().stu_kv4_step(rows.data_ptr(), _row_stride(rows), k4.data_ptr(), v4.data_ptr(), pos.data_ptr(), _p(slopes), out.data_ptr(), B, H,
-                                    kv_heads, hd, slots, window, softcap, int(update_cache), dt, _stream())
+                                    kv_heads, hd, slots, window, softcap, int(update_cache), status_word(qkv.device).data_ptr(), dt, _stream())
     _lib.check(rc, "stu_kv4_step")
-    _count(2 if update_cache else 1)
+    _count()
     return out
 
 

@@ -408,7 +408,7 @@ int stu_kv4_write(const void* qkv, long long row_stride, void* k4, void* v4, int
                   int H, int Hk, int hd, int slots, int dtype, void* stream);
 int stu_kv4_read(const void* k4, const void* v4, void* k, void* v, int B, int Hk, int hd, int slots, int dtype, void* stream);
 int stu_kv4_step(const void* qkv, long long row_stride, void* k4, void* v4, int* pos, const float* slopes, void* out, int B, int H,
-                 int Hk, int hd, int slots, int window, float softcap, int update_cache, int dtype, void* stream);
+                 int Hk, int hd, int slots, int window, float softcap, int update_cache, int* status, int dtype, void* stream);
 
 /* ---- exchange between the GPUs of a tensor-parallel group, fused into the token loop's kernels ----------------
  * The reference is single-GPU (its sub-layers: flash_stu/layers/stu_layer.py:78-98,

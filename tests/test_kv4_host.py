@@ -124,13 +124,13 @@ def test_argument_errors_without_a_gpu():
     from flash_stu_2_b200 import _lib
     lib = _lib.load()
     a = 0x10000   # stands for an aligned device address; the checks return before anything dereferences it
-    assert lib.stu_kv4_step(None, 512, a, a, a, None, a, 1, 2, 1, 64, 16, 15, 0.0, 1, 1, None) == -5
-    assert lib.stu_kv4_step(a, 512, a, a, a, None, a, 1, 2, 1, 64, 16, 16, 0.0, 1, 1, None) == -2
-    assert lib.stu_kv4_step(a, 512, a, a, a, None, a, 1, 3, 2, 64, 16, 15, 0.0, 1, 1, None) == -2
-    assert lib.stu_kv4_step(a, 512, a, a, a, None, a, 1, 2, 1, 64, 24, 15, 0.0, 1, 1, None) == -2
-    assert lib.stu_kv4_step(a, 512, a, a, a, None, a, 1, 2, 1, 60, 16, 15, 0.0, 1, 1, None) == -4
-    assert lib.stu_kv4_step(a, 512, a, a, a, None, a, 1, 2, 1, 64, 16, 15, 0.0, 1, 2, None) == -1
-    assert lib.stu_kv4_step(a, 512, a + 4, a, a, None, a, 1, 2, 1, 64, 16, 15, 0.0, 1, 1, None) == -3
+    assert lib.stu_kv4_step(None, 512, a, a, a, None, a, 1, 2, 1, 64, 16, 15, 0.0, 1, None, 1, None) == -5
+    assert lib.stu_kv4_step(a, 512, a, a, a, None, a, 1, 2, 1, 64, 16, 16, 0.0, 1, None, 1, None) == -2
+    assert lib.stu_kv4_step(a, 512, a, a, a, None, a, 1, 3, 2, 64, 16, 15, 0.0, 1, None, 1, None) == -2
+    assert lib.stu_kv4_step(a, 512, a, a, a, None, a, 1, 2, 1, 64, 24, 15, 0.0, 1, None, 1, None) == -2
+    assert lib.stu_kv4_step(a, 512, a, a, a, None, a, 1, 2, 1, 60, 16, 15, 0.0, 1, None, 1, None) == -4
+    assert lib.stu_kv4_step(a, 512, a, a, a, None, a, 1, 2, 1, 64, 16, 15, 0.0, 1, None, 2, None) == -1
+    assert lib.stu_kv4_step(a, 512, a + 4, a, a, None, a, 1, 2, 1, 64, 16, 15, 0.0, 1, None, 1, None) == -3
     assert lib.stu_kv4_write(a, 255, a, a, a, None, 1, 1, 2, 1, 64, 16, 1, None) == -2
     assert lib.stu_kv4_write(a, 256, a, a, a, None, 2, 3, 2, 1, 64, 16, 1, None) == -2
     assert lib.stu_kv4_read(a, a, a + 8, a, 1, 1, 64, 16, 1, None) == -3
