@@ -91,7 +91,7 @@ __device__ __forceinline__ int slot_of(int t, int slots) { return (int)((unsigne
 
 inline int geometry(int B, int H, int Hk, int hd, int slots, int dtype) {
   if (dtype != STU_F32 && dtype != STU_BF16) return STU_ERR_DTYPE;
-  if (B <= 0 || Hk <= 0 || H < Hk || H % Hk || hd <= 0 || slots <= 0 || slots % 16) return STU_ERR_SHAPE;
+  if (B <= 0 || Hk <= 0 || H < Hk || H % Hk || hd <= 0 || slots <= 0 || slots % 16 || slots > 1 << 24) return STU_ERR_SHAPE;   // (offsets within a head's run fit 32 bits)
   if (hd % 8 || hd > 128) return STU_ERR_UNSUPPORTED;
   return STU_OK;
 }

@@ -8,9 +8,9 @@
 //            a score outgrows it by 2^8
 //   values   mma.sync, weights times the values' steps as rows; a number enters as n - 8 (the tensor core's sums are cut off, not rounded: with 128 + n the error of
 //            16384 of them was four times the output's rounding); what lowest and the 8s add is summed up beside, one number per piece.  The weights' rows are 8 of 16: a
-//            weight is two bf16, its rounding and what that left, in rows r and r + 8 (error 2^-17)
+//            weight is two bf16, its leading bits and what these left, in rows r and r + 8 (error 2^-16)
 // fp32: queries and weights are three bf16 each (the third in a product of its own), and scores are made of n - 8, too.
-// A warp's slots come by bulk copies into two stages of its own, 4.6 KB each (heads of 128).
+// Slots come by bulk copies, 128 at a time for the CTA's four warps, into three stages (18 KB each for heads of 128).
 // Warps are merged through shared memory, CTAs of a cluster through distributed shared memory, in a fixed order; the new token's own key and value join there, as
 // they are.  The ring's slot of the new token holds one that is out of everyone's window; it is written by one warp.
 // Bound by HBM where the grid is large (4.5 bits a number), by latency where it is small.
@@ -26,6 +26,8 @@ int device_sm_count();   // gemm_tc.cu
 namespace {
 
 constexpr int WARPS = 4, TILE = 32;      // warps of a CTA; slots that a warp takes at a time
+constexpr int BLOCK = WARPS * TILE, STAGES = 3;
+constexpr float NOTHING = -3.0e38f;      // the maximum of no scores
 constexpr float LAG = 8.f;               // exp2 domain
 constexpr int STATUS_KV4 = 14;
 constexpr int PITCH = TILE * 2 + 16;     // bytes between rows of weights: eight rows' 16 bytes lie in different banks
@@ -37,15 +39,22 @@ template <typename T, int W> struct Geometry {
   static constexpr int KS = 2 * WPL;                      // steps of 16 dimensions per piece
   static constexpr int NT = W == 32 ? 4 : 8;              // tiles of 8 dimensions per piece
   static constexpr int PROWS = F32 ? 24 : 16;             // rows of weights
-  static constexpr int ROWS_BYTES = TILE * W / 2, SCALE_BYTES = TILE * 4 * NP, STAGE = 2 * (ROWS_BYTES + SCALE_BYTES);   // keys, values, their scales
+  static constexpr int ROWS_BYTES = BLOCK * W / 2, SCALE_BYTES = BLOCK * 4 * NP, STAGE = 2 * (ROWS_BYTES + SCALE_BYTES);   // keys, values, their scales
   static constexpr int P_BYTES = NP * PROWS * PITCH;
-  __host__ __device__ static constexpr int warp_bytes(int rows) { return 2 * STAGE + NP * rows * TILE * 4 + P_BYTES; }
+  __host__ __device__ static constexpr int warp_bytes(int rows) { return NP * rows * TILE * 4 + P_BYTES; }
+  __host__ __device__ static constexpr int bytes(int rows) { return STAGES * STAGE + WARPS * warp_bytes(rows); }
 };
 
 __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// the first of a sum
+__device__ __forceinline__ void mma_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+               : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 __device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t a) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
@@ -53,10 +62,13 @@ __device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t a) {
 __device__ __forceinline__ void ldmatrix_x2(uint32_t (&r)[2], uint32_t a) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x2.shared.b16 {%0,%1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "r"(a) : "memory");
 }
-// numbers s of the two halves of w, as bf16: 128 + n, or n - 8 (CENTRED)
-template <bool CENTRED> __device__ __forceinline__ uint32_t numbers(uint32_t w, int s) {
-  uint32_t v = ((w >> 4 * s) & 0x000f000fu) | 0x43004300u;
-  if (CENTRED) asm("sub.rn.bf16x2 %0, %0, %1;" : "+r"(v) : "r"(0x43084308u));
+// numbers s of the two halves of w, as bf16: 128 + n, or n - 8 (CENTRED).  (mask, base and off: 0x000f000f, 0x43004300 and 0x43084308 from registers, which an
+// instruction takes two of, where it takes one constant)
+struct Bits { uint32_t mask, base, off; };
+template <bool CENTRED> __device__ __forceinline__ uint32_t numbers(uint32_t w, int s, const Bits& k) {
+  uint32_t v;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(v) : "r"(w >> 4 * s), "r"(k.mask), "r"(k.base));   // (w & mask) | base
+  if (CENTRED) asm("sub.rn.bf16x2 %0, %0, %1;" : "+r"(v) : "r"(k.off));
   return v;
 }
 __device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {
@@ -77,7 +89,7 @@ template <int N> __device__ __forceinline__ void load_words(uint32_t (&w)[N], co
 
 // NR: rows of queries that there is room for
 template <typename T, int W, int NR>
-__global__ void __launch_bounds__(WARPS * 32, W == 128 && (sizeof(T) == 4 || NR > 2) ? 3 : 4) kv4_step_kernel(
+__global__ void __launch_bounds__(WARPS * 32, W == 128 ? 3 : 4) kv4_step_kernel(
     const T* __restrict__ qkv, long long row_stride, unsigned char* k4, unsigned char* v4, int* __restrict__ pos, const float* __restrict__ slopes,
     T* __restrict__ out, int B, int H, int Hk, int hd, int slots, int window, float scale, float softcap, int update_cache, int splits, int* status) {
   typedef Geometry<T, W> G;
@@ -89,18 +101,22 @@ __global__ void __launch_bounds__(WARPS * 32, W == 128 && (sizeof(T) == 4 || NR 
   const int g = blockIdx.x / splits, part = blockIdx.x - g * splits, b = blockIdx.y;
   const int R = H / Hk, r0 = blockIdx.z * 8, rows = min(8, R - r0), h0 = g * R + r0;   // the query heads h0 .. h0 + rows - 1
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, gr = lane >> 2, c = lane & 3;
-  __shared__ uint64_t full[WARPS][2];
+  __shared__ uint64_t full[STAGES], empty[STAGES];
   __shared__ int abort_flag;
-  unsigned char* mine = smem + warp * G::warp_bytes(NR);            // two stages
-  float* sS = reinterpret_cast<float*>(mine + 2 * G::STAGE);        // [piece][row][32 keys]
-  unsigned char* sP = mine + 2 * G::STAGE + NP * NR * TILE * 4;     // [piece][hi 8, mid 8 (, lo 8) rows][32 keys] bf16
+  unsigned char* mine = smem + STAGES * G::STAGE + warp * G::warp_bytes(NR);
+  float* sS = reinterpret_cast<float*>(mine);             // [piece][row][32 keys]
+  unsigned char* sP = mine + NP * NR * TILE * 4;          // [piece][hi 8, mid 8 (, lo 8) rows][32 keys] bf16
   for (int e = lane; e < G::P_BYTES / 4; e += 32) reinterpret_cast<uint32_t*>(sP)[e] = 0;   // (rows without a query stay as they are)
-  if (lane == 0) {
-    tma::mbar_init(&full[warp][0], 1);
-    tma::mbar_init(&full[warp][1], 1);
-    if (warp == 0) abort_flag = 0;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < STAGES; i++) {
+      tma::mbar_init(&full[i], 1);
+      tma::mbar_init(&empty[i], WARPS);
+    }
+    abort_flag = 0;
     tma::fence_barrier_init();
   }
+  Bits bits = {0x000f000fu, 0x43004300u, 0x43084308u};
+  asm volatile("" : "+r"(bits.mask), "+r"(bits.base), "+r"(bits.off));
   pdl_trigger();   // launched with the programmatic attribute: resident while the projection in front of it drains
   pdl_wait();
   const int t = pos[2 * b];
@@ -115,38 +131,42 @@ __global__ void __launch_bounds__(WARPS * 32, W == 128 && (sizeof(T) == 4 || NR 
     }
   }
   const int newest = kv4::slot_of(t, slots), live = min(max(t, 0), window);   // the `live` slots before slot `newest`, around the ring's end
-  const int first = newest >= live ? newest - live : newest - live + slots, tiles_all = (slots + TILE - 1) / TILE, tile0 = first / TILE;
+  const int first = newest >= live ? newest - live : newest - live + slots, tiles_all = (slots + BLOCK - 1) / BLOCK, tile0 = first / BLOCK;   // tiles of the CTA: 128 slots
   int tiles = 0;
   if (live > 0) {
     const int last = newest > 0 ? newest - 1 : slots - 1;
-    tiles = first <= last ? last / TILE - tile0 + 1 : min(tiles_all, tiles_all - tile0 + last / TILE + 1);
+    tiles = first <= last ? last / BLOCK - tile0 + 1 : min(tiles_all, tiles_all - tile0 + last / BLOCK + 1);
   }
-  const int parts = min(splits, max(1, (tiles + WARPS - 1) / WARPS));   // CTAs that have something to do (a barrier of the cluster waits for none that has left)
+  const int parts = min(splits, max(1, tiles));   // CTAs that have something to do (a barrier of the cluster waits for none that has left)
   if (part >= parts) return;
   const long long head_bytes = kv4::head_bytes(W, slots);
   unsigned char *kb = k4 + ((long long)b * Hk + g) * head_bytes, *vb = v4 + ((long long)b * Hk + g) * head_bytes;
   const long long scales_at = (long long)slots * (W / 2);
   const T* row = qkv + (long long)b * row_stride;
 
-  auto fetch = [&](int n, int stage) {   // the n-th tile (of the ring's last, what there is)
-    int tile = tile0 + n;
-    if (tile >= tiles_all) tile -= tiles_all;
-    const int s0 = tile * TILE, here = min(TILE, slots - s0);
-    if (lane == 0) {
-      unsigned char* to = mine + stage * G::STAGE;
-      uint64_t* bar = &full[warp][stage];
-      tma::mbar_expect_tx(bar, 2 * here * (W / 2 + 4 * NP));
-      tma::bulk_load(to, kb + (long long)s0 * (W / 2), here * (W / 2), bar);
-      tma::bulk_load(to + 2 * G::ROWS_BYTES, kb + scales_at + (long long)s0 * 4 * NP, here * 4 * NP, bar);
-      tma::bulk_load(to + G::ROWS_BYTES, vb + (long long)s0 * (W / 2), here * (W / 2), bar);
-      tma::bulk_load(to + 2 * G::ROWS_BYTES + G::SCALE_BYTES, vb + scales_at + (long long)s0 * 4 * NP, here * 4 * NP, bar);
+  const unsigned char *kscales = kb + (long long)slots * (W / 2), *vscales = vb + (long long)slots * (W / 2);
+  bool ok = true;
+  auto fetch = [&](int turn) {   // the CTA's turn-th tile (of the ring's last, what there is), by the first warp
+    const int n = part + turn * parts;
+    if (warp != 0 || n >= tiles || !ok) return;
+    const int stage = turn % STAGES;
+    ok = tma::warp_wait_bounded(&empty[stage], ((uint32_t)(turn / STAGES) & 1u) ^ 1u, &abort_flag);
+    if (ok && lane == 0) {
+      const int tile = tile0 + n < tiles_all ? tile0 + n : tile0 + n - tiles_all, here = min(BLOCK, slots - tile * BLOCK);
+      unsigned char* to = smem + stage * G::STAGE;
+      uint64_t* bar = &full[stage];
+      const uint32_t row_at = (uint32_t)tile * G::ROWS_BYTES, scale_at = (uint32_t)tile * G::SCALE_BYTES;
+      const uint32_t row_bytes = here * (W / 2), scale_bytes = here * 4 * NP;
+      tma::mbar_expect_tx(bar, 2 * (row_bytes + scale_bytes));
+      tma::bulk_load(to, kb + row_at, row_bytes, bar);
+      tma::bulk_load(to + 2 * G::ROWS_BYTES, kscales + scale_at, scale_bytes, bar);
+      tma::bulk_load(to + G::ROWS_BYTES, vb + row_at, row_bytes, bar);
+      tma::bulk_load(to + 2 * G::ROWS_BYTES + G::SCALE_BYTES, vscales + scale_at, scale_bytes, bar);
     }
+    __syncwarp();
   };
-  const int stride = parts * WARPS;
-  int n = part * WARPS + warp;
-  __syncwarp();
-  if (n < tiles) fetch(n, 0);
-  if (n + stride < tiles) fetch(n + stride, 1);
+  __syncwarp();   // (the first warp's first lane has made the barriers)
+  for (int turn = 0; turn < STAGES - 1; turn++) fetch(turn);
 
   // queries in the order of the numbers: step u of piece p holds, of word i = 2 c + u / 2 (or c), dimensions s, s + 4 (columns 2 c, 2 c + 1) and s + 1, s + 5
   uint32_t qa[NP][KS][F32 ? 6 : 2];
@@ -201,11 +221,12 @@ __global__ void __launch_bounds__(WARPS * 32, W == 128 && (sizeof(T) == 4 || NR 
     if (on && i == 0) reinterpret_cast<uint32_t*>(ring + scales_at)[(long long)newest * NP + piece] = sc;
   }
 
-  float qs[NR][NP], slope[NR], m[NR], l[NR], low[NR][NP], o[NP][NT][4];
-  const float k0 = softcap > 0.f ? scale / softcap : 0.f, k1 = softcap > 0.f ? softcap * LOG2E : scale * LOG2E;
+  float qs[NR][NP], slope[NR], m[NR], bar[NR], l[NR], low[NR][NP], o[NP][NT][4];   // bar: what a score has to pass for the maximum to move
+  // a score is what is summed up times k_in, or, capped, tanh of that times k_out
+  const float k_in = softcap > 0.f ? scale / softcap : scale * LOG2E, k_out = softcap * LOG2E;
 #pragma unroll
   for (int r = 0; r < NR; r++) {
-    m[r] = -INFINITY;
+    m[r] = bar[r] = NOTHING;
     l[r] = 0.f;
     slope[r] = slopes && r < rows ? slopes[h0 + r] * LOG2E : 0.f;
 #pragma unroll
@@ -224,45 +245,54 @@ __global__ void __launch_bounds__(WARPS * 32, W == 128 && (sizeof(T) == 4 || NR 
   // the column of this lane's key among 16: the keys whose words a lane of the second product takes together, c, c + 4, c + 8 and c + 12, are in rows that lie in
   // more banks than neighbours
   const int column = (lane & 16) + 2 * (lane & 3) + ((lane >> 2) & 1) + (lane & 8);
-  bool ok = true;
-  for (int turn = 0; n < tiles; n += stride, turn++) {   // (the same for the whole warp)
-    int tile = tile0 + n;
-    if (tile >= tiles_all) tile -= tiles_all;
-    const unsigned char* held = mine + (turn & 1) * G::STAGE;
-    ok = tma::warp_wait_bounded(&full[warp][turn & 1], (uint32_t)(turn >> 1) & 1u, &abort_flag);
+  for (int turn = 0, n = part; n < tiles; n += parts, turn++) {   // (the same for the whole CTA)
+    const int tile = tile0 + n < tiles_all ? tile0 + n : tile0 + n - tiles_all, stage = turn % STAGES;
+    const unsigned char *rows_k = smem + stage * G::STAGE + warp * TILE * (W / 2), *rows_v = rows_k + G::ROWS_BYTES;
+    const unsigned char *scale_k = smem + stage * G::STAGE + 2 * G::ROWS_BYTES + (warp * TILE + lane) * 4 * NP, *scale_v = scale_k + G::SCALE_BYTES;
+    const uint32_t phase = (uint32_t)(turn / STAGES) & 1u;
+    fetch(turn + STAGES - 1);
+    ok = ok && (__all_sync(0xffffffffu, tma::mbar_try_wait(&full[stage], phase)) || tma::warp_wait_bounded(&full[stage], phase, &abort_flag));
     if (!ok) break;
-    // ---- scores of 8 queries with 4 x 8 keys
+    // ---- scores of 8 queries with 4 x 8 keys (a product's sum is there for the next 20 clocks later: four sums take turns)
+    {
+      uint32_t k[4][NP * G::WPL];
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
-      uint32_t k[NP * G::WPL];
-      load_words(k, held + (8 * j + gr) * (W / 2) + c * (W / 8));
+      for (int j = 0; j < 4; j++) load_words(k[j], rows_k + (8 * j + gr) * (W / 2) + c * (W / 8));
 #pragma unroll
       for (int p = 0; p < NP; p++) {
-        float s[4] = {0.f, 0.f, 0.f, 0.f};
+        float s[4][4];
 #pragma unroll
-        for (int u = 0; u < KS; u++) {
-          const uint32_t w = k[(u >> 1) * NP + p], b0 = numbers<F32>(w, 2 * (u & 1)), b1 = numbers<F32>(w, 2 * (u & 1) + 1);
-          mma(s, qa[p][u][0], F32 ? qa[p][u][2] : 0u, qa[p][u][1], F32 ? qa[p][u][3] : 0u, b0, b1);
-          if (F32) mma(s, qa[p][u][4], 0u, qa[p][u][5], 0u, b0, b1);
+        for (int u = 0; u < KS; u++)
+#pragma unroll
+          for (int j = 0; j < 4; j++) {
+            const uint32_t w = k[j][(u >> 1) * NP + p], b0 = numbers<F32>(w, 2 * (u & 1), bits), b1 = numbers<F32>(w, 2 * (u & 1) + 1, bits);
+            if (u == 0) mma_first(s[j], qa[p][u][0], F32 ? qa[p][u][2] : 0u, qa[p][u][1], F32 ? qa[p][u][3] : 0u, b0, b1);
+            else mma(s[j], qa[p][u][0], F32 ? qa[p][u][2] : 0u, qa[p][u][1], F32 ? qa[p][u][3] : 0u, b0, b1);
+            if (F32) mma(s[j], qa[p][u][4], 0u, qa[p][u][5], 0u, b0, b1);
+          }
+        if (gr < NR) {
+#pragma unroll
+          for (int j = 0; j < 4; j++)
+            *reinterpret_cast<float2*>(sS + (p * NR + gr) * TILE + 8 * j + 2 * c) = F32 ? make_float2(s[j][0] + s[j][2], s[j][1] + s[j][3]) : make_float2(s[j][0], s[j][1]);
         }
-        if (gr < NR) *reinterpret_cast<float2*>(sS + (p * NR + gr) * TILE + 8 * j + 2 * c) = F32 ? make_float2(s[0] + s[2], s[1] + s[3]) : make_float2(s[0], s[1]);
       }
     }
     __syncwarp();
     // ---- a lane per key
-    const int slot = tile * TILE + lane, behind = newest > slot ? newest - slot : newest - slot + slots;   // 1 .. slots
+    const int slot = tile * BLOCK + warp * TILE + lane, behind = newest > slot ? newest - slot : newest - slot + slots;   // 1 .. slots
     const bool seen = slot < slots && behind <= live;
     const float far = (float)behind;
     float kstep[NP], klow[NP], vstep[NP], vlow[NP];
     uint32_t ks[NP], vs[NP];
-    load_words(ks, held + 2 * G::ROWS_BYTES + lane * 4 * NP);
-    load_words(vs, held + 2 * G::ROWS_BYTES + G::SCALE_BYTES + lane * 4 * NP);
+    load_words(ks, scale_k);
+    load_words(vs, scale_v);
 #pragma unroll
     for (int p = 0; p < NP; p++) {
       kstep[p] = __uint_as_float(ks[p] & 0xffff0000u);
-      klow[p] = fmaf(F32 ? 8.f : -128.f, kstep[p], __uint_as_float(ks[p] << 16));
+      klow[p] = fmaf(F32 ? 8.f : -128.f, kstep[p], __uint_as_float(ks[p] << 16)) * k_in;
+      kstep[p] *= k_in;
       vstep[p] = seen ? __uint_as_float(vs[p] & 0xffff0000u) : 0.f;
-      vlow[p] = seen ? __uint_as_float(vs[p] << 16) : 0.f;
+      vlow[p] = seen ? fmaf(8.f, vstep[p], __uint_as_float(vs[p] << 16)) : 0.f;
     }
     bool moved = false;
     float shrink = 1.f;   // of row gr
@@ -273,31 +303,36 @@ __global__ void __launch_bounds__(WARPS * 32, W == 128 && (sizeof(T) == 4 || NR 
 #pragma unroll
         for (int p = 0; p < NP; p++) x = fmaf(kstep[p], sS[(p * NR + r) * TILE + lane], fmaf(klow[p], qs[r][p], x));
         if (softcap > 0.f) {
-          x *= k0;
           if (F32) x = tanhf(x);
           else asm("tanh.approx.f32 %0, %0;" : "+f"(x));   // relative error 2^-11
+          x *= k_out;
         }
-        x = fmaf(-slope[r], far, x * k1);
-        if (!seen) x = -INFINITY;
-        if (__any_sync(0xffffffffu, x > (m[r] == -INFINITY ? m[r] : m[r] + LAG))) {
+        x = seen ? fmaf(-slope[r], far, x) : -INFINITY;
+        if (__any_sync(0xffffffffu, x > bar[r])) {
           const float top = fmaxf(m[r], warp_max(x)), corr = exp2_fast(m[r] - top);   // (0 where there was no key yet)
           m[r] = top;
+          bar[r] = top + LAG;
           l[r] *= corr;
 #pragma unroll
           for (int p = 0; p < NP; p++) low[r][p] *= corr;
           if (gr == r) shrink = corr;
           moved = true;
         }
-        const float w = seen ? exp2_fast(x - m[r]) : 0.f;
+        const float w = exp2_fast(x - m[r]);
         l[r] += w;
 #pragma unroll
         for (int p = 0; p < NP; p++) {
-          const float a = w * vstep[p], hi = rounded(a), mid = rounded(a - hi);
+          const float a = w * vstep[p];
           __nv_bfloat16* at = reinterpret_cast<__nv_bfloat16*>(sP + (p * G::PROWS + r) * PITCH) + column;
-          at[0] = __float2bfloat16_rn(hi);
-          at[8 * PITCH / 2] = __float2bfloat16_rn(mid);
-          if (F32) at[16 * PITCH / 2] = __float2bfloat16_rn(a - hi - mid);
-          low[r][p] += fmaf(w, vlow[p], 8.f * (F32 ? a : hi + mid));
+          const float mid = a - __uint_as_float(__float_as_uint(a) & 0xffff0000u);   // (cut off, what is left is exact)
+          reinterpret_cast<unsigned short*>(at)[0] = (unsigned short)(__float_as_uint(a) >> 16);
+          if (F32) {
+            reinterpret_cast<unsigned short*>(at)[8 * PITCH / 2] = (unsigned short)(__float_as_uint(mid) >> 16);
+            at[16 * PITCH / 2] = __float2bfloat16_rn(mid - __uint_as_float(__float_as_uint(mid) & 0xffff0000u));
+          } else {
+            at[8 * PITCH / 2] = __float2bfloat16_rn(mid);
+          }
+          low[r][p] = fmaf(w, vlow[p], low[r][p]);
         }
       }
     }
@@ -315,7 +350,7 @@ __global__ void __launch_bounds__(WARPS * 32, W == 128 && (sizeof(T) == 4 || NR 
     for (int kk = 0; kk < 2; kk++) {
       uint32_t v[4][NP];   // (of a head of 32 a lane's word holds its four numbers and those of the next row's lane)
 #pragma unroll
-      for (int e = 0; e < 4; e++) load_words(v[e], held + G::ROWS_BYTES + (16 * kk + c + 4 * e) * (W / 2) + (W == 32 ? gr >> 1 : gr * NP) * 4);
+      for (int e = 0; e < 4; e++) load_words(v[e], rows_v + (16 * kk + c + 4 * e) * (W / 2) + (W == 32 ? gr >> 1 : gr * NP) * 4);
 #pragma unroll
       for (int p = 0; p < NP; p++) {
         uint32_t a[4], a3[2] = {0u, 0u};
@@ -331,14 +366,14 @@ __global__ void __launch_bounds__(WARPS * 32, W == 128 && (sizeof(T) == 4 || NR 
         }
 #pragma unroll
         for (int d = 0; d < NT; d++) {
-          const uint32_t b0 = numbers<true>(d < 4 ? lo[0] : hi[0], d & 3), b1 = numbers<true>(d < 4 ? lo[1] : hi[1], d & 3);
+          const uint32_t b0 = numbers<true>(d < 4 ? lo[0] : hi[0], d & 3, bits), b1 = numbers<true>(d < 4 ? lo[1] : hi[1], d & 3, bits);
           mma(o[p][d], a[0], a[1], a[2], a[3], b0, b1);
           if (F32) mma(o[p][d], a3[0], 0u, a3[1], 0u, b0, b1);
         }
       }
     }
     __syncwarp();
-    if (n + 2 * stride < tiles) fetch(n + 2 * stride, turn & 1);
+    if (lane == 0) tma::mbar_arrive(&empty[stage]);
   }
   // ---- this warp's rows; then the CTA's
   __syncthreads();   // (what they are written to is other warps' scratch)
@@ -375,13 +410,13 @@ __global__ void __launch_bounds__(WARPS * 32, W == 128 && (sizeof(T) == 4 || NR 
   const bool one = parts == 1;
   for (int e = threadIdx.x; e < rows * W; e += WARPS * 32) {
     const int r = e / W, d = e % W;
-    float top = one ? s_own[r] : -INFINITY, num = 0.f, den = 0.f;
+    float top = one ? s_own[r] : NOTHING, num = 0.f, den = 0.f;
 #pragma unroll
     for (int w = 0; w < WARPS; w++) top = fmaxf(top, s_m[w][r]);
 #pragma unroll
     for (int w = 0; w < WARPS; w++) {
-      const float f = s_m[w][r] > -INFINITY ? exp2_fast(s_m[w][r] - top) : (s_l[w][r] == s_l[w][r] ? 0.f : s_l[w][r]);   // (a warp that saw NaN alone has no maximum)
-      if (s_m[w][r] > -INFINITY || !(f == 0.f)) num = fmaf(sO[(w * NR + r) * W + d], f, num);
+      const float f = exp2_fast(s_m[w][r] - top);
+      num = fmaf(sO[(w * NR + r) * W + d], f, num);
       den = fmaf(s_l[w][r], f, den);
     }
     if (one) {
@@ -401,14 +436,12 @@ __global__ void __launch_bounds__(WARPS * 32, W == 128 && (sizeof(T) == 4 || NR 
   if (part == 0) {
     for (int e = threadIdx.x; e < rows * W; e += WARPS * 32) {
       const int r = e / W, d = e % W;
-      float ms[8], top = s_own[r];
-      for (int i = 0; i < parts; i++) top = fmaxf(top, ms[i & 7] = *cluster.map_shared_rank(&c_m[r], i));
-      float num = 0.f, den = 0.f;
+      float top = s_own[r], num = 0.f, den = 0.f;
+      for (int i = 0; i < parts; i++) top = fmaxf(top, *cluster.map_shared_rank(&c_m[r], i));
       for (int i = 0; i < parts; i++) {
-        const float li = *cluster.map_shared_rank(&c_l[r], i);
-        const float f = ms[i & 7] > -INFINITY ? exp2_fast(ms[i & 7] - top) : (li == li ? 0.f : li);
-        if (!(f == 0.f)) num = fmaf(*cluster.map_shared_rank(&sO[r * W + d], i), f, num);
-        den = fmaf(li, f, den);
+        const float f = exp2_fast(*cluster.map_shared_rank(&c_m[r], i) - top);
+        num = fmaf(*cluster.map_shared_rank(&sO[r * W + d], i), f, num);
+        den = fmaf(*cluster.map_shared_rank(&c_l[r], i), f, den);
       }
       const float f = exp2_fast(s_own[r] - top);
       if (d < hd) out[((long long)b * H + h0 + r) * hd + d] = Elem<T>::from_f(fmaf(f, Elem<T>::to_f(row[(long long)(H + Hk + g) * hd + d]), num) / (den + f));
@@ -421,14 +454,25 @@ template <typename T, int W, int NR>
 int launch(const void* qkv, long long row_stride, void* k4, void* v4, int* pos, const float* slopes, void* out, int B, int H, int Hk, int hd, int slots,
            int window, float softcap, int update_cache, int* status, cudaStream_t st) {
   typedef Geometry<T, W> G;
-  const size_t smem = (size_t)WARPS * G::warp_bytes(NR);
-  static_assert(G::warp_bytes(NR) >= NR * W * 4, "the warps' rows are merged there");
+  const size_t smem = G::bytes(NR);
+  static_assert(G::bytes(NR) >= WARPS * NR * W * 4, "the warps' rows are merged there");
   static SmemLimit limit;
   cudaError_t e = allow_smem((const void*)kv4_step_kernel<T, W, NR>, smem, limit);
   if (e != cudaSuccess) return (int)e;
   const int groups = (H / Hk + 7) / 8;
+  // CTAs that share the keys: the number with which the fullest SM has least to do, a CTA's beginning and end counted as 2 tiles.
+  const long long pairs = (long long)Hk * B * groups, sms = device_sm_count();
+  const int tiles = window / BLOCK + 1, per_sm = W == 128 ? 3 : 4;
   int splits = 1;
-  while (splits < 8 && 2ll * splits * Hk * B * groups <= 4ll * device_sm_count() && window / (2 * splits) >= WARPS * TILE / 2) splits *= 2;
+  double least = 1e30;
+  for (int s = 1; s <= 8 && s <= tiles; s++) {
+    const long long on_one = (pairs * s + sms - 1) / sms;
+    const double cost = (double)on_one * ((double)tiles / s + 2) / (double)(on_one < per_sm ? on_one : per_sm);
+    if (cost < least) {
+      least = cost;
+      splits = s;
+    }
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(Hk * splits, B, groups);
   cfg.blockDim = dim3(WARPS * 32);

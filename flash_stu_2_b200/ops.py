@@ -1152,7 +1152,7 @@ def kv4_rings(batch: int, slots: int, kv_heads: int, hd: int, device):
 
 
 def _kv4_check(k4: torch.Tensor, v4: torch.Tensor, hd: int, what: str) -> int:
-    """Slots of the rings."""
+    """Slots of the rings (at most 2^24)."""
     row = _kv4_row_bytes(hd)
     if k4.dtype != torch.uint8 or v4.dtype != torch.uint8:
         raise TypeError(f"{what}: rings are uint8, got {k4.dtype} and {v4.dtype}")
