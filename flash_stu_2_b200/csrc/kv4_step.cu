@@ -1,7 +1,7 @@
 // Attention of one new token per sequence over its ring of 4 bits (kv4.cuh), which takes the token's key and value in.
 //
 // A CTA (or a cluster of up to 8 that share the keys) works for one key head of one sequence and up to 8 of its query heads; a warp takes 32 slots at a time.
-//   scores   mma.sync, queries as rows, the numbers of 8 keys as columns: a number n becomes bf16 by putting its bits under those of 128 (128 + n is exact), so
+//   scores   mma.sync, the numbers of 16 keys as rows, 8 queries as columns: a number n becomes bf16 by putting its bits under those of 128 (128 + n is exact), so
 //            that two of them cost a shift and a logical operation.  A piece's scale is the same for all of a row's products:
 //              q.k = sum over pieces of  step (q.(128 + n)) + (lowest - 128 step) sum(q)
 //   softmax  a lane per key, the scores handed over through shared memory: cap, ALiBi, window, exponentials in the exp2 domain against a maximum that moves only when
@@ -31,6 +31,7 @@ constexpr float NOTHING = -3.0e38f;      // the maximum of no scores
 constexpr float LAG = 8.f;               // exp2 domain
 constexpr int STATUS_KV4 = 14;
 constexpr int PITCH = TILE * 2 + 16;     // bytes between rows of weights: eight rows' 16 bytes lie in different banks
+constexpr int S_PITCH = TILE + 4;        // numbers between rows of scores: those of 8 keys and 4 queries lie in different banks
 
 template <typename T, int W> struct Geometry {
   static constexpr bool F32 = sizeof(T) == 4;
@@ -41,7 +42,7 @@ template <typename T, int W> struct Geometry {
   static constexpr int PROWS = F32 ? 24 : 16;             // rows of weights
   static constexpr int ROWS_BYTES = BLOCK * W / 2, SCALE_BYTES = BLOCK * 4 * NP, STAGE = 2 * (ROWS_BYTES + SCALE_BYTES);   // keys, values, their scales
   static constexpr int P_BYTES = NP * PROWS * PITCH;
-  __host__ __device__ static constexpr int warp_bytes(int rows) { return NP * rows * TILE * 4 + P_BYTES; }
+  __host__ __device__ static constexpr int warp_bytes(int rows) { return NP * rows * S_PITCH * 4 + P_BYTES; }
   __host__ __device__ static constexpr int bytes(int rows) { return STAGES * STAGE + WARPS * warp_bytes(rows); }
 };
 
@@ -97,7 +98,7 @@ __global__ void __launch_bounds__(WARPS * 32, W == 128 ? 3 : 4) kv4_step_kernel(
   constexpr int NP = G::NP, KS = G::KS, NT = G::NT;
   constexpr float LOG2E = 1.4426950408889634f;
   extern __shared__ __align__(16) unsigned char smem[];
-  __shared__ float s_qsum[8][2], s_own[8], s_m[WARPS][8], s_l[WARPS][8], c_m[8], c_l[8];
+  __shared__ float s_qsum[8][2], s_slope[8], s_own[8], s_m[WARPS][8], s_l[WARPS][8], c_m[8], c_l[8];
   const int g = blockIdx.x / splits, part = blockIdx.x - g * splits, b = blockIdx.y;
   const int R = H / Hk, r0 = blockIdx.z * 8, rows = min(8, R - r0), h0 = g * R + r0;   // the query heads h0 .. h0 + rows - 1
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, gr = lane >> 2, c = lane & 3;
@@ -105,7 +106,7 @@ __global__ void __launch_bounds__(WARPS * 32, W == 128 ? 3 : 4) kv4_step_kernel(
   __shared__ int abort_flag;
   unsigned char* mine = smem + STAGES * G::STAGE + warp * G::warp_bytes(NR);
   float* sS = reinterpret_cast<float*>(mine);             // [piece][row][32 keys]
-  unsigned char* sP = mine + NP * NR * TILE * 4;          // [piece][hi 8, mid 8 (, lo 8) rows][32 keys] bf16
+  unsigned char* sP = mine + NP * NR * S_PITCH * 4;          // [piece][hi 8, mid 8 (, lo 8) rows][32 keys] bf16
   for (int e = lane; e < G::P_BYTES / 4; e += 32) reinterpret_cast<uint32_t*>(sP)[e] = 0;   // (rows without a query stay as they are)
   if (threadIdx.x == 0) {
     for (int i = 0; i < STAGES; i++) {
@@ -206,6 +207,7 @@ __global__ void __launch_bounds__(WARPS * 32, W == 128 ? 3 : 4) kv4_step_kernel(
       s_qsum[r][0] = sum0;
       s_qsum[r][1] = sum1;
       s_own[r] = dot * LOG2E;
+      s_slope[r] = slopes ? slopes[h0 + r] * LOG2E : 0.f;
     }
   }
   __syncthreads();
@@ -221,19 +223,15 @@ __global__ void __launch_bounds__(WARPS * 32, W == 128 ? 3 : 4) kv4_step_kernel(
     if (on && i == 0) reinterpret_cast<uint32_t*>(ring + scales_at)[(long long)newest * NP + piece] = sc;
   }
 
-  float qs[NR][NP], slope[NR], m[NR], bar[NR], l[NR], low[NR][NP], o[NP][NT][4];   // bar: what a score has to pass for the maximum to move
+  float m[NR], bar[NR], l[NR], low[NR][NP], o[NP][NT][4];   // bar: what a score has to pass for the maximum to move
   // a score is what is summed up times k_in, or, capped, tanh of that times k_out
   const float k_in = softcap > 0.f ? scale / softcap : scale * LOG2E, k_out = softcap * LOG2E;
 #pragma unroll
   for (int r = 0; r < NR; r++) {
     m[r] = bar[r] = NOTHING;
     l[r] = 0.f;
-    slope[r] = slopes && r < rows ? slopes[h0 + r] * LOG2E : 0.f;
 #pragma unroll
-    for (int p = 0; p < NP; p++) {
-      low[r][p] = 0.f;
-      qs[r][p] = r < rows ? s_qsum[r][p] : 0.f;
-    }
+    for (int p = 0; p < NP; p++) low[r][p] = 0.f;
   }
 #pragma unroll
   for (int p = 0; p < NP; p++)
@@ -253,29 +251,35 @@ __global__ void __launch_bounds__(WARPS * 32, W == 128 ? 3 : 4) kv4_step_kernel(
     fetch(turn + STAGES - 1);
     ok = ok && (__all_sync(0xffffffffu, tma::mbar_try_wait(&full[stage], phase)) || tma::warp_wait_bounded(&full[stage], phase, &abort_flag));
     if (!ok) break;
-    // ---- scores of 8 queries with 4 x 8 keys (a product's sum is there for the next 20 clocks later: four sums take turns)
+    // ---- scores of 2 x 16 keys with 8 queries (a product's sum is there for the next 20 clocks later: four of them take turns)
     {
       uint32_t k[4][NP * G::WPL];
 #pragma unroll
       for (int j = 0; j < 4; j++) load_words(k[j], rows_k + (8 * j + gr) * (W / 2) + c * (W / 8));
+      float s[NP][2][4];
 #pragma unroll
-      for (int p = 0; p < NP; p++) {
-        float s[4][4];
+      for (int u = 0; u < KS; u++)
 #pragma unroll
-        for (int u = 0; u < KS; u++)
+        for (int p = 0; p < NP; p++)
 #pragma unroll
-          for (int j = 0; j < 4; j++) {
-            const uint32_t w = k[j][(u >> 1) * NP + p], b0 = numbers<F32>(w, 2 * (u & 1), bits), b1 = numbers<F32>(w, 2 * (u & 1) + 1, bits);
-            if (u == 0) mma_first(s[j], qa[p][u][0], F32 ? qa[p][u][2] : 0u, qa[p][u][1], F32 ? qa[p][u][3] : 0u, b0, b1);
-            else mma(s[j], qa[p][u][0], F32 ? qa[p][u][2] : 0u, qa[p][u][1], F32 ? qa[p][u][3] : 0u, b0, b1);
-            if (F32) mma(s[j], qa[p][u][4], 0u, qa[p][u][5], 0u, b0, b1);
+          for (int j = 0; j < 2; j++) {
+            const uint32_t w0 = k[2 * j][(u >> 1) * NP + p], w1 = k[2 * j + 1][(u >> 1) * NP + p];
+            const uint32_t a0 = numbers<F32>(w0, 2 * (u & 1), bits), a1 = numbers<F32>(w1, 2 * (u & 1), bits);
+            const uint32_t a2 = numbers<F32>(w0, 2 * (u & 1) + 1, bits), a3 = numbers<F32>(w1, 2 * (u & 1) + 1, bits);
+            if (u == 0) mma_first(s[p][j], a0, a1, a2, a3, qa[p][u][0], qa[p][u][1]);
+            else mma(s[p][j], a0, a1, a2, a3, qa[p][u][0], qa[p][u][1]);
+            if (F32) {
+              mma(s[p][j], a0, a1, a2, a3, qa[p][u][2], qa[p][u][3]);
+              mma(s[p][j], a0, a1, a2, a3, qa[p][u][4], qa[p][u][5]);
+            }
           }
-        if (gr < NR) {
 #pragma unroll
-          for (int j = 0; j < 4; j++)
-            *reinterpret_cast<float2*>(sS + (p * NR + gr) * TILE + 8 * j + 2 * c) = F32 ? make_float2(s[j][0] + s[j][2], s[j][1] + s[j][3]) : make_float2(s[j][0], s[j][1]);
-        }
-      }
+      for (int p = 0; p < NP; p++)
+#pragma unroll
+        for (int j = 0; j < 2; j++)
+#pragma unroll
+          for (int e = 0; e < 4; e++)
+            if (2 * c + (e & 1) < NR) sS[(p * NR + 2 * c + (e & 1)) * S_PITCH + 16 * j + gr + 8 * (e >> 1)] = s[p][j][e];
     }
     __syncwarp();
     // ---- a lane per key
@@ -301,13 +305,13 @@ __global__ void __launch_bounds__(WARPS * 32, W == 128 ? 3 : 4) kv4_step_kernel(
       if (r < rows) {   // (the same for the whole CTA)
         float x = 0.f;
 #pragma unroll
-        for (int p = 0; p < NP; p++) x = fmaf(kstep[p], sS[(p * NR + r) * TILE + lane], fmaf(klow[p], qs[r][p], x));
+        for (int p = 0; p < NP; p++) x = fmaf(kstep[p], sS[(p * NR + r) * S_PITCH + lane], fmaf(klow[p], s_qsum[r][p], x));
         if (softcap > 0.f) {
           if (F32) x = tanhf(x);
           else asm("tanh.approx.f32 %0, %0;" : "+f"(x));   // relative error 2^-11
           x *= k_out;
         }
-        x = seen ? fmaf(-slope[r], far, x) : -INFINITY;
+        x = seen ? fmaf(-s_slope[r], far, x) : -INFINITY;
         if (__any_sync(0xffffffffu, x > bar[r])) {
           const float top = fmaxf(m[r], warp_max(x)), corr = exp2_fast(m[r] - top);   // (0 where there was no key yet)
           m[r] = top;
