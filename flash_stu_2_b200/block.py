@@ -48,6 +48,7 @@ class FlashSTUBlock(nn.Module):
                 use_approx=kwargs.get("use_approx", True), use_hankel_L=kwargs.get("use_hankel_L", False),
                 softcap=50.0, n_layers=1, bsz=1, vocab_size=1, stu_enable_mlp_sandwich=stu_enable_mlp_sandwich,
                 stu_mlp_hidden_size=stu_mlp_hidden_size, mlp_fp8=kwargs.get("mlp_fp8", False),
+                kv_bits=kwargs.get("kv_bits"),
             )
             for key, value in (attention_config or {}).items():
                 if key in fields:

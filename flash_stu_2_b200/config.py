@@ -17,7 +17,9 @@ class FlashSTUConfig(PretrainedConfig):
     Beyond the reference's: cache_len caps the positions that caches are laid out for; mlp_fp8 runs the layers' MLPs in 8 bits (e4m3
     weights and activations with a power-of-two scale for each 128 of a row, bfloat16 models): checkpoints are the same, the 8-bit
     weights are made from them at the first call.  Prefills and MLPs of 1536 and wider gain; token steps of small layers lose, whose bf16
-    sub-layers are one kernel (a block of d=1024: 8 sequences 21 -> 27 us).
+    sub-layers are one kernel (a block of d=1024: 8 sequences 21 -> 27 us).  kv_bits=4 holds the attention layers' keys and values in 4 bits (with a
+    lowest value and a step for each 64 of a head: 4.5 bits a number, head dimensions of a multiple of 8): a token step reads 3.6 times less of them, and they take as
+    much less memory; each is up to 1/30 of its 64's range off.  Small batches are then stepped layer by layer, not by one kernel for all of them.
     """
     model_type = "FlashSTU"
 
@@ -50,6 +52,7 @@ class FlashSTUConfig(PretrainedConfig):
         d_out_tile: Optional[int] = None,
         cache_len: Optional[int] = None,
         mlp_fp8: bool = False,
+        kv_bits: Optional[int] = None,
         **kwargs,
     ):
         # transformers >= 5 serialises a model's dtype under the key `dtype` (and drops `torch_dtype` from the dict it
@@ -68,6 +71,7 @@ class FlashSTUConfig(PretrainedConfig):
             use_cache=use_cache, use_gradient_checkpointing=use_gradient_checkpointing, softcap=softcap,
             stu_enable_mlp_sandwich=stu_enable_mlp_sandwich, stu_mlp_hidden_size=stu_mlp_hidden_size,
             filter_path=filter_path, d_in_tile=d_in_tile, d_out_tile=d_out_tile, cache_len=cache_len, mlp_fp8=mlp_fp8,
+            kv_bits=kv_bits,
         ).items():
             setattr(self, name, value)
         self.hidden_size = n_embd

@@ -152,15 +152,50 @@ class STULayer(nn.Module):
         _mlp_step(mlp, mid, x2, mlp_norm, True, ops.can_fuse_norm(B, mlp.intermediate_size, d, ops.EPI_GELU_MUL, x.dtype))
         return entry
 
-    def forward(self, x: torch.Tensor, past_key_value=None, use_cache=False):
+    def _packed(self, xc, packed, use_cache: bool):
+        """The prompts one after the other (each has a convolution of its own); the cache holds all of them."""
+        stu = self.stu
+        if use_cache and (not stu.use_approx or stu.use_hankel_L or self.stu_mlp_enabled):
+            raise NotImplementedError("caches of packed prompts stand at different positions: plain approx STU layers step from such")
+        if max(packed.lengths) > stu.capacity:
+            raise ValueError(f"a prompt of {max(packed.lengths)} positions exceeds the capacity {stu.capacity} (seq_len={stu.seq_len})")
+        entry = stu.new_cache(len(packed.lengths), xc.device) if use_cache else None
+        at = 0
+        for s, n in enumerate(packed.lengths):
+            if n:
+                own_entry = None
+                if use_cache:
+                    pos = entry[1][s:s + 1]
+                    pos._host_t, pos._uniform = 0, True
+                    own_entry = (entry[0][s:s + 1], pos)
+                # (not a token step, however short the prompt is)
+                self._several(xc[:, at:at + n], own_entry, use_cache)
+            at += n
+        if use_cache:
+            packed.note(entry[1])
+        return entry
+
+    def forward(self, x: torch.Tensor, past_key_value=None, use_cache=False, packed=None):
         xc = _inplace_target(x)
+        if packed is not None:
+            entry = self._packed(xc, packed, use_cache)
+        elif self.stu_mlp_enabled or xc.shape[1] != 1 or past_key_value is None:
+            entry = self._several(xc, past_key_value, use_cache)
+        else:
+            entry = self._decode(xc, past_key_value)
+        if xc is not x:
+            x.copy_(xc)
+        if use_cache:
+            return x, entry
+        return x
+
+    def _several(self, xc, past_key_value, use_cache):
+        """New positions of every sequence, in place on the contiguous xc [B,T,d]."""
         B, T, d = xc.shape
         if self.stu_mlp_enabled:
             entry = self._sandwich(xc, past_key_value, use_cache)
             x2 = xc.view(B * T, d)
             _mlp_step(self.mlp, x2, x2, self.mlp_norm, False, False)
-        elif T == 1 and past_key_value is not None:
-            entry = self._decode(xc, past_key_value)
         else:
             stu, mlp = child(self, "stu"), child(self, "mlp")
             stu_norm, mlp_norm = child(self, "stu_norm"), child(self, "mlp_norm")
@@ -173,11 +208,7 @@ class STULayer(nn.Module):
             if done != 3:
                 x2 = xc.view(B * T, d)
                 _mlp_step(mlp, x2, x2, mlp_norm, False, False)
-        if xc is not x:
-            x.copy_(xc)
-        if use_cache:
-            return x, entry
-        return x
+        return entry
 
 
 class AttentionLayer(nn.Module):
@@ -189,17 +220,17 @@ class AttentionLayer(nn.Module):
         self.mlp_norm = RMSNorm(config.n_embd, dtype=config.torch_dtype)
         self.mlp = make_mlp(config, dtype=config.torch_dtype)
 
-    def forward(self, x: torch.Tensor, past_key_value=None, use_cache=True):
+    def forward(self, x: torch.Tensor, past_key_value=None, use_cache=True, packed=None):
         xc = _inplace_target(x)
         B, T, d = xc.shape
         x2 = xc.view(B * T, d)
         attn, mlp = child(self, "attn"), child(self, "mlp")
         attn_norm, mlp_norm = child(self, "attn_norm"), child(self, "mlp_norm")
-        if T == 1 and ops.can_fuse_norm(B, 3 * d, d, ops.EPI_STORE, x.dtype):
+        if T == 1 and packed is None and ops.can_fuse_norm(B, 3 * d, d, ops.EPI_STORE, x.dtype):
             y, entry = attn.attend(xc, past_key_value, use_cache, norm_w=param(attn_norm, "weight"), eps=attn_norm.eps)
         else:
             xn = ops.rmsnorm(xc, param(attn_norm, "weight"), attn_norm.eps)
-            y, entry = attn.attend(xn, past_key_value, use_cache)
+            y, entry = attn.attend(xn, past_key_value, use_cache) if packed is None else attn.attend(xn, None, use_cache, packed=packed)
         ov = ops.FLAG_OVERLAP if (T == 1 and ops.overlap_decode) else 0   # token step: weights fetched early
         c_proj = param(child(attn, "c_proj"), "weight")
         if getattr(mlp, "fp8", False):   # the branch joins the stream in the norm

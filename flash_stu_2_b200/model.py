@@ -11,7 +11,7 @@ can observe, all forced by the reference's own gaps:
 import contextlib
 import gc
 import threading
-from typing import Any, Dict, Optional, Tuple
+from typing import Any, Dict, Optional, Sequence, Tuple
 
 import torch
 import torch.nn as nn
@@ -23,7 +23,7 @@ from . import ops
 from .config import FlashSTUConfig
 from .filters import get_spectral_filters, nearest_power_of_two
 from .layers import AttentionLayer, STULayer
-from .modules import STU, Attention, RMSNorm
+from .modules import STU, Attention, Packed, RMSNorm
 from .stream_ahead import StreamAhead
 from .token_step import TokenStep
 
@@ -118,17 +118,31 @@ class FlashSTU(PreTrainedModel):
         self.lm_head = value
 
     # ------------------------------------------------------------------ backbone
-    def _backbone(self, input_ids, past_key_values, use_cache: bool, collect_hidden: bool = False):
+    def _backbone(self, input_ids, past_key_values, use_cache: bool, collect_hidden: bool = False, lengths=None):
         if not input_ids.is_cuda:
             raise RuntimeError("flash_stu_2_b200 has no CPU path: move the model and input_ids to a CUDA device")
         if self.training and self.config.dropout > 0:
             raise NotImplementedError("dropout > 0 in training mode has no kernel here (inference path only)")
+        packed = None
+        if lengths is not None:
+            if input_ids.dim() != 2 or input_ids.shape[0] != 1 or not 0 < sum(lengths) == input_ids.shape[1] or past_key_values is not None:
+                raise ValueError(f"packed prompts are input_ids [1, {sum(lengths)}] (the sum of their lengths) without past_key_values, got "
+                                 f"{tuple(input_ids.shape)}")
+            packed = Packed(lengths, input_ids.device)
+        elif past_key_values is not None and input_ids.shape[1] > 1 and any(
+                e is not None and getattr(e[-1], "_uniform", True) is False for e in past_key_values):
+            raise ValueError("caches at different positions take one token per sequence at a time")
         x = ops.embed(input_ids, self.tok_emb.weight)
         hidden = (x.clone(),) if collect_hidden else None
         cache = () if use_cache else None
         for idx, layer in enumerate(self.layers):
             past = past_key_values[idx] if past_key_values is not None else None
-            if use_cache:
+            if packed is not None:
+                x = layer(x, use_cache=use_cache, packed=packed)
+                if use_cache:
+                    x, present = x
+                    cache = cache + (present,)
+            elif use_cache:
                 x, present = layer(x, past_key_value=past, use_cache=True)
                 cache = cache + (present,)
             else:
@@ -146,15 +160,19 @@ class FlashSTU(PreTrainedModel):
         use_cache: Optional[bool] = None,
         output_hidden_states: Optional[bool] = None,
         return_dict: Optional[bool] = None,
+        lengths: Optional[Sequence[int]] = None,
         **kwargs,
     ):
+        """As the reference's.  Beyond it: `lengths` (numbers on the host): input_ids [1, N] are prompts of these lengths behind one another, each of
+        which sees itself alone; logits are [1, N, V], and the cache (models with kv_bits=4 whose STU layers are plain approx ones) holds a sequence for each
+        prompt, from which calls of one token per sequence, input_ids [prompts, 1], go on."""
         if input_ids is None:
             raise ValueError("input_ids must be provided")
         if labels is not None:
             raise NotImplementedError("the loss/labels path is training code and is not part of this implementation")
         return_dict = True if return_dict is None else return_dict
         use_cache = use_cache if use_cache is not None else bool(getattr(self.config, "use_cache", False))
-        x, cache, hidden = self._backbone(input_ids, past_key_values, use_cache, bool(output_hidden_states))
+        x, cache, hidden = self._backbone(input_ids, past_key_values, use_cache, bool(output_hidden_states), *(() if lengths is None else (lengths,)))
         B, T, d = x.shape
         xn = ops.rmsnorm(x, self.norm.weight, self.norm.eps)
         logits = ops.linear(xn.view(B * T, d), self.lm_head.weight).view(B, T, -1)

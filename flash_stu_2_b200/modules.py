@@ -619,10 +619,29 @@ class STU(nn.Module):
         return y
 
 
+class Packed:
+    """Prompts of different lengths behind one another: the lengths, and where each begins (with the end behind the last) on the device."""
+    __slots__ = ("lengths", "cu")
+
+    def __init__(self, lengths, device):
+        self.lengths = [int(n) for n in lengths]
+        if not self.lengths or min(self.lengths) < 0:
+            raise ValueError(f"lengths of packed prompts are at least one number, none below 0: {self.lengths}")
+        ends = [0]
+        for n in self.lengths:
+            ends.append(ends[-1] + n)
+        self.cu = torch.tensor(ends, dtype=torch.int32, device=device)
+
+    def note(self, pos: torch.Tensor):
+        """What the host knows of positions that stand behind these prompts (_host_t: the furthest)."""
+        pos._host_t, pos._uniform = max(self.lengths), min(self.lengths) == max(self.lengths)
+
+
 class Attention(nn.Module):
     """Causal sliding-window multi-head attention with ALiBi slopes (x0.25) and tanh soft-capping
     (flash_stu/modules/attention.py:16-105).  Cache entry = (k_ring [B,W,d], v_ring [B,W,d], pos [B,2])
-    with W = window+1 slots, exact because older keys can never be attended."""
+    with W = window+1 slots, exact because older keys can never be attended; with config.kv_bits = 4 the rings are
+    in 4 bits (ops.kv4_rings), and keys and values of earlier calls are what these hold."""
 
     def __init__(self, config):
         super().__init__()
@@ -633,6 +652,11 @@ class Attention(nn.Module):
         self.head_dim = config.n_embd // config.n_heads
         if self.head_dim > 128:
             raise NotImplementedError("head_dim > 128 has no kernel here")
+        self.kv_bits = getattr(config, "kv_bits", None)
+        if self.kv_bits not in (None, 4):
+            raise NotImplementedError(f"kv_bits={self.kv_bits}: a cache is held in the model's type (None) or in 4 bits")
+        if self.kv_bits is not None and self.head_dim % 8:
+            raise NotImplementedError(f"kv_bits=4 has kernels for head dimensions of a multiple of 8, not {self.head_dim}")
         self.bsz = config.bsz
         self.c_attn = nn.Linear(config.n_embd, 3 * config.n_embd, bias=False, dtype=config.torch_dtype)
         self.c_proj = nn.Linear(config.n_embd, config.n_embd, bias=False, dtype=config.torch_dtype)
@@ -662,12 +686,14 @@ class Attention(nn.Module):
         d = self.n_heads * self.head_dim
         W = self.window + 1
         dt = self.c_attn.weight.dtype
+        if self.kv_bits is not None:
+            return (*ops.kv4_rings(batch, ops.kv4_slots(self.window), self.n_heads, self.head_dim, device), new_pos(batch, device))
         make = torch.empty if filled >= W else torch.zeros   # a prefill of W positions or more writes every slot
         return make(batch, W, d, dtype=dt, device=device), make(batch, W, d, dtype=dt, device=device), new_pos(batch, device)
 
-    def attend(self, xn: torch.Tensor, entry=None, use_cache: bool = False, norm_w=None, eps: float = 0.0):
+    def attend(self, xn: torch.Tensor, entry=None, use_cache: bool = False, norm_w=None, eps: float = 0.0, packed: Optional["Packed"] = None):
         """Heads merged, before c_proj: returns (y [B,T,d], entry).  With norm_w, xn is the un-normalised layer input
-        and the RMSNorm is applied inside the c_attn kernel (token steps)."""
+        and the RMSNorm is applied inside the c_attn kernel (token steps).  packed: xn [1,N,d] holds these prompts behind one another."""
         B, T, d = xn.shape
         c_attn = param(child(self, "c_attn"), "weight")
         if norm_w is not None:
@@ -675,8 +701,19 @@ class Attention(nn.Module):
         else:
             ov = ops.FLAG_OVERLAP if (T == 1 and ops.overlap_decode) else 0   # token step: weights fetched early
             qkv = ops.linear(xn.reshape(B * T, d), c_attn, epilogue=ops.EPI_STORE | ov).view(B, T, 3 * d)
+        if packed is not None:
+            y = ops.swa_packed(qkv[0], packed.cu, self.alibi_slopes, self.n_heads, self.window, self.softcap).view(B, T, d)
+            if use_cache:
+                if self.kv_bits is None:
+                    raise NotImplementedError("the caches of packed prompts are held in 4 bits (kv_bits=4)")
+                k4, v4, pos = entry = self.new_cache(len(packed.lengths), xn.device)
+                ops.kv4_write(qkv[0], k4, v4, pos, self.n_heads, cu_seqlens=packed.cu)
+                packed.note(pos)
+            return y, entry
         if entry is None and use_cache:
             entry = _cache_for_prefill(self, Attention, B, xn.device, T)
+        if entry is not None and self.kv_bits is not None:
+            return self._attend_kv4(qkv, entry), entry
         if entry is not None:
             k_ring, v_ring, pos = entry
             t0 = host_pos(pos)
@@ -690,6 +727,23 @@ class Attention(nn.Module):
         y = attend(qkv, dummy, dummy, new_pos(B, xn.device), self.alibi_slopes, self.n_heads, self.window,
                    self.softcap, update_cache=False)
         return y, None
+
+    def _attend_kv4(self, qkv: torch.Tensor, entry):
+        """New tokens over rings of 4 bits, which take theirs in.  Several of them: the rings are read back, and the kernels for rings of values run."""
+        k4, v4, pos = entry
+        t0, T = host_pos(pos), qkv.shape[1]
+        if T == 1:
+            y = ops.kv4_step(qkv, k4, v4, pos, self.alibi_slopes, self.n_heads, self.window, self.softcap)
+        else:
+            if uniform_pos(pos) and ops.swa_prefill_tc5_supported(qkv, self.n_heads, t0, self.window):
+                y = ops.swa_prefill_tc5(qkv, qkv, qkv, pos, self.alibi_slopes, self.n_heads, self.window, self.softcap, update_cache=False)
+            else:
+                begun = t0 > 0 or not uniform_pos(pos)
+                k, v = ops.kv4_read(k4, v4, self.head_dim, qkv.dtype) if begun else (torch.zeros(1, 1, 1, dtype=qkv.dtype, device=qkv.device),) * 2
+                y = ops.swa_forward(qkv, k, v, pos, self.alibi_slopes, self.n_heads, self.window, self.softcap, update_cache=False)
+            ops.kv4_write(qkv, k4, v4, pos, self.n_heads)
+        pos._host_t = t0 + T
+        return y
 
     def forward(self, x, past_key_value=None, use_cache=True):
         B, T, d = x.shape

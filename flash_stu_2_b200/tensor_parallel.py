@@ -131,6 +131,8 @@ class TensorParallelFlashSTU:
             raise NotImplementedError("tensor parallelism covers the approx STU variant")
         if getattr(config, "mlp_fp8", False):
             raise NotImplementedError("tensor parallelism has no MLP in 8 bits")
+        if getattr(config, "kv_bits", None) is not None:
+            raise NotImplementedError("tensor parallelism has no cache in 4 bits")
         c = dict(n_embd=config.n_embd, n_heads=config.n_heads)
         if presharded:
             self.sd = {k: v.to(self.device) for k, v in state_dict.items()}

@@ -12,14 +12,14 @@ from .modules import host_pos, uniform_pos
 
 def layer_supported(layer) -> bool:
     """Whether a layer's token step is one the kernel computes: a plain approx STU layer or an attention layer, whose
-    forward() nobody overrides or listens to, with an MLP that is not in 8 bits."""
+    forward() nobody overrides or listens to, with an MLP and a cache that are not in 8 or 4 bits."""
     if type(layer) not in (STULayer, AttentionLayer) or "forward" in vars(layer) or layer._forward_hooks or layer._forward_pre_hooks:
         return False
     if getattr(layer.mlp, "fp8", False):
         return False
     if hasattr(layer, "stu"):
         return layer.stu.use_approx and not layer.stu.use_hankel_L and not layer.stu_mlp_enabled
-    return hasattr(layer, "attn")
+    return hasattr(layer, "attn") and layer.attn.kv_bits is None
 
 
 def layer_weights(layer, d: int, inter: int):

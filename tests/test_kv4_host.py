@@ -138,3 +138,40 @@ def test_argument_errors_without_a_gpu():
     assert lib.stu_swa_packed(a, 256, a, 0, None, a, 128, 5, 2, 1, 64, -1, 0.0, None, 1, None) == -2
     assert lib.stu_swa_packed(a, 800, a, 1, None, a, 400, 5, 2, 1, 200, -1, 0.0, None, 1, None) == -4
     assert lib.stu_swa_packed(a, 256, a, 1, None, None, 128, 5, 2, 1, 64, -1, 0.0, None, 1, None) == -5
+
+
+def test_models_without_a_gpu(tmp_path):
+    import flash_stu_2_b200 as F
+    from flash_stu_2_b200.modules import Packed
+    from flash_stu_2_b200.token_step import layer_supported
+
+    def config(**kw):
+        return F.FlashSTUConfig(**{**dict(n_embd=64, n_heads=4, n_layers=2, seq_len=64, window_size=20, vocab_size=11, mlp_scale=2, num_eigh=4), **kw})
+
+    assert config().kv_bits is None and F.FlashSTUConfig.from_dict(config(kv_bits=4).to_dict()).kv_bits == 4
+    attn = F.Attention(config(kv_bits=4))
+    k4, v4, pos = attn.new_cache(3, "cpu")
+    assert k4.shape == v4.shape == (3, 4, 32 * 20) and pos.shape == (3, 2)
+    assert F.FlashSTUBlock(d_model=64, sequence_length=64, num_filters=4, use_attention=True, kv_bits=4).layer.attn.kv_bits == 4
+    layer = F.AttentionLayer(config(kv_bits=4))
+    assert not layer_supported(layer) and layer_supported(F.AttentionLayer(config()))
+    for bad in (dict(kv_bits=8), dict(kv_bits=4, n_embd=48)):
+        with pytest.raises(NotImplementedError):
+            F.Attention(config(**bad))
+    p = Packed([3, 0, 5], "cpu")
+    assert p.cu.tolist() == [0, 3, 3, 8] and p.cu.dtype == torch.int32
+    for bad in ([], [-1, 2]):
+        with pytest.raises(ValueError):
+            Packed(bad, "cpu")
+
+
+def test_tensor_parallelism_refuses_a_cache_in_4_bits(tmp_path):
+    import torch.distributed as dist
+    import flash_stu_2_b200 as F
+    from flash_stu_2_b200.tensor_parallel import TensorParallelFlashSTU
+    dist.init_process_group("gloo", init_method=f"file://{tmp_path}/rendezvous", rank=0, world_size=1)
+    try:
+        with pytest.raises(NotImplementedError, match="4 bits"):
+            TensorParallelFlashSTU(F.FlashSTUConfig(n_embd=64, n_heads=4, n_layers=2, seq_len=64, window_size=20, vocab_size=11, num_eigh=4, kv_bits=4), {}, "cpu")
+    finally:
+        dist.destroy_process_group()
