@@ -6,6 +6,8 @@
 //   score = cap tanh(q.k / sqrt(hd) / cap) - slope_h (i - j);  out = softmax(score) . V     (flash_stu/modules/attention.py:72-101)
 #include "attention_packed.cuh"
 
+int* device_status_word();   // gemm_tc.cu
+
 namespace {
 
 constexpr int QT = 32, KT = 32;
@@ -115,6 +117,7 @@ extern "C" int stu_swa_packed(const void* qkv, long long row_stride, const int* 
       row_stride < (long long)(H + 2 * Hk) * hd || out_stride < (long long)H * hd)
     return STU_ERR_SHAPE;
   if (hd > 128) return STU_ERR_UNSUPPORTED;
+  if (!status) status = device_status_word();
   cudaStream_t st = (cudaStream_t)stream;
   if (dtype == STU_BF16 && hd % 8 == 0 && aligned16(qkv) && row_stride % 8 == 0 && aligned16(out) && out_stride % 8 == 0)
     return launch_packed_umma(qkv, row_stride, cu_seqlens, S, slopes, out, out_stride, (int)rows, H, Hk, hd, window, softcap, status, st);

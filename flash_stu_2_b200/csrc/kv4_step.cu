@@ -22,6 +22,7 @@
 namespace cg = cooperative_groups;
 
 int device_sm_count();   // gemm_tc.cu
+int* device_status_word();
 
 namespace {
 
@@ -509,6 +510,7 @@ extern "C" int stu_kv4_step(const void* qkv, long long row_stride, void* k4, voi
   if (rc != STU_OK) return rc;
   if (window < 0 || window >= slots || B > 65535 || row_stride < (long long)(H + 2 * Hk) * hd) return STU_ERR_SHAPE;
   if (!aligned16(k4) || !aligned16(v4)) return STU_ERR_ALIGN;
+  if (!status) status = device_status_word();
   const int R = H / Hk < 8 ? H / Hk : 8;
   auto go = [&](auto f) { return f(qkv, row_stride, k4, v4, pos, slopes, out, B, H, Hk, hd, slots, window, softcap, update_cache, status, (cudaStream_t)stream); };
   auto by_rows = [&](auto one, auto two, auto four, auto eight) { return R == 1 ? go(one) : R == 2 ? go(two) : R <= 4 ? go(four) : go(eight); };

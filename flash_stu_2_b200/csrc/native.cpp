@@ -12,7 +12,9 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <atomic>
+#include <cmath>
 #include <stdexcept>
 #include <tuple>
 #include <utility>
@@ -328,6 +330,167 @@ PyObject* rmsnorm_fp8(PyObject*, PyObject* const* args, Py_ssize_t n) {
   }
   Py_RETURN_NONE;
 }
+// Attention over packed prompts and rings of 4 bits (see ops.py): what is as usual is checked and launched here; None: ops.py's own checks follow.
+struct Heads {
+  const at::Tensor* qkv;
+  long long H, kv, hd, rows, stride;
+};
+// qkv's rows of H query heads, kv keys and as many values
+bool heads_of(const at::Tensor* qkv, long long H, long long kv, int dev, Heads* out) {
+  if (!qkv || dtype_code(*qkv) < 0 || qkv->device().index() != dev || qkv->dim() < 2 || H < 1 || kv < 1 || H % kv || H > 65535) return false;
+  const long long cols = qkv->size(-1);
+  if (cols == 0 || cols % (H + 2 * kv)) return false;
+  long long rows, stride;
+  if (!as_rows(*qkv, &rows, &stride)) return false;
+  *out = {qkv, H, kv, cols / (H + 2 * kv), rows, std::max(stride, cols)};
+  return rows > 0 && rows <= INT32_MAX && out->hd <= 128;
+}
+bool is_int32(const at::Tensor* t, int dev) { return t && t->scalar_type() == at::kInt && t->device().index() == dev && t->is_contiguous(); }
+bool are_slopes(const at::Tensor* t, long long H, int dev) {
+  return !t || (t->scalar_type() == at::kFloat && t->device().index() == dev && t->dim() == 1 && t->size(0) == H && t->is_contiguous());
+}
+// Rings of heads of hd dimensions: their slots, or 0
+long long ring_slots(const at::Tensor* k4, const at::Tensor* v4, long long hd, int dev) {
+  if (!k4 || !v4 || hd < 8 || hd % 8 || hd > 128) return 0;
+  for (const at::Tensor* t : {k4, v4})
+    if (t->scalar_type() != at::kByte || t->device().index() != dev || t->dim() != 3 || !t->is_contiguous()) return 0;
+  const long long row = hd <= 32 ? 20 : hd <= 64 ? 36 : 72;
+  return k4->sizes() == v4->sizes() && k4->size(0) > 0 && k4->size(2) % (16 * row) == 0 && k4->size(2) / row <= 1 << 24 ? k4->size(2) / row : 0;
+}
+bool ready(int dev) { return g_ready.load(std::memory_order_relaxed) >> dev & 1; }
+bool is_cap(float softcap) { return softcap >= 0.f && softcap < INFINITY; }
+
+// swa_packed(qkv, cu_seqlens, slopes, H, window (-1: none), softcap, kv_heads) -> y
+PyObject* swa_packed(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 7) {
+    PyErr_SetString(PyExc_TypeError, "7 arguments expected");
+    return nullptr;
+  }
+  try {
+    const at::Tensor *qkv, *cu, *slopes;
+    const int dev = c10::cuda::current_device();
+    Heads h;
+    if (!plain(args[0], &qkv) || !plain(args[1], &cu) || !plain(args[2], &slopes) || !ready(dev)) Py_RETURN_NONE;
+    const int window = value_of<int>(args[4]);
+    const float softcap = value_of<float>(args[5]);
+    if (!heads_of(qkv, value_of<long long>(args[3]), value_of<long long>(args[6]), dev, &h) || qkv->dim() != 2 || !is_int32(cu, dev) || cu->dim() != 1 ||
+        cu->size(0) < 2 || !are_slopes(slopes, h.H, dev) || window < -1 || !is_cap(softcap))
+      Py_RETURN_NONE;
+    at::Tensor y = at::empty({h.rows, h.H * h.hd}, qkv->options());
+    void *p[] = {data_of(qkv), data_of(cu), data_of(slopes), y.data_ptr(), (void*)c10::cuda::getCurrentCUDAStream().stream()};
+    const int S = (int)cu->size(0) - 1, code = dtype_code(*qkv);
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = stu_swa_packed(p[0], h.stride, (const int*)p[1], S, (const float*)p[2], p[3], h.H * h.hd, h.rows, (int)h.H, (int)h.kv, (int)h.hd, window, softcap,
+                        nullptr, code, p[4]);
+    Py_END_ALLOW_THREADS
+    if (raised(rc, "stu_swa_packed")) return nullptr;
+    if (rc == 0) return THPVariable_Wrap(std::move(y));
+  } catch (const BadArgument&) {
+    PyErr_Clear();
+  } catch (const std::exception&) {
+  }
+  Py_RETURN_NONE;
+}
+// kv4_step(qkv, k4, v4, pos, slopes, H, window, softcap, update_cache) -> y
+PyObject* kv4_step(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 9) {
+    PyErr_SetString(PyExc_TypeError, "9 arguments expected");
+    return nullptr;
+  }
+  try {
+    const at::Tensor *qkv, *k4, *v4, *pos, *slopes;
+    const int dev = c10::cuda::current_device();
+    Heads h;
+    if (!plain(args[0], &qkv) || !plain(args[1], &k4) || !plain(args[2], &v4) || !plain(args[3], &pos) || !plain(args[4], &slopes) || !ready(dev) || !k4 ||
+        k4->dim() != 3)
+      Py_RETURN_NONE;
+    const int window = value_of<int>(args[6]), update = value_of<int>(args[8]);
+    const float softcap = value_of<float>(args[7]);
+    const long long B = k4->size(0);
+    if (!heads_of(qkv, value_of<long long>(args[5]), k4->size(1), dev, &h) || qkv->dim() != 3 || qkv->size(0) != B || qkv->size(1) != 1) Py_RETURN_NONE;
+    const long long slots = ring_slots(k4, v4, h.hd, dev);
+    if (!slots || window < 0 || window >= slots || !is_int32(pos, dev) || pos->dim() != 2 || pos->size(0) != B || pos->size(1) != 2 ||
+        !are_slopes(slopes, h.H, dev) || !is_cap(softcap))
+      Py_RETURN_NONE;
+    at::Tensor y = at::empty({B, 1, h.H * h.hd}, qkv->options());
+    void *p[] = {data_of(qkv), data_of(k4), data_of(v4), data_of(pos), data_of(slopes), y.data_ptr(), (void*)c10::cuda::getCurrentCUDAStream().stream()};
+    const int code = dtype_code(*qkv);
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = stu_kv4_step(p[0], h.stride, p[1], p[2], (int*)p[3], (const float*)p[4], p[5], (int)B, (int)h.H, (int)h.kv, (int)h.hd, (int)slots, window, softcap,
+                      update, nullptr, code, p[6]);
+    Py_END_ALLOW_THREADS
+    if (raised(rc, "stu_kv4_step")) return nullptr;
+    if (rc == 0) return THPVariable_Wrap(std::move(y));
+  } catch (const BadArgument&) {
+    PyErr_Clear();
+  } catch (const std::exception&) {
+  }
+  Py_RETURN_NONE;
+}
+// kv4_write(qkv, k4, v4, pos, H, cu_seqlens) -> True
+PyObject* kv4_write(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 6) {
+    PyErr_SetString(PyExc_TypeError, "6 arguments expected");
+    return nullptr;
+  }
+  try {
+    const at::Tensor *qkv, *k4, *v4, *pos, *cu;
+    const int dev = c10::cuda::current_device();
+    Heads h;
+    if (!plain(args[0], &qkv) || !plain(args[1], &k4) || !plain(args[2], &v4) || !plain(args[3], &pos) || !plain(args[5], &cu) || !k4 || k4->dim() != 3)
+      Py_RETURN_NONE;
+    const long long B = k4->size(0);
+    if (!heads_of(qkv, value_of<long long>(args[4]), k4->size(1), dev, &h) || qkv->dim() != (cu ? 2 : 3) || (!cu && qkv->size(0) != B)) Py_RETURN_NONE;
+    const long long slots = ring_slots(k4, v4, h.hd, dev);
+    if (!slots || !is_int32(pos, dev) || pos->dim() != 2 || pos->size(0) != B || pos->size(1) != 2 ||
+        (cu && (!is_int32(cu, dev) || cu->dim() != 1 || cu->size(0) != B + 1)))
+      Py_RETURN_NONE;
+    void *p[] = {data_of(qkv), data_of(k4), data_of(v4), data_of(pos), data_of(cu), (void*)c10::cuda::getCurrentCUDAStream().stream()};
+    const int code = dtype_code(*qkv);
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = stu_kv4_write(p[0], h.stride, p[1], p[2], (int*)p[3], (const int*)p[4], (int)B, h.rows, (int)h.H, (int)h.kv, (int)h.hd, (int)slots, code, p[5]);
+    Py_END_ALLOW_THREADS
+    if (raised(rc, "stu_kv4_write")) return nullptr;
+    if (rc == 0) Py_RETURN_TRUE;
+  } catch (const BadArgument&) {
+    PyErr_Clear();
+  } catch (const std::exception&) {
+  }
+  Py_RETURN_NONE;
+}
+// kv4_read(k4, v4, hd, bf16) -> (k, v)
+PyObject* kv4_read(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 4) {
+    PyErr_SetString(PyExc_TypeError, "4 arguments expected");
+    return nullptr;
+  }
+  try {
+    const at::Tensor *k4, *v4;
+    const int dev = c10::cuda::current_device();
+    if (!plain(args[0], &k4) || !plain(args[1], &v4)) Py_RETURN_NONE;
+    const long long hd = value_of<long long>(args[2]), slots = ring_slots(k4, v4, hd, dev);
+    const int code = value_of<int>(args[3]);
+    if (!slots || (code != 0 && code != 1)) Py_RETURN_NONE;
+    const auto options = k4->options().dtype(code ? at::kBFloat16 : at::kFloat);
+    const long long B = k4->size(0), kv = k4->size(1);
+    std::pair<at::Tensor, at::Tensor> out{at::empty({B, slots, kv * hd}, options), at::empty({B, slots, kv * hd}, options)};
+    void *p[] = {data_of(k4), data_of(v4), out.first.data_ptr(), out.second.data_ptr(), (void*)c10::cuda::getCurrentCUDAStream().stream()};
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = stu_kv4_read(p[0], p[1], p[2], p[3], (int)B, (int)kv, (int)hd, (int)slots, code, p[4]);
+    Py_END_ALLOW_THREADS
+    if (raised(rc, "stu_kv4_read")) return nullptr;
+    if (rc == 0) return pair_of(std::move(out));
+  } catch (const BadArgument&) {
+    PyErr_Clear();
+  } catch (const std::exception&) {
+  }
+  Py_RETURN_NONE;
+}
+
 // linear_fp8(x data, x scales, W data, W scales, columns, W2 data, W2 scales, resid, out, flags) -> y, with W2 (data, scales); or None as above.
 PyObject* linear_fp8(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (n != 10) {
@@ -551,6 +714,10 @@ PyMethodDef methods[] = {
     {"quantize_fp8", (PyCFunction)(void (*)(void))quantize_fp8, METH_FASTCALL, nullptr},
     {"rmsnorm_fp8", (PyCFunction)(void (*)(void))rmsnorm_fp8, METH_FASTCALL, nullptr},
     {"linear_fp8", (PyCFunction)(void (*)(void))linear_fp8, METH_FASTCALL, nullptr},
+    {"swa_packed", (PyCFunction)(void (*)(void))swa_packed, METH_FASTCALL, nullptr},
+    {"kv4_step", (PyCFunction)(void (*)(void))kv4_step, METH_FASTCALL, nullptr},
+    {"kv4_write", (PyCFunction)(void (*)(void))kv4_write, METH_FASTCALL, nullptr},
+    {"kv4_read", (PyCFunction)(void (*)(void))kv4_read, METH_FASTCALL, nullptr},
     {"rmsnorm", (PyCFunction)(void (*)(void))rmsnorm, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

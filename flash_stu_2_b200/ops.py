@@ -1099,6 +1099,12 @@ def swa_packed(qkv: torch.Tensor, cu_seqlens: torch.Tensor, slopes: Optional[tor
     or None; kv_heads: H unless query heads share keys.  Returns [N, H hd]; rows that belong to no sequence are left as they are in `out`, which may not
     lie in qkv's memory."""
     softcap, kv_heads = float(softcap or 0.0), H if kv_heads is None else kv_heads
+    if out is None and (not _arenas or getattr(_local, "arena", None) is None) and (window is None or 0 <= window < 2 ** 31):
+        # checks, output and launch in one native call; None: whatever is out of the ordinary is looked at below
+        y = _lib.native().swa_packed(qkv, cu_seqlens, slopes, H, -1 if window is None else window, softcap, kv_heads)
+        if y is not None:
+            _count()
+            return y
     dt = _dt(qkv)
     hd = _heads_of(qkv, H, kv_heads, "swa_packed")
     if qkv.dim() != 2 or hd > 128:
@@ -1164,6 +1170,9 @@ def _kv4_check(k4: torch.Tensor, v4: torch.Tensor, hd: int, what: str) -> int:
 def kv4_write(qkv: torch.Tensor, k4: torch.Tensor, v4: torch.Tensor, pos: torch.Tensor, H: int, cu_seqlens: Optional[torch.Tensor] = None):
     """The keys and values of new tokens into rings of 4 bits (kv4_rings), which move on: qkv [batch, tokens, (H + 2 kv_heads) hd], or packed rows
     [N, ...] with cu_seqlens as in swa_packed.  Of more tokens than slots the last are kept."""
+    if _lib.native().kv4_write(qkv, k4, v4, pos, H, cu_seqlens):
+        _count()
+        return
     dt = _dt(qkv)
     if k4.dim() != 3:
         raise ValueError(f"kv4_write: {tuple(k4.shape)} is no ring")
@@ -1192,6 +1201,11 @@ def kv4_write(qkv: torch.Tensor, k4: torch.Tensor, v4: torch.Tensor, pos: torch.
 def kv4_read(k4: torch.Tensor, v4: torch.Tensor, hd: int, dtype: torch.dtype):
     """What rings of 4 bits stand for: (keys, values) [batch, slots, kv_heads hd], rings as swa_forward reads them.  Slots that nothing was written to
     are zeros."""
+    if not _arenas or getattr(_local, "arena", None) is None:
+        made = _lib.native().kv4_read(k4, v4, hd, 1 if dtype == torch.bfloat16 else 0 if dtype == torch.float32 else -1)
+        if made is not None:
+            _count()
+            return made
     slots = _kv4_check(k4, v4, hd, "kv4_read")
     if dtype not in (torch.float32, torch.bfloat16):
         raise TypeError(f"kv4_read: values are float32 or bfloat16, not {dtype}")
@@ -1214,7 +1228,13 @@ def kv4_step(qkv: torch.Tensor, k4: torch.Tensor, v4: torch.Tensor, pos: torch.T
              softcap: float = 0.0, update_cache: bool = True):
     """swa_forward of one new token per sequence, qkv [batch, 1, (H + 2 kv_heads) hd], over rings of 4 bits: its own key and value as they are,
     those of the `window` positions before it as the rings hold them.  update_cache: they are stored, and pos moves on.  Returns [batch, 1, H hd]."""
-    softcap, dt = float(softcap or 0.0), _dt(qkv)
+    softcap = float(softcap or 0.0)
+    if not _arenas or getattr(_local, "arena", None) is None:
+        y = _lib.native().kv4_step(qkv, k4, v4, pos, slopes, H, window, softcap, int(update_cache))
+        if y is not None:
+            _count()
+            return y
+    dt = _dt(qkv)
     if k4.dim() != 3:
         raise ValueError(f"kv4_step: {tuple(k4.shape)} is no ring")
     B, kv_heads = k4.shape[:2]

@@ -391,7 +391,7 @@ int stu_swa_prefill_tc5(const void* qkv, void* vt_scratch, void* k_ring, void* v
  * head h reads key head h / (H / Hk)), sequence s in rows cu_seqlens[s] .. cu_seqlens[s + 1] - 1 (int32 [S + 1] on the device, ascending, in
  * 0 .. rows; empty sequences are none).  Causal; window < 0: every earlier position of the sequence is seen, else the last `window`; slopes (fp32
  * [H]) may be NULL; softcap 0: none.  out rows of H * hd values; rows that belong to no sequence are left as they are.  For sequences of one length what
- * stu_swa_forward computes without a cache. */
+ * stu_swa_forward computes without a cache.  status NULL: the registered word (stu_set_status_word). */
 int stu_swa_packed(const void* qkv, long long row_stride, const int* cu_seqlens, int S, const float* slopes, void* out,
                    long long out_stride, long long rows, int H, int Hk, int hd, int window, float softcap, int* status, int dtype,
                    void* stream);
