@@ -27,40 +27,43 @@ __device__ __forceinline__ uint32_t bf16_up(float x) {
   return u != cut && (int)u >= 0 ? cut + 0x10000u : cut;
 }
 
+__device__ __forceinline__ float min_nan(float a, float b) {   // NaN where one is
+  float d;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+
 // Eight lanes hold a piece, x[0 .. 7] each (`there`: whether the head has these dimensions): the word of this lane's and the piece's scale.
-// Called by whole warps.  Every operation is one rounding to fp32 (no contraction is possible: a product is never added to).
+// Called by whole warps.  Every operation is one rounding to fp32, none contracted with another.  Adding 1.5 2^23 rounds to the nearest whole number,
+// ties to even, and leaves it in the lowest bits; none is below 0 or above 15, since lowest is rounded down and the step up.
 __device__ __forceinline__ void quantize(const float* x, bool there, uint32_t& word, uint32_t& scale) {
-  float lo = INFINITY, hi = -INFINITY;
-  bool bad = false;
-  if (there) {
+  float lo = there ? x[0] : INFINITY, hi = there ? x[0] : -INFINITY;
 #pragma unroll
-    for (int e = 0; e < 8; e++) {
-      lo = fminf(lo, x[e]);
-      hi = fmaxf(hi, x[e]);
-      bad |= !(fabsf(x[e]) < INFINITY);
-    }
+  for (int e = 1; e < 8; e++) {
+    lo = there ? min_nan(lo, x[e]) : lo;
+    hi = there ? max_nan(hi, x[e]) : hi;
   }
 #pragma unroll
   for (int o = 1; o < 8; o <<= 1) {
-    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+    lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+    hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
   }
-  const uint32_t lane = threadIdx.x & 31;
-  bad = (__ballot_sync(0xffffffffu, bad) >> (lane & 24) & 0xffu) != 0;
   const float low = __uint_as_float(bf16_down(lo + 0.f));   // (+ 0: zeros without a sign)
   const float spread = (hi - low) + 0.f;
   float step = __uint_as_float(bf16_up(spread * (1.f / 15.f)));
   if (step > 0.f) step = fmaxf(step, 1.17549435e-38f);      // 2^-126: its reciprocal is finite
-  bad |= !(fabsf(low) < INFINITY) || !(step < INFINITY);
+  const bool bad = !(fabsf(low) < INFINITY) || !(spread < INFINITY) || !(step < INFINITY);
   const float inv = step > 0.f ? 1.f / step : 0.f;
   word = 0;
-  if (there && !bad) {
 #pragma unroll
-    for (int e = 0; e < 8; e++) {
-      const int n = min(max(__float2int_rn((x[e] - low) * inv), 0), 15);
-      word |= (uint32_t)n << 4 * e;
-    }
-  }
+  for (int e = 7; e >= 0; e--) word = (word << 4) + __float_as_uint(__fadd_rn(__fmul_rn(x[e] - low, inv), 12582912.f));   // 0x4b400000 + n
+  word -= 0x3f400000u;   // the sum of 0x4b400000 << 4 e
+  if (!there || bad) word = 0;
   scale = bad ? 0x7fc0u : __float_as_uint(low) >> 16 | (__float_as_uint(step) & 0xffff0000u);
 }
 
