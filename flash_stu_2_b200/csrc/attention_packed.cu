@@ -12,11 +12,10 @@ namespace {
 
 constexpr int QT = 32, KT = 32;
 
-// Any head dimension, fp32 or bf16, in fp32 on the CUDA cores: a CTA per 32 queries of one head, eight warps of four queries; keys and values of 32
+// bf16 whose rows the tensor copies cannot take (off the 16-byte grid, heads of no multiple of 8), in fp32 on the CUDA cores: a CTA per 32 queries of one head, eight warps of four queries; keys and values of 32
 // positions in shared memory as fp32 (keys transposed), lane = key for the scores, lane = dimension for the weighted values.
-template <typename T>
-__global__ void __launch_bounds__(256) packed_attend_kernel(const T* __restrict__ qkv, long long row_stride, const int* __restrict__ cu, int S,
-                                                            const float* __restrict__ slopes, T* __restrict__ out, long long out_stride, int rows, int H,
+__global__ void __launch_bounds__(256) packed_attend_kernel(const bf16* __restrict__ qkv, long long row_stride, const int* __restrict__ cu, int S,
+                                                            const float* __restrict__ slopes, bf16* __restrict__ out, long long out_stride, int rows, int H,
                                                             int Hk, int hd, int window, float scale, float softcap) {
   extern __shared__ __align__(16) float smem[];
   __shared__ int first[QT];
@@ -27,7 +26,7 @@ __global__ void __launch_bounds__(256) packed_attend_kernel(const T* __restrict_
   const int h = blockIdx.y, g = h / (H / Hk), q0 = blockIdx.x * QT, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   for (int e = threadIdx.x; e < QT * hdp; e += 256) {
     const int qi = e / hdp, c = e % hdp, i = q0 + qi;
-    Qs[c][qi] = i < rows && c < hd ? Elem<T>::to_f(qkv[i * row_stride + (long long)h * hd + c]) * scale : 0.f;
+    Qs[c][qi] = i < rows && c < hd ? Elem<bf16>::to_f(qkv[i * row_stride + (long long)h * hd + c]) * scale : 0.f;
   }
   if (threadIdx.x < QT) first[threadIdx.x] = packed::first_key(cu, S, q0 + threadIdx.x, rows, window);
   __syncthreads();
@@ -50,9 +49,9 @@ __global__ void __launch_bounds__(256) packed_attend_kernel(const T* __restrict_
     for (int e = threadIdx.x; e < KT * hdp; e += 256) {
       const int kj = e / hdp, c = e % hdp, j = jt + kj;
       const bool ok = j <= j_hi && c < hd;
-      const T* at = qkv + j * row_stride + (long long)(H + g) * hd + c;
-      Kt[c][kj] = ok ? Elem<T>::to_f(*at) : 0.f;
-      Vs[kj * hdp + c] = ok ? Elem<T>::to_f(at[(long long)Hk * hd]) : 0.f;
+      const bf16* at = qkv + j * row_stride + (long long)(H + g) * hd + c;
+      Kt[c][kj] = ok ? Elem<bf16>::to_f(*at) : 0.f;
+      Vs[kj * hdp + c] = ok ? Elem<bf16>::to_f(at[(long long)Hk * hd]) : 0.f;
     }
     __syncthreads();
     const int j = jt + lane;
@@ -102,7 +101,7 @@ __global__ void __launch_bounds__(256) packed_attend_kernel(const T* __restrict_
 #pragma unroll
     for (int e = 0; e < 4; e++) {
       const int c = lane + 32 * e;
-      if (e < dpl && c < hd) out[i * out_stride + (long long)h * hd + c] = Elem<T>::from_f(acc[u][e] * inv);
+      if (e < dpl && c < hd) out[i * out_stride + (long long)h * hd + c] = Elem<bf16>::from_f(acc[u][e] * inv);
     }
   }
 }
@@ -121,20 +120,16 @@ extern "C" int stu_swa_packed(const void* qkv, long long row_stride, const int* 
   cudaStream_t st = (cudaStream_t)stream;
   if (dtype == STU_BF16 && hd % 8 == 0 && aligned16(qkv) && row_stride % 8 == 0 && aligned16(out) && out_stride % 8 == 0)
     return launch_packed_umma(qkv, row_stride, cu_seqlens, S, slopes, out, out_stride, (int)rows, H, Hk, hd, window, softcap, status, st);
+  if (dtype == STU_F32) return launch_packed_f32(qkv, row_stride, cu_seqlens, S, slopes, out, out_stride, (int)rows, H, Hk, hd, window, softcap, st);
   const float scale = 1.0f / sqrtf((float)hd);
   const dim3 grid((unsigned)((rows + QT - 1) / QT), H);
   const int hdp = (hd + 31) & ~31;
   const size_t smem = (size_t)(hdp * QT + hdp * (KT + 1) + KT * hdp) * sizeof(float);
-  static SmemLimit limit, limit16;
-  cudaError_t e = dtype == STU_F32 ? allow_smem((const void*)packed_attend_kernel<float>, 64 * 1024, limit)
-                                   : allow_smem((const void*)packed_attend_kernel<bf16>, 64 * 1024, limit16);
+  static SmemLimit limit;
+  const cudaError_t e = allow_smem((const void*)packed_attend_kernel, 64 * 1024, limit);
   if (e != cudaSuccess) return (int)e;
-  if (dtype == STU_F32)
-    packed_attend_kernel<float><<<grid, 256, smem, st>>>((const float*)qkv, row_stride, cu_seqlens, S, slopes, (float*)out, out_stride, (int)rows, H, Hk,
-                                                         hd, window, scale, softcap);
-  else
-    packed_attend_kernel<bf16><<<grid, 256, smem, st>>>((const bf16*)qkv, row_stride, cu_seqlens, S, slopes, (bf16*)out, out_stride, (int)rows, H, Hk, hd,
-                                                        window, scale, softcap);
+  packed_attend_kernel<<<grid, 256, smem, st>>>((const bf16*)qkv, row_stride, cu_seqlens, S, slopes, (bf16*)out, out_stride, (int)rows, H, Hk, hd, window,
+                                                scale, softcap);
   STU_CHECK_LAUNCH();
   return STU_OK;
 }

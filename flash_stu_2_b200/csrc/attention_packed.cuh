@@ -25,3 +25,6 @@ __device__ __forceinline__ int first_key(const int* __restrict__ cu, int S, int 
 // bf16, hd a multiple of 8 up to 128, rows on the 16-byte grid (attention_packed_umma.cu)
 int launch_packed_umma(const void* qkv, long long row_stride, const int* cu, int S, const float* slopes, void* out, long long out_stride, int rows, int H,
                        int Hk, int hd, int window, float softcap, int* status, cudaStream_t st);
+// fp32, hd up to 128 (attention_packed_f32.cu)
+int launch_packed_f32(const void* qkv, long long row_stride, const int* cu, int S, const float* slopes, void* out, long long out_stride, int rows, int H,
+                      int Hk, int hd, int window, float softcap, cudaStream_t st);
