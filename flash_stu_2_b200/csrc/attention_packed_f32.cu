@@ -110,24 +110,34 @@ __global__ void __launch_bounds__(128) packed_f32_kernel(const float* __restrict
 #pragma unroll
     for (int e = 0; e < 4; e++) o[n][e] = 0.f;
 
+  constexpr int MINE = 2 * BN * (HD / 4) / 128;   // fours of a tile that this thread brings: the next tile's are under way while this one is multiplied
+  float coming[MINE][4];
+  auto fetch = [&](int jt) {
+#pragma unroll
+    for (int i = 0; i < MINE; i++) {
+      const int e = threadIdx.x + 128 * i, which = e / (BN * (HD / 4)), r = e / (HD / 4) % BN, d = e % (HD / 4) * 4;
+      four(jt + r, j_hi + 1, qkv + (long long)(H + which * Hk + g) * hd, d, coming[i]);
+    }
+  };
+  if (j_lo <= j_hi) fetch(j_lo);
   for (int jt = j_lo, turn = 0; jt <= j_hi; jt += BN, turn ^= 1) {
     __syncthreads();   // the tile before has been read
-    for (int e = threadIdx.x; e < 2 * BN * (HD / 4); e += 128) {
-      const int which = e / (BN * (HD / 4)), r = e / (HD / 4) % BN, d = e % (HD / 4) * 4;
-      float x[4];
-      four(jt + r, j_hi + 1, qkv + (long long)(H + which * Hk + g) * hd, d, x);
+#pragma unroll
+    for (int i = 0; i < MINE; i++) {
+      const int e = threadIdx.x + 128 * i, which = e / (BN * (HD / 4)), r = e / (HD / 4) % BN, d = e % (HD / 4) * 4;
       if (which) {
 #pragma unroll
-        for (int i = 0; i < 4; i++)
-          if (!(fabsf(x[i]) < INFINITY)) {
-            x[i] = 0.f;
+        for (int u = 0; u < 4; u++)
+          if (!(fabsf(coming[i][u]) < INFINITY)) {
+            coming[i][u] = 0.f;
             s_odd[turn] = 1;
           }
       }
-      put((which ? Vs : Ks) + r * P + d, L::KV_PART, x);
+      put((which ? Vs : Ks) + r * P + d, L::KV_PART, coming[i]);
     }
     __syncthreads();
     if (threadIdx.x == 0) s_odd[turn ^ 1] = 0;   // (written again behind the next barrier)
+    if (jt + BN <= j_hi) fetch(jt + BN);
     if (jt > w_hi || jt + BN <= w_lo) continue;   // (nothing here for this warp's rows)
     float s[BN / 8][4];
 #pragma unroll
@@ -140,17 +150,19 @@ __global__ void __launch_bounds__(128) packed_f32_kernel(const float* __restrict
 #pragma unroll
       for (int i = 0; i < 3; i++)
         ldmatrix_x4(q[i], Qs + i * L::Q_PART + (warp * 16 + (lane & 15)) * P + ks * 16 + (lane >> 4) * 8);
+      uint32_t k[BN / 16][3][4];   // 16 keys: two tiles of 8
 #pragma unroll
-      for (int np = 0; np < BN / 16; np++) {   // 16 keys: two tiles of 8
-        uint32_t k[3][4];
+      for (int np = 0; np < BN / 16; np++)
 #pragma unroll
         for (int i = 0; i < 3; i++)
-          ldmatrix_x4(k[i], Ks + i * L::KV_PART + (np * 16 + (lane & 7) + 8 * (lane >> 4)) * P + ks * 16 + ((lane >> 3) & 1) * 8);
+          ldmatrix_x4(k[np][i], Ks + i * L::KV_PART + (np * 16 + (lane & 7) + 8 * (lane >> 4)) * P + ks * 16 + ((lane >> 3) & 1) * 8);
 #pragma unroll
-        for (int t = 0; t < 6; t++) {          // the small products first
-          constexpr int A[6] = {2, 0, 1, 1, 0, 0}, B[6] = {0, 2, 1, 0, 1, 0};
-          mma(s[2 * np], q[A[t]], k[B[t]][0], k[B[t]][1]);
-          mma(s[2 * np + 1], q[A[t]], k[B[t]][2], k[B[t]][3]);
+      for (int t = 0; t < 6; t++) {   // the small products first; a product's sum is there 20 clocks later: four of them take turns
+        constexpr int A[6] = {2, 0, 1, 1, 0, 0}, B[6] = {0, 2, 1, 0, 1, 0};
+#pragma unroll
+        for (int np = 0; np < BN / 16; np++) {
+          mma(s[2 * np], q[A[t]], k[np][B[t]][0], k[np][B[t]][1]);
+          mma(s[2 * np + 1], q[A[t]], k[np][B[t]][2], k[np][B[t]][3]);
         }
       }
     }
@@ -194,16 +206,21 @@ __global__ void __launch_bounds__(128) packed_f32_kernel(const float* __restrict
         for (int i = 0; i < 3; i++) w[i][e] = p[i];
       }
 #pragma unroll
-      for (int np = 0; np < HD / 16; np++) {
-        uint32_t v[3][4];
+      for (int np = 0; np < HD / 16; np += 2) {
+        uint32_t v[2][3][4];
 #pragma unroll
-        for (int i = 0; i < 3; i++)
-          ldmatrix_x4_trans(v[i], Vs + i * L::KV_PART + (kk * 16 + (lane & 7) + 8 * ((lane >> 3) & 1)) * P + np * 16 + (lane >> 4) * 8);
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+          for (int i = 0; i < 3; i++)
+            ldmatrix_x4_trans(v[u][i], Vs + i * L::KV_PART + (kk * 16 + (lane & 7) + 8 * ((lane >> 3) & 1)) * P + (np + u) * 16 + (lane >> 4) * 8);
 #pragma unroll
         for (int t = 0; t < 6; t++) {
           constexpr int A[6] = {2, 0, 1, 1, 0, 0}, B[6] = {0, 2, 1, 0, 1, 0};
-          mma(o[2 * np], w[A[t]], v[B[t]][0], v[B[t]][1]);
-          mma(o[2 * np + 1], w[A[t]], v[B[t]][2], v[B[t]][3]);
+#pragma unroll
+          for (int u = 0; u < 2; u++) {
+            mma(o[2 * (np + u)], w[A[t]], v[u][B[t]][0], v[u][B[t]][1]);
+            mma(o[2 * (np + u) + 1], w[A[t]], v[u][B[t]][2], v[u][B[t]][3]);
+          }
         }
       }
     }
