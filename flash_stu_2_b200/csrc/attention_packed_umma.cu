@@ -185,7 +185,6 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
-__device__ __forceinline__ bool seen_bit(const uint32_t (&m)[4], int c) { return m[c >> 5] >> (c & 31) & 1u; }
 
 __device__ __forceinline__ void give_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_OTHERS)); }
 
@@ -293,6 +292,16 @@ __global__ void __launch_bounds__(THREADS, 1) packed_umma_kernel(const __grid_co
     below += __syncthreads_count(at <= row_lo);
     upto += __syncthreads_count(at <= row_hi);
   }
+  if (warp == 9 && elect_one()) {   // the queries, while their keys are looked for
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+      if (max(row_lo, q0 + i * BM) <= min(row_hi, q0 + i * BM + BM - 1)) {   // (a tile that has rows of a sequence, and whose products wait for it)
+        tma::mbar_expect_tx(&ctl.q_full[i], L::TILE);
+#pragma unroll
+        for (int kb = 0; kb < L::KB; kb++) tma::load_3d(smem + i * L::TILE + kb * 16384, &map, &ctl.q_full[i], kb * 64, h, q0 + i * BM);
+      }
+  }
+  __syncwarp();
   const int seq_lo = max(below - 1, 0), seq_hi = max(upto, seq_lo + 1);
   if (threadIdx.x < 2 * BM) {
     const int i = q0 + threadIdx.x;
@@ -335,8 +344,6 @@ __global__ void __launch_bounds__(THREADS, 1) packed_umma_kernel(const __grid_co
       n++;
     };
     for (int t = t_lo; ok && t < t_hi; t++) {
-      for (int i = 0; i < 2; i++)
-        if (t == begin[i] && end[i] > begin[i]) load(smem + i * L::TILE, &ctl.q_full[i], h, q0 + i * BM);
       load_kv(H + g, t);
       load_kv(H + Hk + g, t);
     }
@@ -429,23 +436,21 @@ __global__ void __launch_bounds__(THREADS, 1) packed_umma_kernel(const __grid_co
       tmem_wait_ld(sr);
       const bool interior = whole && jt >= last_first && jt + BN - 1 <= q0 + tile * BM;   // all rows of the tile see all keys of this one
       uint32_t seen[4];
+      uint32_t dead = 0, partly = 0;   // blocks of 32 keys that no row of the warp sees, and that some do not see all of
       if (!interior) {
         const int lo = max(first - jt, 0), hi = first == packed::NOBODY ? -1 : min(i - jt, BN - 1);
 #pragma unroll
         for (int w = 0; w < 4; w++) {
           const int a = max(lo - 32 * w, 0), b = min(hi - 32 * w, 31);
           seen[w] = a > b ? 0u : (0xffffffffu >> (31 - (b - a))) << a;
+          dead |= __any_sync(0xffffffffu, seen[w] != 0u) ? 0u : 1u << w;
+          partly |= __all_sync(0xffffffffu, seen[w] == 0xffffffffu) ? 0u : 1u << w;
         }
       }
       // scores in the exp2 domain, counted from ref: s k1 (or its cap) + c2 (j - i) - ref
       const float base_t = ALIBI ? fmaf(c2, (float)(jt - i), -ref) : -ref;
       const f32x2 bt = pair_of(base_t, base_t);
       if (CAP) {
-        if (!interior) {   // a masked score decides nothing
-#pragma unroll
-          for (int c = 0; c < 128; c++)
-            if (!seen_bit(seen, c)) sr[c] = 0;
-        }
         float most[4] = {0.f, 0.f, 0.f, 0.f};   // (a NaN score is not in it: every form carries it on)
 #pragma unroll
         for (int c = 0; c < 128; c += 2) most[c >> 1 & 3] = max3(most[c >> 1 & 3], fabsf(__uint_as_float(sr[c])), fabsf(__uint_as_float(sr[c + 1])));
@@ -472,11 +477,13 @@ __global__ void __launch_bounds__(THREADS, 1) packed_umma_kernel(const __grid_co
         for (int c = 0; c < 128; c += 2)
           split(fma2(pair_of(sr[c], sr[c + 1]), kp, ALIBI ? fma2(cc, pair_of((float)c, (float)(c + 1)), bt) : bt), sr[c], sr[c + 1]);
       }
-      if (!interior) {
 #pragma unroll
-        for (int c = 0; c < 128; c++)
-          if (!seen_bit(seen, c)) sr[c] = 0xff800000u;   // -infinity
-      }
+      for (int w = 0; w < 4; w++)
+        if (partly >> w & 1u) {
+#pragma unroll
+          for (int c = 0; c < 32; c++)
+            if (!(seen[w] >> c & 1u)) sr[w * 32 + c] = 0xff800000u;   // -infinity
+        }
       float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
       for (int c = 0; c < 128; c += 2) mx[c >> 1 & 3] = max3(mx[c >> 1 & 3], __uint_as_float(sr[c]), __uint_as_float(sr[c + 1]));
@@ -509,18 +516,26 @@ __global__ void __launch_bounds__(THREADS, 1) packed_umma_kernel(const __grid_co
 #pragma unroll
       for (int half = 0; half < 2; half++) {
 #pragma unroll
-        for (int c0 = half * 64; c0 < half * 64 + 64; c0 += 16) {   // 8 pairs: the first POLY of them on the FMA pipe
-          f32x2 p[8];
-          exp2_poly<POLY>(sr + c0, p);
+        for (int w = 2 * half; w < 2 * half + 2; w++) {
+          if (dead >> w & 1u) {
 #pragma unroll
-          for (int u = POLY; u < 8; u++) p[u] = pair_of(exp2_hw(__uint_as_float(sr[c0 + 2 * u])), exp2_hw(__uint_as_float(sr[c0 + 2 * u + 1])));
+            for (int u = 0; u < 16; u++) sr[w * 16 + u] = 0;
+          } else {
 #pragma unroll
-          for (int u = 0; u < 8; u++) sum[u & 1] = add2(sum[u & 1], p[u]);
+            for (int c0 = w * 32; c0 < w * 32 + 32; c0 += 16) {   // 8 pairs: the first POLY of them on the FMA pipe
+              f32x2 p[8];
+              exp2_poly<POLY>(sr + c0, p);
 #pragma unroll
-          for (int u = 0; u < 8; u++) {
-            float p0, p1;
-            split(p[u], p0, p1);
-            sr[(c0 >> 1) + u] = pack_bf16(p0, p1);
+              for (int u = POLY; u < 8; u++) p[u] = pair_of(exp2_hw(__uint_as_float(sr[c0 + 2 * u])), exp2_hw(__uint_as_float(sr[c0 + 2 * u + 1])));
+#pragma unroll
+              for (int u = 0; u < 8; u++) sum[u & 1] = add2(sum[u & 1], p[u]);
+#pragma unroll
+              for (int u = 0; u < 8; u++) {
+                float p0, p1;
+                split(p[u], p0, p1);
+                sr[(c0 >> 1) + u] = pack_bf16(p0, p1);
+              }
+            }
           }
         }
         tmem_st32(tm_s + half * 32, sr + half * 32);
