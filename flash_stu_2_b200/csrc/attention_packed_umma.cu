@@ -257,7 +257,6 @@ __global__ void __launch_bounds__(THREADS, 1) packed_umma_kernel(const __grid_co
                                                              long long out_stride, int rows, int H, int Hk, int hd, int window, float scale,
                                                              float softcap, int* status) {
   typedef Smem<HD> L;
-  constexpr int POLY = CAP ? 2 : POLY_OF_8;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   __shared__ Ctl ctl;
@@ -491,7 +490,7 @@ __global__ void __launch_bounds__(THREADS, 1) packed_umma_kernel(const __grid_co
       const bool grow = top > (any_key ? LAG : -INFINITY);   // the row has outgrown ref, or has its first key: ref moves, and what has been summed up shrinks
       if (__any_sync(0xffffffffu, grow)) {
         // (ALiBi alone lifts what is to come by up to c2 (i - the last key here): ref is set as high, or heads with steep slopes would move it in every tile)
-        const float rise = ALIBI ? c2 * (float)max(i - jt - (BN - 1), 0) : 0.f;
+        const float rise = ALIBI ? fmaxf(c2, 0.f) * (float)max(i - jt - (BN - 1), 0) : 0.f;
         const float shift = grow ? top + rise : 0.f, corr = grow && any_key ? exp2_hw(-shift) : 1.f;
         const f32x2 neg = pair_of(-shift, -shift);
         ref += shift;
@@ -522,11 +521,11 @@ __global__ void __launch_bounds__(THREADS, 1) packed_umma_kernel(const __grid_co
             for (int u = 0; u < 16; u++) sr[w * 16 + u] = 0;
           } else {
 #pragma unroll
-            for (int c0 = w * 32; c0 < w * 32 + 32; c0 += 16) {   // 8 pairs: the first POLY of them on the FMA pipe
+            for (int c0 = w * 32; c0 < w * 32 + 32; c0 += 16) {   // 8 pairs: the first of them on the FMA pipe
               f32x2 p[8];
-              exp2_poly<POLY>(sr + c0, p);
+              exp2_poly<POLY_OF_8>(sr + c0, p);
 #pragma unroll
-              for (int u = POLY; u < 8; u++) p[u] = pair_of(exp2_hw(__uint_as_float(sr[c0 + 2 * u])), exp2_hw(__uint_as_float(sr[c0 + 2 * u + 1])));
+              for (int u = POLY_OF_8; u < 8; u++) p[u] = pair_of(exp2_hw(__uint_as_float(sr[c0 + 2 * u])), exp2_hw(__uint_as_float(sr[c0 + 2 * u + 1])));
 #pragma unroll
               for (int u = 0; u < 8; u++) sum[u & 1] = add2(sum[u & 1], p[u]);
 #pragma unroll

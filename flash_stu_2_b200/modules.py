@@ -642,6 +642,7 @@ class Attention(nn.Module):
     (flash_stu/modules/attention.py:16-105).  Cache entry = (k_ring [B,W,d], v_ring [B,W,d], pos [B,2])
     with W = window+1 slots, exact because older keys can never be attended; with config.kv_bits = 4 the rings are
     in 4 bits (ops.kv4_rings), and keys and values of earlier calls are what these hold."""
+    kv_bits = None
 
     def __init__(self, config):
         super().__init__()

@@ -19,7 +19,7 @@ def layer_supported(layer) -> bool:
         return False
     if hasattr(layer, "stu"):
         return layer.stu.use_approx and not layer.stu.use_hankel_L and not layer.stu_mlp_enabled
-    return hasattr(layer, "attn") and layer.attn.kv_bits is None
+    return hasattr(layer, "attn") and getattr(layer.attn, "kv_bits", None) is None
 
 
 def layer_weights(layer, d: int, inter: int):

@@ -442,3 +442,72 @@ def test_streams_and_graphs(dt):
 
     got = run(packed, replayed)
     assert all(torch.equal(a, b) for a, b in zip(want[0], got[0])) and all(torch.equal(a, b) for a, b in zip(want[1:], got[1:]))
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("slopes", [(-0.25, -0.01, 0.0, 3.0), (40.0, -3.0, 0.5, 1e-6)])
+def test_packed_takes_any_slopes(dt, slopes):
+    """Slopes that lift far keys, and such as leave a row its own key alone."""
+    from flash_stu_2_b200 import ops
+    g, lengths = gen(21), (400, 130)
+    qkv, sl = activations(g, 530, 4, 4, 64, dt), torch.tensor(slopes, device=dev())
+    for window in (None, 300):
+        want, tol = R.packed(qkv, lengths, 0, sl, 4, 4, window, 0.0, dt)
+        R.check(ops.swa_packed(qkv, cu_of(lengths), sl, 4, window), want, tol)
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("alibi", [False, True])
+def test_packed_of_extreme_scores(dt, alibi):
+    """Scores of thousands apart, larger ones behind smaller ones and before them: weights of 0 and 1, rows whose first keys are far above all that follow."""
+    from flash_stu_2_b200 import ops
+    g, H, hd, lengths = gen(22), 2, 64, (700, 65)
+    for factor in (0.0, 30.0, 1000.0):
+        qkv = activations(g, 765, H, H, hd, dt)
+        qkv[:, :H * hd] *= factor
+        for rising in (True, False):
+            x = qkv.clone()
+            ramp = torch.linspace(0.1, 1, 765, device=dev())
+            x[:, H * hd:2 * H * hd] *= (ramp if rising else ramp.flip(0))[:, None].to(dt)
+            slopes = slopes_of(H) if alibi else None
+            want, tol = R.packed(x, lengths, 0, slopes, H, H, None, 0.0, dt)
+            R.check(ops.swa_packed(x, cu_of(lengths), slopes, H), want, tol)
+
+
+@pytest.mark.parametrize("cap", [1.0, 8.0, 40.0])
+def test_packed_caps_of_every_size(cap):
+    """Scores below a fifth of the cap, below half of it and above, in one tile and apart: each row by the form that its scores call for."""
+    from flash_stu_2_b200 import ops
+    g, H, hd, lengths = gen(23), 2, 128, (300, 200)
+    qkv = activations(g, 500, H, H, hd, torch.bfloat16)
+    qkv[100:, :H * hd] *= 0.02
+    qkv[200:260, :H * hd] *= 10
+    want, tol = R.packed(qkv, lengths, 0, slopes_of(H), H, H, 150, cap, torch.bfloat16)
+    R.check(ops.swa_packed(qkv, cu_of(lengths), slopes_of(H), H, 150, cap), want, tol)
+
+
+def test_offsets_past_32_bits():
+    """Rows of qkv and rings behind more than 2^32 bytes."""
+    from flash_stu_2_b200 import ops
+    g, H, kv, hd, dt = gen(31), 12, 12, 128, torch.bfloat16
+    N, tail = 720000, 300
+    qkv = torch.zeros(N, (H + 2 * kv) * hd, device=dev(), dtype=dt)                  # 6.6 GB
+    qkv[N - tail:] = activations(g, tail, H, kv, hd, dt)
+    out = ops.swa_packed(qkv, cu_of([N - tail, tail]), slopes_of(H), H, 40, 50.0)
+    alone = ops.swa_packed(qkv[N - tail:].clone(), cu_of([tail]), slopes_of(H), H, 40, 50.0)
+    assert float((out[N - tail:].double() - alone.double()).norm() / alone.double().norm()) < 2.0 ** -7 and not bool(out[:N - tail].any())
+    B, slots = 64, 80016
+    k4, v4 = ops.kv4_rings(B, slots, kv, hd, dev())                                   # 4.4 GB each
+    one = ops.kv4_rings(1, slots, kv, hd, dev())
+    pos, pos1 = positions(*([slots - 3] * B)), positions(slots - 3)
+    rows = activations(g, 8, H, kv, hd, dt)
+    ops.kv4_write(rows.expand(B, 8, -1), k4, v4, pos, H)
+    ops.kv4_write(rows[None], *one, pos1, H)
+    new = activations(g, 1, H, kv, hd, dt)[None]
+    got, want = ops.kv4_step(new.expand(B, 1, -1), k4, v4, pos, slopes_of(H), H, 100, 50.0), ops.kv4_step(new, *one, pos1, slopes_of(H), H, 100, 50.0)
+    assert float((got[-1].double() - want[0].double()).norm() / want.double().norm()) < 2.0 ** -7
+    assert torch.equal(k4[-1], one[0][0]) and torch.equal(v4[-1], one[1][0]) and torch.equal(k4[0], k4[-1])
+    del qkv, out
+    k, v = ops.kv4_read(k4[-2:], v4[-2:], hd, dt)
+    k1, v1 = ops.kv4_read(*one, hd, dt)
+    assert torch.equal(k[1:], k1) and torch.equal(v[1:], v1)

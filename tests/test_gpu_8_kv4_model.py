@@ -70,7 +70,7 @@ def test_attention_layer_holds_what_it_says(dt, calls, heads, d):
 
 
 @pytest.mark.parametrize("dt", DTYPES)
-@pytest.mark.parametrize("B", [1, 3])
+@pytest.mark.parametrize("B", [1, 3, 20])
 def test_generate(dt, B):
     """Replayed steps are the layers' own; the rings' rounding changes logits by little."""
     m, plain = model(dt), model(dt, kv_bits=None)
