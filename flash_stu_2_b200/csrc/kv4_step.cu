@@ -4,8 +4,8 @@
 //   scores   mma.sync, the numbers of 16 keys as rows, 8 queries as columns: a number n becomes bf16 by putting its bits under those of 128 (128 + n is exact), so
 //            that two of them cost a shift and a logical operation.  A piece's scale is the same for all of a row's products:
 //              q.k = sum over pieces of  step (q.(128 + n)) + (lowest - 128 step) sum(q)
-//   softmax  a lane per key, the scores handed over through shared memory: cap, ALiBi, window, exponentials in the exp2 domain against a maximum that moves only when
-//            a score outgrows it by 2^8
+//   softmax  a lane per key, the scores handed over through shared memory, a key's queries side by side (one access of 16 bytes for four scores or eight weights): cap, ALiBi,
+//            window, exponentials in the exp2 domain against a maximum that moves only when a score outgrows it by 2^8, one vote of the warp for all rows
 //   values   mma.sync, weights times the values' steps as rows; a number enters as n - 8 (the tensor core's sums are cut off, not rounded: with 128 + n the error of
 //            16384 of them was four times the output's rounding); what lowest and the 8s add is summed up beside, one number per piece.  The weights' rows are 8 of 16: a
 //            weight is two bf16, its leading bits and what these left, in rows r and r + 8 (error 2^-16)
@@ -31,8 +31,6 @@ constexpr int BLOCK = WARPS * TILE, STAGES = 3;
 constexpr float NOTHING = -3.0e38f;      // the maximum of no scores
 constexpr float LAG = 8.f;               // exp2 domain
 constexpr int STATUS_KV4 = 14;
-constexpr int PITCH = TILE * 2 + 16;     // bytes between rows of weights: eight rows' 16 bytes lie in different banks
-constexpr int S_PITCH = TILE + 4;        // numbers between rows of scores: those of 8 keys and 4 queries lie in different banks
 
 template <typename T, int W> struct Geometry {
   static constexpr bool F32 = sizeof(T) == 4;
@@ -40,10 +38,10 @@ template <typename T, int W> struct Geometry {
   static constexpr int WPL = W == 32 ? 1 : 2;             // words of a key's piece per lane
   static constexpr int KS = 2 * WPL;                      // steps of 16 dimensions per piece
   static constexpr int NT = W == 32 ? 4 : 8;              // tiles of 8 dimensions per piece
-  static constexpr int PROWS = F32 ? 24 : 16;             // rows of weights
+  static constexpr int PARTS = F32 ? 3 : 2;               // bf16 that a weight is
   static constexpr int ROWS_BYTES = BLOCK * W / 2, SCALE_BYTES = BLOCK * 4 * NP, STAGE = 2 * (ROWS_BYTES + SCALE_BYTES);   // keys, values, their scales
-  static constexpr int P_BYTES = NP * PROWS * PITCH;
-  __host__ __device__ static constexpr int warp_bytes(int rows) { return NP * rows * S_PITCH * 4 + P_BYTES; }
+  static constexpr int P_BYTES = NP * PARTS * TILE * 16;
+  __host__ __device__ static constexpr int warp_bytes(int rows) { return NP * rows * TILE * 4 + P_BYTES; }
   __host__ __device__ static constexpr int bytes(int rows) { return STAGES * STAGE + WARPS * warp_bytes(rows); }
 };
 
@@ -58,11 +56,11 @@ __device__ __forceinline__ void mma_first(float (&c)[4], uint32_t a0, uint32_t a
                : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
-__device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t a) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], uint32_t a) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
 }
-__device__ __forceinline__ void ldmatrix_x2(uint32_t (&r)[2], uint32_t a) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x2.shared.b16 {%0,%1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "r"(a) : "memory");
+__device__ __forceinline__ void ldmatrix_x2_trans(uint32_t (&r)[2], uint32_t a) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0,%1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "r"(a) : "memory");
 }
 // numbers s of the two halves of w, as bf16: 128 + n, or n - 8 (CENTRED).  (mask, base and off: 0x000f000f, 0x43004300 and 0x43084308 from registers, which an
 // instruction takes two of, where it takes one constant)
@@ -88,6 +86,21 @@ template <int N> __device__ __forceinline__ void load_words(uint32_t (&w)[N], co
   if constexpr (N == 2) *reinterpret_cast<uint2*>(w) = *reinterpret_cast<const uint2*>(p);
   if constexpr (N == 1) w[0] = *reinterpret_cast<const uint32_t*>(p);
 }
+template <int N> __device__ __forceinline__ void load_rows(uint32_t (&w)[N], const float* p) {
+  if constexpr (N == 8) {
+    load_words(*reinterpret_cast<uint32_t(*)[4]>(w), reinterpret_cast<const unsigned char*>(p));
+    load_words(*reinterpret_cast<uint32_t(*)[4]>(w + 4), reinterpret_cast<const unsigned char*>(p + 4));
+  } else {
+    load_words(w, reinterpret_cast<const unsigned char*>(p));
+  }
+}
+// bf16 v[0], v[1], ... from p on
+template <int N> __device__ __forceinline__ void store_halves(unsigned char* p, const uint32_t* v) {
+  if constexpr (N == 8) *reinterpret_cast<uint4*>(p) = make_uint4(v[0], v[1], v[2], v[3]);
+  if constexpr (N == 4) *reinterpret_cast<uint2*>(p) = make_uint2(v[0], v[1]);
+  if constexpr (N == 2) *reinterpret_cast<uint32_t*>(p) = v[0];
+  if constexpr (N == 1) *reinterpret_cast<unsigned short*>(p) = (unsigned short)v[0];
+}
 
 // NR: rows of queries that there is room for
 template <typename T, int W, int NR>
@@ -99,16 +112,17 @@ __global__ void __launch_bounds__(WARPS * 32, W == 128 ? 3 : 4) kv4_step_kernel(
   constexpr int NP = G::NP, KS = G::KS, NT = G::NT;
   constexpr float LOG2E = 1.4426950408889634f;
   extern __shared__ __align__(16) unsigned char smem[];
-  __shared__ float s_qsum[8][2], s_slope[8], s_own[8], s_m[WARPS][8], s_l[WARPS][8], c_m[8], c_l[8];
+  __shared__ __align__(16) float s_qsum[2][8], s_slope[8];
+  __shared__ float s_own[8], s_m[WARPS][8], s_l[WARPS][8], c_m[8], c_l[8];
   const int g = blockIdx.x / splits, part = blockIdx.x - g * splits, b = blockIdx.y;
   const int R = H / Hk, r0 = blockIdx.z * 8, rows = min(8, R - r0), h0 = g * R + r0;   // the query heads h0 .. h0 + rows - 1
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, gr = lane >> 2, c = lane & 3;
   __shared__ uint64_t full[STAGES], empty[STAGES];
   __shared__ int abort_flag;
   unsigned char* mine = smem + STAGES * G::STAGE + warp * G::warp_bytes(NR);
-  float* sS = reinterpret_cast<float*>(mine);             // [piece][row][32 keys]
-  unsigned char* sP = mine + NP * NR * S_PITCH * 4;          // [piece][hi 8, mid 8 (, lo 8) rows][32 keys] bf16
-  for (int e = lane; e < G::P_BYTES / 4; e += 32) reinterpret_cast<uint32_t*>(sP)[e] = 0;   // (rows without a query stay as they are)
+  float* sS = reinterpret_cast<float*>(mine);             // [piece][32 keys][row]; of 8 rows the halves change places with every fourth key (banks)
+  unsigned char* sP = mine + NP * NR * TILE * 4;          // [piece][hi, mid (, lo)][32 keys][8 rows] bf16
+  for (int e = lane; e < G::P_BYTES / 4; e += 32) reinterpret_cast<uint32_t*>(sP)[e] = 0;   // (rows that there is no room for stay as they are)
   if (threadIdx.x == 0) {
     for (int i = 0; i < STAGES; i++) {
       tma::mbar_init(&full[i], 1);
@@ -192,6 +206,8 @@ __global__ void __launch_bounds__(WARPS * 32, W == 128 ? 3 : 4) kv4_step_kernel(
           }
         }
   }
+  if (threadIdx.x < 8) s_qsum[0][threadIdx.x] = s_qsum[1][threadIdx.x] = s_slope[threadIdx.x] = 0.f;   // rows without a query are computed beside the others
+  __syncthreads();
   for (int r = warp; r < rows; r += WARPS) {   // each query's sums, and its score with the new token's own key
     const T *q = row + (long long)(h0 + r) * hd, *k = row + (long long)(H + g) * hd;
     float sum0 = 0.f, sum1 = 0.f, dot = 0.f;
@@ -205,8 +221,8 @@ __global__ void __launch_bounds__(WARPS * 32, W == 128 ? 3 : 4) kv4_step_kernel(
     dot = warp_sum(dot) * scale;
     if (softcap > 0.f) dot = softcap * tanhf(dot / softcap);
     if (lane == 0) {
-      s_qsum[r][0] = sum0;
-      s_qsum[r][1] = sum1;
+      s_qsum[0][r] = sum0;
+      s_qsum[1][r] = sum1;
       s_own[r] = dot * LOG2E;
       s_slope[r] = slopes ? slopes[h0 + r] * LOG2E : 0.f;
     }
@@ -279,8 +295,12 @@ __global__ void __launch_bounds__(WARPS * 32, W == 128 ? 3 : 4) kv4_step_kernel(
 #pragma unroll
         for (int j = 0; j < 2; j++)
 #pragma unroll
-          for (int e = 0; e < 4; e++)
-            if (2 * c + (e & 1) < NR) sS[(p * NR + 2 * c + (e & 1)) * S_PITCH + 16 * j + gr + 8 * (e >> 1)] = s[p][j][e];
+          for (int e = 0; e < 2; e++)   // key 16 j + gr + 8 e, queries 2 c and 2 c + 1
+            if (2 * c < NR) {
+              float* at = sS + (p * TILE + 16 * j + gr + 8 * e) * NR + (NR == 8 ? (2 * c) ^ (gr & 4) : 2 * c);
+              if (NR == 1) *at = s[p][j][2 * e];
+              else *reinterpret_cast<float2*>(at) = make_float2(s[p][j][2 * e], s[p][j][2 * e + 1]);
+            }
     }
     __syncwarp();
     // ---- a lane per key
@@ -299,47 +319,76 @@ __global__ void __launch_bounds__(WARPS * 32, W == 128 ? 3 : 4) kv4_step_kernel(
       vstep[p] = seen ? __uint_as_float(vs[p] & 0xffff0000u) : 0.f;
       vlow[p] = seen ? fmaf(8.f, vstep[p], __uint_as_float(vs[p] << 16)) : 0.f;
     }
-    bool moved = false;
-    float shrink = 1.f;   // of row gr
+    float x[NR];   // scores, then weights
+#pragma unroll
+    for (int r = 0; r < NR; r++) x[r] = 0.f;
+#pragma unroll
+    for (int p = 0; p < NP; p++) {
+      uint32_t raw[NR], qsum[NR];
+      load_rows(qsum, s_qsum[p]);
+      const float* at = sS + (p * TILE + lane) * NR;
+      if constexpr (NR == 8) {
+        load_words(*reinterpret_cast<uint32_t(*)[4]>(raw), reinterpret_cast<const unsigned char*>(at + (lane & 4)));
+        load_words(*reinterpret_cast<uint32_t(*)[4]>(raw + 4), reinterpret_cast<const unsigned char*>(at + (4 ^ (lane & 4))));
+      } else {
+        load_words(raw, reinterpret_cast<const unsigned char*>(at));
+      }
+#pragma unroll
+      for (int r = 0; r < NR; r++) x[r] = fmaf(kstep[p], __uint_as_float(raw[r]), fmaf(klow[p], __uint_as_float(qsum[r]), x[r]));
+    }
+    bool over = false;
+    uint32_t slope[NR];
+    load_rows(slope, s_slope);
 #pragma unroll
     for (int r = 0; r < NR; r++) {
-      if (r < rows) {   // (the same for the whole CTA)
-        float x = 0.f;
+      if (softcap > 0.f) {
+        if (F32) x[r] = tanhf(x[r]);
+        else asm("tanh.approx.f32 %0, %0;" : "+f"(x[r]));   // relative error 2^-11
+        x[r] *= k_out;
+      }
+      x[r] = seen ? fmaf(-__uint_as_float(slope[r]), far, x[r]) : -INFINITY;
+      over = over || x[r] > bar[r];
+    }
+    const bool moved = __any_sync(0xffffffffu, over);   // seldom: one vote for all rows
+    float shrink = 1.f;   // of row gr
+    if (moved) {
 #pragma unroll
-        for (int p = 0; p < NP; p++) x = fmaf(kstep[p], sS[(p * NR + r) * S_PITCH + lane], fmaf(klow[p], s_qsum[r][p], x));
-        if (softcap > 0.f) {
-          if (F32) x = tanhf(x);
-          else asm("tanh.approx.f32 %0, %0;" : "+f"(x));   // relative error 2^-11
-          x *= k_out;
-        }
-        x = seen ? fmaf(-s_slope[r], far, x) : -INFINITY;
-        if (__any_sync(0xffffffffu, x > bar[r])) {
-          const float top = fmaxf(m[r], warp_max(x)), corr = exp2_fast(m[r] - top);   // (0 where there was no key yet)
-          m[r] = top;
-          bar[r] = top + LAG;
-          l[r] *= corr;
+      for (int r = 0; r < NR; r++) {
+        const float top = fmaxf(m[r], warp_max(x[r])), corr = exp2_fast(m[r] - top);   // (0 where there was no key yet)
+        m[r] = top;
+        bar[r] = top + LAG;
+        l[r] *= corr;
 #pragma unroll
-          for (int p = 0; p < NP; p++) low[r][p] *= corr;
-          if (gr == r) shrink = corr;
-          moved = true;
-        }
-        const float w = exp2_fast(x - m[r]);
-        l[r] += w;
+        for (int p = 0; p < NP; p++) low[r][p] *= corr;
+        if (gr == r) shrink = corr;
+      }
+    }
 #pragma unroll
-        for (int p = 0; p < NP; p++) {
-          const float a = w * vstep[p];
-          __nv_bfloat16* at = reinterpret_cast<__nv_bfloat16*>(sP + (p * G::PROWS + r) * PITCH) + column;
-          const float mid = a - __uint_as_float(__float_as_uint(a) & 0xffff0000u);   // (cut off, what is left is exact)
-          reinterpret_cast<unsigned short*>(at)[0] = (unsigned short)(__float_as_uint(a) >> 16);
-          if (F32) {
-            reinterpret_cast<unsigned short*>(at)[8 * PITCH / 2] = (unsigned short)(__float_as_uint(mid) >> 16);
-            at[16 * PITCH / 2] = __float2bfloat16_rn(mid - __uint_as_float(__float_as_uint(mid) & 0xffff0000u));
-          } else {
-            at[8 * PITCH / 2] = __float2bfloat16_rn(mid);
-          }
-          low[r][p] = fmaf(w, vlow[p], low[r][p]);
+    for (int r = 0; r < NR; r++) {
+      x[r] = exp2_fast(x[r] - m[r]);
+      l[r] += x[r];
+    }
+#pragma unroll
+    for (int p = 0; p < NP; p++) {
+      unsigned char* at = sP + (p * G::PARTS * TILE + column) * 16;
+      uint32_t hi[(NR + 1) / 2], mid[(NR + 1) / 2], lo[(NR + 1) / 2];
+#pragma unroll
+      for (int r = 0; r < NR; r += 2) {   // what is left of a weight that is cut off is exact
+        const float a0 = x[r] * vstep[p], a1 = r + 1 < NR ? x[r + 1 < NR ? r + 1 : r] * vstep[p] : 0.f;
+        const float b0 = a0 - __uint_as_float(__float_as_uint(a0) & 0xffff0000u), b1 = a1 - __uint_as_float(__float_as_uint(a1) & 0xffff0000u);
+        hi[r / 2] = __byte_perm(__float_as_uint(a0), __float_as_uint(a1), 0x7632);
+        if (F32) {
+          mid[r / 2] = __byte_perm(__float_as_uint(b0), __float_as_uint(b1), 0x7632);
+          lo[r / 2] = bf16_pair(b0 - __uint_as_float(__float_as_uint(b0) & 0xffff0000u), b1 - __uint_as_float(__float_as_uint(b1) & 0xffff0000u));
+        } else {
+          mid[r / 2] = bf16_pair(b0, b1);
         }
       }
+      store_halves<NR>(at, hi);
+      store_halves<NR>(at + TILE * 16, mid);
+      if (F32) store_halves<NR>(at + 2 * TILE * 16, lo);
+#pragma unroll
+      for (int r = 0; r < NR; r++) low[r][p] = fmaf(x[r], vlow[p], low[r][p]);
     }
     if (moved) {   // (for the whole warp)
 #pragma unroll
@@ -359,9 +408,10 @@ __global__ void __launch_bounds__(WARPS * 32, W == 128 ? 3 : 4) kv4_step_kernel(
 #pragma unroll
       for (int p = 0; p < NP; p++) {
         uint32_t a[4], a3[2] = {0u, 0u};
-        const uint32_t at = (uint32_t)__cvta_generic_to_shared(sP + (p * G::PROWS + (lane & 15)) * PITCH + kk * 32 + (lane >> 4) * 16);
-        ldmatrix_x4(a, at);   // rows 0 - 7 and 8 - 15 of keys 0 - 7, then of keys 8 - 15
-        if (F32) ldmatrix_x2(a3, (uint32_t)__cvta_generic_to_shared(sP + (p * G::PROWS + 16 + (lane & 7)) * PITCH + kk * 32 + ((lane >> 3) & 1) * 16));
+        const uint32_t at = (uint32_t)__cvta_generic_to_shared(sP + (p * G::PARTS * TILE + 16 * kk + (lane & 7)) * 16);
+        // rows 0 - 7 (leading bits) and 8 - 15 (what they left) of keys 0 - 7, then of keys 8 - 15
+        ldmatrix_x4_trans(a, at + ((lane & 8) ? TILE * 16 : 0) + (lane >> 4) * 128);
+        if (F32) ldmatrix_x2_trans(a3, at + 2 * TILE * 16 + ((lane & 8) ? 128 : 0));
         uint32_t lo[2], hi[2];   // numbers 0 - 3 and 4 - 7 of two keys
 #pragma unroll
         for (int e = 0; e < 2; e++) {
