@@ -9,6 +9,8 @@
 // has any.  (An infinite query or key has NaN scores: so do its parts' products.)
 // The keys' first tile is the first that any row sees.  Six products instead of one on the older tensor path (1024 multiply-adds a clock and SM) leave 90 TFLOP/s; the CUDA cores'
 // 74 need both operands of every product from shared memory or registers.  Shared memory: 120 KB for heads of 128 (one CTA per SM), 60 for heads of 64.
+// Measured: 128 + 700 tokens, 8 heads of 64, 51 us where there are only 104 CTAs: a warp per scheduler, whose products (24 % of the pipe), cutting up and softmax follow one another.  On the CUDA
+// cores the same took 379 us.
 #include "attention_packed.cuh"
 
 namespace {
