@@ -156,7 +156,8 @@ extern "C" int stu_kv4_write(const void* qkv, long long row_stride, void* k4, vo
   if (!qkv || !k4 || !v4 || !pos) return STU_ERR_NULL;
   const int rc = kv4::geometry(B, H, Hk, hd, slots, dtype);
   if (rc != STU_OK) return rc;
-  if (rows <= 0 || rows > 0x7fff0000ll || row_stride < (long long)(H + 2 * Hk) * hd || (!cu_seqlens && rows % B)) return STU_ERR_SHAPE;
+  // (above the last row there is room for a grid's warps, 512 per SM: the rows' count passes no 32 bits)
+  if (rows <= 0 || rows > 0x7ff00000ll || row_stride < (long long)(H + 2 * Hk) * hd || (!cu_seqlens && rows % B)) return STU_ERR_SHAPE;
   if (!aligned16(k4) || !aligned16(v4)) return STU_ERR_ALIGN;
   const int per_seq = cu_seqlens ? 0 : (int)(rows / B);
   return dtype == STU_F32 ? launch_write<float>(qkv, row_stride, k4, v4, pos, cu_seqlens, B, rows, per_seq, H, Hk, hd, slots, (cudaStream_t)stream)

@@ -175,3 +175,12 @@ def test_tensor_parallelism_refuses_a_cache_in_4_bits(tmp_path):
             TensorParallelFlashSTU(F.FlashSTUConfig(n_embd=64, n_heads=4, n_layers=2, seq_len=64, window_size=20, vocab_size=11, num_eigh=4, kv_bits=4), {}, "cpu")
     finally:
         dist.destroy_process_group()
+
+
+def test_rows_of_a_write_stay_below_32_bits():
+    from flash_stu_2_b200 import _lib
+    lib = _lib.load()
+    a = 0x10000   # as above: refused before anything dereferences it (a + 4: were the rows allowed, the ring's alignment would refuse the call)
+    most = 0x7ff00000
+    assert lib.stu_kv4_write(a, 256, a + 4, a, a, None, 1, most, 2, 1, 64, 16, 1, None) == -3
+    assert lib.stu_kv4_write(a, 256, a + 4, a, a, None, 1, most + 1, 2, 1, 64, 16, 1, None) == -2
