@@ -23,7 +23,7 @@ from . import ops
 from .config import FlashSTUConfig
 from .filters import get_spectral_filters, nearest_power_of_two
 from .layers import AttentionLayer, STULayer
-from .modules import STU, Attention, Packed, RMSNorm
+from .modules import STU, Attention, Packed, RMSNorm, common_pos
 from .stream_ahead import StreamAhead
 from .token_step import TokenStep
 
@@ -129,9 +129,10 @@ class FlashSTU(PreTrainedModel):
                 raise ValueError(f"packed prompts are input_ids [1, {sum(lengths)}] (the sum of their lengths) without past_key_values, got "
                                  f"{tuple(input_ids.shape)}")
             packed = Packed(lengths, input_ids.device)
-        elif past_key_values is not None and input_ids.shape[1] > 1 and any(
-                e is not None and getattr(e[-1], "_uniform", True) is False for e in past_key_values):
-            raise ValueError("caches at different positions take one token per sequence at a time")
+        elif past_key_values is not None and input_ids.shape[1] > 1:   # (before any layer has moved its cache on)
+            for e in past_key_values:
+                if e is not None:
+                    common_pos(e[-1])
         x = ops.embed(input_ids, self.tok_emb.weight)
         hidden = (x.clone(),) if collect_hidden else None
         cache = () if use_cache else None

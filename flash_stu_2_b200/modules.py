@@ -51,12 +51,12 @@ def unwritten_pos(batch: int, device) -> torch.Tensor:
 
 
 def host_pos(pos: torch.Tensor) -> int:
-    """Host-side mirror of pos[0,0]; falls back to a device read when the tensor was re-created
+    """Host-side mirror of the furthest position, pos[:,0].max(); falls back to a device read when the tensor was re-created
     (e.g. by _reorder_cache), which also re-checks whether all sequences share one position."""
     t = getattr(pos, "_host_t", None)
     if t is None:
         col = pos[:, 0].tolist()
-        t = int(col[0])
+        t = max(col, default=0)
         pos._host_t = t
         pos._uniform = all(v == t for v in col)
     return t
@@ -64,6 +64,14 @@ def host_pos(pos: torch.Tensor) -> int:
 
 def uniform_pos(pos: torch.Tensor) -> bool:
     return getattr(pos, "_uniform", False)
+
+
+def common_pos(pos: torch.Tensor) -> int:
+    """host_pos for kernels that take one position for all sequences."""
+    t = host_pos(pos)
+    if getattr(pos, "_uniform", True) is False:
+        raise ValueError("caches at different positions take one token per sequence at a time, in attention and plain approx STU layers")
+    return t
 
 
 def param(module: nn.Module, name: str):
@@ -368,7 +376,7 @@ class STU(nn.Module):
         t0 = 0
         if entry is not None:
             hist, pos = entry
-            t0 = host_pos(pos)
+            t0 = common_pos(pos)
         elif use_cache:
             hist, pos = self.new_cache(B, xn.device)
         else:
@@ -434,7 +442,7 @@ class STU(nn.Module):
         phi, Mcat = self.prepared_full()
         B, d, _, Lh = hist.shape
         K, nsign = self.K, (1 if self.use_hankel_L else 2)
-        t = host_pos(pos)
+        t = common_pos(pos)
         if t + 1 > self.capacity:
             raise ValueError(f"sequence position {t + 1} exceeds the capacity {self.capacity} (seq_len={self.seq_len})")
         if (Lh == self.Lh and ops.full_decode_step_supported(x2d, hist, K)
@@ -467,7 +475,7 @@ class STU(nn.Module):
         t0, fresh = 0, False
         if entry is not None:
             hist, pos = entry
-            t0 = host_pos(pos)
+            t0 = common_pos(pos)
         if t0 + T > self.capacity:
             raise ValueError(f"sequence position {t0 + T} exceeds the capacity {self.capacity} (seq_len={self.seq_len}: "
                              f"the filters have seq_len taps; cache_len={self.cache_len})")
@@ -500,7 +508,7 @@ class STU(nn.Module):
         t0 = 0
         if entry is not None:
             hist, pos = entry
-            t0 = host_pos(pos)
+            t0 = common_pos(pos)
         elif use_cache:
             hist, pos = _cache_for_prefill(self, STU, B, xn.device, T if T <= self.capacity else 0)
         else:

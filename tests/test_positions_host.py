@@ -1,0 +1,56 @@
+"""What the host knows of a cache's positions once its tensors have been made anew (reordered, cloned, joined), and the calls that need them all alike."""
+from types import SimpleNamespace
+
+import pytest
+import torch
+
+from flash_stu_2_b200 import FlashSTU, modules
+from flash_stu_2_b200.modules import STU
+
+
+def ragged(*t):
+    """Positions that nothing is known of on the host, as index_select leaves them."""
+    pos = modules.new_pos(len(t), "cpu")
+    pos[:, 0] = torch.tensor(t, dtype=torch.int32)
+    return pos.index_select(0, torch.arange(len(t)))
+
+
+def test_the_furthest_position_counts():
+    for t in ((5, 250, 7), (250, 5, 7), (3,), (4, 4)):
+        pos = ragged(*t)
+        assert modules.host_pos(pos) == max(t) and modules.uniform_pos(pos) == (len(set(t)) == 1)
+    assert modules.common_pos(ragged(9, 9)) == 9 and modules.common_pos(modules.new_pos(2, "cpu")) == 0
+    noted = modules.new_pos(2, "cpu")
+    noted._host_t, noted._uniform = 8, False
+    for pos in (ragged(9, 8), ragged(0, 1, 0), noted):
+        with pytest.raises(ValueError, match="different positions"):
+            modules.common_pos(pos)
+
+
+@pytest.mark.parametrize("t", [(5, 250), (250, 5), (0, 3)])
+def test_models_refuse_several_tokens(t):
+    model = SimpleNamespace(training=False, config=SimpleNamespace(dropout=0.0), tok_emb=SimpleNamespace(weight=None), layers=())
+    ids = SimpleNamespace(is_cuda=True, shape=(2, 3))
+    with pytest.raises(ValueError, match="different positions"):
+        FlashSTU._backbone(model, ids, [None, (None, ragged(*t))], True)
+
+
+@pytest.mark.parametrize("t", [(5, 25), (25, 5)])
+def test_layers_refuse_one_position_for_all(t):
+    """Layers called by themselves: a prefill's histories go where one number says, and so does every step of the full variant and of the single branch."""
+    stu = SimpleNamespace(use_approx=True, use_hankel_L=False, capacity=100, K=4, seq_len=100, cache_len=None, Lh=56, prepared=lambda: (None,) * 3,
+                          prepared_full=lambda: (None, None))
+    x, hist = torch.zeros(2, 3, 8), torch.zeros(2, 8, 2, 56)
+    for call in (lambda: STU.add_to_residual(stu, x, x, (hist, ragged(*t))),
+                 lambda: STU.layer_prefill(stu, x, (hist, ragged(*t)), True, None, None, None),
+                 lambda: STU.full_forward(stu, x, None, x, (hist, ragged(*t))),
+                 lambda: STU.full_decode_step(stu, x[:, 0], None, x[:, 0], (hist, ragged(*t)))):
+        with pytest.raises(ValueError, match="different positions"):
+            call()
+
+
+def test_the_furthest_position_is_held_to_the_capacity():
+    stu = SimpleNamespace(use_approx=True, use_hankel_L=False, capacity=100, seq_len=100, prepared=lambda: (None,) * 3)
+    for t in ((100, 5), (5, 100)):
+        with pytest.raises(ValueError, match="exceeds the capacity"):
+            STU.decode_step(stu, torch.zeros(2, 8), None, 1e-6, (torch.zeros(2, 8, 2, 56), ragged(*t)), torch.zeros(2, 8))
