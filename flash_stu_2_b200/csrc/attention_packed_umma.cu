@@ -156,17 +156,21 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
+__device__ __forceinline__ float max_nan(float a, float b) {   // NaN where one is
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
 // 2^x on the FMA pipe, beside the special-function unit, which takes 8 clocks of a warp for every exponential: x = k + f with f in [-1/2, 1/2] (adding 1.5 2^23
-// rounds to whole numbers), a polynomial of degree 3 in f (minimax, relative error 7.5e-5 against 2^-9 of the weights' rounding), k added to the exponent.  At least 2^-125: what is
-// masked adds that to the sum of weights and to none of the products of finite values, as far as fp32 tells.  NaN stays NaN.
+// rounds to whole numbers), a polynomial of degree 3 in f (minimax among those that are 1 at 0, relative error 1.02e-4 against 2^-9 of the weights' rounding), k added
+// to the exponent.  x is raised to -127, where f is 0, the polynomial 1 and the sum 0: what is masked has no weight at all (a small one in its place would be seen in the
+// products: 2^-125 of the largest finite value is 8).  Between -127 and -126 the sum is below 2^-126, whatever it is.  NaN leaves as a number that bf16 rounds to
+// infinity: its row's result is not finite, is computed again, and is NaN.
 template <int N> __device__ __forceinline__ void exp2_poly(const uint32_t* x, f32x2* y) {
   f32x2 f[N], t[N], p[N];
   const f32x2 big = pair_of(12582912.f, 12582912.f), unbig = pair_of(-12582912.f, -12582912.f), minus = pair_of(-1.f, -1.f);
 #pragma unroll
-  for (int u = 0; u < N; u++) {
-    const float x0 = __uint_as_float(x[2 * u]), x1 = __uint_as_float(x[2 * u + 1]);
-    f[u] = pair_of(x0 < -125.f ? -125.f : x0, x1 < -125.f ? -125.f : x1);
-  }
+  for (int u = 0; u < N; u++) f[u] = pair_of(max_nan(__uint_as_float(x[2 * u]), -127.f), max_nan(__uint_as_float(x[2 * u + 1]), -127.f));
 #pragma unroll
   for (int u = 0; u < N; u++) t[u] = add2(f[u], big);
 #pragma unroll
@@ -174,11 +178,11 @@ template <int N> __device__ __forceinline__ void exp2_poly(const uint32_t* x, f3
 #pragma unroll
   for (int u = 0; u < N; u++) f[u] = fma2(p[u], minus, f[u]);
 #pragma unroll
-  for (int u = 0; u < N; u++) p[u] = fma2(f[u], pair_of(0.05517167f, 0.05517167f), pair_of(0.24261112f, 0.24261112f));
+  for (int u = 0; u < N; u++) p[u] = fma2(f[u], pair_of(0.0550089329f, 0.0550089329f), pair_of(0.242210969f, 0.242210969f));
 #pragma unroll
-  for (int u = 0; u < N; u++) p[u] = fma2(f[u], p[u], pair_of(0.69326099f, 0.69326099f));
+  for (int u = 0; u < N; u++) p[u] = fma2(f[u], p[u], pair_of(0.693282902f, 0.693282902f));
 #pragma unroll
-  for (int u = 0; u < N; u++) p[u] = fma2(f[u], p[u], pair_of(0.99992807f, 0.99992807f));
+  for (int u = 0; u < N; u++) p[u] = fma2(f[u], p[u], pair_of(1.f, 1.f));
 #pragma unroll
   for (int u = 0; u < N; u++) {
     uint32_t p0, p1, t0, t1;

@@ -2,6 +2,8 @@
 import pytest
 import torch
 
+import kv4_reference as R
+from test_gpu_7_kv4 import activations, cu_of, gen, slopes_of
 from test_gpu_8_kv4_model import SAME, dev, far, model
 
 pytestmark = pytest.mark.gpu
@@ -67,3 +69,55 @@ def test_layers_by_themselves_refuse_different_positions():
         for e in (past[0], tuple(t.clone() for t in past[0])):
             with pytest.raises(ValueError, match="different positions"):
                 m.layers[0](x, past_key_value=e, use_cache=True)
+
+
+# ---------------------------------------------------------------------------------------------------- huge finite values
+def huge(dt):
+    most = torch.finfo(dt).max
+    return (most, -most, 3e38, -3e38, 1e36)
+
+
+def check_rows(got, want, tol, rows):
+    R.check(got[rows], want[rows], tol[rows])
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16])
+@pytest.mark.parametrize("hd", [64, 128, 40, 13])
+@pytest.mark.parametrize("cap,window", [(50.0, None), (0.0, 30)])
+def test_packed_huge_values_are_for_those_who_see_them(dt, hd, cap, window):
+    """Finite values as large as the type's, in one sequence or at one key: no other sequence and no earlier row has anything of them, and rows that
+    are past the key's window neither.  (All but the weights of what is seen are the same for them, so the reference's tolerance is too.)"""
+    from flash_stu_2_b200 import ops
+    g, H, kv, lengths = gen(hd), 2, 1, (70, 33, 200, 5)
+    qkv, cu, slopes = activations(g, sum(lengths), H, kv, hd, dt), cu_of(lengths), slopes_of(H)
+    want, tol = R.packed(qkv, lengths, 0, slopes, H, kv, window, cap, dt)
+    for value in huge(dt):
+        for bad in range(4):
+            x = qkv.clone()
+            a, b = int(cu[bad]), int(cu[bad + 1])
+            x[a:b, H * hd:] = value
+            got = ops.swa_packed(x, cu, slopes, H, window, cap, kv_heads=kv)
+            check_rows(torch.cat([got[:a], got[b:]]), torch.cat([want[:a], want[b:]]), torch.cat([tol[:a], tol[b:]]), slice(None))
+        x = qkv.clone()
+        x[150, (H + kv) * hd:] = value              # one value in the third, whose rows are 103 .. 302
+        got = ops.swa_packed(x, cu, slopes, H, window, cap, kv_heads=kv)
+        some = list(range(150)) + list(range(303, 308)) + (list(range(150 + window + 1, 303)) if window else [])
+        check_rows(got, want, tol, some)
+        seen, loose = R.packed(x, lengths, 0, slopes, H, kv, window, cap, dt)
+        check_rows(got, seen, loose, slice(150, 150 + window + 1 if window else 303))
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_packed_huge_values_far_away(dt, hd):
+    """A huge value that is seen from so far that ALiBi leaves nothing of it: e^-390 of it is below 10^-130."""
+    from flash_stu_2_b200 import ops
+    g, H, kv, n = gen(hd + 1), 2, 2, 400
+    qkv, cu, slopes = activations(g, n, H, kv, hd, dt), cu_of([n]), torch.tensor([8.0, 4.0], device=dev())
+    for cap in (0.0, 50.0):
+        want, tol = R.packed(qkv, [n], 0, slopes, H, kv, None, cap, dt)
+        for value in huge(dt):
+            x = qkv.clone()
+            x[96:100, (H + kv) * hd:] = value
+            got = ops.swa_packed(x, cu, slopes, H, None, cap)
+            check_rows(got, want, tol, list(range(96)) + list(range(200, n)))
