@@ -75,7 +75,7 @@ __global__ void __launch_bounds__(256) packed_attend_kernel(const bf16* __restri
       if (softcap > 0.f) sc = softcap * tanhf(sc / softcap);
       sc = seen[u] ? sc - slope * (float)(i - j) : -INFINITY;
       const float top = fmaxf(m[u], warp_max(sc)), corr = top == -INFINITY ? 1.f : __expf(m[u] - top);
-      pr[u] = seen[u] ? __expf(sc - top) : 0.f;
+      pr[u] = sc == -INFINITY ? 0.f : __expf(sc - top);   // (what is not seen, and what is, with no weight: there may be no maximum yet)
       l[u] = l[u] * corr + warp_sum(pr[u]);
       m[u] = top;
 #pragma unroll

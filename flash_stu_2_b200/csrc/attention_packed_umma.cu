@@ -249,7 +249,8 @@ __device__ void row_again(const bf16* __restrict__ qkv, long long row_stride, bf
     s = warp_sum(s);
     if (softcap > 0.f) s = softcap * tanhf(s / softcap);
     s -= slope * (float)(i - j);
-    const float top = fmaxf(m, s), corr = top == -INFINITY ? 1.f : __expf(m - top), p = __expf(s - top);
+    // (a score of minus infinity weighs nothing, the first ones too, behind which there is no maximum yet)
+    const float top = fmaxf(m, s), corr = top == -INFINITY ? 1.f : __expf(m - top), p = s == -INFINITY ? 0.f : __expf(s - top);
     m = top;
     l = l * corr + p;
 #pragma unroll

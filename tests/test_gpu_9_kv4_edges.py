@@ -121,3 +121,68 @@ def test_packed_huge_values_far_away(dt, hd):
             x[96:100, (H + kv) * hd:] = value
             got = ops.swa_packed(x, cu, slopes, H, None, cap)
             check_rows(got, want, tol, list(range(96)) + list(range(200, n)))
+
+
+# ---------------------------------------------------------------------------------------------------- infinite scores
+def by_hand(qkv, lengths, slopes, H, kv, window, cap, dt, unseen):
+    """R.packed where nobody sees the rows `unseen`."""
+    x = qkv.double().view(qkv.shape[0], H + 2 * kv, -1)
+    out, tol, at = [], [], 0
+    for n in lengths:
+        p = torch.arange(n, device=qkv.device)
+        behind = p[:, None] - p
+        seen = (behind >= 0) & (behind <= window)
+        for j in unseen:
+            if at <= j < at + n:
+                seen[:, j - at] = False
+        rows = [R.attention(x[at:at + n, h], x[at:at + n, H + h * kv // H], x[at:at + n, H + kv + h * kv // H], behind, seen, float(slopes[h]), cap)
+                for h in range(H)]
+        out.append(torch.stack([o for o, _ in rows], 1))
+        tol.append(torch.stack([R.tolerance(o, t, dt, R.WEIGHTS_PACKED[dt], R.TANH[dt]) for o, t in rows], 1))
+        at += n
+    out, tol = torch.cat(out).flatten(1), torch.cat(tol).flatten(1)
+    return out, tol
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16])
+@pytest.mark.parametrize("hd", [64, 128, 13])
+@pytest.mark.parametrize("beside", [False, True])
+def test_packed_keys_of_no_weight(dt, hd, beside):
+    """Keys whose scores are minus infinity weigh nothing, the first that a row sees and the first of a tile among them; a row that sees only such has no
+    result.  beside: NaN in the keys and values of the next sequence, for which rows are computed in another way."""
+    from flash_stu_2_b200 import ops
+    g, H, kv, lengths, window = gen(hd + 3), 2, 1, (100, 60), 10
+    qkv, cu, slopes = activations(g, sum(lengths), H, kv, hd, dt), cu_of(lengths), slopes_of(H)
+    x = qkv.view(-1, H + 2 * kv, hd)
+    x[:, :H, 3] = x[:, :H, 3].abs() + 1
+    none = [0, 1, 22, 53, 54, 85, 99]
+    want, tol = by_hand(qkv, lengths, slopes, H, kv, window, 0.0, dt, none)
+    x[none, H:H + kv] = 0.0
+    x[none, H:H + kv, 3] = float("-inf")
+    if beside:
+        x[100:, H:] = float("nan")
+    got = ops.swa_packed(qkv, cu, slopes, H, window, 0.0, kv_heads=kv)
+    assert bool(got[:2].isnan().all()) and bool(got[100:].isnan().all()) == beside
+    R.check(got[2:100], want[2:100], tol[2:100])
+    if not beside:
+        R.check(got[100:], want[100:], tol[100:])
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16])
+@pytest.mark.parametrize("hd", [64, 128, 13])
+def test_packed_infinite_scores_are_capped(dt, hd):
+    """A soft cap makes a finite score of an infinite one, the same as of one that is far past it."""
+    from flash_stu_2_b200 import ops
+    g, H, kv, lengths, window, cap = gen(hd + 4), 2, 1, (100, 60), 10, 3.0
+    qkv, cu, slopes = activations(g, sum(lengths), H, kv, hd, dt), cu_of(lengths), slopes_of(H)
+    x = qkv.view(-1, H + 2 * kv, hd)
+    x[:, :H, 3] = x[:, :H, 3].abs() + 1
+    for sign in (1.0, -1.0):
+        for j in (0, 22, 53, 159):
+            x[j, H:H + kv] = 0.0
+            x[j, H:H + kv, 3] = sign * 60 * hd ** 0.5      # a score of 60 and more: tanh(20) is 1 - 2^-56
+        want, tol = R.packed(qkv, lengths, 0, slopes, H, kv, window, cap, dt)
+        y = x.clone()
+        for j in (0, 22, 53, 159):
+            y[j, H:H + kv, 3] = sign * float("inf")
+        R.check(ops.swa_packed(y.flatten(1), cu, slopes, H, window, cap, kv_heads=kv), want, tol)
