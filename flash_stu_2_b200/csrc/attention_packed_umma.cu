@@ -587,8 +587,9 @@ __global__ void __launch_bounds__(THREADS, 1) packed_umma_kernel(const __grid_co
           }
         }
       }
+      __syncwarp();   // a row that is computed again has been stored by its thread, and is stored by all of them below: in this order
       uint32_t again = __ballot_sync(0xffffffffu, first != packed::NOBODY && (l < LEAST || (!finite && fabsf(l) < INFINITY)));
-      for (; again; again &= again - 1) {   // (stored above by the row's thread, here by all of them: the ballot has ordered the two)
+      for (; again; again &= again - 1) {
         const int r = tile * BM + quarter * 32 + __ffs(again) - 1;
         row_again(qkv, row_stride, out + (long long)(q0 + r) * out_stride + (long long)h * hd, q0 + r, ctl.first[r], h, g, H, Hk, hd, ALIBI ? slopes[h] : 0.f,
                   scale, CAP ? softcap : 0.f, lane);
