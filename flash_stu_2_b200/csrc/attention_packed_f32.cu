@@ -5,11 +5,12 @@
 //   S = Q K^T   the queries' three parts stay in shared memory, as do the keys' and values' of a tile, which are cut up as they come in
 //   softmax     in registers, against the running maximum (exp2 domain, tanh of the library for the cap)
 //   O += P V    the weights' three parts are made from the accumulators where they lie
-// A product takes all values of a tile, masked ones with a weight of 0: infinite ones and NaN are zeros there, and are added for the rows that see them, where a tile
-// has any.  (An infinite query or key has NaN scores: so do its parts' products.)
+// A product takes all values of a tile, masked ones with a weight of 0: those whose leading part would not be finite (infinities, NaN, and what bf16 rounds to infinity,
+// from 2^128 - 2^119 on) are zeros there, and are added for the rows that see them, where a tile has any.  Queries and keys as large have their scores from fp32
+// products on the CUDA cores, as their parts' products would be NaN.  (NaN itself is NaN in its parts' products too.)
 // The keys' first tile is the first that any row sees.  Six products instead of one on the older tensor path (1024 multiply-adds a clock and SM) leave 90 TFLOP/s; the CUDA cores'
 // 74 need both operands of every product from shared memory or registers.  Shared memory: 120 KB for heads of 128 (one CTA per SM), 60 for heads of 64.
-// Measured: 128 + 700 tokens, 8 heads of 64, 51 us where there are only 104 CTAs: a warp per scheduler, whose products (24 % of the pipe), cutting up and softmax follow one another.  On the CUDA
+// Measured: 128 + 700 tokens, 8 heads of 64, 53 us where there are only 104 CTAs: a warp per scheduler, whose products (24 % of the pipe), cutting up and softmax follow one another.  On the CUDA
 // cores the same took 379 us.
 #include "attention_packed.cuh"
 
@@ -17,6 +18,7 @@ namespace {
 
 constexpr int BM = 64, BN = 32;
 constexpr float LOG2E = 1.4426950408889634f;
+constexpr float MOST = 0x1.ffp127f;   // what is smaller rounds to a finite bf16
 
 template <int HD> struct Smem {
   static constexpr int PITCH = HD + 8;                          // bf16 values between rows: eight rows' 16 bytes lie in different banks
@@ -65,7 +67,7 @@ __global__ void __launch_bounds__(128) packed_f32_kernel(const float* __restrict
   constexpr int P = L::PITCH;
   extern __shared__ __align__(16) bf16 smem[];
   bf16 *Qs = smem, *Ks = Qs + 3 * L::Q_PART, *Vs = Ks + 3 * L::KV_PART;   // [part][row][PITCH]
-  __shared__ int s_first[BM], s_odd[2];   // s_odd: whether a tile has values that are not finite (this and the next tile's)
+  __shared__ int s_first[BM], s_odd[2];   // whether a tile has values past MOST (this and the next tile's)
   const int h = blockIdx.y, g = h / (H / Hk), q0 = (int)(gridDim.x - 1 - blockIdx.x) * BM;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, gr = lane >> 2, c = lane & 3;
   // 4 values of a row of qkv, zeros past the head and past the rows
@@ -86,13 +88,16 @@ __global__ void __launch_bounds__(128) packed_f32_kernel(const float* __restrict
   };
   if (threadIdx.x < BM) s_first[threadIdx.x] = packed::first_key(cu, S, q0 + threadIdx.x, rows, window);
   if (threadIdx.x < 2) s_odd[threadIdx.x] = 0;
+  bool big = false;
   for (int e = threadIdx.x; e < BM * (HD / 4); e += 128) {
     const int r = e / (HD / 4), d = e % (HD / 4) * 4;
     float x[4];
     four(q0 + r, rows, qkv + (long long)h * hd, d, x);
+#pragma unroll
+    for (int u = 0; u < 4; u++) big |= fabsf(x[u]) >= MOST;
     put(Qs + r * P + d, L::Q_PART, x);
   }
-  __syncthreads();
+  const bool big_queries = __syncthreads_or(big);
   int j_lo = packed::NOBODY, j_hi = -1;   // keys that any row of the tile sees
   for (int r = 0; r < BM; r++) {
     j_lo = min(j_lo, s_first[r]);
@@ -124,20 +129,24 @@ __global__ void __launch_bounds__(128) packed_f32_kernel(const float* __restrict
   if (j_lo <= j_hi) fetch(j_lo);
   for (int jt = j_lo, turn = 0; jt <= j_hi; jt += BN, turn ^= 1) {
     __syncthreads();   // the tile before has been read
+    big = false;
 #pragma unroll
     for (int i = 0; i < MINE; i++) {
       const int e = threadIdx.x + 128 * i, which = e / (BN * (HD / 4)), r = e / (HD / 4) % BN, d = e % (HD / 4) * 4;
       if (which) {
 #pragma unroll
         for (int u = 0; u < 4; u++)
-          if (!(fabsf(coming[i][u]) < INFINITY)) {
+          if (!(fabsf(coming[i][u]) < MOST)) {
             coming[i][u] = 0.f;
             s_odd[turn] = 1;
           }
+      } else {
+#pragma unroll
+        for (int u = 0; u < 4; u++) big |= fabsf(coming[i][u]) >= MOST;
       }
       put((which ? Vs : Ks) + r * P + d, L::KV_PART, coming[i]);
     }
-    __syncthreads();
+    const bool big_scores = __syncthreads_or(big) || big_queries;   // (the same for the whole CTA)
     if (threadIdx.x == 0) s_odd[turn ^ 1] = 0;   // (written again behind the next barrier)
     if (jt + BN <= j_hi) fetch(jt + BN);
     if (jt > w_hi || jt + BN <= w_lo) continue;   // (nothing here for this warp's rows)
@@ -167,6 +176,20 @@ __global__ void __launch_bounds__(128) packed_f32_kernel(const float* __restrict
           mma(s[2 * np + 1], q[A[t]], k[np][B[t]][2], k[np][B[t]][3]);
         }
       }
+    }
+    if (big_scores) {
+#pragma unroll
+      for (int n = 0; n < BN / 8; n++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          const int j = jt + n * 8 + 2 * c + (e & 1), i = q0 + r0 + 8 * (e >> 1);
+          if (j < first[e >> 1] || j > i) continue;
+          const float *q = qkv + i * row_stride + (long long)h * hd, *k = qkv + j * row_stride + (long long)(H + g) * hd;
+          float x = 0.f;
+#pragma unroll 1
+          for (int d = 0; d < hd; d++) x = fmaf(q[d], k[d], x);
+          s[n][e] = x;
+        }
     }
     float top[2] = {m[0], m[1]};
 #pragma unroll
@@ -241,7 +264,7 @@ __global__ void __launch_bounds__(128) packed_f32_kernel(const float* __restrict
             for (int e = 0; e < 2; e++) {
               const int d = d8 * 8 + 2 * c + e;
               const float x = d < hd ? v[d] : 0.f;
-              if (!(fabsf(x) < INFINITY)) {
+              if (!(fabsf(x) < MOST)) {
                 if (j >= first[0] && j <= q0 + r0) o[d8][e] = fmaf(w0, x, o[d8][e]);
                 if (j >= first[1] && j <= q0 + r0 + 8) o[d8][2 + e] = fmaf(w1, x, o[d8][2 + e]);
               }

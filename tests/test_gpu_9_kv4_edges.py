@@ -81,7 +81,7 @@ def check_rows(got, want, tol, rows):
     R.check(got[rows], want[rows], tol[rows])
 
 
-@pytest.mark.parametrize("dt", [torch.bfloat16])
+@pytest.mark.parametrize("dt", DTYPES)
 @pytest.mark.parametrize("hd", [64, 128, 40, 13])
 @pytest.mark.parametrize("cap,window", [(50.0, None), (0.0, 30)])
 def test_packed_huge_values_are_for_those_who_see_them(dt, hd, cap, window):
@@ -107,7 +107,7 @@ def test_packed_huge_values_are_for_those_who_see_them(dt, hd, cap, window):
         check_rows(got, seen, loose, slice(150, 150 + window + 1 if window else 303))
 
 
-@pytest.mark.parametrize("dt", [torch.bfloat16])
+@pytest.mark.parametrize("dt", DTYPES)
 @pytest.mark.parametrize("hd", [64, 128])
 def test_packed_huge_values_far_away(dt, hd):
     """A huge value that is seen from so far that ALiBi leaves nothing of it: e^-390 of it is below 10^-130."""
@@ -121,6 +121,25 @@ def test_packed_huge_values_far_away(dt, hd):
             x[96:100, (H + kv) * hd:] = value
             got = ops.swa_packed(x, cu, slopes, H, None, cap)
             check_rows(got, want, tol, list(range(96)) + list(range(200, n)))
+
+
+@pytest.mark.parametrize("hd", [64, 128, 30])
+@pytest.mark.parametrize("cap", [0.0, 50.0])
+def test_packed_huge_queries_and_keys(hd, cap):
+    """The largest fp32 numbers in queries and keys, where the other side is 0: they add nothing to a score."""
+    from flash_stu_2_b200 import ops
+    g, H, kv, lengths, dt = gen(hd + 2), 4, 2, (50, 90), torch.float32
+    qkv, cu, slopes = activations(g, sum(lengths), H, kv, hd, dt), cu_of(lengths), slopes_of(H)
+    x = qkv.view(-1, H + 2 * kv, hd)
+    x[:, :H, 5] = 0.0
+    x[:, H:H + kv, 7] = 0.0
+    want, tol = R.packed(qkv, lengths, 0, slopes, H, kv, 40, cap, dt)
+    for value in huge(dt):
+        y = qkv.clone().view(-1, H + 2 * kv, hd)
+        y[33, H:H + kv, 5] = value
+        y[70, :H, 7] = value
+        y[139, H + 1, 5] = value
+        R.check(ops.swa_packed(y.flatten(1), cu, slopes, H, 40, cap, kv_heads=kv), want, tol)
 
 
 # ---------------------------------------------------------------------------------------------------- infinite scores
@@ -144,7 +163,7 @@ def by_hand(qkv, lengths, slopes, H, kv, window, cap, dt, unseen):
     return out, tol
 
 
-@pytest.mark.parametrize("dt", [torch.bfloat16])
+@pytest.mark.parametrize("dt", DTYPES)
 @pytest.mark.parametrize("hd", [64, 128, 13])
 @pytest.mark.parametrize("beside", [False, True])
 def test_packed_keys_of_no_weight(dt, hd, beside):
@@ -168,7 +187,7 @@ def test_packed_keys_of_no_weight(dt, hd, beside):
         R.check(got[100:], want[100:], tol[100:])
 
 
-@pytest.mark.parametrize("dt", [torch.bfloat16])
+@pytest.mark.parametrize("dt", DTYPES)
 @pytest.mark.parametrize("hd", [64, 128, 13])
 def test_packed_infinite_scores_are_capped(dt, hd):
     """A soft cap makes a finite score of an infinite one, the same as of one that is far past it."""
