@@ -71,10 +71,7 @@ __global__ void __launch_bounds__(256) kv4_write_kernel(const T* __restrict__ qk
   }
   __shared__ int last;
   __syncthreads();
-  if (threadIdx.x == 0) {
-    __threadfence();
-    last = atomicAdd(&pos[1], 1) == (int)gridDim.x - 1;
-  }
+  if (threadIdx.x == 0) last = kv4::last_to_arrive(&pos[1], (int)gridDim.x);
   __syncthreads();
   if (last) {
     for (int b = threadIdx.x; b < B; b += 256) pos[2 * b] += cu ? max(cu[b + 1] - cu[b], 0) : per_seq;

@@ -92,6 +92,14 @@ __device__ __forceinline__ int word_at(int i, int piece, int pieces) { return i 
 // Slot of the token at position t.  (A position that no sequence has, below 0, still falls into the ring.)
 __device__ __forceinline__ int slot_of(int t, int slots) { return (int)((unsigned)t % (unsigned)slots); }
 
+// One thread of each CTA, behind a barrier that all of the CTA's threads pass once they have read the positions: whether the CTA is the last, which moves the positions
+// on.  Release keeps each CTA's reading ahead of its arrival, acquire the last one's writing behind all arrivals.
+__device__ __forceinline__ bool last_to_arrive(int* counter, int ctas) {
+  int before;
+  asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(before) : "l"(counter) : "memory");
+  return before == ctas - 1;
+}
+
 inline int geometry(int B, int H, int Hk, int hd, int slots, int dtype) {
   if (dtype != STU_F32 && dtype != STU_BF16) return STU_ERR_DTYPE;
   if (B <= 0 || Hk <= 0 || H < Hk || H % Hk || hd <= 0 || slots <= 0 || slots % 16 || slots > 1 << 24) return STU_ERR_SHAPE;   // (offsets within a head's run fit 32 bits)

@@ -138,12 +138,10 @@ __global__ void __launch_bounds__(WARPS * 32, W == 128 ? 3 : 4) kv4_step_kernel(
   const int t = pos[2 * b];
   if (update_cache) {   // every CTA has read its position before it arrives here; the last one to arrive moves all of them on
     __syncthreads();
-    if (threadIdx.x == 0) {
-      const int total = gridDim.x * gridDim.y * gridDim.z;
-      if (atomicAdd(&pos[1], 1) == total - 1) {
-        pos[1] = 0;
-        for (int i = 0; i < B; i++) pos[2 * i] += 1;
-      }
+    // (The first warp has the copies to ask for.  Ordered arrivals take a step of 32 sequences 0.7 us of 23.4; by the first warp 0.3, and one of one sequence 0.6 of 9.2.)
+    if (threadIdx.x == 32 && kv4::last_to_arrive(&pos[1], gridDim.x * gridDim.y * gridDim.z)) {
+      pos[1] = 0;
+      for (int i = 0; i < B; i++) pos[2 * i] += 1;
     }
   }
   const int newest = kv4::slot_of(t, slots), live = min(max(t, 0), window);   // the `live` slots before slot `newest`, around the ring's end
