@@ -77,7 +77,9 @@ class StreamAhead:
         """The buffers for steps from here to position `last`, or None."""
         if not cls.supported(layers, past, B):
             return None
-        ring = sum(2 * e[0].numel() * e[0].element_size() * min(last, e[0].shape[1]) // e[0].shape[1] for e in past if e is not None and len(e) == 3)
+        # (rings of values and of 4 bits alike: what the window's part of them holds by then)
+        ring = sum(2 * e[0].numel() * e[0].element_size() * min(last, layer.attn.window + 1) // (layer.attn.window + 1)
+                   for layer, e in zip(layers, past) if e is not None and len(e) == 3)
         stus = [(layer, e) for layer, e in zip(layers, past) if hasattr(layer, "stu")]
         hist, d = stus[0][1][0], stus[0][1][0].shape[1]
         apart = not all(ops.can_fuse_norm(B, layer.mlp.intermediate_size, d, ops.EPI_GELU_MUL, hist.dtype) for layer, _ in stus)

@@ -54,3 +54,22 @@ def test_the_furthest_position_is_held_to_the_capacity():
     for t in ((100, 5), (5, 100)):
         with pytest.raises(ValueError, match="exceeds the capacity"):
             STU.decode_step(stu, torch.zeros(2, 8), None, 1e-6, (torch.zeros(2, 8, 2, 56), ragged(*t)), torch.zeros(2, 8))
+
+
+@pytest.mark.parametrize("kv_bits", [None, 4])
+@pytest.mark.parametrize("last", [10, 63, 200])
+def test_streams_count_what_rings_hold(monkeypatch, kv_bits, last):
+    """The bytes of keys and values that steps up to position `last` read, by the window and not by the rings' second axis (of 4 bits: heads)."""
+    import flash_stu_2_b200 as F
+    from flash_stu_2_b200.stream_ahead import StreamAhead
+    asked = []
+    monkeypatch.setattr(StreamAhead, "supported", staticmethod(lambda *a: True))
+    monkeypatch.setattr(StreamAhead, "sms", staticmethod(lambda *a: asked.append(a) or 0))
+    monkeypatch.setattr("flash_stu_2_b200.stream_ahead._sm_count", lambda dev: 148)
+    cfg = F.FlashSTUConfig(n_embd=64, n_heads=4, n_layers=2, seq_len=256, window_size=63, vocab_size=11, mlp_scale=2, num_eigh=4, kv_bits=kv_bits,
+                           torch_dtype=torch.bfloat16)
+    m = F.FlashSTU(cfg)
+    past = [layer.stu.new_cache(16, "cpu") if hasattr(layer, "stu") else layer.attn.new_cache(16, "cpu") for layer in m.layers]
+    assert StreamAhead.plan(m.layers, past, 16, last, 1000) is None
+    row = 4 * 20 if kv_bits else 64 * 2                      # bytes of a position's keys: heads of 16 in 4 bits are 20, a row of 64 bf16 128
+    assert asked[0][6] == 2 * 16 * row * min(last, 64)
