@@ -1226,7 +1226,7 @@ def kv4_read(k4: torch.Tensor, v4: torch.Tensor, hd: int, dtype: torch.dtype):
 
 def kv4_step(qkv: torch.Tensor, k4: torch.Tensor, v4: torch.Tensor, pos: torch.Tensor, slopes: Optional[torch.Tensor], H: int, window: int,
              softcap: float = 0.0, update_cache: bool = True):
-    """swa_forward of one new token per sequence, qkv [batch, 1, (H + 2 kv_heads) hd], over rings of 4 bits: its own key and value as they are,
+    """swa_forward of one new token per sequence (at most 65535 of them), qkv [batch, 1, (H + 2 kv_heads) hd], over rings of 4 bits: its own key and value as they are,
     those of the `window` positions before it as the rings hold them.  update_cache: they are stored, and pos moves on.  Returns [batch, 1, H hd]."""
     softcap = float(softcap or 0.0)
     if not _arenas or getattr(_local, "arena", None) is None:
@@ -1244,6 +1244,8 @@ def kv4_step(qkv: torch.Tensor, k4: torch.Tensor, v4: torch.Tensor, pos: torch.T
     _check_scores(slopes, H, softcap, "kv4_step")
     if qkv.dim() != 3 or qkv.shape[:2] != (B, 1):
         raise ValueError(f"kv4_step: qkv {tuple(qkv.shape)} is not one token for each of {B} sequences")
+    if B > 65535:
+        raise ValueError(f"kv4_step: {B} sequences are more than a call takes (65535)")
     if not 0 <= window < slots:
         raise ValueError(f"kv4_step: a window of {window} earlier positions and the new one do not fit {slots} slots")
     _cuda(qkv, k4, v4, pos, slopes)

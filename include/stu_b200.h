@@ -402,7 +402,7 @@ int stu_swa_packed(const void* qkv, long long row_stride, const int* cu_seqlens,
  * stu_kv4_write: the keys and values of qkv's rows (as in stu_swa_packed; without cu_seqlens rows / B of each sequence) from position pos[2 b] on, of each
  * sequence the last `slots`; pos moves on by all of them.
  * stu_kv4_read: both rings as values [B][slots][Hk * hd], in the order of the slots.
- * stu_kv4_step: attention of one new token per sequence (qkv: B rows) over its own key and value, as they are, and the last `window` < slots earlier
+ * stu_kv4_step: attention of one new token per sequence (qkv: B <= 65535 rows) over its own key and value, as they are, and the last `window` < slots earlier
  * ones, as the rings hold them; out [B][H * hd].  update_cache: the new key and value are stored, and pos moves on. */
 int stu_kv4_write(const void* qkv, long long row_stride, void* k4, void* v4, int* pos, const int* cu_seqlens, int B, long long rows,
                   int H, int Hk, int hd, int slots, int dtype, void* stream);

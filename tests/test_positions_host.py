@@ -73,3 +73,11 @@ def test_streams_count_what_rings_hold(monkeypatch, kv_bits, last):
     assert StreamAhead.plan(m.layers, past, 16, last, 1000) is None
     row = 4 * 20 if kv_bits else 64 * 2                      # bytes of a position's keys: heads of 16 in 4 bits are 20, a row of 64 bf16 128
     assert asked[0][6] == 2 * 16 * row * min(last, 64)
+
+
+def test_steps_of_too_many_sequences_are_refused():
+    from flash_stu_2_b200 import ops
+    k4, v4 = ops.kv4_rings(65536, 16, 1, 8, "cpu")
+    qkv, pos = torch.zeros(65536, 1, 24), torch.zeros(65536, 2, dtype=torch.int32)
+    with pytest.raises(ValueError, match="65535"):
+        ops.kv4_step(qkv, k4, v4, pos, None, 1, 15)
