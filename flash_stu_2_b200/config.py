@@ -19,7 +19,7 @@ class FlashSTUConfig(PretrainedConfig):
     weights are made from them at the first call.  Prefills and MLPs of 1536 and wider gain; token steps of small layers lose, whose bf16
     sub-layers are one kernel (a block of d=1024: 8 sequences 21 -> 27 us).  kv_bits=4 holds the attention layers' keys and values in 4 bits (with a
     lowest value and a step for each 64 of a head: 4.5 bits a number, head dimensions of a multiple of 8): a token step reads 3.6 times less of them, and they take as
-    much less memory; each is up to 1/30 of its 64's range off.  Small batches are then stepped layer by layer, not by one kernel for all of them.
+    much less memory; each is up to 1/30 of its 64's range off, to which the rounding of their lowest adds up to 2^-7 of that.  Small batches are then stepped layer by layer, not by one kernel for all of them.
     """
     model_type = "FlashSTU"
 

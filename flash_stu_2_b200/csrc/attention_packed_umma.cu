@@ -15,11 +15,12 @@
 // is the output's rounding).
 // With ALiBi the maximum is taken for what it will be at the row's end if the scores stay as they are.  Where they do not, all of a row's weights may be too small for fp32:
 // the row is computed again, as below.
-// Measured: 16384 tokens, 16 heads of 128 on 2, 1070 to 1115 us (1 PFLOP/s, the tensor pipe 58 % busy at the 1.45 GHz that the power limit leaves); 16 prompts of 14140 tokens, 12 heads of 128,
-// window 1024, cap and ALiBi, 141 us (380 TFLOP/s); 9311 tokens, 12 heads of 64, window 512, 73 us.  Bound by the softmax where there is a cap or a short window (2900 clocks of a warp for a tile
-// whose products take 1024), else by power and by the chain from scores to the next scores.  Instead: key tiles of 64 1115 to 1240 us for the 16384 tokens, an issuer per tile of queries 1258.
+// Measured: 16384 tokens, 16 heads of 128 on 2, 1120 to 1150 us (0.96 to 0.98 PFLOP/s, the tensor pipe 58 % busy at 1.45 GHz, where the library's products keep it 87 % busy at 1.3); 16 prompts of
+// 14140 tokens, 12 heads of 128, window 1024, cap and ALiBi, 141 us (380 TFLOP/s); 9311 tokens, 12 heads of 64, window 512, 73 us.  Bound by the softmax where there is a cap or a short window (2900
+// clocks of a warp for a tile whose products take 1024), else by the chain from scores to the next scores.  Instead: key tiles of 64 1115 to 1240 us for the 16384 tokens, an issuer per tile of queries 1258.
 // The tensor core adds 0 times what a masked key's value holds: where that is NaN or infinite, a row with a finite sum of weights has a result that is not, and is
-// computed again on the CUDA cores over the keys that it sees.
+// computed again on the CUDA cores over the keys that it sees.  (One key after the other by a warp, and a warp's rows in turn: many such rows of many keys take far longer than the rest, by estimate 0.2 s
+// for 16384 tokens of 16 heads that all meet one.)
 #include <cuda.h>
 
 #include "attention_packed.cuh"
@@ -33,11 +34,11 @@ constexpr int BM = 128, BN = 128, STAGES = 4;
 constexpr int THREADS = 384, REGS_SOFTMAX = 208, REGS_OTHERS = 80;
 constexpr int STATUS_PACKED = 13;
 constexpr float LOG2E = 1.4426950408889634f;
-// tanh(y) = y (T0 + T1 y^2 + T2 y^4) for |y| <= 1/2: relative error 2.3e-5 (these and exp2's coefficients: Remez' exchange on the relative error)
+// tanh(y) = y (T0 + T1 y^2 + T2 y^4) for |y| <= 1/2: relative error 2.3e-5 (Chebyshev interpolation on [0, 1/4] in y^2)
 constexpr float T0 = 0.999977239f, T1 = -0.331685329f, T2 = 0.115185198f;
-// ... = y (T0_TINY + T1_TINY y^2) for |y| <= 1/5: 2.6e-5
+// ... = y (T0_TINY + T1_TINY y^2) for |y| <= 1/5: 2.6e-5 (the least there is)
 constexpr float T0_TINY = 0.999973796f, T1_TINY = -0.328076375f;
-// How far a score may outgrow what scores are counted from; the least sum of weights (what it leaves out is below 2^-126 a key)
+// How far a score may outgrow what scores are counted from (heads of 64, 9311 tokens, with 2 instead of 8: error against 64 bits 2.02e-3 instead of 2.05e-3, 75 us instead of 73); the least sum of weights (what it leaves out is below 2^-126 a key)
 constexpr float LAG = 8.f, LEAST = 0x1p-90f;
 
 // Of 8 pairs of weights those that the FMA pipe makes (16384 tokens: 1140 us with 1 of them, 1070 to 1115 with 2, 1144 with 3, 1236 with 4); pairs whose arithmetic is interleaved

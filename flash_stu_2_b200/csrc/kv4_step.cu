@@ -13,7 +13,7 @@
 // Slots come by bulk copies, 128 at a time for the CTA's four warps, into three stages (18 KB each for heads of 128).
 // Warps are merged through shared memory, CTAs of a cluster through distributed shared memory, in a fixed order; the new token's own key and value join there, as
 // they are.  The ring's slot of the new token holds one that is out of everyone's window; it is written by one warp.
-// Bound by HBM where the grid is large (4.5 bits a number), by latency where it is small.
+// Bound by instructions and a warp's chain of scores, softmax and values where the grid is large (32 sequences, 12 heads of 128, 1024 keys: 23.4 us, 2.4 TB/s of HBM's 6.5), by latency where it is small.
 #include <cooperative_groups.h>
 
 #include "kv4.cuh"
@@ -515,7 +515,7 @@ int launch(const void* qkv, long long row_stride, void* k4, void* v4, int* pos, 
   const int groups = (H / Hk + 7) / 8;
   // CTAs that share the keys: as many as take least by rounds of what the SMs hold at a time, times a CTA's tiles with its beginning and end (3 tiles, with a cluster 5), three tenths more for
   // each further CTA on an SM.  Of 37 measured sizes (12 to 1536 sequences' heads, 500 to 16384 keys, heads of 64 and 128) the time is 2 % above the best number's on average, at most 28 %;
-  // with the fullest SM's work alone, as if clusters began as places become free, it was 8 %.  Heads of 128, us with 1, 2, 3, 4, 8 CTAs: 12 heads of 1025 keys 14.3, 11.9, 10.2, 10.0, 8.6; 384
+  // with the fullest SM's work alone, as if clusters began as places become free, it was 8 % (all without ordered arrivals).  Heads of 128, us with 1, 2, 3, 4, 8 CTAs: 12 heads of 1025 keys 14.3, 11.9, 10.2, 10.0, 8.6; 384
   // of them 22.7, 31.4, 36.1, 45.3, 78.4; 128 of 16385 keys, 8 queries each, 309, 170, 119, 154, 158.
   const long long pairs = (long long)Hk * B * groups, sms = device_sm_count();
   const int tiles = window / BLOCK + 1, per_sm = W == 128 ? 3 : 4;
